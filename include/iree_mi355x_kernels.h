@@ -272,6 +272,115 @@ int32_t iree_mi355x_classify_attention(const iree_mi355x_attention_t *args,
 size_t iree_mi355x_attention_workspace_bytes(
     const iree_mi355x_attention_t *args);
 
+// ---------------------------------------------------------- paged KV cache
+//
+// A KV cache in pages, for a batch of requests of any lengths: the tables that
+// say where a request's tokens are, the rows appended to it, and the attention
+// that reads it. The reference has none of it: its attention reads a slice of
+// one contiguous cache (integration_tests/models/micro/
+// attention-cache-slice-f16/model.py:10-29). Lengths and tables are device
+// data, so a step can be captured once and replayed with other lengths. What
+// they say is checked on the device: a negative count is 0, a page or slot
+// outside the cache is skipped.
+//
+// The new tokens of a step are packed rows: request b's are rows
+// row_starts[b] .. row_starts[b + 1] - 1.
+
+// Tables of one step from its requests' lengths: the tokens of each that the
+// pages hold (cached) and that the step adds (added). With up(x) = ceil(x /
+// page_size), b in [0, batch):
+//   row_starts[b] = sum_{i<b} added[i], row_starts[batch] their sum
+//   lengths[b] = cached[b] + added[b]
+//   take[b] = min(up(lengths[b]), table_width) - min(up(cached[b]),
+//     table_width), needed[0] = sum take
+//   block_table[b][up(cached[b]) + j] = free_pages[sum_{i<b} take[i] + j],
+//     j in [0, take[b]); -1 past free_count
+//   slots[row_starts[b] + i] = page * page_size + place of token cached[b] + i,
+//     i in [0, added[b]); -1 where it has no page, and for rows past the last
+// Other entries of the table are left as they were. Sums stop at 2^31 - 1;
+// only `rows` slots are written. needed[0] > free_count tells that the list
+// was too short; needed[0] entries of it are used up.
+typedef struct iree_mi355x_page_tables_t {
+  const int32_t *cached;      // [batch]
+  const int32_t *added;       // [batch]
+  const int32_t *free_pages;  // [free_count]
+  int32_t *block_table;       // [batch, table_width], row pitch table_stride
+  int32_t *row_starts;        // [batch + 1]
+  int32_t *lengths;           // [batch]
+  int32_t *slots;             // [rows]
+  int32_t *needed;            // [1]
+  int64_t batch, free_count, page_size;
+  int64_t table_width, table_stride;
+  int64_t rows;
+} iree_mi355x_page_tables_t;
+int iree_mi355x_page_tables(const iree_mi355x_page_tables_t *args,
+                            void *stream);
+
+// The cache of one layer: f16 [pages, kv_heads, page_size, head dim] through
+// (page, head, token) element strides, the head dim contiguous; K and V
+// apart. Head dims are multiples of 8 up to 256, strides multiples of 8,
+// bases 16-byte aligned; the rows of a head lie within 64 GiB.
+typedef struct iree_mi355x_kv_cache_t {
+  void *k, *v;
+  int64_t pages, page_size, kv_heads;
+  int64_t head_dim, head_dim_v;
+  int64_t k_strides[3], v_strides[3];
+} iree_mi355x_kv_cache_t;
+
+// Appends rows: k [rows, kv_heads, head_dim], v [rows, kv_heads, head_dim_v]
+// through (row, head) element strides, aligned as the cache, row r to slot
+// slots[r] (page slots[r] / page_size, token slots[r] % page_size). A row
+// whose slot is not in the cache is skipped. The slots of a call are
+// different ones; where two rows name one, each 16 bytes of it come from
+// either.
+int iree_mi355x_append_kv_f16(const iree_mi355x_kv_cache_t *cache,
+                              const void *k, const void *v, int64_t rows,
+                              const int64_t k_strides[2],
+                              const int64_t v_strides[2],
+                              const int32_t *slots, void *stream);
+
+// Attention of packed rows over the cache, f16 in and out, f32 scores and
+// softmax. All requests share a prefix of prefix_length tokens in the pages
+// prefix_pages (0: none, paged attention); request b's own tokens are the
+// first lengths[b] of the pages block_table[b]. Row row_starts[b] + i sees
+// the prefix and own tokens 0 .. lengths[b] - added[b] + i, added[b] =
+// row_starts[b + 1] - row_starts[b]: the new tokens are its last ones.
+//   o[row, h] = softmax(q[row, h] k^T * scale) v, KV head h / (heads /
+//   kv_heads); 0 for a row that sees no key
+// Tokens in pages outside the cache are not seen, nor those past table_width
+// pages. Rows from row_starts[batch] on are left as they were. A NaN or
+// infinity in the V of a token that a row does not see may reach it where
+// another row of its tile does (0 times it).
+// The prefix's keys are read once for tiles of rows of the whole batch where
+// requests bring few rows each, which takes a workspace; without one every
+// request reads them. A call runs with any workspace or none. Unlike the
+// matmuls' it needs no zero-filled contents; its first 256 KiB (their
+// counters) are left alone. row_starts must ascend from 0.
+typedef struct iree_mi355x_paged_attention_t {
+  iree_mi355x_kv_cache_t cache;
+  const void *q;               // [rows, heads, head_dim]
+  void *o;                     // [rows, heads, head_dim_v]
+  const int32_t *row_starts;   // [batch + 1]
+  const int32_t *lengths;      // [batch]
+  const int32_t *block_table;  // [batch, table_width], row pitch table_stride
+  const int32_t *prefix_pages;  // at least ceil(prefix_length / page_size)
+  int64_t rows, heads, batch;
+  int64_t table_width, table_stride;
+  int64_t prefix_length;
+  int64_t q_strides[2], o_strides[2];  // (row, head); q's multiples of 8 and
+                                       // 16-byte aligned, o's of 4 and 8-byte
+  float scale;
+  uint32_t flags;  // 0
+} iree_mi355x_paged_attention_t;
+int iree_mi355x_shared_prefix_attention_f16(
+    const iree_mi355x_paged_attention_t *args, void *workspace,
+    size_t workspace_bytes, void *stream);
+
+// The workspace a call of these extents can use (0: none); pointers and
+// strides are not looked at.
+size_t iree_mi355x_shared_prefix_attention_workspace_bytes(
+    const iree_mi355x_paged_attention_t *args);
+
 // Workspace a matmul_f16 / matmul_i8 / w8a16_matmul call of this shape
 // needs (split-K
 // partials and arrival counters), 0 if none. Mirrors the scratch query of the

@@ -86,6 +86,9 @@ EXPORTED_SYMBOLS = (
     "iree_mi355x_loaded_executable_release",
     "iree_mi355x_matmul_f16_no_alloc",
     "iree_mi355x_match_linalg_op", "iree_mi355x_match_dispatch_region",
+    "iree_mi355x_page_tables", "iree_mi355x_append_kv_f16",
+    "iree_mi355x_shared_prefix_attention_f16",
+    "iree_mi355x_shared_prefix_attention_workspace_bytes",
 )
 
 # Activations of the fused matmul epilogue (include/iree_mi355x_kernels.h).
@@ -304,6 +307,11 @@ def library():
     lib.iree_mi355x_attention_workspace_bytes.restype = sz
     lib.iree_mi355x_attention_workspace_bytes.argtypes = [p]
     lib.iree_mi355x_classify_attention.argtypes = [p, sz]
+    lib.iree_mi355x_page_tables.argtypes = [p, p]
+    lib.iree_mi355x_append_kv_f16.argtypes = [p, p, p, i64, p, p, p, p]
+    lib.iree_mi355x_shared_prefix_attention_f16.argtypes = [p, p, sz, p]
+    lib.iree_mi355x_shared_prefix_attention_workspace_bytes.restype = sz
+    lib.iree_mi355x_shared_prefix_attention_workspace_bytes.argtypes = [p]
     lib.iree_mi355x_matmul_workspace_bytes.restype = sz
     lib.iree_mi355x_matmul_workspace_bytes.argtypes = [i64, i64, i64, u32]
     lib.iree_mi355x_batch_matmul_f16.argtypes = [
@@ -1160,6 +1168,245 @@ def attention(q, k, v, o=None, *, causal=True, scale=None, mask=None,
     _call(lib.iree_mi355x_attention_with_workspace, (args,), need,
           q.get_device(), stp)
     return o
+
+
+# ------------------------------------------------------- paged KV cache ----
+
+class PageTablesArgs(ctypes.Structure):
+    """iree_mi355x_page_tables_t."""
+    _fields_ = [(n, ctypes.c_void_p) for n in (
+        "cached", "added", "free_pages", "block_table", "row_starts",
+        "lengths", "slots", "needed")] + [(n, ctypes.c_int64) for n in (
+            "batch", "free_count", "page_size", "table_width",
+            "table_stride", "rows")]
+
+
+class KvCache(ctypes.Structure):
+    """iree_mi355x_kv_cache_t."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p)] + [
+        (n, ctypes.c_int64) for n in ("pages", "page_size", "kv_heads",
+                                      "head_dim", "head_dim_v")] + [
+        ("k_strides", ctypes.c_int64 * 3), ("v_strides", ctypes.c_int64 * 3)]
+
+
+class PagedAttentionArgs(ctypes.Structure):
+    """iree_mi355x_paged_attention_t."""
+    _fields_ = [("cache", KvCache)] + [(n, ctypes.c_void_p) for n in (
+        "q", "o", "row_starts", "lengths", "block_table",
+        "prefix_pages")] + [(n, ctypes.c_int64) for n in (
+            "rows", "heads", "batch", "table_width", "table_stride",
+            "prefix_length")] + [
+        ("q_strides", ctypes.c_int64 * 2), ("o_strides", ctypes.c_int64 * 2),
+        ("scale", ctypes.c_float), ("flags", ctypes.c_uint32)]
+
+
+# The structures above as bytes.
+_PAGE_TABLES = struct.Struct("@8P6q")
+_KV_CACHE = struct.Struct("@2P11q")
+_PAIR = struct.Struct("@2q")
+_PAGED_ATTENTION = struct.Struct("@2P11q6P10qfI")
+
+
+def _ints(t, name, dims=1):
+    """A device table: int32, its rows contiguous."""
+    import torch
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32:
+        raise TypeError(f"{name} must be an int32 tensor")
+    if t.dim() != dims or not (_unit_col(t) or t.numel() == 0):
+        raise ValueError(f"{name} must be {dims}-D with unit column stride")
+
+
+def _cache_fields(k_cache, v_cache):
+    """(the fields of iree_mi355x_kv_cache_t after its pointers, the caches
+    checked)."""
+    import torch
+    for t, nm in ((k_cache, "k_cache"), (v_cache, "v_cache")):
+        if (not isinstance(t, torch.Tensor) or t.dtype != torch.float16
+                or t.dim() != 4 or not _unit_col(t)):
+            raise TypeError(f"{nm} must be a 4-D f16 tensor with unit "
+                            "stride along head_dim")
+    pages, heads, page, d = k_cache.shape
+    dv = v_cache.shape[3]
+    _shape(v_cache, (pages, heads, page, dv), "v_cache")
+    return (pages, page, heads, d, dv, *k_cache.stride()[:3],
+            *v_cache.stride()[:3])
+
+
+def _rows_of(t, name):
+    import torch
+    if (not isinstance(t, torch.Tensor) or t.dtype != torch.float16
+            or t.dim() != 3 or not _unit_col(t)):
+        raise TypeError(f"{name} must be a 3-D f16 tensor with unit stride "
+                        "along head_dim")
+
+
+def _run_on(index, stream, call):
+    """call(raw stream) with device `index` current: the current stream of
+    that device unless one is given."""
+    import torch
+    if index == torch.cuda.current_device():
+        return call(_stream_ptr(stream))
+    with torch.cuda.device(index):
+        return call(_stream_ptr(stream))
+
+
+def page_tables(cached, added, free_pages, block_table, page_size, rows, *,
+                stream=None):
+    """Tables of one step of a paged KV cache, from device lengths: `cached`
+    [B] tokens of each request are in its pages, `added` [B] more come. Takes
+    the pages that they need from `free_pages` [F] in the requests' order,
+    writes them into `block_table` [B, W] in place, and returns (row_starts
+    [B + 1], lengths [B], slots [rows], needed [1]): where each request's new
+    rows start among the packed rows, the tokens after the step, every new
+    row's page * page_size + place (-1: none, or a row past the last), and
+    how many pages were taken (more than F: the list was too short, and the
+    pages past it are -1). All tables are int32."""
+    import torch
+    for t, nm in ((cached, "cached"), (added, "added"),
+                  (free_pages, "free_pages")):
+        _ints(t, nm)
+    _ints(block_table, "block_table", 2)
+    batch = cached.shape[0]
+    _shape(added, (batch,), "added")
+    width = block_table.shape[1]
+    _shape(block_table, (batch, width), "block_table")
+    if page_size < 1 or rows < 0:
+        raise ValueError(f"page_size {page_size} and rows {rows} must be at "
+                         "least 1 and 0")
+    _on_device((cached, "cached"), (added, "added"),
+               (free_pages, "free_pages"), (block_table, "block_table"))
+    lib = library()
+
+    def call(s):
+        out = torch.empty(2 * batch + 2 + rows, dtype=torch.int32,
+                          device=cached.device)
+        starts, lengths, needed, slots = out.split(
+            (batch + 1, batch, 1, rows))
+        at = out.data_ptr()
+        _check(lib.iree_mi355x_page_tables(_PAGE_TABLES.pack(
+            cached.data_ptr(), added.data_ptr(), free_pages.data_ptr(),
+            block_table.data_ptr(), at, at + 4 * (batch + 1),
+            at + 4 * (2 * batch + 2), at + 4 * (2 * batch + 1), batch,
+            free_pages.shape[0], page_size, width, block_table.stride(0),
+            rows), s))
+        return starts, lengths, slots, needed
+
+    return _run_on(cached.get_device(), stream, call)
+
+
+def append_kv(k, v, k_cache, v_cache, slots, *, stream=None):
+    """Writes rows k [T, Hkv, D] and v [T, Hkv, Dv] (f16, any row and head
+    strides that are multiples of 8) into the pages of k_cache [P, Hkv, S, D]
+    and v_cache [P, Hkv, S, Dv], row t to place slots[t] % S of page slots[t]
+    // S. Rows whose slot is negative or past the cache are skipped; two rows
+    must not name one slot. A cache in [page, token, head] order is passed as
+    a permuted view."""
+    fields = _cache_fields(k_cache, v_cache)
+    _rows_of(k, "k")
+    _rows_of(v, "v")
+    rows = k.shape[0]
+    _shape(k, (rows, fields[2], fields[3]), "k")
+    _shape(v, (rows, fields[2], fields[4]), "v")
+    _ints(slots, "slots")
+    _shape(slots, (rows,), "slots")
+    _on_device((k, "k"), (v, "v"), (k_cache, "k_cache"),
+               (v_cache, "v_cache"), (slots, "slots"))
+    lib = library()
+    cache = _KV_CACHE.pack(k_cache.data_ptr(), v_cache.data_ptr(), *fields)
+    _run_on(k.get_device(), stream, lambda s: _check(
+        lib.iree_mi355x_append_kv_f16(
+            cache, k.data_ptr(), v.data_ptr(), rows,
+            _PAIR.pack(*k.stride()[:2]), _PAIR.pack(*v.stride()[:2]),
+            slots.data_ptr(), s)))
+
+
+@functools.lru_cache(maxsize=4096)
+def _paged_workspace_need(rows, batch, h, hkv, d, dv, page, width,
+                          prefix) -> int:
+    a = PagedAttentionArgs(rows=rows, batch=batch, heads=h,
+                           table_width=width, prefix_length=prefix)
+    a.cache.kv_heads, a.cache.page_size = hkv, page
+    a.cache.head_dim, a.cache.head_dim_v = d, dv
+    return library().iree_mi355x_shared_prefix_attention_workspace_bytes(
+        ctypes.byref(a))
+
+
+def shared_prefix_attention(q, k_cache, v_cache, row_starts, lengths,
+                            block_table, prefix_pages=None, prefix_length=0,
+                            o=None, *, scale=None, stream=None):
+    """Attention of a batch's new tokens over a paged KV cache, the keys of a
+    prefix that all requests share read once for all of them. q [T, H, D]
+    holds the requests' rows one after the other, request b's at row_starts[b]
+    .. row_starts[b + 1] - 1; its own tokens are the first lengths[b] of the
+    pages block_table[b] (the new ones included, appended before), and the
+    prefix the first prefix_length tokens of prefix_pages. A row sees the
+    prefix and its request's own tokens up to itself. k_cache [P, Hkv, S, D]
+    and v_cache [P, Hkv, S, Dv] as in append_kv; o [T, H, Dv] f16 keeps the
+    rows past row_starts[B]. Tables are int32, from page_tables. With
+    prefix_length 0 this is paged attention."""
+    import torch
+    fields = _cache_fields(k_cache, v_cache)
+    _, page, hkv, d, dv = fields[:5]
+    _rows_of(q, "q")
+    rows, h = q.shape[:2]
+    _shape(q, (rows, h, d), "q")
+    if hkv < 1 or h % hkv:
+        raise ValueError(f"{h} query heads are not a multiple of {hkv} KV "
+                         "heads")
+    if o is not None:
+        _rows_of(o, "o")
+        _shape(o, (rows, h, dv), "o")
+    _ints(lengths, "lengths")
+    _ints(row_starts, "row_starts")
+    _ints(block_table, "block_table", 2)
+    batch, width = lengths.shape[0], block_table.shape[1]
+    _shape(row_starts, (batch + 1,), "row_starts")
+    _shape(block_table, (batch, width), "block_table")
+    if prefix_length < 0:
+        raise ValueError(f"prefix_length {prefix_length} is negative")
+    if prefix_length:
+        if prefix_pages is None:
+            raise ValueError("prefix_length needs prefix_pages")
+        _ints(prefix_pages, "prefix_pages")
+        if prefix_pages.shape[0] * page < prefix_length:
+            raise ValueError(f"prefix_pages hold {prefix_pages.shape[0]} "
+                             f"pages of {page}, fewer than {prefix_length} "
+                             "tokens")
+    else:
+        prefix_pages = None
+    _on_device((q, "q"), (k_cache, "k_cache"), (v_cache, "v_cache"),
+               (row_starts, "row_starts"), (lengths, "lengths"),
+               (block_table, "block_table"), (prefix_pages, "prefix_pages"),
+               (o, "o"))
+    lib = library()
+    if scale is None:
+        scale = d ** -0.5
+    index = q.get_device()
+
+    def call(s):
+        out = torch.empty(rows, h, dv, dtype=torch.float16,
+                          device=q.device) if o is None else o
+        args = _PAGED_ATTENTION.pack(
+            k_cache.data_ptr(), v_cache.data_ptr(), *fields, q.data_ptr(),
+            out.data_ptr(), row_starts.data_ptr(), lengths.data_ptr(),
+            block_table.data_ptr(),
+            0 if prefix_pages is None else prefix_pages.data_ptr(), rows, h,
+            batch, width, block_table.stride(0), prefix_length,
+            *q.stride()[:2], *out.stride()[:2], scale, 0)
+        need = _paged_workspace_need(rows, batch, h, hkv, d, dv, page, width,
+                                     prefix_length)
+        ws = wsb = held = None
+        if need > 0 and s and _capturing(s):
+            # the graph's own: its replays share it with no other's
+            held = torch.empty(need, dtype=torch.uint8, device=q.device)
+            ws, wsb = held.data_ptr(), need
+        elif need > 0:
+            ws, wsb = _call_workspace(need, index, s)
+        _check(lib.iree_mi355x_shared_prefix_attention_f16(
+            args, ws, wsb or 0, s))
+        return out
+
+    return _run_on(index, stream, call)
 
 
 def matmul_mfma_config(index, a, b, c, *, scale=None, splits=0, accumulate=False,

@@ -33,7 +33,7 @@ int fail(int status, const char *fmt, ...) {
   return status;
 }
 
-static int ok() {
+int ok() {
   g_last_error[0] = 0;
   return IREE_MI355X_OK;
 }
@@ -63,7 +63,6 @@ static bool aligned(const void *p, size_t a) {
   return ((uintptr_t)p % a) == 0;
 }
 
-static const int64_t kMaxExtent = (int64_t)1 << 31;
 
 // The split-K partials and arrival counters of a call come from the
 // caller's workspace: the library allocates no device memory. A call whose
@@ -118,7 +117,7 @@ static int scratch_address(void **out) {
   return IREE_MI355X_OK;
 }
 
-static int launch_status(hipError_t e, const char *what) {
+int launch_status(hipError_t e, const char *what) {
   if (e != hipSuccess)
     return fail(IREE_MI355X_LAUNCH_FAILED, "%s: %s", what, hipGetErrorString(e));
   return ok();

@@ -106,6 +106,15 @@ inline bool fast_operand(const void *p, int64_t ld_bytes,
          ld_bytes < kMaxFastPitchBytes && batch_stride_bytes % 16 == 0;
 }
 
+// The C-ABI's statuses (abi.cpp): records the message of a failure, clears
+// it, or reports what a launch returned.
+int fail(int status, const char *fmt, ...);
+int ok();
+int launch_status(hipError_t e, const char *what);
+
+// Extents are below this: 32-bit row and tile counters.
+constexpr int64_t kMaxExtent = (int64_t)1 << 31;
+
 // While set, the C-ABI entry points on this thread validate and plan only:
 // no allocation, no launch; the workspace the call needs is written to
 // *sink. nullptr ends it.
@@ -338,6 +347,66 @@ hipError_t launch_attention_rows(const void *q, const void *k, const void *v,
                                  const AttentionRowsPlan &plan, int out_f32,
                                  void *workspace, void *stream);
 const KernelEntry *attention_rows_kernels(int *count);
+
+// The paged KV cache (paged_cache.hip): see iree_mi355x_page_tables_t.
+struct PageTables {
+  const int32_t *cached, *added, *free_pages;
+  int32_t *table, *row_starts, *lengths, *slots, *needed;
+  int64_t batch, free_count, width, table_stride, rows;
+  int page_size;
+};
+hipError_t launch_page_tables(const PageTables &tables, void *stream);
+
+// Rows of K and V into the cache, 16 bytes at a time: element strides of the
+// cache's (page, head, token) and of the rows' (row, head), all multiples of
+// 8, every base 16-byte aligned (checked on the host); chunks: 16-byte pieces
+// of a head's row.
+struct AppendKv {
+  const _Float16 *k, *v;
+  _Float16 *k_cache, *v_cache;
+  const int32_t *slots;
+  int64_t rows, slot_count;
+  int64_t ks[2], vs[2], kc[3], vc[3];
+  int kv_heads, chunks_k, chunks_v, page_size;
+};
+hipError_t launch_append_kv(const AppendKv &append, void *stream);
+const KernelEntry *paged_cache_kernels(int *count);
+
+// Attention over the paged cache (attention_paged.hip). Strides in elements;
+// a cache row's place within its head is counted in 16 bytes, in 32 bits
+// (checked on the host).
+struct PagedAttention {
+  const _Float16 *q, *k_cache, *v_cache;
+  _Float16 *o;
+  const int32_t *row_starts, *lengths, *table, *prefix_pages;
+  float *partials, *part_ml;  // null: the tiles store the result
+  int64_t q_row, q_head, o_row, o_head, k_head, v_head, table_stride;
+  int64_t packed;             // rows of a KV head: rows * group
+  uint64_t page_magic;        // key / page_size = key * magic >> shift
+  uint32_t k_page16, k_row16, v_page16, v_row16;
+  int page_shift, page_size, pages;
+  int batch, rows, kv_heads, group, dqk, dv;
+  int prefix, capacity;       // prefix keys, keys that a table row can name
+  float scale;
+  int prefix_tiles, prefix_splits, own_tiles, own_splits;
+};
+// Workgroups wanted: two a CU. A part of a tile's keys is at least 2 blocks a
+// wave.
+constexpr int64_t kPagedTargetWgs = 512;
+constexpr int kPagedSplitBlocks = 8;
+struct PagedPlan {
+  int dp, rp, ro;  // head-dim bucket, 16-row fragments of a tile
+  int64_t prefix_tiles, prefix_splits, own_tiles, own_splits;
+  int64_t items, workspace;
+};
+PagedPlan plan_attention_paged(int64_t rows, int64_t batch, int64_t kv_heads,
+                               int64_t group, int64_t prefix, int64_t capacity,
+                               int64_t head_dim, int64_t head_dim_v,
+                               size_t workspace_limit);
+hipError_t launch_attention_paged(const PagedAttention &attention,
+                                  const PagedPlan &plan, void *workspace,
+                                  void *stream);
+const KernelEntry *attention_paged_kernels(int *count);
 
 #ifdef __HIP_DEVICE_COMPILE__
 #define IHP_HD __device__

@@ -10,10 +10,6 @@
 #include "../../include/iree_mi355x_kernels.h"
 #include "kernels_internal.h"
 
-namespace ihp {
-int fail(int status, const char *fmt, ...);
-}
-
 namespace {
 
 using ihp::fail;
@@ -376,6 +372,7 @@ const ihp::KernelEntry *kernel_at(int index) {
   const ihp::KernelEntry *(*lists[])(int *) = {
       ihp::gemm_kernels, ihp::gemv_kernels, ihp::attention_kernels,
       ihp::attention_general_kernels, ihp::attention_rows_kernels,
+      ihp::paged_cache_kernels, ihp::attention_paged_kernels,
       ihp::runtime_kernels};
   for (auto list : lists) {
     int n = 0;
@@ -400,6 +397,10 @@ extern "C" int iree_mi355x_kernel_count(void) {
   ihp::attention_general_kernels(&n);
   total += n;
   ihp::attention_rows_kernels(&n);
+  total += n;
+  ihp::paged_cache_kernels(&n);
+  total += n;
+  ihp::attention_paged_kernels(&n);
   total += n;
   ihp::runtime_kernels(&n);
   return total + n;

@@ -1,0 +1,610 @@
+"""The paged KV cache on the GPU: tables built from lengths, rows appended to
+pages, attention of a batch behind a shared prefix, and the three in turn.
+
+Whole numbers are compared for equality with a plain loop. Attention is
+compared with the definition in 64 bits (`Attention`, which also says how far
+a result may be off, from the roundings that the kernel makes).
+"""
+import ctypes
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+H, I32 = torch.float16, torch.int32
+NAN, INF = float("nan"), float("inf")
+
+
+def up(n, page):
+    return -(-n // page)
+
+
+def ints(values):
+    return torch.tensor(values, dtype=I32, device="cuda")
+
+
+# ------------------------------------------------------------------- tables --
+
+def plain_tables(cached, added, free, table, page, rows):
+    """The definition: (table, row_starts, lengths, slots, needed)."""
+    table = [list(r) for r in table]
+    width = len(table[0]) if table else 0
+    starts, lengths, slots, taken = [0], [], [-1] * rows, 0
+    for b, (c, a) in enumerate(zip(cached, added)):
+        c, a = max(c, 0), max(a, 0)
+        for column in range(min(up(c, page), width),
+                            min(up(c + a, page), width)):
+            table[b][column] = free[taken] if taken < len(free) else -1
+            taken += 1
+        for i in range(a):
+            row, at = starts[b] + i, c + i
+            if row >= rows:
+                break
+            if at // page < width and table[b][at // page] >= 0:
+                slot = table[b][at // page] * page + at % page
+                slots[row] = slot if slot < 2 ** 31 else -1
+        starts.append(starts[b] + a)
+        lengths.append(c + a)
+    top = 2 ** 31 - 1
+    return (table, [min(s, top) for s in starts],
+            [min(n, top) for n in lengths], slots, [min(taken, top)])
+
+
+def check_tables(pkg, cached, added, free, table, page, rows, pitch=0):
+    width = len(table[0]) if table else 0
+    buf = torch.full((len(table), width + pitch), 77, dtype=I32,
+                     device="cuda")
+    got = buf[:, :width]
+    if width:
+        got.copy_(ints(table))
+    starts, lengths, slots, needed = pkg.page_tables(
+        ints(cached), ints(added), ints(free), got, page, rows)
+    want = plain_tables(cached, added, free, table, page, rows)
+    for g, w, n in zip((got, starts, lengths, slots, needed), want,
+                       ("table", "starts", "lengths", "slots", "needed")):
+        assert g.dtype == I32 and g.tolist() == w, n
+    assert bool((buf[:, width:] == 77).all()), "write past the table's rows"
+
+
+@pytest.mark.parametrize("batch", [0, 1, 2, 63, 64, 65, 511, 512, 513, 1500])
+@pytest.mark.parametrize("page", [1, 7, 16, 64])
+def test_tables(pkg, dev, batch, page):
+    g = torch.Generator().manual_seed(batch * 100 + page)
+
+    def draw(lo, hi, n):
+        return torch.randint(lo, hi, (n,), generator=g).tolist()
+
+    print(f"tables {batch} {page}", flush=True)
+    cached, added = draw(0, 60, batch), draw(0, 30, batch)
+    width = up(90, page) + 2
+    free = torch.randperm(40 * batch + 99, generator=g).tolist()
+    table = [[draw(0, 5000, 1)[0] if c < up(n, page) else -9
+              for c in range(width)] for n in cached]
+    total = sum(added)
+    need = sum(up(c + a, page) - up(c, page) for c, a in zip(cached, added))
+    for rows, have, pitch in ((total, need, 0), (total + 40, need + 9, 3),
+                              (total // 2, need // 2, 0), (0, 0, 1)):
+        check_tables(pkg, cached, added, (free * 30)[:have], table, page,
+                     rows, pitch)
+
+
+def test_tables_one_long_request(pkg, dev):
+    """Many rows of one request among single tokens; no tokens at all."""
+    added = [1] * 40 + [9000] + [0] * 5 + [1] * 30
+    cached = [17 * i % 50 for i in range(len(added))]
+    table = [[3 * i + c for c in range(600)] for i in range(len(added))]
+    check_tables(pkg, cached, added, list(range(2000)), table, 16,
+                 sum(added))
+    check_tables(pkg, cached, [0] * len(added), [5], table, 16, 12)
+
+
+def test_tables_bounds(pkg, dev):
+    """Requests longer than their table's row, counts below 0 and at the type's
+    end, pages whose slots pass 32 bits, rows without a table."""
+    top = 2 ** 31 - 1
+    table = [[1, 2, 3]] * 6
+    check_tables(pkg, [0, 40, 47, 48, 200, -5], [70, 9, 1, 3, 4, 20],
+                 list(range(9)), table, 16, 107)
+    # 600 such requests: sums past 32 bits, in more than one round
+    check_tables(pkg, [top, -top - 1, 5] * 200, [top, -3, top] * 200,
+                 list(range(7)), [[4, 4]] * 600, 16, 50)
+    check_tables(pkg, [15, 0], [1, 2], [top, 2 ** 27], [[2 ** 27], [-1]],
+                 16, 3)
+    check_tables(pkg, [15, 0], [1, 2], [2 ** 27 - 1], [[2 ** 27 - 1], [-1]],
+                 16, 3)
+    check_tables(pkg, [3, 0], [1, 2], [], [[], []], 16, 3)
+    check_tables(pkg, [0], [top], [], [[0, 0]], top, 2)
+
+
+# ------------------------------------------------------------------- append --
+
+def plain_append(cache, rows, slots):
+    flat = cache.transpose(1, 2).reshape(-1, *cache.shape[1::2]).clone()
+    for r, s in enumerate(slots):
+        if 0 <= s < flat.shape[0]:
+            flat[s] = rows[r]
+    return flat.unflatten(0, cache.shape[::2][:2]).transpose(1, 2)
+
+
+def new_cache(g, pages, heads, page, d, token_major=False, pad=0):
+    """A cache and the buffer it is a view of."""
+    shape = (pages, page, heads) if token_major else (pages, heads, page)
+    buf = torch.randn(*shape, d + pad, generator=g).half().cuda()
+    view = buf[..., :d]
+    return (view.permute(0, 2, 1, 3) if token_major else view), buf
+
+
+@pytest.mark.parametrize("token_major", [False, True])
+@pytest.mark.parametrize("rows,heads,d,dv,page,pages", [
+    (1, 1, 8, 8, 1, 1), (5, 3, 64, 64, 16, 4), (70, 8, 128, 128, 16, 9),
+    (333, 2, 40, 24, 7, 60), (9, 32, 256, 200, 24, 3),
+    (5000, 2, 64, 128, 64, 90)])
+def test_append(pkg, dev, token_major, rows, heads, d, dv, page, pages):
+    g = torch.Generator().manual_seed(rows + d)
+    print(f"append {rows} {heads} {d} {dv} {page}", flush=True)
+    kc, kbuf = new_cache(g, pages, heads, page, d, token_major, pad=8)
+    vc, vbuf = new_cache(g, pages, heads, page, dv, token_major)
+    # rows of one fused buffer, heads apart by more than their size
+    kv = torch.randn(rows, heads, d + dv + 16, generator=g).half().cuda()
+    k, v = kv[..., :d], kv[..., d + 8:d + 8 + dv]
+    slots = torch.randperm(pages * page, generator=g)[:rows].tolist()
+    slots += [-1] * (rows - len(slots))
+    if rows > 3:  # outside the cache
+        slots[1], slots[2], slots[3] = -1, pages * page, -2 ** 31
+        slots[0] = 2 ** 31 - 1 if rows > 5 else slots[0]
+    want_k = plain_append(kc, k, slots)
+    want_v = plain_append(vc, v, slots)
+    beside = kbuf[..., d:].clone()
+    pkg.append_kv(k, v, kc, vc, ints(slots))
+    assert torch.equal(kc, want_k) and torch.equal(vc, want_v)
+    assert torch.equal(kbuf[..., d:], beside)
+
+
+def test_append_far_pages(pkg, dev):
+    """Pages whose elements pass 32 bits."""
+    pages, heads, page, d = 5, 1, 2, 8
+    stride = 1 << 30  # elements: 4 pages reach 2^32
+    buf = torch.zeros(stride * (pages - 1) + 64, dtype=H, device="cuda")
+    kc = buf.as_strided((pages, heads, page, d), (stride, 16, 8, 1))
+    vc = torch.zeros(pages, heads, page, d, dtype=H, device="cuda")
+    k = torch.arange(1, 17, device="cuda").half().reshape(2, 1, 8)
+    pkg.append_kv(k, k, kc, vc, ints([9, 7]))
+    assert torch.equal(kc[4, 0, 1], k[0, 0]) and torch.equal(kc[3, 0, 1],
+                                                             k[1, 0])
+    assert int((kc != 0).sum()) == 16 and int((buf[:4096] != 0).sum()) == 0
+    q = torch.ones(1, 1, 8, dtype=H, device="cuda")
+    o = pkg.shared_prefix_attention(q, kc, kc, ints([0, 1]), ints([1]),
+                                    ints([[4]]), ints([3]), 2)
+    # keys: place 0 and 1 of page 3 (0 and k[1]), place 0 of page 4 (0)
+    w = torch.softmax(torch.tensor([0.0, float(k[1].sum()) * 8 ** -0.5, 0.0],
+                                   dtype=torch.float64), 0)[1]
+    assert (o[0, 0].double().cpu() - w * k[1, 0].double().cpu()).abs().max() \
+        <= 16 * 2 ** -11 * 2
+
+
+# ---------------------------------------------------------------- attention --
+
+class Attention:
+    """A batch's tensors, their definition in 64 bits, and how far a result
+    may be off it.
+
+    The kernel rounds each weight 2^(s - m) <= 1 to f16, by 2^-11 of it or, under
+    2^-14, by 2^-25, sums the rounded ones, and rounds the result. Over a row's
+    n keys the sum is at least 1 (the largest weight is 1), so with p the
+    softmax and A = sum p |v| + |o|
+      |got - o| <= 2^-11 |o| + 2^-11 A + n 2^-25 (max |v| + |o|) + 2^-25
+    (the last: a result in f16's subnormal range), to which the 32-bit sums
+    add n 2^-24 A and the scores (d + 8) 2^-24 S A, S = max_j scale sum |q k_j|
+    (the scale's and the logarithm's roundings among the 8), all to first
+    order: 2 % more, for exp2's last bit and the products of these.
+    """
+
+    def __init__(self, cached, added, heads, hk, d, dv, page, prefix=0, pad=0,
+                 spare=1, token_major=False, seed=0, q_scale=1.0):
+        g = torch.Generator().manual_seed(seed)
+        self.cached, self.added, self.prefix = cached, added, prefix
+        self.heads, self.hk, self.d, self.dv, self.page = heads, hk, d, dv, page
+        self.rows = sum(added) + pad
+        lengths = [c + a for c, a in zip(cached, added)]
+        lead = up(prefix, page)
+        held = [up(n, page) for n in lengths]
+        pages = lead + sum(held) + 2
+        order = torch.randperm(pages, generator=g).tolist()
+        self.prefix_pages = order[:lead]
+        width = max(held + [0]) + spare
+        self.table, at = [], lead
+        for n in held:
+            self.table.append(order[at:at + n] + [-1] * (width - n))
+            at += n
+        self.width, self.lengths = width, lengths
+        self.starts = [sum(added[:b]) for b in range(len(added) + 1)]
+        self.q = (torch.randn(self.rows, heads, d, generator=g)
+                  * q_scale).half().cuda()
+        self.kc, _ = new_cache(g, pages, hk, page, d, token_major)
+        self.vc, _ = new_cache(g, pages, hk, page, dv, token_major)
+        # tokens past the lengths, and the pages of no one, hold anything
+        taken = torch.zeros(pages, page, dtype=torch.bool)
+        for pp, n in [(self.prefix_pages, prefix)] + list(
+                zip(self.table, lengths)):
+            for j in range(n):
+                taken[pp[j // page], j % page] = True
+        rest = (~taken).cuda()
+        for c in (self.kc, self.vc):
+            c.transpose(1, 2)[rest] = NAN
+        self.scale = d ** -0.5
+
+    def call(self, pkg, o=None, **kw):
+        if o is None:
+            o = torch.full((self.rows, self.heads, self.dv), 9.0, dtype=H,
+                           device="cuda")
+        batch = len(self.added)
+        table = (ints(self.table) if batch and self.width else
+                 torch.empty(batch, self.width, dtype=I32, device="cuda"))
+        out = pkg.shared_prefix_attention(
+            self.q, self.kc, self.vc, ints(self.starts), ints(self.lengths),
+            table, ints(self.prefix_pages), self.prefix, o, **kw)
+        assert out is o
+        return o
+
+    def keys(self, b, g):
+        """(K, V) of request b's prefix and own tokens, in 64 bits; a page
+        that is not in the cache is zeros that `there` tells."""
+        ks, vs, there = [], [], []
+        for pages, n in ((self.prefix_pages, self.prefix),
+                         (self.table[b], self.lengths[b])):
+            n = max(0, min(n, len(pages) * self.page))
+            for j in range(n):
+                p = pages[j // self.page]
+                ok = 0 <= p < self.kc.shape[0]
+                there.append(ok)
+                ks.append(self.kcpu[p, g, j % self.page] if ok else
+                          torch.zeros(self.d, dtype=torch.float64))
+                vs.append(self.vcpu[p, g, j % self.page] if ok else
+                          torch.zeros(self.dv, dtype=torch.float64))
+        if not ks:
+            return (torch.zeros(0, self.d, dtype=torch.float64),
+                    torch.zeros(0, self.dv, dtype=torch.float64),
+                    torch.zeros(0, dtype=torch.bool))
+        return torch.stack(ks), torch.stack(vs), torch.tensor(there)
+
+    def expected(self):
+        """(o, bound), NaN where the rows are not written."""
+        self.kcpu, self.vcpu = self.kc.double().cpu(), self.vc.double().cpu()
+        q = self.q.double().cpu()
+        o = torch.full((self.rows, self.heads, self.dv), NAN,
+                       dtype=torch.float64)
+        bound = o.clone()
+        group = self.heads // self.hk
+        for b, a in enumerate(self.added):
+            first = self.starts[b]
+            if not a:
+                continue
+            for g in range(self.hk):
+                k, v, there = self.keys(b, g)
+                own = torch.arange(len(k)) - self.prefix
+                for i in range(a):
+                    sees = there & ((own < 0)
+                                    | (own <= self.lengths[b] - a + i))
+                    kk, vv = k[sees], v[sees]
+                    for h in range(g * group, (g + 1) * group):
+                        row = q[first + i, h]
+                        if not len(kk):
+                            o[first + i, h] = bound[first + i, h] = 0
+                            continue
+                        s = kk @ row * self.scale
+                        p = torch.softmax(s, 0)
+                        r = p @ vv
+                        big = (kk.abs() @ row.abs()).max() * abs(self.scale)
+                        spread = p @ vv.abs() + r.abs()
+                        n = len(kk)
+                        far = (2 ** -11 * (r.abs() + spread) + 2 ** -25
+                               + n * 2 ** -25 * (vv.abs().amax(0) + r.abs())
+                               + (n + (self.d + 8) * big) * 2 ** -24 * spread)
+                        o[first + i, h] = r
+                        bound[first + i, h] = 1.02 * far
+        return o, bound
+
+    def check(self, got):
+        want, bound = self.expected()
+        got = got.double().cpu()
+        written = ~want.isnan()
+        assert bool((got[~written] == 9).all()), "a row past the last"
+        off = (got - want).abs()[written] - bound[written]
+        assert bool((off <= 0).all()), float(off.max())
+        return want
+
+
+# tokens, drafts and prompts; few keys and many; sizes short of their bucket
+SHAPES = [
+    # cached, added, heads, kv heads, d, dv, page, prefix
+    ([5], [1], 1, 1, 8, 8, 16, 0),
+    ([0], [1], 4, 4, 64, 64, 16, 0),
+    ([0], [1], 8, 1, 128, 128, 16, 1),
+    ([3, 0, 40, 31], [1, 1, 1, 1], 9, 3, 64, 64, 16, 64),
+    ([100, 7, 0, 333], [1, 1, 1, 1], 8, 2, 128, 128, 7, 300),
+    ([0, 9, 60], [3, 0, 5], 6, 2, 80, 80, 24, 33),
+    ([10, 0, 200], [2, 17, 1], 4, 1, 192, 128, 8, 100),
+    ([63, 64, 65], [1, 2, 4], 2, 2, 256, 256, 64, 31),
+    ([0, 50], [40, 33], 6, 2, 96, 96, 16, 0),
+    ([20, 0, 5], [70, 130, 2], 8, 2, 64, 64, 32, 96),
+    ([12], [150], 3, 1, 128, 128, 16, 129),
+    ([0, 1], [64, 64], 2, 1, 40, 24, 5, 65),
+    ([1000], [1], 8, 1, 64, 64, 16, 2000),
+    ([700, 3, 0], [1, 1, 1], 4, 2, 128, 128, 1, 40),
+]
+
+
+@pytest.mark.parametrize("token_major", [False, True])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_attention(pkg, dev, shape, token_major):
+    cached, added, heads, hk, d, dv, page, prefix = shape
+    print(f"attention {shape} {token_major}", flush=True)
+    a = Attention(cached, added, heads, hk, d, dv, page, prefix, pad=3,
+                  token_major=token_major, seed=len(cached) + d)
+    a.check(a.call(pkg))
+
+
+@pytest.mark.parametrize("batch", [33, 64, 65, 200])
+def test_attention_batches(pkg, dev, batch):
+    """Requests are found among their tiles, 64 at a step."""
+    g = torch.Generator().manual_seed(batch)
+    cached = torch.randint(0, 70, (batch,), generator=g).tolist()
+    added = torch.randint(0, 4, (batch,), generator=g).tolist()
+    print(f"batch {batch}", flush=True)
+    for prefix in (0, 50):
+        a = Attention(cached, added, 2, 1, 64, 64, 16, prefix, seed=batch)
+        a.check(a.call(pkg))
+
+
+def test_attention_empty(pkg, dev):
+    """Requests without keys or rows, a batch of them, no rows at all."""
+    a = Attention([0, 0], [0, 0], 2, 1, 64, 64, 16, 40, pad=4)
+    a.check(a.call(pkg))
+    # fewer tokens than new rows: the first rows see only the prefix, or none
+    for prefix in (0, 40):
+        a = Attention([0, 0, 9], [3, 40, 2], 4, 2, 64, 64, 16, prefix)
+        a.lengths = [1, 7, 0]
+        want = a.check(a.call(pkg))
+        assert bool((want[:2] == 0).all()) == (prefix == 0)
+        # a length below 0 is none
+        a.lengths = [-4, 7, -2 ** 31]
+        o = a.call(pkg)
+        a.lengths = [0, 7, 0]
+        a.check(o)
+    # a table without columns, a cache without pages
+    a = Attention([0], [2], 2, 1, 64, 64, 16, 20, spare=0)
+    a.table, a.width = [[]], 0
+    a.check(a.call(pkg))
+    a.kc, a.vc = a.kc[:0], a.vc[:0]
+    assert bool((a.call(pkg) == 0).all())
+    a = Attention([], [], 2, 1, 64, 64, 16, 20, pad=2)
+    assert bool((a.call(pkg) == 9).all())
+
+
+@pytest.mark.parametrize("added", [[1, 1, 1], [60, 2, 33]])
+def test_attention_pages_outside_the_cache(pkg, dev, added):
+    """Tokens in pages that the cache does not have are not seen; lengths past
+    the table's row stop there."""
+    a = Attention([40, 100, 70], added, 4, 2, 64, 64, 16, 70, spare=0)
+    pages = a.kc.shape[0]
+    a.table[0][1], a.table[1][0] = -1, pages
+    a.table[2][2] = 2 ** 31 - 1
+    a.prefix_pages[1] = -2 ** 31
+    a.check(a.call(pkg))
+    a.prefix_pages = [pages + 5] * len(a.prefix_pages)
+    a.table = [[-1] * a.width] * 3
+    assert bool((a.call(pkg) == 0).all())
+    a = Attention([40, 100, 70], added, 4, 2, 64, 64, 16, 0, spare=0)
+    a.lengths = [n + 1000 for n in a.lengths]
+    full = a.width * 16
+    a.table[0] = a.table[1] = a.table[2] = max(a.table, key=lambda t: min(t))
+    a.vc.nan_to_num_(0.5)
+    a.kc.nan_to_num_(0.5)
+    o = a.call(pkg)
+    assert a.lengths[0] > full
+    a.check(o)
+
+
+def test_attention_infinities(pkg, dev):
+    """A NaN in a row's query, or in a key that it sees, makes it NaN and no
+    other request's; keys it does not see do nothing to it."""
+    a = Attention([40, 9, 300], [1, 2, 1], 4, 2, 64, 64, 16, 70)
+    want = a.call(pkg).clone()
+    a.q[1, 2, 5] = NAN
+    o = a.call(pkg)
+    bad = o.isnan().all(-1)
+    assert bool(bad[1, 2]) and int(o.isnan().any(-1).sum()) == 1
+    assert torch.equal(o[~bad], want[~bad])
+    a.q[1, 2, 5] = 0.5
+    want = a.call(pkg).clone()
+    # a key of request 2's own: its row alone
+    p, at = a.table[2][100 // 16], 100 % 16
+    a.kc[p, 1, at, 3] = NAN
+    o = a.call(pkg)
+    assert bool(o[3, 2:].isnan().all()) and not bool(o[3, :2].isnan().any())
+    assert torch.equal(o[:3], want[:3])
+    a.kc[p, 1, at, 3] = 0.5
+    # an infinite value of the prefix reaches every row's column
+    a.vc[a.prefix_pages[0], 0, 3, 7] = INF
+    o = a.call(pkg)
+    assert bool(o[:4, :2, 7].isinf().all())
+    assert torch.equal(o[:4, 2:], a.call(pkg)[:4, 2:])
+    assert bool(o[:4, 2:].isfinite().all())
+    a.vc[a.prefix_pages[0], 0, 3, 7] = 0
+    # scores far apart, at f16's largest values
+    a.q.fill_(1.0)
+    a.kc.nan_to_num_(0.0)
+    a.kc.mul_(0.0)
+    a.kc[a.prefix_pages[0], :, 0] = -65504.0
+    a.kc[a.table[1][0], :, 0] = 65504.0
+    a.vc.nan_to_num_(0.0)
+    o = a.call(pkg)
+    top = a.vc[a.table[1][0], :, 0].repeat_interleave(2, 0)
+    assert torch.equal(o[1], top) and torch.equal(o[2], top)
+    a.check(o)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.3, 2.0])
+def test_attention_scale(pkg, dev, scale):
+    a = Attention([40, 9], [1, 50], 4, 2, 64, 64, 16, 70)
+    a.scale = scale
+    a.check(a.call(pkg, scale=scale))
+
+
+def test_attention_strides(pkg, dev):
+    """q and o as parts of wider rows, heads out of order in memory."""
+    a = Attention([40, 9, 0], [1, 2, 20], 6, 2, 64, 64, 16, 70, pad=2)
+    wide = torch.full((a.rows, 3 * 64 * 6 + 8), 7.0, dtype=H, device="cuda")
+    q = wide[:, 64:64 + 64 * 6].unflatten(1, (6, 64))
+    q.copy_(a.q)
+    a.q = q
+    o = wide[:, 64 * 7 + 4:64 * 13 + 4].unflatten(1, (6, 64))
+    o.fill_(9.0)
+    a.check(a.call(pkg, o))
+    o.fill_(7.0)
+    q.fill_(7.0)
+    assert bool((wide == 7).all()), "write past o's rows"
+    # [head, row] order
+    buf = torch.full((6, a.rows, 64), 9.0, dtype=H, device="cuda")
+    a.q = torch.randn(6, a.rows, 64, device="cuda").half().transpose(0, 1)
+    a.check(a.call(pkg, buf.transpose(0, 1)))
+
+
+def test_attention_workspaces(pkg, dev):
+    """No workspace, short ones and all it can use give the same within the
+    roundings; nothing past its end or in its first 256 KiB is written."""
+    a = Attention([900, 40, 300], [1, 2, 1], 8, 2, 64, 64, 16, 1500)
+    args = pkg.PagedAttentionArgs(
+        q=a.q.data_ptr(), rows=a.rows, heads=8, batch=3, table_width=a.width,
+        table_stride=a.width, prefix_length=a.prefix, scale=a.scale)
+    keep = [ints(x) for x in (a.starts, a.lengths, a.table, a.prefix_pages)]
+    for n, t in zip(("row_starts", "lengths", "block_table", "prefix_pages"),
+                    keep):
+        setattr(args, n, t.data_ptr())
+    c = args.cache
+    c.k, c.v = a.kc.data_ptr(), a.vc.data_ptr()
+    c.pages, c.kv_heads, c.page_size, c.head_dim = a.kc.shape
+    c.head_dim_v = 64
+    c.k_strides[:], c.v_strides[:] = a.kc.stride()[:3], a.vc.stride()[:3]
+    args.q_strides[:] = args.o_strides[:] = a.q.stride()[:2]
+    lib, s = pkg.library(), torch.cuda.current_stream().cuda_stream
+    full = lib.iree_mi355x_shared_prefix_attention_workspace_bytes(
+        ctypes.byref(args))
+    head = 256 << 10
+    assert full > head
+    part = 2 * 4 * a.rows * 66 * 4
+    for size in (0, 100, head, head + part, head + 2 * part,
+                 head + 2 * part + 99, head + 5 * part, full, full + 4096):
+        ws = torch.full((size + 256,), 0xA5, dtype=torch.uint8,
+                        device="cuda")
+        o = torch.full((a.rows, 8, 64), 9.0, dtype=H, device="cuda")
+        args.o = o.data_ptr()
+        print(f"workspace {size} of {full}", flush=True)
+        assert lib.iree_mi355x_shared_prefix_attention_f16(
+            ctypes.byref(args), ws.data_ptr() if size else None, size,
+            s) == pkg.OK
+        a.check(o)
+        assert bool((ws[size:] == 0xA5).all()) and bool(
+            (ws[:min(size, head)] == 0xA5).all())
+
+
+def test_two_streams_and_capture(pkg, dev):
+    """Calls on two streams at once, and two graphs captured on one stream and
+    replayed together, with eager calls between."""
+    batches = [Attention([900, 40, 300 + s], [1, 2, 1], 8, 2, 64, 64, 16,
+                         1500 + s, seed=s) for s in range(2)]
+    want = [a.call(pkg).clone() for a in batches]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for _ in range(5):
+        for a, s, g in zip(batches, streams, got):
+            with torch.cuda.stream(s):
+                g.append(a.call(pkg))
+    torch.cuda.synchronize()
+    for g, w in zip(got, want):
+        assert all(torch.equal(o, w) for o in g)
+    graphs, outs = [], []
+    state = []
+    for a in batches:
+        t = [ints(x) for x in (a.starts, a.lengths, a.table, a.prefix_pages)]
+        o = torch.empty_like(want[0])
+        state.append(t)
+        outs.append(o)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=streams[0]):
+            pkg.shared_prefix_attention(a.q, a.kc, a.vc, *t, a.prefix, o)
+        graphs.append(graph)
+    for turn in range(4):
+        for o in outs:
+            o.fill_(3.0)
+        torch.cuda.synchronize()
+        for graph, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                graph.replay()
+        eager = batches[0].call(pkg)
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, w) for o, w in zip(outs, want)), turn
+        assert torch.equal(eager, want[0])
+    # the captured call reads the lengths of its replay
+    state[0][1].copy_(ints([500, 42, 301]))
+    graphs[0].replay()
+    batches[0].lengths = [500, 42, 301]
+    torch.cuda.synchronize()
+    batches[0].check(outs[0])
+
+
+# ------------------------------------------------------------- all together --
+
+def test_steps(pkg, dev):
+    """A batch behind a prefix over several steps: tables, rows appended, and
+    attention, against one contiguous cache for each request."""
+    g = torch.Generator().manual_seed(5)
+    heads, hk, d, page, prefix, batch = 6, 2, 64, 16, 37, 4
+    pages, width = 60, 8
+    kc, vc = (torch.full((pages, hk, page, d), NAN, dtype=H, device="cuda")
+              for _ in range(2))
+    free = torch.randperm(pages, generator=g).to(I32).cuda()
+    table = torch.full((batch + 1, width), -1, dtype=I32, device="cuda")
+    past = [[] for _ in range(batch + 1)]  # (k, v) rows, the prefix last
+    cached = torch.zeros(batch + 1, dtype=I32, device="cuda")
+    steps = [[0, 0, 0, 0, prefix], [20, 1, 0, 33, 0], [1, 1, 1, 1, 0],
+             [1, 0, 5, 1, 0], [1, 1, 1, 17, 0], [1, 1, 1, 1, 0]]
+    for added in steps:
+        rows = sum(added) + 2
+        k, v = (torch.randn(rows, hk, d, generator=g).half().cuda()
+                for _ in range(2))
+        q = torch.randn(rows, heads, d, generator=g).half().cuda()
+        starts, lengths, slots, needed = pkg.page_tables(
+            cached, ints(added), free, table, page, rows)
+        pkg.append_kv(k, v, kc, vc, slots)
+        at = 0
+        for b, n in enumerate(added):
+            past[b] += [(k[at + i], v[at + i]) for i in range(n)]
+            at += n
+        free, cached = free[int(needed):], lengths
+        if added[batch]:
+            continue
+        o = pkg.shared_prefix_attention(
+            q, kc, vc, starts[:batch + 1], lengths[:batch], table[:batch],
+            table[batch], prefix)
+        at = 0
+        for b, n in enumerate(added[:batch]):
+            if not n:
+                continue
+            seq = past[batch] + past[b]
+            keys = torch.stack([x for x, _ in seq], 1)[None]
+            vals = torch.stack([x for _, x in seq], 1)[None]
+            hidden = torch.zeros(n, len(seq), dtype=H, device="cuda")
+            for i in range(n):
+                hidden[i, len(seq) - n + i + 1:] = -INF
+            want = pkg.attention(
+                q[at:at + n].transpose(0, 1)[None], keys, vals, causal=False,
+                mask=hidden)[0].transpose(0, 1)
+            got = o[at:at + n]
+            # either is within 3 f16 roundings of values up to max |v| (see
+            # Attention), an eighth of one more for the 32-bit sums
+            assert (got.float() - want.float()).abs().max() \
+                <= 6.25 * 2 ** -11 * vals.abs().max().float()
+            at += n
