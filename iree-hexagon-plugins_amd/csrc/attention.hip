@@ -30,6 +30,7 @@
 //    masked, and the grid runs the heaviest query blocks first.
 #include <type_traits>
 
+#include "attention_common.h"
 #include "device_common.h"
 #include "kernels_internal.h"
 
@@ -47,54 +48,6 @@ typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 constexpr float kLazyMax = 8.0f;
 // K fragment reads in flight ahead of the S^T MFMA that takes them.
 constexpr int kKReadAhead = 3;
-
-template <int N, int I = 0, typename F>
-__device__ __forceinline__ void static_for(F &&f) {
-  if constexpr (I < N) {
-    f(std::integral_constant<int, I>());
-    static_for<N, I + 1>(f);
-  }
-}
-
-__device__ __forceinline__ void tie2(i32x2 &v) { asm volatile("" : "+v"(v)); }
-
-// Transposed 8-byte LDS read (ds_read_b64_tr_b16) with an immediate byte
-// offset: within each 16-lane block, lane i receives element i%4 of the
-// 8-byte loads of lanes 4r + i/4, r = 0..3. The caller waits with
-// lgkm_wait<N>() and ties the result before use.
-template <int OFF>
-__device__ __forceinline__ i32x2 lds_read_tr16_at(const IHP_LDS char *p) {
-  static_assert(OFF >= 0 && OFF < 65536, "ds offset range");
-  i32x2 v;
-  asm volatile("ds_read_b64_tr_b16 %0, %1 offset:%2"
-               : "=v"(v)
-               : "v"((unsigned)(uintptr_t)p), "i"(OFF));
-  return v;
-}
-
-// x[l % 32] op x[l % 32 + 32] in every lane l (the two lane halves hold
-// different keys of the same query row). v_permlane32_swap_b32 exchanges
-// lanes 32..63 of its first operand with lanes 0..31 of its second: with
-// both set to x, one then holds x[0..31] twice and the other x[32..63]
-// twice. Issued as asm with both operands tied: the compiler's builtin for
-// it maps both results to one register. s_nop 1 covers the VALU-write ->
-// permlane-read wait states the compiler inserts before it.
-__device__ __forceinline__ void half_swap(float x, float &lo, float &hi) {
-  lo = x;
-  hi = x;
-  asm volatile("s_nop 1\n\tv_permlane32_swap_b32 %0, %1"
-               : "+v"(lo), "+v"(hi));
-}
-__device__ __forceinline__ float pair_max(float x) {
-  float a, b;
-  half_swap(x, a, b);
-  return fmaxf(a, b);
-}
-__device__ __forceinline__ float pair_sum(float x) {
-  float a, b;
-  half_swap(x, a, b);
-  return a + b;
-}
 }  // namespace
 
 // K and V blocks are copied HBM -> LDS with global_load_lds into two-slot

@@ -7,18 +7,26 @@
 //   m = max_j s_j, l = sum_j 2^(s_j - m), a = sum_j 2^(s_j - m) v_j
 // of any set of keys (s = q . k * scale * log2 e), two sets join as
 //   m = max(m1, m2), l = l1 2^(m1 - m) + l2 2^(m2 - m), a alike, o = a / l,
-// so the prefix is computed for tiles of rows of the whole batch, each
-// request's own keys for tiles of its own rows, both by key splits, and a
-// second kernel joins the parts of each row. Where requests bring enough rows
-// to fill tiles, a tile walks the prefix and its own keys in turn and stores
-// the result itself.
+// so the prefix can be computed for tiles of rows of the whole batch, each
+// request's own keys for tiles of its own rows, and any tile's keys in pieces;
+// a second kernel joins the parts of each row. Where requests bring enough
+// rows to fill tiles, a tile walks the prefix and its own keys in turn.
 //
-// A workgroup takes a tile of 16 or 32 rows, its 4 waves blocks of 32 keys in
-// turn, each alone: K rows go from memory into MFMA fragments (S^T = K Q^T; a
-// lane holds 4 + 4 keys of one row), V rows through the wave's LDS tile, from
-// which transposed reads take the key order that S^T has, so P stays in
-// registers for O^T += V^T P. The next block's rows are in flight during the
-// current one, and the page numbers of the one after it.
+// The tiles of a KV head, one after the other with the keys of each, are a
+// line that a fixed number of workgroups share out evenly, whatever the
+// lengths are: every workgroup finds its stretch of the line by itself. A tile
+// that one workgroup has whole needs no joining.
+//
+// Tiles of up to 16 rows (a token or a few of a request): the 4 waves take
+// blocks of 32 keys in turn, each alone: K rows go from memory into MFMA
+// fragments (S^T = K Q^T; a lane holds 4 + 4 keys of one row), V rows through
+// the wave's LDS tile, from which transposed reads take the key order that S^T
+// has, so P stays in registers for O^T += V^T P. The next block's rows are in
+// flight during the current one, and the page numbers of the one after it.
+// Wide tiles (128 rows, 32 a wave): K and V of 64 keys are copied straight
+// into a two-slot LDS ring that all waves read, one barrier a block; two such
+// workgroups share a CU, so one's softmax runs beside the other's MFMAs.
+#include "attention_common.h"
 #include "device_common.h"
 #include "kernels_internal.h"
 
@@ -28,26 +36,21 @@ namespace {
 
 constexpr int kPagedThreads = 256;
 constexpr int kPagedWaves = kPagedThreads / 64;
-constexpr int kBlockKeys = 32;
+constexpr int kBlockKeys = 32;   // of a narrow tile's wave
+constexpr int kStepKeys = 64;    // of a wide tile's block; pieces of a line
+constexpr int kNarrowRows = 16;
+constexpr int kWideRows = 128;
 constexpr float kNegInf = -__builtin_inff();
 constexpr float kLog2e = 1.4426950408889634f;
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 
-// Chunk swizzle of a staged V row (key) of NCH 16-byte chunks: a transposed
-// read takes 4 rows of one 32-byte window per 16-lane block, two blocks (rows
-// 4 apart) at a time, and all of it must spread over the 64 banks.
-template <int NCH>
-__device__ __forceinline__ int v_swizzle(int k) {
-  return NCH >= 16 ? (4 * (k & 3)) ^ (2 * ((k >> 2) & 1))
-                   : (2 * ((k >> 1) & 1)) ^ (4 * ((k >> 2) & 1));
+// The same value in every lane, in scalar registers.
+__device__ __forceinline__ int uniform(int x) {
+  return __builtin_amdgcn_readfirstlane(x);
 }
-
-__device__ __forceinline__ float across_groups_max(float x) {
-  x = fmaxf(x, __shfl_xor(x, 16));
-  return fmaxf(x, __shfl_xor(x, 32));
-}
-__device__ __forceinline__ float across_groups_sum(float x) {
-  x += __shfl_xor(x, 16);
-  return x + __shfl_xor(x, 32);
+__device__ __forceinline__ int64_t uniform(int64_t x) {
+  return (int64_t)((uint64_t)(uint32_t)uniform((int)x) |
+                   (uint64_t)(uint32_t)uniform((int)(x >> 32)) << 32);
 }
 
 // row_starts[b], within the rows that there are whatever it holds.
@@ -56,48 +59,85 @@ __device__ __forceinline__ int row_start(const PagedAttention &p, int b) {
   return r < 0 ? 0 : r > p.rows ? p.rows : r;
 }
 
-// The request of tile `tile` where request b's tiles of RM rows start at
-// row_starts[b] * group / RM + b: at least as many numbers as it has tiles,
-// with no sum over the requests. 64 of them are looked at a step.
-template <int RM>
-__device__ __forceinline__ int request_of(const PagedAttention &p, int tile) {
-  const int lane = threadIdx.x & 63;
-  int lo = 0, n = p.batch;
-  while (n > 1) {
-    const int step = (n + 63) / 64;
-    const int b = lo + lane * step;
-    const bool at = lane * step < n &&
-                    (int64_t)row_start(p, b) * p.group / RM + b <= tile;
-    // lanes ascend: the last one that holds
-    const int last = 63 - __builtin_clzll(__ballot(at) | 1);
-    lo += last * step;
-    n = n - last * step < step ? n - last * step : step;
+// One tile's work: rows r0 .. r_end - 1 (of a KV head) against steps
+// s_begin .. s_end - 1 of 64 keys, the first `lead` of them the prefix's.
+struct PagedTile {
+  int kv_head, r0, r_end;
+  int lead;
+  const int32_t *table;  // the request's pages
+  int own_end;           // own keys that its pages hold
+  int seen;              // own keys that the tile's last row sees
+  int base, first;       // row r sees own keys .. base + r / group - first
+  int s_begin, s_end;
+  int64_t part;          // where row 0's part would be; -1: the result
+};
+
+// Own keys that row r sees.
+__device__ __forceinline__ int sees(const PagedAttention &p,
+                                    const PagedTile &t, int r) {
+  const int64_t n = (int64_t)t.base + r / p.group - t.first + 1;
+  return n < 0 ? 0 : n > t.own_end ? t.own_end : (int)n;
+}
+
+// Pages of the KEYS keys of a block: a lane's key, its table's page number
+// (find, a block ahead of the rows) and the places in the caches that `place`
+// makes of it, in 16 bytes. A page that the cache does not have hides its
+// keys.
+template <int KEYS>
+struct PagedBlock {
+  typedef typename std::conditional<KEYS == 64, uint64_t, uint32_t>::type Mask;
+  int found = 0, inside = 0;
+  uint32_t k = 0, v = 0;
+  Mask there = 0;  // bit i: key i of the block is there
+
+  // `lead`: the prefix's blocks of KEYS keys.
+  __device__ __forceinline__ void find(const PagedAttention &p,
+                                       const PagedTile &t, int lead, int c) {
+    const bool own = c >= lead;
+    const int end = own ? t.own_end : p.prefix;
+    const int32_t *table = own ? t.table : p.prefix_pages;
+    int key = (own ? c - lead : c) * KEYS + ((int)threadIdx.x & (KEYS - 1));
+    key = key < end ? key : end - 1;
+    const int column =
+        (int)(((uint64_t)(uint32_t)key * p.page_magic) >> p.page_shift);
+    inside = key - column * p.page_size;
+    found = table[column];
   }
-  return lo;
+  __device__ __forceinline__ void place(const PagedAttention &p,
+                                        const PagedTile &t, int lead, int c) {
+    const bool own = c >= lead;
+    const int left =
+        (own ? t.own_end - (c - lead) * KEYS : p.prefix - c * KEYS);
+    const bool has = (uint32_t)found < (uint32_t)p.pages;
+    const uint32_t page = has ? (uint32_t)found : 0u;
+    k = page * p.k_page16 + (uint32_t)inside * p.k_row16;
+    v = page * p.v_page16 + (uint32_t)inside * p.v_row16;
+    there = (Mask)__ballot(has);
+    if (left < KEYS)
+      there = left > 0 ? there & (((Mask)1 << left) - 1) : 0;
+  }
+};
+
+// Where a row's result or part goes.
+__device__ __forceinline__ f16 *result_row(const PagedAttention &p, int kv_head,
+                                           int row) {
+  return p.o + (int64_t)(row / p.group) * p.o_row +
+         (int64_t)(kv_head * p.group + row % p.group) * p.o_head;
+}
+__device__ __forceinline__ int64_t part_row(const PagedAttention &p,
+                                            const PagedTile &t, int row) {
+  return (int64_t)t.kv_head * p.part_rows + t.part + row;
 }
 
 }  // namespace
 
-// One tile's work: rows r0 .. r_end - 1 (of a KV head) against key blocks
-// c_begin .. c_end - 1, the first `lead` of them the prefix's.
-struct PagedTile {
-  int kv_head, r0, r_end;
-  int lead;            // prefix blocks
-  int prefix;          // prefix keys
-  const int32_t *table;  // the request's pages
-  int own_end;         // own keys that its pages hold
-  int base, first;     // row r sees own keys .. base + r / group - first
-  int c_begin, c_end;
-  int part;            // which part of the rows' keys this is
-};
-
-// DP: the head-dim bucket (64, 128 or 256, at least both head dims); RF:
-// 16-row fragments a tile.
-template <int DP, int RF>
-__device__ __forceinline__ void paged_tile(const PagedAttention &p,
-                                           const PagedTile &t, char *smem,
-                                           float (*wave_m)[32],
-                                           float (*wave_l)[32]) {
+// A tile of up to 16 rows. DP: the head-dim bucket (64, 128 or 256, at least
+// both head dims).
+template <int DP>
+__device__ __forceinline__ void narrow_tile(const PagedAttention &p,
+                                            const PagedTile &t, char *smem,
+                                            float (*wave_m)[kNarrowRows],
+                                            float (*wave_l)[kNarrowRows]) {
   constexpr int KS = DP / 32;           // head-dim steps of S
   constexpr int DB = DP / 16;           // 16-wide d blocks of O
   constexpr int NCH = DP / 8;           // 16-byte chunks of a V row
@@ -112,30 +152,22 @@ __device__ __forceinline__ void paged_tile(const PagedAttention &p,
   const char *Kp = (const char *)(p.k_cache + (int64_t)t.kv_head * p.k_head);
   const char *Vp = (const char *)(p.v_cache + (int64_t)t.kv_head * p.v_head);
 
-  // This lane's query rows (rows past the end repeat the last one) and the
-  // own keys that they see.
-  auto sees = [&](int r) {
-    const int64_t n = (int64_t)t.base + r / p.group - t.first + 1;
-    return n < 0 ? 0 : n > t.own_end ? t.own_end : (int)n;
-  };
-  i32x4 qf[RF][KS];
-  int limit[RF];
-#pragma unroll
-  for (int f = 0; f < RF; ++f) {
-    int r = t.r0 + f * 16 + l15;
-    r = r < t.r_end ? r : t.r_end - 1;
-    limit[f] = sees(r);
-    const f16 *qp = p.q + (int64_t)(r / p.group) * p.q_row +
-                    (int64_t)(t.kv_head * p.group + r % p.group) * p.q_head;
+  // This lane's query row (rows past the end repeat the last one), the own
+  // keys that it sees, and those that every row sees.
+  const int r_mine = t.r0 + l15 < t.r_end ? t.r0 + l15 : t.r_end - 1;
+  const int limit = sees(p, t, r_mine), all_own = sees(p, t, t.r0);
+  i32x4 qf[KS];
+  {
+    const f16 *qp = p.q + (int64_t)(r_mine / p.group) * p.q_row +
+                    (int64_t)(t.kv_head * p.group + r_mine % p.group) * p.q_head;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
       const int c = 32 * ks + 8 * lg;
-      qf[f][ks] = i32x4{0, 0, 0, 0};
+      qf[ks] = i32x4{0, 0, 0, 0};
       if (c < p.dqk)
-        qf[f][ks] = *(const i32x4 *)(qp + c);
+        qf[ks] = *(const i32x4 *)(qp + c);
     }
   }
-  const int all_own = sees(t.r0);  // own keys that every row sees
 
   // Chunks of a row past the head dim: K's are zeroed before use, V's reach
   // columns that are not stored; both are loaded from inside the row.
@@ -149,40 +181,17 @@ __device__ __forceinline__ void paged_tile(const PagedAttention &p,
   const int vrow = lane / NCH, vch = lane % NCH;
   const int voff = 2 * (8 * vch < p.dv ? 8 * vch : p.dv - 8);
 
-  // Block c's page number and place in it of key lane % 32: loaded (find)
-  // one block ahead of the rows, whose places (in 16 bytes) `place` makes of
-  // it. A page that the cache does not have hides its keys.
-  int found = 0, inside = 0;
-  auto find = [&](int c) __attribute__((always_inline)) {
-    const bool own = c >= t.lead;
-    const int end = own ? t.own_end : t.prefix;
-    const int32_t *table = own ? t.table : p.prefix_pages;
-    int key = (own ? c - t.lead : c) * kBlockKeys + (lane & 31);
-    key = key < end ? key : end - 1;
-    const int column =
-        (int)(((uint64_t)(uint32_t)key * p.page_magic) >> p.page_shift);
-    inside = key - column * p.page_size;
-    found = table[column];
-  };
-  uint32_t kat = 0, vat = 0, there = 0;
-  auto place = [&](int c) __attribute__((always_inline)) {
-    const bool own = c >= t.lead;
-    const int end = own ? t.own_end : t.prefix;
-    const int left = end - (own ? c - t.lead : c) * kBlockKeys;
-    const bool has = (uint32_t)found < (uint32_t)p.pages;
-    const uint32_t page = has ? (uint32_t)found : 0u;
-    kat = page * p.k_page16 + (uint32_t)inside * p.k_row16;
-    vat = page * p.v_page16 + (uint32_t)inside * p.v_row16;
-    there = (uint32_t)__ballot(has);
-    if (left < kBlockKeys)
-      there &= (1u << left) - 1;
-  };
-
+  const int lead = t.lead * (kStepKeys / kBlockKeys);
+  const int c_begin = t.s_begin * (kStepKeys / kBlockKeys);
+  int c_end = lead + (t.seen + kBlockKeys - 1) / kBlockKeys;
+  if (c_end > t.s_end * (kStepKeys / kBlockKeys))
+    c_end = t.s_end * (kStepKeys / kBlockKeys);
+  PagedBlock<kBlockKeys> block;
   i32x4 kf[2][KS], vf[VP];
   auto load_k = [&]() __attribute__((always_inline)) {
 #pragma unroll
     for (int f = 0; f < 2; ++f) {
-      const uint32_t at = (uint32_t)__shfl((int)kat, f * 16 + l15);
+      const uint32_t at = (uint32_t)__shfl((int)block.k, f * 16 + l15);
       const char *row = Kp + (uint64_t)at * 16;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks)
@@ -192,115 +201,93 @@ __device__ __forceinline__ void paged_tile(const PagedAttention &p,
   auto load_v = [&]() __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < VP; ++i) {
-      const uint32_t at = (uint32_t)__shfl((int)vat, i * VROWS + vrow);
+      const uint32_t at = (uint32_t)__shfl((int)block.v, i * VROWS + vrow);
       vf[i] = *(const i32x4 *)(Vp + (uint64_t)at * 16 + voff);
     }
   };
 
-  f32x4 o[RF][DB];
-  float m_ref[RF], l_sum[RF];
+  f32x4 o[DB];
 #pragma unroll
-  for (int f = 0; f < RF; ++f) {
-    m_ref[f] = kNegInf;
-    l_sum[f] = 0.0f;
-#pragma unroll
-    for (int d = 0; d < DB; ++d)
-      o[f][d] = f32x4{0, 0, 0, 0};
-  }
+  for (int d = 0; d < DB; ++d)
+    o[d] = f32x4{0, 0, 0, 0};
+  float m_ref = kNegInf, l_sum = 0.0f;
   char *vs = smem + wave * VBYTES;
   const float scale = p.scale * kLog2e;
   const f16x2 ones = {(f16)1.0f, (f16)1.0f};
 
-  int c = t.c_begin + wave;
-  if (c < t.c_end) {
-    find(c);
-    place(c);
+  // Every wave has finished with the LDS of the tile before.
+  __syncthreads();
+  int c = c_begin + wave;
+  if (c < c_end) {
+    block.find(p, t, lead, c);
+    block.place(p, t, lead, c);
     load_k();
     load_v();
-    if (c + kPagedWaves < t.c_end)
-      find(c + kPagedWaves);
+    if (c + kPagedWaves < c_end)
+      block.find(p, t, lead, c + kPagedWaves);
   }
-  for (; c < t.c_end; c += kPagedWaves) {
-    const bool more = c + kPagedWaves < t.c_end;
-    const bool own = c >= t.lead;
-    const int key0 = (own ? c - t.lead : c) * kBlockKeys;
-    const uint32_t live = there;
+  for (; c < c_end; c += kPagedWaves) {
+    const bool more = c + kPagedWaves < c_end;
+    const bool own = c >= lead;
+    const int key0 = (own ? c - lead : c) * kBlockKeys;
+    const uint32_t live = block.there;
     if (pad_k) {
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks)
         if (32 * ks + 8 * lg >= p.dqk)
           kf[0][ks] = kf[1][ks] = i32x4{0, 0, 0, 0};
     }
-    f32x4 s[RF][2];
+    f32x4 s[2];
 #pragma unroll
-    for (int r = 0; r < RF; ++r)
+    for (int f = 0; f < 2; ++f) {
+      s[f] = f32x4{0, 0, 0, 0};
 #pragma unroll
-      for (int f = 0; f < 2; ++f) {
-        s[r][f] = f32x4{0, 0, 0, 0};
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
-          s[r][f] = Mfma16<f16>::mma(kf[f][ks], qf[r][ks], s[r][f]);
-        s[r][f] *= scale;
-      }
+      for (int ks = 0; ks < KS; ++ks)
+        s[f] = Mfma16<f16>::mma(kf[f][ks], qf[ks], s[f]);
+      s[f] *= scale;
+    }
     if (live != 0xffffffffu || (own && key0 + kBlockKeys > all_own)) {
+      const int end = (own ? limit : p.prefix) - key0;
 #pragma unroll
-      for (int r = 0; r < RF; ++r) {
-        const int end = own ? limit[r] : t.prefix;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int key = 16 * (e >> 2) + 4 * lg + (e & 3);
-          if (key0 + key >= end || !(live >> key & 1))
-            s[r][e >> 2][e & 3] = kNegInf;
-        }
+      for (int e = 0; e < 8; ++e) {
+        const int key = 16 * (e >> 2) + 4 * lg + (e & 3);
+        if (key >= end || !(live >> key & 1))
+          s[e >> 2][e & 3] = kNegInf;
       }
     }
     if (more) {
-      place(c + kPagedWaves);
+      block.place(p, t, lead, c + kPagedWaves);
       load_k();
-      if (c + 2 * kPagedWaves < t.c_end)
-        find(c + 2 * kPagedWaves);
+      if (c + 2 * kPagedWaves < c_end)
+        block.find(p, t, lead, c + 2 * kPagedWaves);
     }
 
-    float top[RF];
-    bool move = false;
+    float top = s[0][0];
 #pragma unroll
-    for (int r = 0; r < RF; ++r) {
-      float x = s[r][0][0];
+    for (int e = 1; e < 8; ++e)
+      top = fmaxf(top, s[e >> 2][e & 3]);
+    if (__any(top > m_ref)) {
+      const float x = fmaxf(m_ref, across_groups_max(top));
+      const float keep =
+          x == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(m_ref - x);
+      m_ref = x;
+      l_sum *= keep;
 #pragma unroll
-      for (int e = 1; e < 8; ++e)
-        x = fmaxf(x, s[r][e >> 2][e & 3]);
-      top[r] = x;
-      move |= x > m_ref[r];
-    }
-    if (__any(move)) {
-#pragma unroll
-      for (int r = 0; r < RF; ++r) {
-        const float x = fmaxf(m_ref[r], across_groups_max(top[r]));
-        const float keep =
-            x == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(m_ref[r] - x);
-        m_ref[r] = x;
-        l_sum[r] *= keep;
-#pragma unroll
-        for (int d = 0; d < DB; ++d)
-          o[r][d] *= keep;
-      }
+      for (int d = 0; d < DB; ++d)
+        o[d] *= keep;
     }
     // The weights are rounded to f16 for the matrix instruction, by at most
-    // 2^-11 of each and, the largest being 1, 2^-25 of the sum's least; the
-    // sum is of the rounded ones.
-    i32x4 pf[RF];
+    // 2^-11 of each or, the largest being 1, 2^-25; the sum is of the rounded
+    // ones.
+    const float ref = m_ref == kNegInf ? 0.0f : m_ref;
+    i32x4 pf;
 #pragma unroll
-    for (int r = 0; r < RF; ++r) {
-      const float ref = m_ref[r] == kNegInf ? 0.0f : m_ref[r];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float x0 = s[r][e >> 1][2 * (e & 1)];
-        const float x1 = s[r][e >> 1][2 * (e & 1) + 1];
-        const f16x2 p2 = {(f16)__builtin_amdgcn_exp2f(x0 - ref),
-                          (f16)__builtin_amdgcn_exp2f(x1 - ref)};
-        l_sum[r] = __builtin_amdgcn_fdot2(p2, ones, l_sum[r], false);
-        pf[r][e] = __builtin_bit_cast(int, p2);
-      }
+    for (int e = 0; e < 4; ++e) {
+      const float x0 = s[e >> 1][2 * (e & 1)], x1 = s[e >> 1][2 * (e & 1) + 1];
+      const f16x2 p2 = {(f16)__builtin_amdgcn_exp2f(x0 - ref),
+                        (f16)__builtin_amdgcn_exp2f(x1 - ref)};
+      l_sum = __builtin_amdgcn_fdot2(p2, ones, l_sum, false);
+      pf[e] = __builtin_bit_cast(int, p2);
     }
 
     // V through this wave's LDS tile; keys that are not there are zeros.
@@ -309,7 +296,8 @@ __device__ __forceinline__ void paged_tile(const PagedAttention &p,
       const int k = i * VROWS + vrow;
       if (!(live >> k & 1))
         vf[i] = i32x4{0, 0, 0, 0};
-      *(i32x4 *)(vs + k * (DP * 2) + ((vch ^ v_swizzle<NCH>(k)) << 4)) = vf[i];
+      *(i32x4 *)(vs + k * (DP * 2) + ((vch ^ row_v_swizzle<NCH>(k)) << 4)) =
+          vf[i];
     }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
@@ -322,16 +310,13 @@ __device__ __forceinline__ void paged_tile(const PagedAttention &p,
       const int byte = 2 * (16 * d + 4 * (l15 & 3));
       const IHP_LDS char *at =
           (const IHP_LDS char *)vs + k * (DP * 2) +
-          (((byte >> 4) ^ v_swizzle<NCH>(k)) << 4) + (byte & 15);
+          (((byte >> 4) ^ row_v_swizzle<NCH>(k)) << 4) + (byte & 15);
       const i32x2 lo = __builtin_bit_cast(
           i32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((IHP_LDS s16x4 *)at));
       const i32x2 hi = __builtin_bit_cast(
           i32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                      (IHP_LDS s16x4 *)(at + 16 * (DP * 2))));
-      const i32x4 v = {lo[0], lo[1], hi[0], hi[1]};
-#pragma unroll
-      for (int r = 0; r < RF; ++r)
-        o[r][d] = Mfma16<f16>::mma(v, pf[r], o[r][d]);
+      o[d] = Mfma16<f16>::mma(i32x4{lo[0], lo[1], hi[0], hi[1]}, pf, o[d]);
     }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
@@ -339,151 +324,567 @@ __device__ __forceinline__ void paged_tile(const PagedAttention &p,
 
   // Merge the waves: a common max per row, O scaled to it. A row whose
   // scores are all NaN has m -inf and l NaN, which the sums keep.
-#pragma unroll
-  for (int r = 0; r < RF; ++r) {
-    const float l = across_groups_sum(l_sum[r]);
-    if (lg == 0) {
-      wave_m[wave][r * 16 + l15] = m_ref[r];
-      wave_l[wave][r * 16 + l15] = l;
-    }
+  const float l_row = across_groups_sum(l_sum);
+  if (lg == 0) {
+    wave_m[wave][l15] = m_ref;
+    wave_l[wave][l15] = l_row;
   }
   __syncthreads();
-  // Thread (q, dq) of the merge: row q of a fragment, DP / 16 columns from dq.
+  float *om = (float *)smem;
+  {
+    float top = kNegInf;
+#pragma unroll
+    for (int w = 0; w < kPagedWaves; ++w)
+      top = fmaxf(top, wave_m[w][l15]);
+    const float f =
+        m_ref == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(m_ref - top);
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+      *(f32x4 *)(om + (wave * 16 + l15) * OPITCH + 16 * d + 4 * lg) = o[d] * f;
+  }
+  __syncthreads();
+  // Thread (q, dq): row q, DP / 16 columns from dq.
   constexpr int CPT = DP / 16;
   const int q = tid >> 4, dq = (tid & 15) * CPT;
+  const int row = t.r0 + q;
+  if (row >= t.r_end)
+    return;
+  float top = kNegInf, sum = 0.0f;
 #pragma unroll
-  for (int r = 0; r < RF; ++r) {
-    float *om = (float *)smem;
-    {
-      float top = kNegInf;
+  for (int w = 0; w < kPagedWaves; ++w)
+    top = fmaxf(top, wave_m[w][q]);
 #pragma unroll
-      for (int w = 0; w < kPagedWaves; ++w)
-        top = fmaxf(top, wave_m[w][r * 16 + l15]);
-      const float f =
-          m_ref[r] == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(m_ref[r] - top);
+  for (int w = 0; w < kPagedWaves; ++w)
+    sum += wave_l[w][q] * (wave_m[w][q] == kNegInf
+                               ? 0.0f
+                               : __builtin_amdgcn_exp2f(wave_m[w][q] - top));
+  f32x4 acc[CPT / 4];
 #pragma unroll
-      for (int d = 0; d < DB; ++d)
-        *(f32x4 *)(om + (wave * 16 + l15) * OPITCH + 16 * d + 4 * lg) =
-            o[r][d] * f;
-    }
-    __syncthreads();
-    float top = kNegInf, sum = 0.0f;
-#pragma unroll
-    for (int w = 0; w < kPagedWaves; ++w)
-      top = fmaxf(top, wave_m[w][r * 16 + q]);
+  for (int e = 0; e < CPT / 4; ++e) {
+    acc[e] = f32x4{0, 0, 0, 0};
 #pragma unroll
     for (int w = 0; w < kPagedWaves; ++w)
-      sum += wave_l[w][r * 16 + q] *
-             (wave_m[w][r * 16 + q] == kNegInf
-                  ? 0.0f
-                  : __builtin_amdgcn_exp2f(wave_m[w][r * 16 + q] - top));
-    float acc[CPT];
+      acc[e] += *(const f32x4 *)(om + (w * 16 + q) * OPITCH + dq + 4 * e);
+  }
+  if (t.part < 0) {
+    const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+    f16 *dst = result_row(p, t.kv_head, row) + dq;
 #pragma unroll
-    for (int e = 0; e < CPT; ++e) {
-      acc[e] = 0.0f;
+    for (int e = 0; e < CPT / 4; ++e)
+      if (dq + 4 * e < p.dv)  // dv is a multiple of 8
+        *(f16x4 *)(dst + 4 * e) =
+            f16x4{(f16)(acc[e][0] * inv), (f16)(acc[e][1] * inv),
+                  (f16)(acc[e][2] * inv), (f16)(acc[e][3] * inv)};
+  } else {
+    const int64_t at = part_row(p, t, row);
 #pragma unroll
-      for (int w = 0; w < kPagedWaves; ++w)
-        acc[e] += om[(w * 16 + q) * OPITCH + dq + e];
-    }
-    __syncthreads();  // before the next fragment's rows
-    const int row = t.r0 + r * 16 + q;
-    if (row >= t.r_end)
-      continue;
-    if (!p.partials) {
-      const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
-      f16 *dst = p.o + (int64_t)(row / p.group) * p.o_row +
-                 (int64_t)(t.kv_head * p.group + row % p.group) * p.o_head + dq;
-#pragma unroll
-      for (int e = 0; e < CPT; e += 4)
-        if (dq + e < p.dv)  // dv is a multiple of 8
-          *(f16x4 *)(dst + e) =
-              f16x4{(f16)(acc[e] * inv), (f16)(acc[e + 1] * inv),
-                    (f16)(acc[e + 2] * inv), (f16)(acc[e + 3] * inv)};
-    } else {
-      const int64_t at =
-          ((int64_t)t.part * p.kv_heads + t.kv_head) * p.packed + row;
-      float *dst = p.partials + at * DP + dq;
-#pragma unroll
-      for (int e = 0; e < CPT; e += 4)
-        *(f32x4 *)(dst + e) = f32x4{acc[e], acc[e + 1], acc[e + 2], acc[e + 3]};
-      if (dq == 0) {
-        p.part_ml[2 * at] = top;
-        p.part_ml[2 * at + 1] = sum;
-      }
-    }
+    for (int e = 0; e < CPT / 4; ++e)
+      *(f32x4 *)(p.partials + at * DP + dq + 4 * e) = acc[e];
+    if (dq == 0)
+      *(f32x2 *)(p.part_ml + 2 * at) = f32x2{top, sum};
   }
 }
 
-// Grid: the prefix's items (tile, KV head, split), then the requests' own.
-template <int DP, int RP, int RO>
+// A tile of up to 128 rows, 32 a wave: K and V of 64 keys in a two-slot LDS
+// ring, rows of 16-byte chunks swizzled on the copy side (as attention.hip's):
+// K is read 16 lanes = 16 keys at one chunk, V transposed, 32 lanes = 4 keys
+// x 32 columns.
+template <int DP>
+__device__ __forceinline__ int wide_k_swizzle(int key) {
+  return DP == 128 ? (key & 15) : ((key >> 1) & 7);
+}
+template <int DP>
+__device__ __forceinline__ int wide_v_swizzle(int key) {
+  return DP == 128 ? 4 * (key & 3) : 4 * ((key >> 1) & 1);
+}
+
+template <int DP>
+__device__ __forceinline__ void wide_tile(const PagedAttention &p,
+                                          const PagedTile &t, char *smem) {
+  constexpr int DS = DP / 16;         // 16-wide d steps of S^T = K Q^T
+  constexpr int DT = DP / 32;         // 32-row d tiles of O^T
+  constexpr int ROW = DP * 2;         // bytes of a staged row
+  constexpr int CH = ROW / 16;        // its 16-byte chunks
+  constexpr int BLK = kStepKeys * ROW;
+  constexpr int ROWS = 64 / CH;       // rows a copy instruction moves
+  constexpr int PASSES = kStepKeys / (kPagedWaves * ROWS);
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int g = lane >> 5, l32 = lane & 31;
+  const char *Kp = (const char *)(p.k_cache + (int64_t)t.kv_head * p.k_head);
+  const char *Vp = (const char *)(p.v_cache + (int64_t)t.kv_head * p.v_head);
+
+  // This lane's query row (rows past the end repeat the last one) and the own
+  // keys that it sees; those that every row of the wave sees.
+  const int r_wave = t.r0 + 32 * wave;
+  const int r_mine = r_wave + l32 < t.r_end ? r_wave + l32 : t.r_end - 1;
+  const bool idle = r_wave >= t.r_end;  // no rows: the wave only copies
+  const int limit = sees(p, t, r_mine);
+  const int all_own = sees(p, t, r_wave < t.r_end ? r_wave : t.r_end - 1);
+  i32x4 qf[DS];
+  {
+    const f16 *qp = p.q + (int64_t)(r_mine / p.group) * p.q_row +
+                    (int64_t)(t.kv_head * p.group + r_mine % p.group) * p.q_head;
+#pragma unroll
+    for (int s = 0; s < DS; ++s) {
+      const int c = 16 * s + 8 * g;
+      qf[s] = i32x4{0, 0, 0, 0};
+      if (c < p.dqk)
+        qf[s] = *(const i32x4 *)(qp + c);
+    }
+  }
+
+  // Copy side: a lane's (row, chunk) of an instruction, the logical chunk
+  // that belongs there, and whether it lies within the head dim (the LDS past
+  // it is zeroed once and never written).
+  const int c_row = lane / CH, c_phys = lane % CH;
+  IHP_LDS char *lds = (IHP_LDS char *)smem;
+  PagedBlock<kStepKeys> block;
+  auto copy = [&](int slot) {
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i) {
+      const int row0 = (i * kPagedWaves + wave) * ROWS;
+      const int row = row0 + c_row;
+      const int chunk = c_phys ^ wide_k_swizzle<DP>(row);
+      const uint32_t at = (uint32_t)__shfl((int)block.k, row);
+      if (8 * chunk < p.dqk)
+        global_to_lds_16(Kp + ((uint64_t)at + (uint32_t)chunk) * 16,
+                         lds + slot * BLK + row0 * ROW);
+    }
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i) {
+      const int row0 = (i * kPagedWaves + wave) * ROWS;
+      const int row = row0 + c_row;
+      const int chunk = c_phys ^ wide_v_swizzle<DP>(row);
+      const uint32_t at = (uint32_t)__shfl((int)block.v, row);
+      if (8 * chunk < p.dv)
+        global_to_lds_16(Vp + ((uint64_t)at + (uint32_t)chunk) * 16,
+                         lds + (2 + slot) * BLK + row0 * ROW);
+    }
+  };
+
+  // K read base of this lane in slot 0; a d step's address is it XOR 32 s (the
+  // ring is aligned, and the swizzle flips chunk bits only). V^T reads: load
+  // lane j = lane % 16 of block b = lane / 16 reads row kstart + j / 4,
+  // columns 32 dt + 16 (b % 2) + 4 (j % 4) .. + 3.
+  const int k_sw = wide_k_swizzle<DP>(l32);
+  const uint32_t ka =
+      (uint32_t)(uintptr_t)lds +
+      (uint32_t)(l32 * ROW + 16 * (g ^ (k_sw & 1)) + 32 * (k_sw >> 1));
+  const int vj = lane & 15, vb = lane >> 4;
+  int v_off[DT];
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt) {
+    const int b0 = 64 * dt + 2 * (16 * (vb & 1) + 4 * (vj & 3));
+    v_off[dt] = (4 * g + (vj >> 2)) * ROW +
+                (((b0 >> 4) ^ wide_v_swizzle<DP>(vj >> 2)) << 4) + (b0 & 15);
+  }
+
+  f32x16 o[DT], st[2];
+#pragma unroll
+  for (int dt = 0; dt < DT; ++dt)
+    o[dt] = f32x16{};
+  float m_run = kNegInf, l_run = 0.0f;  // l_run: this lane half's keys
+  const float scale = p.scale * kLog2e;
+
+  const int lead = t.lead;
+  int c_end = lead + (t.seen + kStepKeys - 1) / kStepKeys;
+  if (c_end > t.s_end)
+    c_end = t.s_end;
+  int c = t.s_begin;
+  // Every wave has finished with the LDS of the tile before.
+  wait_lgkmcnt0();
+  block_barrier();
+  if (p.dqk != DP || p.dv != DP) {
+    for (int i = tid * 16; i < 4 * BLK; i += kPagedThreads * 16)
+      *(IHP_LDS i32x4 *)(lds + i) = i32x4{0, 0, 0, 0};
+    wait_lgkmcnt0();
+    block_barrier();
+  }
+  if (c < c_end) {
+    block.find(p, t, lead, c);
+    block.place(p, t, lead, c);
+    copy(0);
+    if (c + 1 < c_end)
+      block.find(p, t, lead, c + 1);
+  }
+  for (int slot = 0; c < c_end; ++c, slot ^= 1) {
+    const bool own = c >= lead;
+    const int key0 = (own ? c - lead : c) * kStepKeys;
+    const uint64_t live = block.there;
+    // This block's rows have landed, and every wave is done with the one
+    // before, whose slot the next one takes.
+    wait_vmcnt<0>();
+    block_barrier();
+    if (live != ~0ull) {  // keys that are not there: their V rows are zeros
+      for (int i = tid; i < kStepKeys * CH; i += kPagedThreads)
+        if (!(live >> (i / CH) & 1))
+          *(IHP_LDS i32x4 *)(lds + (2 + slot) * BLK + i * 16) =
+              i32x4{0, 0, 0, 0};
+      wait_lgkmcnt0();
+      block_barrier();
+    }
+    if (c + 1 < c_end) {
+      block.place(p, t, lead, c + 1);
+      copy(slot ^ 1);
+      if (c + 2 < c_end)
+        block.find(p, t, lead, c + 2);
+    }
+
+    if (idle)
+      continue;
+
+    // S^T: reads run three MFMAs ahead in four rotating registers.
+    {
+      const uint32_t kbase = ka + (uint32_t)(slot * BLK);
+      constexpr int NR = 2 * DS, KW = 3, NB = KW + 1;
+      i32x4 kb[NB];
+      auto issue = [&](auto r_c) {
+        constexpr int R = decltype(r_c)::value;
+        kb[R % NB] = lds_read_16_async<32 * (R % 2) * ROW>(
+            (const IHP_LDS char *)(uintptr_t)(kbase ^ (32u * (R / 2))));
+      };
+      static_for<KW>(issue);
+      static_for<NR>([&](auto r_c) {
+        constexpr int R = decltype(r_c)::value;
+        constexpr int S = R / 2, T = R % 2;
+        constexpr int AHEAD = (R + KW < NR ? R + KW : NR) - R - 1;
+        lgkm_wait<AHEAD>();
+        lgkm_tie(kb[R % NB]);
+        st[T] = Mfma32<f16>::mma(kb[R % NB], qf[S], S == 0 ? f32x16{} : st[T]);
+        if constexpr (R + KW < NR)
+          issue(std::integral_constant<int, R + KW>());
+      });
+    }
+
+    // Softmax. Element (t, r) of S^T is key 32 t + 8 (r / 4) + 4 g + r % 4.
+    float sc = scale;
+    if (live != ~0ull || (own && key0 + kStepKeys > all_own) || scale <= 0.0f) {
+      const int end = (own ? limit : p.prefix) - key0 - 4 * g;
+      const uint64_t mine = live >> (4 * g);
+#pragma unroll
+      for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int key = 32 * tt + 8 * (r >> 2) + (r & 3);
+          st[tt][r] = key < end && (mine >> key & 1) ? st[tt][r] * scale
+                                                     : kNegInf;
+        }
+      sc = 1.0f;
+    }
+    float top[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      top[i] = kNegInf;
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        top[i] = fmaxf(top[i], st[i >> 1][8 * (i & 1) + e]);
+    }
+    const float mx =
+        pair_max(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * sc);
+    if (!__all(mx <= m_run)) {
+      const float m_new = fmaxf(m_run, mx);
+      const float keep =
+          m_new == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(m_run - m_new);
+      m_run = m_new;
+      l_run *= keep;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+        o[dt] *= keep;
+    }
+    const float m_use = m_run == kNegInf ? 0.0f : m_run;
+    // Weights rounded to f16 as in a narrow tile.
+    i32x4 pw[4];
+#pragma unroll
+    for (int f = 0; f < 4; ++f)
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float p0 = __builtin_amdgcn_exp2f(
+            __builtin_fmaf(st[f >> 1][8 * (f & 1) + 2 * w], sc, -m_use));
+        const float p1 = __builtin_amdgcn_exp2f(
+            __builtin_fmaf(st[f >> 1][8 * (f & 1) + 2 * w + 1], sc, -m_use));
+        const f16x2 h = __builtin_convertvector(f32x2{p0, p1}, f16x2);
+        pw[f][w] = __builtin_bit_cast(int, h);
+      }
+
+    // O^T += V^T P^T, 16 keys an MFMA; the V^T fragments of the next key step
+    // are read before the MFMAs of this one.
+    {
+      float psum[4];
+      const IHP_LDS char *vs = lds + (2 + slot) * BLK;
+      i32x2 vr[2][DT][2];
+      auto read_v = [&](auto step_c) {
+        constexpr int ST = decltype(step_c)::value;
+        constexpr int KOFF = 16 * ST * ROW;
+        static_for<DT>([&](auto dt) {
+          constexpr int DTI = decltype(dt)::value;
+          vr[ST % 2][DTI][0] = lds_read_tr16_at<KOFF>(vs + v_off[DTI]);
+          vr[ST % 2][DTI][1] = lds_read_tr16_at<KOFF + 8 * ROW>(vs + v_off[DTI]);
+        });
+      };
+      read_v(std::integral_constant<int, 0>());
+      static_for<4>([&](auto step_c) {
+        constexpr int ST = decltype(step_c)::value;
+        if constexpr (ST < 3)
+          read_v(std::integral_constant<int, ST + 1>());
+        lgkm_wait<ST < 3 ? 2 * DT : 0>();
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+          tie2(vr[ST % 2][dt][0]);
+          tie2(vr[ST % 2][dt][1]);
+          const i32x4 vf = i32x4{vr[ST % 2][dt][0][0], vr[ST % 2][dt][0][1],
+                                 vr[ST % 2][dt][1][0], vr[ST % 2][dt][1][1]};
+          o[dt] = Mfma32<f16>::mma(vf, pw[ST], o[dt]);
+        }
+        psum[ST] = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const int word = pw[ST][w];
+          psum[ST] = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, word),
+                                            f16x2{1, 1}, psum[ST], false);
+        }
+      });
+      l_run += (psum[0] + psum[1]) + (psum[2] + psum[3]);
+    }
+  }
+
+  // Register quarter (dt, q) of O^T holds columns 32 dt + 8 q + 4 g .. + 3 of
+  // the lane's row.
+  const float sum = pair_sum(l_run);
+  const int row = r_wave + l32;
+  if (row >= t.r_end)
+    return;
+  if (t.part < 0) {
+    const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+    f16 *dst = result_row(p, t.kv_head, row) + 4 * g;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (32 * dt + 8 * q < p.dv)  // dv is a multiple of 8
+          *(f16x4 *)(dst + 32 * dt + 8 * q) =
+              f16x4{(f16)(o[dt][4 * q] * inv), (f16)(o[dt][4 * q + 1] * inv),
+                    (f16)(o[dt][4 * q + 2] * inv),
+                    (f16)(o[dt][4 * q + 3] * inv)};
+  } else {
+    const int64_t at = part_row(p, t, row);
+    float *dst = p.partials + at * DP + 4 * g;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        *(f32x4 *)(dst + 32 * dt + 8 * q) =
+            f32x4{o[dt][4 * q], o[dt][4 * q + 1], o[dt][4 * q + 2],
+                  o[dt][4 * q + 3]};
+    if (g == 0)
+      *(f32x2 *)(p.part_ml + 2 * at) = f32x2{m_run, sum};
+  }
+}
+
+// ----------------------------------------------------------------------------
+// The line of a KV head's tiles.
+// ----------------------------------------------------------------------------
+
+namespace {
+
+// Rows of a tile where `rows` of them belong together.
+template <int DP>
+__device__ __forceinline__ int tile_rows(int64_t rows) {
+  return DP >= 256 || rows <= kNarrowRows ? kNarrowRows : kWideRows;
+}
+
+// Request b's tiles on the line: tile i takes a + i * step keys, near what it
+// walks, so that their sums have a closed form.
+struct Request {
+  int begin, end, tile, tiles;  // rows' tokens, rows a tile
+  int own_end, base;
+  int64_t a, step;
+  __device__ __forceinline__ int64_t before(int64_t i) const {
+    return i * a + step * (i * (i - 1) / 2);
+  }
+};
+// UNIFORM: b is the same in every lane.
+template <int DP, bool UNIFORM = true>
+__device__ __forceinline__ Request request(const PagedAttention &p, int b,
+                                           int64_t lead_keys) {
+  Request q;
+  q.begin = row_start(p, b);
+  q.end = row_start(p, b + 1);
+  int length = p.lengths[b];
+  if (UNIFORM) {
+    q.begin = uniform(q.begin);
+    q.end = uniform(q.end);
+    length = uniform(length);
+  }
+  const int added = q.end > q.begin ? q.end - q.begin : 0;
+  q.end = q.begin + added;
+  const int64_t rows = (int64_t)added * p.group;
+  q.tile = tile_rows<DP>(rows);
+  q.tiles = (int)((rows + q.tile - 1) / q.tile);
+  length = length > 0 ? length : 0;
+  q.own_end = length < p.capacity ? length : p.capacity;
+  q.base = length - added;
+  const int tokens = q.tile / p.group > 1 ? q.tile / p.group : 1;
+  if (q.base >= 0 && length <= p.capacity) {
+    q.a = lead_keys + q.base + (added < tokens ? added : tokens);
+    q.step = q.tiles > 1 ? tokens : 0;
+  } else {
+    q.a = lead_keys + q.own_end + 1;
+    q.step = 0;
+  }
+  return q;
+}
+
+}  // namespace
+
+template <int DP>
 __global__ __launch_bounds__(kPagedThreads, DP >= 256 ? 1 : 2) void
 attention_paged_kernel(PagedAttention p) {
   constexpr int VBYTES = kBlockKeys * DP * 2;
   constexpr int MERGE = kPagedWaves * 16 * (DP + 4) * 4;
-  constexpr int SMEM = kPagedWaves * VBYTES > MERGE ? kPagedWaves * VBYTES : MERGE;
+  constexpr int WIDE = DP >= 256 ? 0 : 4 * kStepKeys * DP * 2;
+  constexpr int NARROW =
+      kPagedWaves * VBYTES > MERGE ? kPagedWaves * VBYTES : MERGE;
+  constexpr int SMEM = NARROW > WIDE ? NARROW : WIDE;
   __shared__ __attribute__((aligned(1024))) char smem[SMEM];
-  __shared__ float wave_m[kPagedWaves][32], wave_l[kPagedWaves][32];
-  const int prefix_items = p.prefix_tiles * p.kv_heads * p.prefix_splits;
-  PagedTile t;
-  t.prefix = p.prefix;
-  const int prefix_blocks = (p.prefix + kBlockKeys - 1) / kBlockKeys;
-  if ((int)blockIdx.x < prefix_items) {
-    // Consecutive tiles of one (head, split) read the same keys: one XCD's.
-    int item, unused;
-    xcd_tile_order((int)blockIdx.x, prefix_items, prefix_items, 1, 1, &item,
-                   &unused);
-    const int tile = item % p.prefix_tiles, rest = item / p.prefix_tiles;
-    t.part = rest % p.prefix_splits;
-    t.kv_head = rest / p.prefix_splits;
-    t.r0 = tile * (RP * 16);
-    t.r_end = row_start(p, p.batch) * p.group;
-    if (t.r0 >= t.r_end)
-      return;
-    t.lead = prefix_blocks;
-    t.table = nullptr;
-    t.own_end = t.base = t.first = 0;
-    const int per = (prefix_blocks + p.prefix_splits - 1) / p.prefix_splits;
-    t.c_begin = t.part * per;
-    t.c_end = t.c_begin + per < prefix_blocks ? t.c_begin + per : prefix_blocks;
-    paged_tile<DP, RP>(p, t, smem, wave_m, wave_l);
-    return;
-  }
-  constexpr int RM = RO * 16;
-  const int own_items = (int)gridDim.x - prefix_items;
+  __shared__ float wave_m[kPagedWaves][kNarrowRows],
+      wave_l[kPagedWaves][kNarrowRows];
+
+  const int lane = threadIdx.x & 63;
+  // Consecutive stretches of one head's line read the same prefix: one XCD's.
   int item, unused;
-  xcd_tile_order((int)blockIdx.x - prefix_items, own_items, own_items, 1, 1,
-                 &item, &unused);
-  const int tile = item % p.own_tiles, rest = item / p.own_tiles;
-  const int split = rest % p.own_splits;
-  t.kv_head = rest / p.own_splits;
-  const int b = __builtin_amdgcn_readfirstlane(request_of<RM>(p, tile));
-  const int begin = row_start(p, b), end = row_start(p, b + 1);
-  const int64_t r0 = (int64_t)begin * p.group +
-                     (int64_t)(tile - ((int64_t)begin * p.group / RM + b)) * RM;
-  if (r0 < (int64_t)begin * p.group || r0 >= (int64_t)end * p.group)
+  xcd_tile_order((int)blockIdx.x, (int)gridDim.x, (int)gridDim.x, 1, 1, &item,
+                 &unused);
+  PagedTile t;
+  t.kv_head = item / p.ways;
+  const int way = item % p.ways;
+
+  // The line: the prefix's tiles (rows of the whole batch), then the
+  // requests'. Lane l sums requests l * each .. + each - 1.
+  const int prefix_steps = (p.prefix + kStepKeys - 1) / kStepKeys;
+  const int64_t prefix_keys = (int64_t)prefix_steps * kStepKeys;
+  const int packed = uniform(row_start(p, p.batch)) * p.group;
+  const int shared_tile = tile_rows<DP>(p.packed);
+  const int shared_tiles =
+      p.shared ? (packed + shared_tile - 1) / shared_tile : 0;
+  const int64_t shared_keys = shared_tiles * prefix_keys;
+  const int64_t lead_keys = p.shared ? 0 : prefix_keys;
+  const int each = (p.batch + 63) / 64;
+  int64_t mine = 0;
+  for (int i = 0; i < each; ++i) {
+    const int b = lane * each + i;
+    if (b < p.batch) {
+      const Request q = request<DP, false>(p, b, lead_keys);
+      mine += q.before(q.tiles);
+    }
+  }
+  int64_t upto = mine;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int64_t x = __shfl_up(upto, d);
+    if (lane >= d)
+      upto += x;
+  }
+  const int64_t total = shared_keys + uniform(__shfl(upto, 63));
+  int64_t per = (total + p.ways - 1) / p.ways;
+  per = per < p.least ? p.least : per;
+  int64_t x = way * per;
+  const int64_t x_end = x + per < total ? x + per : total;
+  if (x >= x_end)
     return;
-  t.r0 = (int)r0;
-  t.r_end = end * p.group;
-  const int length = p.lengths[b];
-  t.own_end = length < 0 ? 0 : length < p.capacity ? length : p.capacity;
-  t.base = (length < 0 ? 0 : length) - (end - begin);
-  t.first = begin;
-  t.table = p.table + (int64_t)b * p.table_stride;
-  // Blocks up to the last key that the tile's last row sees.
-  const int r_last = t.r0 + RM < t.r_end ? t.r0 + RM - 1 : t.r_end - 1;
-  int seen = t.base + r_last / p.group - begin + 1;
-  seen = seen < 0 ? 0 : seen > t.own_end ? t.own_end : seen;
-  t.lead = p.prefix_splits ? 0 : prefix_blocks;
-  const int blocks = t.lead + (seen + kBlockKeys - 1) / kBlockKeys;
-  int per = (blocks + p.own_splits - 1) / p.own_splits;
-  per = per < kPagedSplitBlocks ? kPagedSplitBlocks : per;
-  t.part = p.prefix_splits + split;
-  t.c_begin = split * per < blocks ? split * per : blocks;
-  t.c_end = blocks - t.c_begin < per ? blocks : t.c_begin + per;
-  paged_tile<DP, RO>(p, t, smem, wave_m, wave_l);
+
+  // Where the stretch begins: among the prefix's tiles, or in the request that
+  // holds it: the last lane whose requests start at or before it, then that
+  // lane's one after the other; its tile by bisection.
+  bool lead = x < shared_keys;
+  int b = -1, i = 0;
+  int64_t start = 0;  // where the tiles of b (or of the prefix) start
+  Request q = {};
+  q.tiles = shared_tiles;
+  q.tile = shared_tile;
+  q.a = prefix_keys;
+  if (lead) {
+    i = uniform((int)(x / prefix_keys));
+  } else {
+    const int64_t y = x - shared_keys;
+    const int lane_of =
+        uniform(63 - __builtin_clzll(__ballot(upto - mine <= y) | 1));
+    start = shared_keys + uniform(__shfl(upto - mine, lane_of));
+    b = lane_of * each;
+    q = request<DP>(p, b, lead_keys);
+    while (start + q.before(q.tiles) <= x && b + 1 < p.batch) {
+      start += q.before(q.tiles);
+      q = request<DP>(p, ++b, lead_keys);
+    }
+    for (int span = q.tiles; span > 1;) {
+      const int half = span / 2;
+      const bool past = start + q.before(i + half) <= x;
+      i += past ? half : 0;
+      span = past ? span - half : half;
+    }
+  }
+
+  while (x < x_end) {
+    if (i >= q.tiles) {  // on to the next request
+      start += q.before(q.tiles);
+      lead = false;
+      if (++b >= p.batch)
+        return;
+      q = request<DP>(p, b, lead_keys);
+      i = 0;
+      continue;
+    }
+    // Keys from .. to - 1 of the `keys` that the tile has on the line.
+    const int64_t at = start + q.before(i), keys = q.a + q.step * i;
+    const int64_t from = x - at;
+    int64_t to = x_end - at < keys ? x_end - at : keys;
+    x = at + to;
+    t.r0 = q.begin * p.group + i * q.tile;
+    t.r_end = lead ? packed : q.end * p.group;
+    t.r_end = t.r_end - t.r0 < q.tile ? t.r_end : t.r0 + q.tile;
+    t.first = q.begin;
+    t.base = q.base;
+    t.own_end = lead ? 0 : q.own_end;
+    t.table = p.table + (int64_t)(lead ? 0 : b) * p.table_stride;
+    t.lead = lead || !p.shared ? prefix_steps : 0;
+    t.seen = lead ? 0 : uniform(sees(p, t, t.r_end - 1));
+    const int steps = t.lead + (t.seen + kStepKeys - 1) / kStepKeys;
+    ++i;
+    int64_t first = 0;
+    int count = 1;
+    if (p.partials) {
+      first = at / per;
+      count = (int)((at + keys - 1) / per - first) + 1;
+    } else {
+      // without a workspace a workgroup takes the tiles that start in its
+      // stretch, whole
+      if (from > 0)
+        continue;
+      to = keys;
+    }
+    auto step_at = [&](int64_t key) {
+      const int64_t s = (key + kStepKeys - 1) / kStepKeys;
+      return key >= keys || s > steps ? steps : (int)s;
+    };
+    t.s_begin = step_at(from);
+    t.s_end = step_at(to);
+    const bool whole = count == 1 && !p.shared;
+    const int64_t line = p.shared && !lead ? p.packed : 0;
+    t.part = whole ? -1 : line + (int64_t)kWideRows * way;
+    if (p.partials && from == 0 && t.kv_head == 0)
+      for (int r = t.r0 + (int)threadIdx.x; r < t.r_end; r += kPagedThreads)
+        p.part_of[line + r] = i32x2{(int)first, whole ? 0 : count};
+    if (q.tile == kNarrowRows)
+      narrow_tile<DP>(p, t, smem, wave_m, wave_l);
+    else if constexpr (DP < 256)
+      wide_tile<DP>(p, t, smem);
+  }
 }
 
-// Joins the parts of every row: DP / 4 threads a row, 4 columns each.
+// Joins the parts of every row that has some: DP / 4 threads a row, 4 columns
+// each. A row's parts of one kind (the prefix's and its own, or both at once)
+// are kWideRows rows apart, part_of telling the first and how many.
 template <int DP>
 __global__ __launch_bounds__(kPagedThreads) void attention_paged_join_kernel(
     PagedAttention p) {
@@ -495,43 +896,55 @@ __global__ __launch_bounds__(kPagedThreads) void attention_paged_join_kernel(
   if (kv_head >= p.kv_heads || row >= row_start(p, p.batch) * p.group ||
       dq >= p.dv)
     return;
-  const int parts = p.prefix_splits + p.own_splits;
-  const int64_t step = (int64_t)p.kv_heads * p.packed;
   float top = kNegInf, sum = 0.0f;
   f32x4 acc = {0, 0, 0, 0};
-  // 4 parts' loads in flight; a part past the last repeats it with weight 0
-  for (int s0 = 0; s0 < parts; s0 += 4) {
-    float m[4], l[4];
-    f32x4 v[4];
+  int parts = 0;
+  for (int kind = 0; kind <= p.shared; ++kind) {
+    const int64_t line = kind * p.packed + row;
+    const i32x2 of = p.part_of[line];
+    // within the workgroups of the line, whatever it holds
+    const int first = of[0] < 0 ? 0 : of[0] < p.ways ? of[0] : p.ways - 1;
+    const int count = of[1] < p.ways - first ? of[1] : p.ways - first;
+    const int64_t at0 = (int64_t)kv_head * p.part_rows + line +
+                        (int64_t)kWideRows * first;
+    // 4 parts' loads in flight; a part past the last repeats it with weight 0
+    for (int s0 = 0; s0 < count; s0 += 4) {
+      f32x2 ml[4];
+      f32x4 v[4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int64_t i = at + (s0 + u < parts ? s0 + u : parts - 1) * step;
-      m[u] = p.part_ml[2 * i];
-      l[u] = p.part_ml[2 * i + 1];
-      v[u] = *(const f32x4 *)(p.partials + i * DP + dq);
-    }
-    float x = top;
-#pragma unroll
-    for (int u = 0; u < 4; ++u)
-      x = fmaxf(x, m[u]);
-    const float keep = top == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(top - x);
-    top = x;
-    sum *= keep;
-    acc *= keep;
-#pragma unroll
-    for (int u = 0; u < 4; ++u)
-      if (s0 + u < parts) {
-        const float f =
-            m[u] == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(m[u] - x);
-        sum += f * l[u];
-        acc += f * v[u];
+      for (int u = 0; u < 4; ++u) {
+        const int64_t i =
+            at0 + (int64_t)kWideRows * (s0 + u < count ? s0 + u : count - 1);
+        ml[u] = *(const f32x2 *)(p.part_ml + 2 * i);
+        v[u] = *(const f32x4 *)(p.partials + i * DP + dq);
       }
+      float x = top;
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        x = fmaxf(x, ml[u][0]);
+      const float keep =
+          top == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(top - x);
+      top = x;
+      sum *= keep;
+      acc *= keep;
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (s0 + u < count) {
+          const float f = ml[u][0] == kNegInf
+                              ? 0.0f
+                              : __builtin_amdgcn_exp2f(ml[u][0] - x);
+          sum += f * ml[u][1];
+          acc += f * v[u];
+        }
+    }
+    parts += count > 0 ? count : 0;
   }
+  if (parts == 0)
+    return;  // stored by the workgroup that had the tile whole
   const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
-  f16 *dst = p.o + (int64_t)(row / p.group) * p.o_row +
-             (int64_t)(kv_head * p.group + row % p.group) * p.o_head + dq;
-  *(f16x4 *)dst = f16x4{(f16)(acc[0] * inv), (f16)(acc[1] * inv),
-                          (f16)(acc[2] * inv), (f16)(acc[3] * inv)};
+  *(f16x4 *)(result_row(p, kv_head, row) + dq) =
+      f16x4{(f16)(acc[0] * inv), (f16)(acc[1] * inv), (f16)(acc[2] * inv),
+            (f16)(acc[3] * inv)};
 }
 
 // ----------------------------------------------------------------------------
@@ -542,26 +955,24 @@ namespace {
 
 struct PagedKernel {
   const char *name;
-  int dp, rp, ro;
+  int dp;
   const void *fn;
 };
-#define IHP_PAGED(DP, RP, RO)                                                  \
-  {"attention_paged_d" #DP "_r" #RP "_r" #RO, DP, RP, RO,                      \
-   (const void *)&attention_paged_kernel<DP, RP, RO>}
 const PagedKernel kPagedKernels[] = {
-    IHP_PAGED(64, 2, 1),  IHP_PAGED(64, 2, 2),  IHP_PAGED(128, 2, 1),
-    IHP_PAGED(128, 2, 2), IHP_PAGED(256, 1, 1),
+    {"attention_paged_d64", 64, (const void *)&attention_paged_kernel<64>},
+    {"attention_paged_d128", 128, (const void *)&attention_paged_kernel<128>},
+    {"attention_paged_d256", 256, (const void *)&attention_paged_kernel<256>},
+};
+const PagedKernel kJoinKernels[] = {
+    {"attention_paged_join_d64", 64,
+     (const void *)&attention_paged_join_kernel<64>},
+    {"attention_paged_join_d128", 128,
+     (const void *)&attention_paged_join_kernel<128>},
+    {"attention_paged_join_d256", 256,
+     (const void *)&attention_paged_join_kernel<256>},
 };
 constexpr int kPagedKernelCount =
     sizeof(kPagedKernels) / sizeof(kPagedKernels[0]);
-const PagedKernel kJoinKernels[] = {
-    {"attention_paged_join_d64", 64, 0, 0,
-     (const void *)&attention_paged_join_kernel<64>},
-    {"attention_paged_join_d128", 128, 0, 0,
-     (const void *)&attention_paged_join_kernel<128>},
-    {"attention_paged_join_d256", 256, 0, 0,
-     (const void *)&attention_paged_join_kernel<256>},
-};
 
 }  // namespace
 
@@ -573,48 +984,22 @@ PagedPlan plan_attention_paged(int64_t rows, int64_t batch, int64_t kv_heads,
   const int64_t d = head_dim > head_dim_v ? head_dim : head_dim_v;
   p.dp = d <= 64 ? 64 : d <= 128 ? 128 : 256;
   const int64_t packed = rows * group;
-  p.rp = p.dp < 256 ? 2 : 1;
-  p.ro = p.dp < 256 && packed > 16 * batch ? 2 : 1;
-  p.own_tiles = packed / (16 * p.ro) + batch;
-  const int64_t part_bytes = kv_heads * packed * (p.dp + 2) * 4;
-  const int64_t most_parts =
-      workspace_limit <= kWorkspaceCounterBytes
-          ? 0
-          : (int64_t)((workspace_limit - kWorkspaceCounterBytes) /
-                      (size_t)part_bytes);
-  auto clamp = [](int64_t v, int64_t lo, int64_t hi) {
-    return v < lo ? lo : v > hi ? hi : v;
-  };
-  const int64_t prefix_blocks = (prefix + kBlockKeys - 1) / kBlockKeys;
-  const int64_t own_blocks = (capacity + kBlockKeys - 1) / kBlockKeys;
-  // Requests whose rows fill tiles walk the prefix themselves.
-  const bool shared = prefix > 0 && packed < 32 * batch && most_parts >= 2;
-  int64_t own_keys = own_blocks + (shared ? 0 : prefix_blocks);
-  p.own_splits = clamp(kPagedTargetWgs / (p.own_tiles * kv_heads), 1, 16);
-  p.own_splits =
-      clamp(p.own_splits, 1, (own_keys + kPagedSplitBlocks - 1) / kPagedSplitBlocks);
-  if (shared) {
-    p.prefix_tiles = (packed + 16 * p.rp - 1) / (16 * p.rp);
-    p.prefix_splits =
-        clamp(kPagedTargetWgs / (p.prefix_tiles * kv_heads), 1, 32);
-    p.prefix_splits =
-        clamp(p.prefix_splits, 1,
-              (prefix_blocks + kPagedSplitBlocks - 1) / kPagedSplitBlocks);
-    if (p.prefix_splits + p.own_splits > most_parts) {
-      // as many parts as fit, the prefix's first
-      p.own_splits = clamp(p.own_splits, 1, most_parts / 2);
-      p.prefix_splits = clamp(p.prefix_splits, 1, most_parts - p.own_splits);
-    }
-  } else if (p.own_splits > 1) {
-    p.own_splits = clamp(p.own_splits, 1, most_parts < 1 ? 1 : most_parts);
+  // Requests that fill wide tiles walk the prefix themselves, as one alone.
+  p.shared = prefix > 0 && batch > 1 && packed < kWideRows * batch;
+  const int64_t wgs = p.dp < 256 ? kPagedTargetWgs : kPagedTargetWgs / 2;
+  p.ways = wgs / kv_heads > 1 ? wgs / kv_heads : 1;
+  p.least = kPagedLeastKeys;
+  p.part_rows = 2 * packed + kWideRows * p.ways;
+  p.workspace = (int64_t)kWorkspaceCounterBytes + 2 * packed * 8 +
+                kv_heads * p.part_rows * (p.dp + 2) * 4;
+  if ((uint64_t)p.workspace > workspace_limit) {
+    // every tile whole, one workgroup each at the most
+    p.shared = false;
+    p.workspace = p.part_rows = 0;
+    p.ways = batch + packed / 16;
+    p.ways = p.ways < 2 * wgs / kv_heads + 1 ? p.ways : 2 * wgs / kv_heads + 1;
+    p.least = 1;
   }
-  if (p.own_splits < 1)
-    p.own_splits = 1;
-  const int64_t parts = p.prefix_splits + p.own_splits;
-  p.workspace =
-      parts > 1 ? (int64_t)kWorkspaceCounterBytes + parts * part_bytes : 0;
-  p.items = (p.prefix_tiles * p.prefix_splits + p.own_tiles * p.own_splits) *
-            kv_heads;
   return p;
 }
 
@@ -622,51 +1007,49 @@ hipError_t launch_attention_paged(const PagedAttention &attention,
                                   const PagedPlan &plan, void *workspace,
                                   void *stream) {
   PagedAttention a = attention;
-  a.prefix_tiles = (int)plan.prefix_tiles;
-  a.prefix_splits = (int)plan.prefix_splits;
-  a.own_tiles = (int)plan.own_tiles;
-  a.own_splits = (int)plan.own_splits;
-  const int64_t parts = plan.prefix_splits + plan.own_splits;
+  a.ways = (int)plan.ways;
+  a.least = (int)plan.least;
+  a.shared = plan.shared ? 1 : 0;
+  a.part_rows = plan.part_rows;
+  a.part_of = nullptr;
+  a.partials = a.part_ml = nullptr;
   const int64_t all = (int64_t)a.kv_heads * a.packed;
-  a.partials = nullptr;
-  a.part_ml = nullptr;
-  if (parts > 1) {
+  if (plan.workspace) {
     a.partials = (float *)((char *)workspace + kWorkspaceCounterBytes);
-    a.part_ml = a.partials + parts * all * plan.dp;
+    a.part_ml = a.partials + a.kv_heads * plan.part_rows * plan.dp;
+    a.part_of = (i32x2 *)(a.part_ml + a.kv_heads * plan.part_rows * 2);
   }
-  const void *kernel = nullptr;
-  for (const PagedKernel &k : kPagedKernels)
-    if (k.dp == plan.dp && k.rp == plan.rp && k.ro == plan.ro)
-      kernel = k.fn;
+  const void *kernel = nullptr, *join = nullptr;
+  for (int i = 0; i < kPagedKernelCount; ++i)
+    if (kPagedKernels[i].dp == plan.dp) {
+      kernel = kPagedKernels[i].fn;
+      join = kJoinKernels[i].fn;
+    }
   if (!kernel)
     return hipErrorInvalidValue;
   void *args[] = {&a};
-  hipError_t e = hipLaunchKernel(kernel, dim3((unsigned)plan.items),
-                                 dim3(kPagedThreads), args, 0,
-                                 (hipStream_t)stream);
-  if (e != hipSuccess || parts == 1)
+  hipError_t e =
+      hipLaunchKernel(kernel, dim3((unsigned)(plan.ways * a.kv_heads)),
+                      dim3(kPagedThreads), args, 0, (hipStream_t)stream);
+  if (e != hipSuccess || !plan.workspace)
     return e;
-  for (const PagedKernel &k : kJoinKernels)
-    if (k.dp == plan.dp)
-      kernel = k.fn;
   const int per = kPagedThreads / (plan.dp / 4);
-  return hipLaunchKernel(kernel, dim3((unsigned)((all + per - 1) / per)),
+  return hipLaunchKernel(join, dim3((unsigned)((all + per - 1) / per)),
                          dim3(kPagedThreads), args, 0, (hipStream_t)stream);
 }
 
 const KernelEntry *attention_paged_kernels(int *count) {
-  constexpr int kJoins = sizeof(kJoinKernels) / sizeof(kJoinKernels[0]);
-  static KernelEntry all[kPagedKernelCount + kJoins];
+  static KernelEntry all[2 * kPagedKernelCount];
   static const bool filled = [] {
-    for (int i = 0; i < kPagedKernelCount; ++i)
+    for (int i = 0; i < kPagedKernelCount; ++i) {
       all[i] = {kPagedKernels[i].name, kPagedKernels[i].fn, kPagedThreads, 0};
-    for (int i = 0; i < kJoins; ++i)
       all[kPagedKernelCount + i] = {kJoinKernels[i].name, kJoinKernels[i].fn,
                                     kPagedThreads, 0};
+    }
     return true;
   }();
   (void)filled;
-  *count = kPagedKernelCount + kJoins;
+  *count = 2 * kPagedKernelCount;
   return all;
 }
 

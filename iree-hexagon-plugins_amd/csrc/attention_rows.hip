@@ -30,6 +30,7 @@
 // when they are many, where the fused kernel takes over (abi.cpp, rows_us).
 #include <type_traits>
 
+#include "attention_common.h"
 #include "device_common.h"
 #include "kernels_internal.h"
 
@@ -48,24 +49,6 @@ typedef i32x4 __attribute__((aligned(2))) i32x4_u;
 typedef i32x2 __attribute__((aligned(2))) i32x2_u;
 typedef f16x4 __attribute__((aligned(2))) f16x4_u;
 typedef f32x4 __attribute__((aligned(4))) f32x4_u;
-
-// Chunk swizzle of a staged V row (key) of NCH 16-byte chunks: a transposed
-// read takes 4 rows of one 32-byte window per 16-lane block, two blocks (rows
-// 4 apart) at a time, and all of it must spread over the 64 banks.
-template <int NCH>
-__device__ __forceinline__ int v_swizzle(int k) {
-  return NCH >= 16 ? (4 * (k & 3)) ^ (2 * ((k >> 2) & 1))
-                   : (2 * ((k >> 1) & 1)) ^ (4 * ((k >> 2) & 1));
-}
-
-__device__ __forceinline__ float across_groups_max(float x) {
-  x = fmaxf(x, __shfl_xor(x, 16));
-  return fmaxf(x, __shfl_xor(x, 32));
-}
-__device__ __forceinline__ float across_groups_sum(float x) {
-  x += __shfl_xor(x, 16);
-  return x + __shfl_xor(x, 32);
-}
 
 }  // namespace
 
@@ -308,7 +291,7 @@ attention_rows_kernel(const f16 *__restrict__ Q, const f16 *__restrict__ K,
       const int k = p * VROWS + vrow;
       if (c * kBlockKeys + k >= L.seq_kv)
         vf[p] = i32x4{0, 0, 0, 0};
-      *(i32x4 *)(vs + k * (DP * 2) + ((vch ^ v_swizzle<NCH>(k)) << 4)) = vf[p];
+      *(i32x4 *)(vs + k * (DP * 2) + ((vch ^ row_v_swizzle<NCH>(k)) << 4)) = vf[p];
     }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
@@ -321,7 +304,7 @@ attention_rows_kernel(const f16 *__restrict__ Q, const f16 *__restrict__ K,
       const int byte = 2 * (16 * d + 4 * (l15 & 3));
       const IHP_LDS char *p =
           (const IHP_LDS char *)vs + k * (DP * 2) +
-          (((byte >> 4) ^ v_swizzle<NCH>(k)) << 4) + (byte & 15);
+          (((byte >> 4) ^ row_v_swizzle<NCH>(k)) << 4) + (byte & 15);
       const i32x2 lo = __builtin_bit_cast(
           i32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((IHP_LDS s16x4 *)p));
       const i32x2 hi = __builtin_bit_cast(

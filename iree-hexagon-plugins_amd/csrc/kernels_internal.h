@@ -379,7 +379,6 @@ struct PagedAttention {
   const _Float16 *q, *k_cache, *v_cache;
   _Float16 *o;
   const int32_t *row_starts, *lengths, *table, *prefix_pages;
-  float *partials, *part_ml;  // null: the tiles store the result
   int64_t q_row, q_head, o_row, o_head, k_head, v_head, table_stride;
   int64_t packed;             // rows of a KV head: rows * group
   uint64_t page_magic;        // key / page_size = key * magic >> shift
@@ -388,16 +387,28 @@ struct PagedAttention {
   int batch, rows, kv_heads, group, dqk, dv;
   int prefix, capacity;       // prefix keys, keys that a table row can name
   float scale;
-  int prefix_tiles, prefix_splits, own_tiles, own_splits;
+  // Workgroups that share a KV head's tiles, the keys that one takes at
+  // least, and whether the prefix has tiles of its own.
+  int ways, least, shared;
+  // Parts (no workspace: null): a row's f32 part of workgroup w at row
+  // line + 128 w of its KV head's part_rows, line = its row, plus `packed`
+  // for its own keys where the prefix has tiles of its own; their (max, sum);
+  // and per line the first workgroup and how many (0: none, the result is
+  // stored). Distinct on the line of tiles: from one tile to the next the row
+  // moves on by the tile's at most 128 rows, from one workgroup to the next w
+  // does.
+  int64_t part_rows;
+  float *partials, *part_ml;
+  int __attribute__((ext_vector_type(2))) *part_of;
 };
-// Workgroups wanted: two a CU. A part of a tile's keys is at least 2 blocks a
-// wave.
+// Workgroups wanted (two a CU where head dims allow it), and the keys that
+// one takes at least.
 constexpr int64_t kPagedTargetWgs = 512;
-constexpr int kPagedSplitBlocks = 8;
+constexpr int64_t kPagedLeastKeys = 128;
 struct PagedPlan {
-  int dp, rp, ro;  // head-dim bucket, 16-row fragments of a tile
-  int64_t prefix_tiles, prefix_splits, own_tiles, own_splits;
-  int64_t items, workspace;
+  int dp;  // head-dim bucket
+  bool shared;
+  int64_t ways, least, part_rows, workspace;
 };
 PagedPlan plan_attention_paged(int64_t rows, int64_t batch, int64_t kv_heads,
                                int64_t group, int64_t prefix, int64_t capacity,

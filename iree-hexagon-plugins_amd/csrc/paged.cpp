@@ -305,7 +305,7 @@ int iree_mi355x_shared_prefix_attention_f16(
   const PagedPlan plan = plan_of(b, workspace ? workspace_bytes : 0);
   // A launch has fewer than 2^32 threads.
   const int64_t most = (int64_t)1 << 24;
-  if (plan.items >= most ||
+  if (plan.ways * c.kv_heads >= most ||
       (plan.workspace && p.packed * p.kv_heads / (1024 / plan.dp) >= most - 1))
     return fail(IREE_MI355X_UNSUPPORTED, "%s: problem too large", who);
   return launch_status(launch_attention_paged(p, plan, workspace, stream),

@@ -215,7 +215,7 @@ def test_attention_argument_errors(pkg):
         assert attend(pkg, **kw) == pkg.MISALIGNED, kw
     for kw in (dict(rows=1 << 30), dict(batch=1 << 31),
                dict(prefix_length=1 << 30), dict(heads=1 << 17),
-               dict(rows=1 << 27, table_width=0, prefix_length=0)):
+               dict(rows=1 << 27, ws=FAKE, wsb=1 << 62)):
         assert attend(pkg, **kw) == pkg.UNSUPPORTED, kw
     # nothing to do
     for kw in (dict(rows=0), dict(heads=0), dict(batch=0)):
@@ -223,20 +223,19 @@ def test_attention_argument_errors(pkg):
 
 
 def test_attention_workspace(pkg):
-    """Tokens behind a prefix split the keys over parts and need a workspace;
-    rows that fill tiles, and few keys, need none."""
+    """Parts of rows: 512 workgroups' of 128 rows and both kinds of every
+    row, whatever the lengths are."""
     def need(**kw):
         a = paged(pkg, **kw)
         return (pkg.library().
                 iree_mi355x_shared_prefix_attention_workspace_bytes(
                     ctypes.byref(a)))
 
-    # a prefix part and an own part, f32 rows of 64 and their (max, sum)
-    assert need() >= (256 << 10) + 2 * 6 * 8 * (64 + 2) * 4
-    assert need(prefix_length=8192) > need()
-    assert need(prefix_length=0) == 0
-    assert need(prefix_length=0, table_width=100) > 256 << 10
-    assert need(rows=5000, prefix_length=1000) == 0
+    # f32 rows of the head-dim bucket, their (max, sum), and where they are
+    rows = 2 * 6 * 8 + 512 * 128
+    assert need() == (256 << 10) + rows * (64 + 2) * 4 + 2 * 6 * 4 * 8
+    assert need(prefix_length=8192) == need(table_width=99) == need()
+    assert need(rows=5000) > need() + 2 * 8 * 4994 * 66 * 4
     for kw in (dict(rows=0), dict(heads=7), dict(batch=0), dict(rows=1 << 40),
                dict(prefix_length=-1)):
         assert need(**kw) == 0
