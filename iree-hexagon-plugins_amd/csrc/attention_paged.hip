@@ -40,6 +40,11 @@ constexpr int kBlockKeys = 32;   // of a narrow tile's wave
 constexpr int kStepKeys = 64;    // of a wide tile's block; pieces of a line
 constexpr int kNarrowRows = 16;
 constexpr int kWideRows = 128;
+// How far (in log2) a wide tile's row maximum may pass its reference before
+// the reference moves and O is rescaled: the sums are exact in either case,
+// and the weights' roundings relative, so a lag of 4 is 0-5 % further from 64
+// bits than none (rounding N(0, 1) scores and values of 64 to 5000 keys).
+constexpr float kLag = 4.0f;
 constexpr float kNegInf = -__builtin_inff();
 constexpr float kLog2e = 1.4426950408889634f;
 typedef float f32x2 __attribute__((ext_vector_type(2)));
@@ -48,9 +53,13 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ int uniform(int x) {
   return __builtin_amdgcn_readfirstlane(x);
 }
-__device__ __forceinline__ int64_t uniform(int64_t x) {
-  return (int64_t)((uint64_t)(uint32_t)uniform((int)x) |
-                   (uint64_t)(uint32_t)uniform((int)(x >> 32)) << 32);
+
+// The kernel's arguments, read where they are used: held in registers from the
+// kernel's start they pushed the tiles' own out of theirs.
+__device__ __forceinline__ const PagedAttention &arguments() {
+  auto *at = __builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(at));
+  return *(const PagedAttention *)at;
 }
 
 // row_starts[b], within the rows that there are whatever it holds.
@@ -90,14 +99,18 @@ struct PagedBlock {
   uint32_t k = 0, v = 0;
   Mask there = 0;  // bit i: key i of the block is there
 
-  // `lead`: the prefix's blocks of KEYS keys.
+  // `lead`: the prefix's blocks of KEYS keys. Keys past the end are the last
+  // one, or those of the last aligned `group` keys (which a page that is a
+  // multiple of them holds whole).
   __device__ __forceinline__ void find(const PagedAttention &p,
-                                       const PagedTile &t, int lead, int c) {
+                                       const PagedTile &t, int lead, int c,
+                                       int group = 1) {
     const bool own = c >= lead;
     const int end = own ? t.own_end : p.prefix;
     const int32_t *table = own ? t.table : p.prefix_pages;
     int key = (own ? c - lead : c) * KEYS + ((int)threadIdx.x & (KEYS - 1));
-    key = key < end ? key : end - 1;
+    if (key >= end)
+      key = ((end - 1) & -group) + (key & (group - 1));
     const int column =
         (int)(((uint64_t)(uint32_t)key * p.page_magic) >> p.page_shift);
     inside = key - column * p.page_size;
@@ -134,10 +147,10 @@ __device__ __forceinline__ int64_t part_row(const PagedAttention &p,
 // A tile of up to 16 rows. DP: the head-dim bucket (64, 128 or 256, at least
 // both head dims).
 template <int DP>
-__device__ __forceinline__ void narrow_tile(const PagedAttention &p,
-                                            const PagedTile &t, char *smem,
+__device__ __forceinline__ void narrow_tile(const PagedTile &t, char *smem,
                                             float (*wave_m)[kNarrowRows],
                                             float (*wave_l)[kNarrowRows]) {
+  const PagedAttention &p = arguments();
   constexpr int KS = DP / 32;           // head-dim steps of S
   constexpr int DB = DP / 16;           // 16-wide d blocks of O
   constexpr int NCH = DP / 8;           // 16-byte chunks of a V row
@@ -399,8 +412,8 @@ __device__ __forceinline__ int wide_v_swizzle(int key) {
 }
 
 template <int DP>
-__device__ __forceinline__ void wide_tile(const PagedAttention &p,
-                                          const PagedTile &t, char *smem) {
+__device__ __forceinline__ void wide_tile(const PagedTile &t, char *smem) {
+  const PagedAttention &p = arguments();
   constexpr int DS = DP / 16;         // 16-wide d steps of S^T = K Q^T
   constexpr int DT = DP / 32;         // 32-row d tiles of O^T
   constexpr int ROW = DP * 2;         // bytes of a staged row
@@ -435,32 +448,61 @@ __device__ __forceinline__ void wide_tile(const PagedAttention &p,
     }
   }
 
-  // Copy side: a lane's (row, chunk) of an instruction, the logical chunk
-  // that belongs there, and whether it lies within the head dim (the LDS past
-  // it is zeroed once and never written).
+  // Copy side: an instruction moves ROWS rows of CH chunks, lane -> (row,
+  // physical chunk), fetching the logical chunk that belongs there if it lies
+  // within the head dim (the LDS past it is zeroed once and never written).
+  // The swizzles repeat every 16 rows, so the chunk is the same in all passes.
+  // Where pages are multiples of ROWS tokens an instruction's rows follow one
+  // another in a page: their base is scalar, a lane's offset the same for all
+  // of them, and a copy takes no vector instruction. Otherwise every lane's
+  // place comes from the lane that has the key: 90 instead of 16 vector and
+  // LDS instructions a block of 8 copies a wave.
   const int c_row = lane / CH, c_phys = lane % CH;
+  const int k_chunk = c_phys ^ wide_k_swizzle<DP>(wave * ROWS + c_row);
+  const int v_chunk = c_phys ^ wide_v_swizzle<DP>(wave * ROWS + c_row);
+  const bool k_in = 8 * k_chunk < p.dqk, v_in = 8 * v_chunk < p.dv;
+  const bool grouped = p.page_size % ROWS == 0 &&
+                       p.k_row16 < (1u << 24) && p.v_row16 < (1u << 24);
+  const int group = grouped ? ROWS : 1;
+  const uint32_t k_lane = ((uint32_t)c_row * p.k_row16 + k_chunk) * 16;
+  const uint32_t v_lane = ((uint32_t)c_row * p.v_row16 + v_chunk) * 16;
   IHP_LDS char *lds = (IHP_LDS char *)smem;
   PagedBlock<kStepKeys> block;
   auto copy = [&](int slot) {
+    IHP_LDS char *kd = lds + slot * BLK + wave * (ROWS * ROW);
+    IHP_LDS char *vd = kd + 2 * BLK;
+    if (grouped) {
+      auto rows = [&](const char *base, uint32_t at, uint32_t mine, bool in,
+                      IHP_LDS char *to) {
 #pragma unroll
-    for (int i = 0; i < PASSES; ++i) {
-      const int row0 = (i * kPagedWaves + wave) * ROWS;
-      const int row = row0 + c_row;
-      const int chunk = c_phys ^ wide_k_swizzle<DP>(row);
-      const uint32_t at = (uint32_t)__shfl((int)block.k, row);
-      if (8 * chunk < p.dqk)
-        global_to_lds_16(Kp + ((uint64_t)at + (uint32_t)chunk) * 16,
-                         lds + slot * BLK + row0 * ROW);
-    }
+        for (int i = 0; i < PASSES; ++i) {
+          const uint32_t row0 = (uint32_t)__builtin_amdgcn_readlane(
+              (int)at, (i * kPagedWaves + wave) * ROWS);
+          if (in)
+            global_to_lds_16s(base + (uint64_t)row0 * 16, mine,
+                              to + i * kPagedWaves * ROWS * ROW);
+        }
+      };
+      rows(Kp, block.k, k_lane, k_in, kd);
+      rows(Vp, block.v, v_lane, v_in, vd);
+    } else {
+      uint32_t at[2 * PASSES];
 #pragma unroll
-    for (int i = 0; i < PASSES; ++i) {
-      const int row0 = (i * kPagedWaves + wave) * ROWS;
-      const int row = row0 + c_row;
-      const int chunk = c_phys ^ wide_v_swizzle<DP>(row);
-      const uint32_t at = (uint32_t)__shfl((int)block.v, row);
-      if (8 * chunk < p.dv)
-        global_to_lds_16(Vp + ((uint64_t)at + (uint32_t)chunk) * 16,
-                         lds + (2 + slot) * BLK + row0 * ROW);
+      for (int i = 0; i < PASSES; ++i) {
+        const int row = (i * kPagedWaves + wave) * ROWS + c_row;
+        at[i] = (uint32_t)__shfl((int)block.k, row);
+        at[PASSES + i] = (uint32_t)__shfl((int)block.v, row);
+      }
+#pragma unroll
+      for (int i = 0; i < PASSES; ++i) {
+        if (k_in)
+          global_to_lds_16(Kp + ((uint64_t)at[i] + (uint32_t)k_chunk) * 16,
+                           kd + i * kPagedWaves * ROWS * ROW);
+        if (v_in)
+          global_to_lds_16(
+              Vp + ((uint64_t)at[PASSES + i] + (uint32_t)v_chunk) * 16,
+              vd + i * kPagedWaves * ROWS * ROW);
+      }
     }
   };
 
@@ -503,11 +545,11 @@ __device__ __forceinline__ void wide_tile(const PagedAttention &p,
     block_barrier();
   }
   if (c < c_end) {
-    block.find(p, t, lead, c);
+    block.find(p, t, lead, c, group);
     block.place(p, t, lead, c);
     copy(0);
     if (c + 1 < c_end)
-      block.find(p, t, lead, c + 1);
+      block.find(p, t, lead, c + 1, group);
   }
   for (int slot = 0; c < c_end; ++c, slot ^= 1) {
     const bool own = c >= lead;
@@ -529,13 +571,15 @@ __device__ __forceinline__ void wide_tile(const PagedAttention &p,
       block.place(p, t, lead, c + 1);
       copy(slot ^ 1);
       if (c + 2 < c_end)
-        block.find(p, t, lead, c + 2);
+        block.find(p, t, lead, c + 2, group);
     }
 
     if (idle)
       continue;
 
-    // S^T: reads run three MFMAs ahead in four rotating registers.
+    // S^T: reads run three MFMAs ahead in four rotating registers. The other
+    // workgroup's wave on the SIMD leaves its softmax for these.
+    __builtin_amdgcn_s_setprio(1);
     {
       const uint32_t kbase = ka + (uint32_t)(slot * BLK);
       constexpr int NR = 2 * DS, KW = 3, NB = KW + 1;
@@ -557,6 +601,8 @@ __device__ __forceinline__ void wide_tile(const PagedAttention &p,
           issue(std::integral_constant<int, R + KW>());
       });
     }
+
+    __builtin_amdgcn_s_setprio(0);
 
     // Softmax. Element (t, r) of S^T is key 32 t + 8 (r / 4) + 4 g + r % 4.
     float sc = scale;
@@ -583,7 +629,7 @@ __device__ __forceinline__ void wide_tile(const PagedAttention &p,
     }
     const float mx =
         pair_max(fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * sc);
-    if (!__all(mx <= m_run)) {
+    if (!__all(mx <= m_run + kLag)) {
       const float m_new = fmaxf(m_run, mx);
       const float keep =
           m_new == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(m_run - m_new);
@@ -610,6 +656,7 @@ __device__ __forceinline__ void wide_tile(const PagedAttention &p,
 
     // O^T += V^T P^T, 16 keys an MFMA; the V^T fragments of the next key step
     // are read before the MFMAs of this one.
+    __builtin_amdgcn_s_setprio(1);
     {
       float psum[4];
       const IHP_LDS char *vs = lds + (2 + slot) * BLK;
@@ -647,6 +694,7 @@ __device__ __forceinline__ void wide_tile(const PagedAttention &p,
       });
       l_run += (psum[0] + psum[1]) + (psum[2] + psum[3]);
     }
+    __builtin_amdgcn_s_setprio(0);
   }
 
   // Register quarter (dt, q) of O^T holds columns 32 dt + 8 q + 4 g .. + 3 of
@@ -694,45 +742,44 @@ __device__ __forceinline__ int tile_rows(int64_t rows) {
   return DP >= 256 || rows <= kNarrowRows ? kNarrowRows : kWideRows;
 }
 
-// Request b's tiles on the line: tile i takes a + i * step keys, near what it
-// walks, so that their sums have a closed form.
+// Request b's tiles on the line: tile i takes a + i * step units, near the keys
+// that it walks and what a tile costs besides, so that their sums have a
+// closed form. A unit is 2^unit keys, which keeps the line below 2^31.
 struct Request {
   int begin, end, tile, tiles;  // rows' tokens, rows a tile
   int own_end, base;
-  int64_t a, step;
-  __device__ __forceinline__ int64_t before(int64_t i) const {
+  uint32_t a, step;
+  __device__ __forceinline__ uint32_t before(uint32_t i) const {
     return i * a + step * (i * (i - 1) / 2);
   }
 };
-// UNIFORM: b is the same in every lane.
-template <int DP, bool UNIFORM = true>
-__device__ __forceinline__ Request request(const PagedAttention &p, int b,
-                                           int64_t lead_keys) {
+// A workgroup's place on the line.
+struct Line {
+  uint32_t x, x_end, start, per;
+  float inv_per;
+  int packed, kv_head, way, b, i;
   Request q;
-  q.begin = row_start(p, b);
-  q.end = row_start(p, b + 1);
-  int length = p.lengths[b];
-  if (UNIFORM) {
-    q.begin = uniform(q.begin);
-    q.end = uniform(q.end);
-    length = uniform(length);
-  }
-  const int added = q.end > q.begin ? q.end - q.begin : 0;
-  q.end = q.begin + added;
-  const int64_t rows = (int64_t)added * p.group;
+};
+
+template <int DP>
+__device__ __forceinline__ Request request(const PagedAttention &p, int begin,
+                                           int end, int length, int lead) {
+  Request q;
+  const int added = end > begin ? end - begin : 0;
+  q.begin = begin;
+  q.end = begin + added;
+  const int rows = added * p.group;
   q.tile = tile_rows<DP>(rows);
-  q.tiles = (int)((rows + q.tile - 1) / q.tile);
+  q.tiles = (rows + q.tile - 1) / q.tile;
   length = length > 0 ? length : 0;
   q.own_end = length < p.capacity ? length : p.capacity;
   q.base = length - added;
-  const int tokens = q.tile / p.group > 1 ? q.tile / p.group : 1;
-  if (q.base >= 0 && length <= p.capacity) {
-    q.a = lead_keys + q.base + (added < tokens ? added : tokens);
-    q.step = q.tiles > 1 ? tokens : 0;
-  } else {
-    q.a = lead_keys + q.own_end + 1;
-    q.step = 0;
-  }
+  const int tokens = rows <= q.tile ? added : q.tile / p.group;
+  const bool whole = q.base >= 0 && length <= p.capacity && tokens > 0;
+  const uint32_t keys =
+      (uint32_t)lead + (uint32_t)(whole ? q.base + tokens : q.own_end);
+  q.a = (keys >> p.unit) + p.tile_units;
+  q.step = whole && q.tiles > 1 ? (uint32_t)tokens >> p.unit : 0;
   return q;
 }
 
@@ -740,7 +787,7 @@ __device__ __forceinline__ Request request(const PagedAttention &p, int b,
 
 template <int DP>
 __global__ __launch_bounds__(kPagedThreads, DP >= 256 ? 1 : 2) void
-attention_paged_kernel(PagedAttention p) {
+attention_paged_kernel(PagedAttention) {
   constexpr int VBYTES = kBlockKeys * DP * 2;
   constexpr int MERGE = kPagedWaves * 16 * (DP + 4) * 4;
   constexpr int WIDE = DP >= 256 ? 0 : 4 * kStepKeys * DP * 2;
@@ -750,95 +797,123 @@ attention_paged_kernel(PagedAttention p) {
   __shared__ __attribute__((aligned(1024))) char smem[SMEM];
   __shared__ float wave_m[kPagedWaves][kNarrowRows],
       wave_l[kPagedWaves][kNarrowRows];
+  // Where each wave is on the line, and the requests' row starts and lengths
+  // where every lane has one: kept here, out of the tiles' registers.
+  __shared__ Line line_at[kPagedWaves];
+  __shared__ int request_of[kPagedWaves][3][64];
 
+  const PagedAttention &p = arguments();
+  // Lane l sums requests l * each .. + each - 1; its first one's row starts
+  // and length stay in registers.
   const int lane = threadIdx.x & 63;
+  const int each = (p.batch + 63) / 64;
+  const int rows_end = row_start(p, p.batch);
+  int begin = 0, end = 0, length = 0;
+  if (lane * each < p.batch) {
+    begin = row_start(p, lane * each);
+    end = row_start(p, lane * each + 1);
+    length = p.lengths[lane * each];
+  }
   // Consecutive stretches of one head's line read the same prefix: one XCD's.
   int item, unused;
   xcd_tile_order((int)blockIdx.x, (int)gridDim.x, (int)gridDim.x, 1, 1, &item,
                  &unused);
   PagedTile t;
   t.kv_head = item / p.ways;
-  const int way = item % p.ways;
+  int way = item % p.ways;
 
   // The line: the prefix's tiles (rows of the whole batch), then the
-  // requests'. Lane l sums requests l * each .. + each - 1.
+  // requests'.
   const int prefix_steps = (p.prefix + kStepKeys - 1) / kStepKeys;
-  const int64_t prefix_keys = (int64_t)prefix_steps * kStepKeys;
-  const int packed = uniform(row_start(p, p.batch)) * p.group;
-  const int shared_tile = tile_rows<DP>(p.packed);
-  const int shared_tiles =
-      p.shared ? (packed + shared_tile - 1) / shared_tile : 0;
-  const int64_t shared_keys = shared_tiles * prefix_keys;
-  const int64_t lead_keys = p.shared ? 0 : prefix_keys;
-  const int each = (p.batch + 63) / 64;
-  int64_t mine = 0;
-  for (int i = 0; i < each; ++i) {
+  const int lead_keys = p.shared ? 0 : prefix_steps * kStepKeys;
+  uint32_t mine = 0;
+  for (int i = 0; i < each && lane * each + i < p.batch; ++i) {
     const int b = lane * each + i;
-    if (b < p.batch) {
-      const Request q = request<DP, false>(p, b, lead_keys);
-      mine += q.before(q.tiles);
-    }
+    const Request q =
+        i == 0 ? request<DP>(p, begin, end, length, lead_keys)
+               : request<DP>(p, row_start(p, b), row_start(p, b + 1),
+                             p.lengths[b], lead_keys);
+    mine += q.before(q.tiles);
   }
-  int64_t upto = mine;
+  uint32_t upto = mine;
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
-    const int64_t x = __shfl_up(upto, d);
+    const uint32_t y = __shfl_up(upto, d);
     if (lane >= d)
-      upto += x;
+      upto += y;
   }
-  const int64_t total = shared_keys + uniform(__shfl(upto, 63));
-  int64_t per = (total + p.ways - 1) / p.ways;
-  per = per < p.least ? p.least : per;
-  int64_t x = way * per;
-  const int64_t x_end = x + per < total ? x + per : total;
-  if (x >= x_end)
+  Request q = {};
+  int packed = uniform(rows_end) * p.group;
+  q.tile = tile_rows<DP>(p.packed);
+  q.tiles = p.shared ? (packed + q.tile - 1) / q.tile : 0;
+  q.a = ((uint32_t)(prefix_steps * kStepKeys) >> p.unit) + p.tile_units;
+  const uint32_t shared_units = q.before(q.tiles);
+  const uint32_t total = shared_units + (uint32_t)uniform((int)__shfl(upto, 63));
+  uint32_t per = (total + (uint32_t)p.ways - 1) / (uint32_t)p.ways;
+  per = per < (uint32_t)p.least ? p.least : per;
+  float inv_per = 1.0f / (float)per;
+  uint32_t x = (uint32_t)way * per;  // below 2^31 + 2^31
+  if (x >= total)
     return;
+  uint32_t x_end = x + per < total ? x + per : total;
+
+  const int wave = uniform((int)threadIdx.x >> 6);
+  request_of[wave][0][lane] = begin;
+  request_of[wave][1][lane] = end;
+  request_of[wave][2][lane] = length;
+  auto request_at = [&](int b) {
+    int of[3];
+    if (p.batch <= 64) {
+#pragma unroll
+      for (int k = 0; k < 3; ++k)
+        of[k] = uniform(request_of[wave][k][b]);
+    } else {
+      of[0] = uniform(row_start(p, b));
+      of[1] = uniform(row_start(p, b + 1));
+      of[2] = uniform(p.lengths[b]);
+    }
+    return request<DP>(p, of[0], of[1], of[2], p.shared ? 0 : prefix_steps * kStepKeys);
+  };
 
   // Where the stretch begins: among the prefix's tiles, or in the request that
   // holds it: the last lane whose requests start at or before it, then that
   // lane's one after the other; its tile by bisection.
-  bool lead = x < shared_keys;
   int b = -1, i = 0;
-  int64_t start = 0;  // where the tiles of b (or of the prefix) start
-  Request q = {};
-  q.tiles = shared_tiles;
-  q.tile = shared_tile;
-  q.a = prefix_keys;
-  if (lead) {
-    i = uniform((int)(x / prefix_keys));
-  } else {
-    const int64_t y = x - shared_keys;
-    const int lane_of =
-        uniform(63 - __builtin_clzll(__ballot(upto - mine <= y) | 1));
-    start = shared_keys + uniform(__shfl(upto - mine, lane_of));
+  uint32_t start = 0;  // where the tiles of b (or of the prefix) start
+  if (x >= shared_units) {
+    const int lane_of = uniform(
+        63 - __builtin_clzll(
+                 __ballot(shared_units + upto - mine <= x) | 1));
+    start = shared_units + (uint32_t)uniform((int)__shfl(upto - mine, lane_of));
     b = lane_of * each;
-    q = request<DP>(p, b, lead_keys);
+    q = request_at(b);
     while (start + q.before(q.tiles) <= x && b + 1 < p.batch) {
       start += q.before(q.tiles);
-      q = request<DP>(p, ++b, lead_keys);
+      q = request_at(++b);
     }
-    for (int span = q.tiles; span > 1;) {
-      const int half = span / 2;
-      const bool past = start + q.before(i + half) <= x;
-      i += past ? half : 0;
-      span = past ? span - half : half;
-    }
+  }
+  for (int span = q.tiles; span > 1;) {
+    const int half = span / 2;
+    const bool past = start + q.before(i + half) <= x;
+    i += past ? half : 0;
+    span = past ? span - half : half;
   }
 
   while (x < x_end) {
+    const PagedAttention &p = arguments();
     if (i >= q.tiles) {  // on to the next request
       start += q.before(q.tiles);
-      lead = false;
       if (++b >= p.batch)
         return;
-      q = request<DP>(p, b, lead_keys);
+      q = request_at(b);
       i = 0;
       continue;
     }
-    // Keys from .. to - 1 of the `keys` that the tile has on the line.
-    const int64_t at = start + q.before(i), keys = q.a + q.step * i;
-    const int64_t from = x - at;
-    int64_t to = x_end - at < keys ? x_end - at : keys;
+    // Units from .. to - 1 of the `units` that the tile has on the line.
+    const bool lead = b < 0;
+    const uint32_t at = start + q.before(i), units = q.a + q.step * i;
+    const uint32_t from = x - at;
+    uint32_t to = x_end - at < units ? x_end - at : units;
     x = at + to;
     t.r0 = q.begin * p.group + i * q.tile;
     t.r_end = lead ? packed : q.end * p.group;
@@ -851,21 +926,28 @@ attention_paged_kernel(PagedAttention p) {
     t.seen = lead ? 0 : uniform(sees(p, t, t.r_end - 1));
     const int steps = t.lead + (t.seen + kStepKeys - 1) / kStepKeys;
     ++i;
-    int64_t first = 0;
-    int count = 1;
+    int first = 0, count = 1;
     if (p.partials) {
-      first = at / per;
-      count = (int)((at + keys - 1) / per - first) + 1;
+      // quotients that the float is off by one of at most
+      auto way_of = [&](uint32_t u) {
+        int w = (int)((float)u * inv_per);
+        w -= (uint64_t)w * per > u;
+        return w + ((uint64_t)(w + 1) * per <= u);
+      };
+      first = uniform(way_of(at));
+      count = uniform(way_of(at + units - 1)) - first + 1;
     } else {
       // without a workspace a workgroup takes the tiles that start in its
       // stretch, whole
       if (from > 0)
         continue;
-      to = keys;
+      to = units;
     }
-    auto step_at = [&](int64_t key) {
-      const int64_t s = (key + kStepKeys - 1) / kStepKeys;
-      return key >= keys || s > steps ? steps : (int)s;
+    // A tile's own units come first, before its keys.
+    auto step_at = [&](uint32_t u) {
+      const uint32_t n = u > (uint32_t)p.tile_units ? u - p.tile_units : 0;
+      const uint64_t s = (((uint64_t)n << p.unit) + kStepKeys - 1) / kStepKeys;
+      return u >= units || s > (uint64_t)steps ? steps : (int)s;
     };
     t.s_begin = step_at(from);
     t.s_end = step_at(to);
@@ -874,32 +956,55 @@ attention_paged_kernel(PagedAttention p) {
     t.part = whole ? -1 : line + (int64_t)kWideRows * way;
     if (p.partials && from == 0 && t.kv_head == 0)
       for (int r = t.r0 + (int)threadIdx.x; r < t.r_end; r += kPagedThreads)
-        p.part_of[line + r] = i32x2{(int)first, whole ? 0 : count};
-    if (q.tile == kNarrowRows)
-      narrow_tile<DP>(p, t, smem, wave_m, wave_l);
+        p.part_of[line + r] = i32x2{first, whole ? 0 : count};
+    const int tile = q.tile;
+    line_at[wave] = {x, x_end, start, per, inv_per, packed, t.kv_head, way,
+                     b, i, q};
+    if (tile == kNarrowRows)
+      narrow_tile<DP>(t, smem, wave_m, wave_l);
     else if constexpr (DP < 256)
-      wide_tile<DP>(p, t, smem);
+      wide_tile<DP>(t, smem);
+    asm volatile("" ::: "memory");
+    const Line &l = line_at[wave];
+    x = (uint32_t)uniform((int)l.x);
+    x_end = (uint32_t)uniform((int)l.x_end);
+    start = (uint32_t)uniform((int)l.start);
+    per = (uint32_t)uniform((int)l.per);
+    inv_per = __builtin_bit_cast(float, uniform(__builtin_bit_cast(int, l.inv_per)));
+    packed = uniform(l.packed);
+    t.kv_head = uniform(l.kv_head);
+    way = uniform(l.way);
+    b = uniform(l.b);
+    i = uniform(l.i);
+    q.begin = uniform(l.q.begin);
+    q.end = uniform(l.q.end);
+    q.tile = uniform(l.q.tile);
+    q.tiles = uniform(l.q.tiles);
+    q.own_end = uniform(l.q.own_end);
+    q.base = uniform(l.q.base);
+    q.a = (uint32_t)uniform((int)l.q.a);
+    q.step = (uint32_t)uniform((int)l.q.step);
   }
 }
 
-// Joins the parts of every row that has some: DP / 4 threads a row, 4 columns
-// each. A row's parts of one kind (the prefix's and its own, or both at once)
-// are kWideRows rows apart, part_of telling the first and how many.
-template <int DP>
+// Joins the parts of every row that has some: DP / 4 threads, 4 columns each,
+// for every GROUPS-th four of a row's parts, then the GROUPS sums through LDS.
+// A row's parts of one kind (the prefix's and its own, or both at once) are
+// kWideRows rows apart, part_of telling the first and how many.
+template <int DP, int GROUPS>
 __global__ __launch_bounds__(kPagedThreads) void attention_paged_join_kernel(
     PagedAttention p) {
-  constexpr int TPR = DP / 4;
-  const int64_t at = (int64_t)blockIdx.x * (kPagedThreads / TPR) +
-                     threadIdx.x / TPR;
-  const int dq = 4 * ((int)threadIdx.x % TPR);
+  constexpr int TPR = DP / 4, ROWS = kPagedThreads / TPR / GROUPS;
+  const int tid = threadIdx.x;
+  const int g = tid / TPR % GROUPS, dq = 4 * (tid % TPR);
+  const int64_t at = (int64_t)blockIdx.x * ROWS + tid / (TPR * GROUPS);
   const int kv_head = (int)(at / p.packed), row = (int)(at % p.packed);
-  if (kv_head >= p.kv_heads || row >= row_start(p, p.batch) * p.group ||
-      dq >= p.dv)
-    return;
+  const bool real =
+      kv_head < p.kv_heads && row < row_start(p, p.batch) * p.group;
   float top = kNegInf, sum = 0.0f;
   f32x4 acc = {0, 0, 0, 0};
   int parts = 0;
-  for (int kind = 0; kind <= p.shared; ++kind) {
+  for (int kind = 0; real && kind <= p.shared; ++kind) {
     const int64_t line = kind * p.packed + row;
     const i32x2 of = p.part_of[line];
     // within the workgroups of the line, whatever it holds
@@ -908,7 +1013,7 @@ __global__ __launch_bounds__(kPagedThreads) void attention_paged_join_kernel(
     const int64_t at0 = (int64_t)kv_head * p.part_rows + line +
                         (int64_t)kWideRows * first;
     // 4 parts' loads in flight; a part past the last repeats it with weight 0
-    for (int s0 = 0; s0 < count; s0 += 4) {
+    for (int s0 = 4 * g; s0 < count; s0 += 4 * GROUPS) {
       f32x2 ml[4];
       f32x4 v[4];
 #pragma unroll
@@ -939,8 +1044,31 @@ __global__ __launch_bounds__(kPagedThreads) void attention_paged_join_kernel(
     }
     parts += count > 0 ? count : 0;
   }
-  if (parts == 0)
-    return;  // stored by the workgroup that had the tile whole
+  if constexpr (GROUPS > 1) {
+    __shared__ f32x4 group_acc[kPagedThreads];
+    __shared__ f32x2 group_ml[kPagedThreads];
+    group_acc[tid] = acc;
+    group_ml[tid] = f32x2{top, sum};
+    __syncthreads();
+    if (g > 0)
+      return;
+#pragma unroll
+    for (int u = 1; u < GROUPS; ++u)
+      top = fmaxf(top, group_ml[tid + u * TPR][0]);
+    sum = 0.0f;
+    acc = f32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int u = 0; u < GROUPS; ++u) {
+      const f32x2 ml = group_ml[tid + u * TPR];
+      const float f =
+          ml[0] == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(ml[0] - top);
+      sum += f * ml[1];
+      acc += f * group_acc[tid + u * TPR];
+    }
+  }
+  // Without parts the workgroup that had the tile whole stored the row.
+  if (!real || parts == 0 || dq >= p.dv)
+    return;
   const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
   *(f16x4 *)(result_row(p, kv_head, row) + dq) =
       f16x4{(f16)(acc[0] * inv), (f16)(acc[1] * inv), (f16)(acc[2] * inv),
@@ -955,21 +1083,25 @@ namespace {
 
 struct PagedKernel {
   const char *name;
-  int dp;
+  int dp, groups;  // groups: of a joined row's parts
   const void *fn;
 };
 const PagedKernel kPagedKernels[] = {
-    {"attention_paged_d64", 64, (const void *)&attention_paged_kernel<64>},
-    {"attention_paged_d128", 128, (const void *)&attention_paged_kernel<128>},
-    {"attention_paged_d256", 256, (const void *)&attention_paged_kernel<256>},
-};
-const PagedKernel kJoinKernels[] = {
-    {"attention_paged_join_d64", 64,
-     (const void *)&attention_paged_join_kernel<64>},
-    {"attention_paged_join_d128", 128,
-     (const void *)&attention_paged_join_kernel<128>},
-    {"attention_paged_join_d256", 256,
-     (const void *)&attention_paged_join_kernel<256>},
+    {"attention_paged_d64", 64, 0, (const void *)&attention_paged_kernel<64>},
+    {"attention_paged_d128", 128, 0,
+     (const void *)&attention_paged_kernel<128>},
+    {"attention_paged_d256", 256, 0,
+     (const void *)&attention_paged_kernel<256>},
+#define IHP_JOIN(DP, GROUPS)                                                   \
+  {"attention_paged_join_d" #DP "_g" #GROUPS, DP, GROUPS,                      \
+   (const void *)&attention_paged_join_kernel<DP, GROUPS>}
+    IHP_JOIN(64, 1),
+    IHP_JOIN(64, 8),
+    IHP_JOIN(128, 1),
+    IHP_JOIN(128, 8),
+    IHP_JOIN(256, 1),
+    IHP_JOIN(256, 4),
+#undef IHP_JOIN
 };
 constexpr int kPagedKernelCount =
     sizeof(kPagedKernels) / sizeof(kPagedKernels[0]);
@@ -988,7 +1120,16 @@ PagedPlan plan_attention_paged(int64_t rows, int64_t batch, int64_t kv_heads,
   p.shared = prefix > 0 && batch > 1 && packed < kWideRows * batch;
   const int64_t wgs = p.dp < 256 ? kPagedTargetWgs : kPagedTargetWgs / 2;
   p.ways = wgs / kv_heads > 1 ? wgs / kv_heads : 1;
-  p.least = kPagedLeastKeys;
+  // The line in 32 bits, also where row_starts do not ascend and every request
+  // has all rows.
+  const int64_t each = packed / (p.dp < 256 ? kWideRows : kNarrowRows) + 2;
+  const double line = (double)(batch * each + packed) *
+                      (double)(prefix + capacity + rows + 512);
+  while (line / (double)((int64_t)1 << p.unit) >= 1e9)
+    ++p.unit;
+  auto units = [&](int64_t keys) { return (keys >> p.unit) + 1; };
+  p.least = units(kPagedLeastKeys + kPagedTileKeys);
+  p.tile_units = units(kPagedTileKeys);
   p.part_rows = 2 * packed + kWideRows * p.ways;
   p.workspace = (int64_t)kWorkspaceCounterBytes + 2 * packed * 8 +
                 kv_heads * p.part_rows * (p.dp + 2) * 4;
@@ -998,7 +1139,6 @@ PagedPlan plan_attention_paged(int64_t rows, int64_t batch, int64_t kv_heads,
     p.workspace = p.part_rows = 0;
     p.ways = batch + packed / 16;
     p.ways = p.ways < 2 * wgs / kv_heads + 1 ? p.ways : 2 * wgs / kv_heads + 1;
-    p.least = 1;
   }
   return p;
 }
@@ -1009,6 +1149,8 @@ hipError_t launch_attention_paged(const PagedAttention &attention,
   PagedAttention a = attention;
   a.ways = (int)plan.ways;
   a.least = (int)plan.least;
+  a.unit = (int)plan.unit;
+  a.tile_units = (int)plan.tile_units;
   a.shared = plan.shared ? 1 : 0;
   a.part_rows = plan.part_rows;
   a.part_of = nullptr;
@@ -1019,37 +1161,38 @@ hipError_t launch_attention_paged(const PagedAttention &attention,
     a.part_ml = a.partials + a.kv_heads * plan.part_rows * plan.dp;
     a.part_of = (i32x2 *)(a.part_ml + a.kv_heads * plan.part_rows * 2);
   }
-  const void *kernel = nullptr, *join = nullptr;
-  for (int i = 0; i < kPagedKernelCount; ++i)
-    if (kPagedKernels[i].dp == plan.dp) {
-      kernel = kPagedKernels[i].fn;
-      join = kJoinKernels[i].fn;
+  // Few rows, whose parts can be many: a row's are dealt to groups.
+  const bool few = all <= kPagedFewRows;
+  const PagedKernel *kernel = nullptr, *join = nullptr;
+  for (const PagedKernel &k : kPagedKernels)
+    if (k.dp == plan.dp) {
+      if (k.groups == 0)
+        kernel = &k;
+      else if ((k.groups > 1) == few)
+        join = &k;
     }
-  if (!kernel)
+  if (!kernel || !join)
     return hipErrorInvalidValue;
   void *args[] = {&a};
   hipError_t e =
-      hipLaunchKernel(kernel, dim3((unsigned)(plan.ways * a.kv_heads)),
+      hipLaunchKernel(kernel->fn, dim3((unsigned)(plan.ways * a.kv_heads)),
                       dim3(kPagedThreads), args, 0, (hipStream_t)stream);
   if (e != hipSuccess || !plan.workspace)
     return e;
-  const int per = kPagedThreads / (plan.dp / 4);
-  return hipLaunchKernel(join, dim3((unsigned)((all + per - 1) / per)),
+  const int per = kPagedThreads / (plan.dp / 4) / join->groups;
+  return hipLaunchKernel(join->fn, dim3((unsigned)((all + per - 1) / per)),
                          dim3(kPagedThreads), args, 0, (hipStream_t)stream);
 }
 
 const KernelEntry *attention_paged_kernels(int *count) {
-  static KernelEntry all[2 * kPagedKernelCount];
+  static KernelEntry all[kPagedKernelCount];
   static const bool filled = [] {
-    for (int i = 0; i < kPagedKernelCount; ++i) {
+    for (int i = 0; i < kPagedKernelCount; ++i)
       all[i] = {kPagedKernels[i].name, kPagedKernels[i].fn, kPagedThreads, 0};
-      all[kPagedKernelCount + i] = {kJoinKernels[i].name, kJoinKernels[i].fn,
-                                    kPagedThreads, 0};
-    }
     return true;
   }();
   (void)filled;
-  *count = 2 * kPagedKernelCount;
+  *count = kPagedKernelCount;
   return all;
 }
 

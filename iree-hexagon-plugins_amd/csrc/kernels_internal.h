@@ -387,9 +387,10 @@ struct PagedAttention {
   int batch, rows, kv_heads, group, dqk, dv;
   int prefix, capacity;       // prefix keys, keys that a table row can name
   float scale;
-  // Workgroups that share a KV head's tiles, the keys that one takes at
-  // least, and whether the prefix has tiles of its own.
-  int ways, least, shared;
+  // Workgroups that share a KV head's tiles, the units of 2^unit keys that one
+  // takes at least, the units that a tile counts for besides its keys, and
+  // whether the prefix has tiles of its own.
+  int ways, least, unit, tile_units, shared;
   // Parts (no workspace: null): a row's f32 part of workgroup w at row
   // line + 128 w of its KV head's part_rows, line = its row, plus `packed`
   // for its own keys where the prefix has tiles of its own; their (max, sum);
@@ -401,14 +402,17 @@ struct PagedAttention {
   float *partials, *part_ml;
   int __attribute__((ext_vector_type(2))) *part_of;
 };
-// Workgroups wanted (two a CU where head dims allow it), and the keys that
-// one takes at least.
+// Workgroups wanted (two a CU where head dims allow it), the keys that one
+// takes at least, and the keys that a tile's start and end cost as much as.
 constexpr int64_t kPagedTargetWgs = 512;
 constexpr int64_t kPagedLeastKeys = 128;
+constexpr int64_t kPagedTileKeys = 256;
+// Rows (of all heads) up to which a row's parts are joined by several groups.
+constexpr int64_t kPagedFewRows = 8192;
 struct PagedPlan {
   int dp;  // head-dim bucket
   bool shared;
-  int64_t ways, least, part_rows, workspace;
+  int64_t ways, least, unit, tile_units, part_rows, workspace;
 };
 PagedPlan plan_attention_paged(int64_t rows, int64_t batch, int64_t kv_heads,
                                int64_t group, int64_t prefix, int64_t capacity,
