@@ -1210,44 +1210,60 @@ _PAGED_ATTENTION = struct.Struct("@2P11q6P10qfI")
 def _ints(t, name, dims=1):
     """A device table: int32, its rows contiguous."""
     import torch
-    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32:
+    if not isinstance(t, torch.Tensor) or t.dtype is not torch.int32:
         raise TypeError(f"{name} must be an int32 tensor")
-    if t.dim() != dims or not (_unit_col(t) or t.numel() == 0):
+    if t.dim() != dims or (t.stride(-1) != 1 and t.shape[-1] != 1
+                           and t.numel()):
         raise ValueError(f"{name} must be {dims}-D with unit column stride")
 
 
-def _cache_fields(k_cache, v_cache):
-    """(the fields of iree_mi355x_kv_cache_t after its pointers, the caches
-    checked)."""
+def _rows_of(t, name, dims):
+    """Shape of f16 rows, the head dim contiguous."""
     import torch
-    for t, nm in ((k_cache, "k_cache"), (v_cache, "v_cache")):
-        if (not isinstance(t, torch.Tensor) or t.dtype != torch.float16
-                or t.dim() != 4 or not _unit_col(t)):
-            raise TypeError(f"{nm} must be a 4-D f16 tensor with unit "
-                            "stride along head_dim")
-    pages, heads, page, d = k_cache.shape
-    dv = v_cache.shape[3]
-    _shape(v_cache, (pages, heads, page, dv), "v_cache")
+    if (not isinstance(t, torch.Tensor) or t.dtype is not torch.float16
+            or t.dim() != dims or (t.stride(-1) != 1 and t.shape[-1] != 1)):
+        raise TypeError(f"{name} must be a {dims}-D f16 tensor with unit "
+                        "stride along head_dim")
+    return t.shape
+
+
+def _cache_fields(k_cache, v_cache):
+    """The fields of iree_mi355x_kv_cache_t after its pointers, of checked
+    caches."""
+    pages, heads, page, d = _rows_of(k_cache, "k_cache", 4)
+    *rest, dv = _rows_of(v_cache, "v_cache", 4)
+    if rest != [pages, heads, page]:
+        _shape(v_cache, (pages, heads, page, dv), "v_cache")
     return (pages, page, heads, d, dv, *k_cache.stride()[:3],
             *v_cache.stride()[:3])
 
 
-def _rows_of(t, name):
-    import torch
-    if (not isinstance(t, torch.Tensor) or t.dtype != torch.float16
-            or t.dim() != 3 or not _unit_col(t)):
-        raise TypeError(f"{name} must be a 3-D f16 tensor with unit stride "
-                        "along head_dim")
+def _one_device(first, name, *named):
+    """_on_device, and the index of the device; nothing is looked up where all
+    is well."""
+    index = first.get_device()
+    for t, _ in named:
+        if t is not None and (t.get_device() != index or index < 0):
+            _on_device((first, name), *named)
+    return index
 
 
-def _run_on(index, stream, call):
-    """call(raw stream) with device `index` current: the current stream of
-    that device unless one is given."""
+def _stream_on(index, stream):
+    """The raw stream of a call on device `index`, which the caller made
+    current (None: its current one)."""
+    if stream is None:
+        import torch
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        if raw is not None:
+            return raw(index)
+    return _stream_ptr(stream)
+
+
+def _other_device(index) -> bool:
+    """Whether device `index` is not the current one: the call is then made
+    again with it current, on its current stream unless one is given."""
     import torch
-    if index == torch.cuda.current_device():
-        return call(_stream_ptr(stream))
-    with torch.cuda.device(index):
-        return call(_stream_ptr(stream))
+    return index != torch.cuda.current_device()
 
 
 def page_tables(cached, added, free_pages, block_table, page_size, rows, *,
@@ -1261,37 +1277,40 @@ def page_tables(cached, added, free_pages, block_table, page_size, rows, *,
     row's page * page_size + place (-1: none, or a row past the last), and
     how many pages were taken (more than F: the list was too short, and the
     pages past it are -1). All tables are int32."""
-    import torch
-    for t, nm in ((cached, "cached"), (added, "added"),
-                  (free_pages, "free_pages")):
-        _ints(t, nm)
+    _ints(cached, "cached")
+    _ints(added, "added")
+    _ints(free_pages, "free_pages")
     _ints(block_table, "block_table", 2)
     batch = cached.shape[0]
-    _shape(added, (batch,), "added")
-    width = block_table.shape[1]
-    _shape(block_table, (batch, width), "block_table")
+    if added.shape[0] != batch:
+        _shape(added, (batch,), "added")
+    have, width = block_table.shape
+    if have != batch:
+        _shape(block_table, (batch, width), "block_table")
     if page_size < 1 or rows < 0:
         raise ValueError(f"page_size {page_size} and rows {rows} must be at "
                          "least 1 and 0")
-    _on_device((cached, "cached"), (added, "added"),
-               (free_pages, "free_pages"), (block_table, "block_table"))
-    lib = library()
-
-    def call(s):
-        out = torch.empty(2 * batch + 2 + rows, dtype=torch.int32,
-                          device=cached.device)
-        starts, lengths, needed, slots = out.split(
-            (batch + 1, batch, 1, rows))
-        at = out.data_ptr()
-        _check(lib.iree_mi355x_page_tables(_PAGE_TABLES.pack(
-            cached.data_ptr(), added.data_ptr(), free_pages.data_ptr(),
-            block_table.data_ptr(), at, at + 4 * (batch + 1),
-            at + 4 * (2 * batch + 2), at + 4 * (2 * batch + 1), batch,
-            free_pages.shape[0], page_size, width, block_table.stride(0),
-            rows), s))
-        return starts, lengths, slots, needed
-
-    return _run_on(cached.get_device(), stream, call)
+    index = _one_device(cached, "cached", (added, "added"),
+                        (free_pages, "free_pages"),
+                        (block_table, "block_table"))
+    if _other_device(index):
+        import torch
+        with torch.cuda.device(index):
+            return page_tables(cached, added, free_pages, block_table,
+                               page_size, rows, stream=stream)
+    out = cached.new_empty(2 * batch + 2 + rows)
+    at = out.data_ptr()
+    starts, lengths, needed, slots = out.split_with_sizes(
+        (batch + 1, batch, 1, rows))
+    st = library().iree_mi355x_page_tables(_PAGE_TABLES.pack(
+        cached.data_ptr(), added.data_ptr(), free_pages.data_ptr(),
+        block_table.data_ptr(), at, at + 4 * (batch + 1),
+        at + 4 * (2 * batch + 2), at + 4 * (2 * batch + 1), batch,
+        free_pages.shape[0], page_size, width, block_table.stride(0), rows),
+        _stream_on(index, stream))
+    if st != OK:
+        _check(st)
+    return starts, lengths, slots, needed
 
 
 def append_kv(k, v, k_cache, v_cache, slots, *, stream=None):
@@ -1302,22 +1321,28 @@ def append_kv(k, v, k_cache, v_cache, slots, *, stream=None):
     must not name one slot. A cache in [page, token, head] order is passed as
     a permuted view."""
     fields = _cache_fields(k_cache, v_cache)
-    _rows_of(k, "k")
-    _rows_of(v, "v")
-    rows = k.shape[0]
-    _shape(k, (rows, fields[2], fields[3]), "k")
-    _shape(v, (rows, fields[2], fields[4]), "v")
+    _, _, heads, d, dv = fields[:5]
+    rows, *of_k = _rows_of(k, "k", 3)
+    if of_k != [heads, d]:
+        _shape(k, (rows, heads, d), "k")
+    if tuple(_rows_of(v, "v", 3)) != (rows, heads, dv):
+        _shape(v, (rows, heads, dv), "v")
     _ints(slots, "slots")
-    _shape(slots, (rows,), "slots")
-    _on_device((k, "k"), (v, "v"), (k_cache, "k_cache"),
-               (v_cache, "v_cache"), (slots, "slots"))
-    lib = library()
-    cache = _KV_CACHE.pack(k_cache.data_ptr(), v_cache.data_ptr(), *fields)
-    _run_on(k.get_device(), stream, lambda s: _check(
-        lib.iree_mi355x_append_kv_f16(
-            cache, k.data_ptr(), v.data_ptr(), rows,
-            _PAIR.pack(*k.stride()[:2]), _PAIR.pack(*v.stride()[:2]),
-            slots.data_ptr(), s)))
+    if slots.shape[0] != rows:
+        _shape(slots, (rows,), "slots")
+    index = _one_device(k, "k", (v, "v"), (k_cache, "k_cache"),
+                        (v_cache, "v_cache"), (slots, "slots"))
+    if _other_device(index):
+        import torch
+        with torch.cuda.device(index):
+            return append_kv(k, v, k_cache, v_cache, slots, stream=stream)
+    st = library().iree_mi355x_append_kv_f16(
+        _KV_CACHE.pack(k_cache.data_ptr(), v_cache.data_ptr(), *fields),
+        k.data_ptr(), v.data_ptr(), rows, _PAIR.pack(*k.stride()[:2]),
+        _PAIR.pack(*v.stride()[:2]), slots.data_ptr(),
+        _stream_on(index, stream))
+    if st != OK:
+        _check(st)
 
 
 @functools.lru_cache(maxsize=4096)
@@ -1344,24 +1369,25 @@ def shared_prefix_attention(q, k_cache, v_cache, row_starts, lengths,
     and v_cache [P, Hkv, S, Dv] as in append_kv; o [T, H, Dv] f16 keeps the
     rows past row_starts[B]. Tables are int32, from page_tables. With
     prefix_length 0 this is paged attention."""
-    import torch
     fields = _cache_fields(k_cache, v_cache)
     _, page, hkv, d, dv = fields[:5]
-    _rows_of(q, "q")
-    rows, h = q.shape[:2]
-    _shape(q, (rows, h, d), "q")
+    rows, h, of_q = _rows_of(q, "q", 3)
+    if of_q != d:
+        _shape(q, (rows, h, d), "q")
     if hkv < 1 or h % hkv:
         raise ValueError(f"{h} query heads are not a multiple of {hkv} KV "
                          "heads")
-    if o is not None:
-        _rows_of(o, "o")
+    if o is not None and tuple(_rows_of(o, "o", 3)) != (rows, h, dv):
         _shape(o, (rows, h, dv), "o")
     _ints(lengths, "lengths")
     _ints(row_starts, "row_starts")
     _ints(block_table, "block_table", 2)
-    batch, width = lengths.shape[0], block_table.shape[1]
-    _shape(row_starts, (batch + 1,), "row_starts")
-    _shape(block_table, (batch, width), "block_table")
+    batch = lengths.shape[0]
+    if row_starts.shape[0] != batch + 1:
+        _shape(row_starts, (batch + 1,), "row_starts")
+    have, width = block_table.shape
+    if have != batch:
+        _shape(block_table, (batch, width), "block_table")
     if prefix_length < 0:
         raise ValueError(f"prefix_length {prefix_length} is negative")
     if prefix_length:
@@ -1374,39 +1400,42 @@ def shared_prefix_attention(q, k_cache, v_cache, row_starts, lengths,
                              "tokens")
     else:
         prefix_pages = None
-    _on_device((q, "q"), (k_cache, "k_cache"), (v_cache, "v_cache"),
-               (row_starts, "row_starts"), (lengths, "lengths"),
-               (block_table, "block_table"), (prefix_pages, "prefix_pages"),
-               (o, "o"))
-    lib = library()
-    if scale is None:
-        scale = d ** -0.5
-    index = q.get_device()
-
-    def call(s):
-        out = torch.empty(rows, h, dv, dtype=torch.float16,
-                          device=q.device) if o is None else o
-        args = _PAGED_ATTENTION.pack(
-            k_cache.data_ptr(), v_cache.data_ptr(), *fields, q.data_ptr(),
-            out.data_ptr(), row_starts.data_ptr(), lengths.data_ptr(),
-            block_table.data_ptr(),
-            0 if prefix_pages is None else prefix_pages.data_ptr(), rows, h,
-            batch, width, block_table.stride(0), prefix_length,
-            *q.stride()[:2], *out.stride()[:2], scale, 0)
-        need = _paged_workspace_need(rows, batch, h, hkv, d, dv, page, width,
-                                     prefix_length)
-        ws = wsb = held = None
-        if need > 0 and s and _capturing(s):
-            # the graph's own: its replays share it with no other's
+    index = _one_device(q, "q", (k_cache, "k_cache"), (v_cache, "v_cache"),
+                        (row_starts, "row_starts"), (lengths, "lengths"),
+                        (block_table, "block_table"),
+                        (prefix_pages, "prefix_pages"), (o, "o"))
+    if _other_device(index):
+        import torch
+        with torch.cuda.device(index):
+            return shared_prefix_attention(
+                q, k_cache, v_cache, row_starts, lengths, block_table,
+                prefix_pages, prefix_length, o, scale=scale, stream=stream)
+    if o is None:
+        o = q.new_empty((rows, h, dv))
+    qs, os_ = q.stride(), o.stride()
+    args = _PAGED_ATTENTION.pack(
+        k_cache.data_ptr(), v_cache.data_ptr(), *fields, q.data_ptr(),
+        o.data_ptr(), row_starts.data_ptr(), lengths.data_ptr(),
+        block_table.data_ptr(),
+        0 if prefix_pages is None else prefix_pages.data_ptr(), rows, h,
+        batch, width, block_table.stride(0), prefix_length, qs[0], qs[1],
+        os_[0], os_[1], d ** -0.5 if scale is None else scale, 0)
+    s = _stream_on(index, stream)
+    need = _paged_workspace_need(rows, batch, h, hkv, d, dv, page, width,
+                                 prefix_length)
+    ws, wsb = None, 0
+    if need > 0:
+        if s and _capturing(s):
+            # the graph's own: no other graph's replays share it
+            import torch
             held = torch.empty(need, dtype=torch.uint8, device=q.device)
             ws, wsb = held.data_ptr(), need
-        elif need > 0:
+        else:
             ws, wsb = _call_workspace(need, index, s)
-        _check(lib.iree_mi355x_shared_prefix_attention_f16(
-            args, ws, wsb or 0, s))
-        return out
-
-    return _run_on(index, stream, call)
+    st = library().iree_mi355x_shared_prefix_attention_f16(args, ws, wsb, s)
+    if st != OK:
+        _check(st)
+    return o
 
 
 def matmul_mfma_config(index, a, b, c, *, scale=None, splits=0, accumulate=False,

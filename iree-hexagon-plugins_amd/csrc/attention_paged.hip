@@ -1133,12 +1133,16 @@ PagedPlan plan_attention_paged(int64_t rows, int64_t batch, int64_t kv_heads,
   p.part_rows = 2 * packed + kWideRows * p.ways;
   p.workspace = (int64_t)kWorkspaceCounterBytes + 2 * packed * 8 +
                 kv_heads * p.part_rows * (p.dp + 2) * 4;
-  if ((uint64_t)p.workspace > workspace_limit) {
-    // every tile whole, one workgroup each at the most
+  if (prefix + capacity <= kPagedWholeKeys ||
+      (uint64_t)p.workspace > workspace_limit) {
+    // every tile whole, at most one a workgroup as far as they go: a stretch
+    // is no longer than the shortest tile's units
     p.shared = false;
     p.workspace = p.part_rows = 0;
-    p.ways = batch + packed / 16;
-    p.ways = p.ways < 2 * wgs / kv_heads + 1 ? p.ways : 2 * wgs / kv_heads + 1;
+    p.least = p.tile_units;
+    const int64_t tiles =
+        batch + packed / (p.dp < 256 ? kWideRows : kNarrowRows);
+    p.ways = 4 * p.ways < 3 * tiles + 1 ? 4 * p.ways : 3 * tiles + 1;
   }
   return p;
 }

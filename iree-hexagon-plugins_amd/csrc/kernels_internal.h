@@ -407,6 +407,8 @@ struct PagedAttention {
 constexpr int64_t kPagedTargetWgs = 512;
 constexpr int64_t kPagedLeastKeys = 128;
 constexpr int64_t kPagedTileKeys = 256;
+// Keys up to which a tile is not split: its parts would take longer to join.
+constexpr int64_t kPagedWholeKeys = 512;
 // Rows (of all heads) up to which a row's parts are joined by several groups.
 constexpr int64_t kPagedFewRows = 8192;
 struct PagedPlan {

@@ -215,7 +215,7 @@ def test_attention_argument_errors(pkg):
         assert attend(pkg, **kw) == pkg.MISALIGNED, kw
     for kw in (dict(rows=1 << 30), dict(batch=1 << 31),
                dict(prefix_length=1 << 30), dict(heads=1 << 17),
-               dict(rows=1 << 27, ws=FAKE, wsb=1 << 62)):
+               dict(rows=1 << 27, prefix_length=9999, ws=FAKE, wsb=1 << 62)):
         assert attend(pkg, **kw) == pkg.UNSUPPORTED, kw
     # nothing to do
     for kw in (dict(rows=0), dict(heads=0), dict(batch=0)):
@@ -233,9 +233,12 @@ def test_attention_workspace(pkg):
 
     # f32 rows of the head-dim bucket, their (max, sum), and where they are
     rows = 2 * 6 * 8 + 512 * 128
-    assert need() == (256 << 10) + rows * (64 + 2) * 4 + 2 * 6 * 4 * 8
-    assert need(prefix_length=8192) == need(table_width=99) == need()
-    assert need(rows=5000) > need() + 2 * 8 * 4994 * 66 * 4
+    full = (256 << 10) + rows * (64 + 2) * 4 + 2 * 6 * 4 * 8
+    assert need(prefix_length=8192) == need(table_width=99) == full
+    assert need(rows=5000, prefix_length=8192) > full + 2 * 8 * 4994 * 66 * 4
+    # up to 512 keys no row has parts
+    assert need() == need(prefix_length=512 - 32) == 0
+    assert need(prefix_length=513 - 32) == full
     for kw in (dict(rows=0), dict(heads=7), dict(batch=0), dict(rows=1 << 40),
                dict(prefix_length=-1)):
         assert need(**kw) == 0
