@@ -54,6 +54,14 @@ __device__ __forceinline__ int uniform(int x) {
   return __builtin_amdgcn_readfirstlane(x);
 }
 
+// A value kept in a scalar register: the compiler would read an argument again
+// at its uses in a loop, and wait for it among the LDS reads.
+template <typename T>
+__device__ __forceinline__ T held(T x) {
+  asm volatile("" : "+s"(x));
+  return x;
+}
+
 // The kernel's arguments, read where they are used: held in registers from the
 // kernel's start they pushed the tiles' own out of theirs.
 __device__ __forceinline__ const PagedAttention &arguments() {
@@ -68,10 +76,30 @@ __device__ __forceinline__ int row_start(const PagedAttention &p, int b) {
   return r < 0 ? 0 : r > p.rows ? p.rows : r;
 }
 
-// One tile's work: rows r0 .. r_end - 1 (of a KV head) against steps
-// s_begin .. s_end - 1 of 64 keys, the first `lead` of them the prefix's.
+// The token of a packed row: r / group, of rows below 2^30.
+__device__ __forceinline__ int token_of(const PagedAttention &p, int r) {
+  return p.group == 1 ? r
+                      : (int)(__umulhi((uint32_t)r, p.group_magic) >>
+                              p.group_shift);
+}
+
+// What the workgroup knows of the requests, in LDS: of lane l's `each`
+// requests the first one's row starts and length, and the rows of small
+// requests before them.
+struct Requests {
+  int of[3][64];
+  int small[64];
+};
+
+// Requests of up to 16 rows share tiles of the prefix.
+constexpr int kSmallRows = kNarrowRows;
+
+// One tile's work: rows r0 .. r_end - 1 (of a KV head; `compact`: the small
+// requests' rows alone) against steps s_begin .. s_end - 1 of 64 keys, the
+// first `lead` of them the prefix's.
 struct PagedTile {
   int kv_head, r0, r_end;
+  bool compact;
   int lead;
   const int32_t *table;  // the request's pages
   int own_end;           // own keys that its pages hold
@@ -84,9 +112,79 @@ struct PagedTile {
 // Own keys that row r sees.
 __device__ __forceinline__ int sees(const PagedAttention &p,
                                     const PagedTile &t, int r) {
-  const int64_t n = (int64_t)t.base + r / p.group - t.first + 1;
+  const int64_t n = (int64_t)t.base + token_of(p, r) - t.first + 1;
   return n < 0 ? 0 : n > t.own_end ? t.own_end : (int)n;
 }
+
+// The packed row of the small requests' row r: the last lane whose small rows
+// start at or before it, then its requests one after the other.
+__device__ __forceinline__ int packed_row(const PagedAttention &p,
+                                          const Requests &all, int r) {
+  int l = 0;
+#pragma unroll
+  for (int step = 32; step > 0; step >>= 1)
+    if (all.small[l + step] <= r)
+      l += step;
+  int rest = r - all.small[l];
+  const int each = (p.batch + 63) >> 6;
+  int begin = all.of[0][l];
+  if (each > 1) {
+    int b = l * each;
+    const int last = b + each < p.batch ? b + each - 1 : p.batch - 1;
+    for (;; ++b) {
+      begin = row_start(p, b);
+      const int rows = (row_start(p, b + 1) - begin) * p.group;
+      const int mine = rows > 0 && rows <= kSmallRows ? rows : 0;
+      if (rest < mine || b >= last)
+        break;
+      rest -= mine;
+    }
+  }
+  r = begin * p.group + rest;
+  const int end = p.rows * p.group;
+  return r < end ? r : end - 1;
+}
+
+// The lane's query row of a tile.
+__device__ __forceinline__ const f16 *query_row(const PagedAttention &p,
+                                                const PagedTile &t,
+                                                const Requests &all, int r) {
+  if (t.compact)
+    r = packed_row(p, all, r);
+  const int token = token_of(p, r);
+  return p.q + (int64_t)token * p.q_row +
+         (int64_t)(t.kv_head * p.group + r - token * p.group) * p.q_head;
+}
+
+// Inclusive sums over the lanes.
+__device__ __forceinline__ uint32_t lane_sums(uint32_t x) {
+#define IHP_SHIFTED(CTRL, ROWS)                                                \
+  x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, false)
+  IHP_SHIFTED(0x111, 0xf);  // row_shr 1, 2, 4, 8: sums within 16 lanes
+  IHP_SHIFTED(0x112, 0xf);
+  IHP_SHIFTED(0x114, 0xf);
+  IHP_SHIFTED(0x118, 0xf);
+  IHP_SHIFTED(0x142, 0xa);  // row_bcast 15: rows 1, 3 take rows 0, 2's
+  IHP_SHIFTED(0x143, 0xc);  // row_bcast 31: rows 2, 3 take rows 0 and 1's
+#undef IHP_SHIFTED
+  return x;
+}
+
+// Where a tile's keys are, in scalar registers for the length of its loop.
+struct Pages {
+  const int32_t *prefix_pages, *table;
+  int prefix, own_end;  // keys
+  int pages, page_size, shift, near;
+  uint32_t magic, k_page, k_row, v_page, v_row;
+
+  __device__ __forceinline__ Pages(const PagedAttention &p, const PagedTile &t)
+      : prefix_pages(held(p.prefix_pages)), table(held(t.table)),
+        prefix(held(p.prefix)), own_end(held(t.own_end)), pages(held(p.pages)),
+        page_size(held(p.page_size)), shift(held(p.page_shift)),
+        near(held(p.near)), magic(held(p.page_magic)),
+        k_page(held(p.k_page16)), k_row(held(p.k_row16)),
+        v_page(held(p.v_page16)), v_row(held(p.v_row16)) {}
+};
 
 // Pages of the KEYS keys of a block: a lane's key, its table's page number
 // (find, a block ahead of the rows) and the places in the caches that `place`
@@ -102,29 +200,31 @@ struct PagedBlock {
   // `lead`: the prefix's blocks of KEYS keys. Keys past the end are the last
   // one, or those of the last aligned `group` keys (which a page that is a
   // multiple of them holds whole).
-  __device__ __forceinline__ void find(const PagedAttention &p,
-                                       const PagedTile &t, int lead, int c,
+  __device__ __forceinline__ void find(const Pages &p, int lead, int c,
                                        int group = 1) {
     const bool own = c >= lead;
-    const int end = own ? t.own_end : p.prefix;
-    const int32_t *table = own ? t.table : p.prefix_pages;
+    const int end = own ? p.own_end : p.prefix;
+    const int32_t *table = own ? p.table : p.prefix_pages;
     int key = (own ? c - lead : c) * KEYS + ((int)threadIdx.x & (KEYS - 1));
     if (key >= end)
       key = ((end - 1) & -group) + (key & (group - 1));
     const int column =
-        (int)(((uint64_t)(uint32_t)key * p.page_magic) >> p.page_shift);
+        p.page_size == 1 ? key : (int)(__umulhi((uint32_t)key, p.magic) >> p.shift);
     inside = key - column * p.page_size;
     found = table[column];
   }
-  __device__ __forceinline__ void place(const PagedAttention &p,
-                                        const PagedTile &t, int lead, int c) {
+  __device__ __forceinline__ void place(const Pages &p, int lead, int c) {
     const bool own = c >= lead;
-    const int left =
-        (own ? t.own_end - (c - lead) * KEYS : p.prefix - c * KEYS);
+    const int left = own ? p.own_end - (c - lead) * KEYS : p.prefix - c * KEYS;
     const bool has = (uint32_t)found < (uint32_t)p.pages;
     const uint32_t page = has ? (uint32_t)found : 0u;
-    k = page * p.k_page16 + (uint32_t)inside * p.k_row16;
-    v = page * p.v_page16 + (uint32_t)inside * p.v_row16;
+    if (p.near) {  // every factor below 2^24
+      k = __umul24(page, p.k_page) + __umul24(inside, p.k_row);
+      v = __umul24(page, p.v_page) + __umul24(inside, p.v_row);
+    } else {
+      k = page * p.k_page + (uint32_t)inside * p.k_row;
+      v = page * p.v_page + (uint32_t)inside * p.v_row;
+    }
     there = (Mask)__ballot(has);
     if (left < KEYS)
       there = left > 0 ? there & (((Mask)1 << left) - 1) : 0;
@@ -134,8 +234,9 @@ struct PagedBlock {
 // Where a row's result or part goes.
 __device__ __forceinline__ f16 *result_row(const PagedAttention &p, int kv_head,
                                            int row) {
-  return p.o + (int64_t)(row / p.group) * p.o_row +
-         (int64_t)(kv_head * p.group + row % p.group) * p.o_head;
+  const int token = token_of(p, row);
+  return p.o + (int64_t)token * p.o_row +
+         (int64_t)(kv_head * p.group + row - token * p.group) * p.o_head;
 }
 __device__ __forceinline__ int64_t part_row(const PagedAttention &p,
                                             const PagedTile &t, int row) {
@@ -144,15 +245,16 @@ __device__ __forceinline__ int64_t part_row(const PagedAttention &p,
 
 }  // namespace
 
-// A tile of up to 16 rows. DP: the head-dim bucket (64, 128 or 256, at least
-// both head dims).
-template <int DP>
-__device__ __forceinline__ void narrow_tile(const PagedTile &t, char *smem,
+// A tile of up to 16 rows. DP: the row of a staged key (64, 128 or 256); DX:
+// a multiple of 32 up to it, at least both head dims.
+template <int DP, int DX>
+__device__ __forceinline__ void narrow_tile(const PagedTile &t,
+                                            const Requests &all, char *smem,
                                             float (*wave_m)[kNarrowRows],
                                             float (*wave_l)[kNarrowRows]) {
   const PagedAttention &p = arguments();
-  constexpr int KS = DP / 32;           // head-dim steps of S
-  constexpr int DB = DP / 16;           // 16-wide d blocks of O
+  constexpr int KS = DX / 32;           // head-dim steps of S
+  constexpr int DB = DX / 16;           // 16-wide d blocks of O
   constexpr int NCH = DP / 8;           // 16-byte chunks of a V row
   constexpr int VROWS = 64 / NCH;       // V rows per load
   constexpr int VP = kBlockKeys / VROWS;
@@ -171,8 +273,7 @@ __device__ __forceinline__ void narrow_tile(const PagedTile &t, char *smem,
   const int limit = sees(p, t, r_mine), all_own = sees(p, t, t.r0);
   i32x4 qf[KS];
   {
-    const f16 *qp = p.q + (int64_t)(r_mine / p.group) * p.q_row +
-                    (int64_t)(t.kv_head * p.group + r_mine % p.group) * p.q_head;
+    const f16 *qp = query_row(p, t, all, r_mine);
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
       const int c = 32 * ks + 8 * lg;
@@ -184,7 +285,7 @@ __device__ __forceinline__ void narrow_tile(const PagedTile &t, char *smem,
 
   // Chunks of a row past the head dim: K's are zeroed before use, V's reach
   // columns that are not stored; both are loaded from inside the row.
-  const bool pad_k = p.dqk != DP;
+  const bool pad_k = p.dqk != DX;
   int koff[KS];
 #pragma unroll
   for (int ks = 0; ks < KS; ++ks) {
@@ -199,6 +300,7 @@ __device__ __forceinline__ void narrow_tile(const PagedTile &t, char *smem,
   int c_end = lead + (t.seen + kBlockKeys - 1) / kBlockKeys;
   if (c_end > t.s_end * (kStepKeys / kBlockKeys))
     c_end = t.s_end * (kStepKeys / kBlockKeys);
+  const Pages pages(p, t);
   PagedBlock<kBlockKeys> block;
   i32x4 kf[2][KS], vf[VP];
   auto load_k = [&]() __attribute__((always_inline)) {
@@ -232,12 +334,12 @@ __device__ __forceinline__ void narrow_tile(const PagedTile &t, char *smem,
   __syncthreads();
   int c = c_begin + wave;
   if (c < c_end) {
-    block.find(p, t, lead, c);
-    block.place(p, t, lead, c);
+    block.find(pages, lead, c);
+    block.place(pages, lead, c);
     load_k();
     load_v();
     if (c + kPagedWaves < c_end)
-      block.find(p, t, lead, c + kPagedWaves);
+      block.find(pages, lead, c + kPagedWaves);
   }
   for (; c < c_end; c += kPagedWaves) {
     const bool more = c + kPagedWaves < c_end;
@@ -260,7 +362,7 @@ __device__ __forceinline__ void narrow_tile(const PagedTile &t, char *smem,
       s[f] *= scale;
     }
     if (live != 0xffffffffu || (own && key0 + kBlockKeys > all_own)) {
-      const int end = (own ? limit : p.prefix) - key0;
+      const int end = (own ? limit : pages.prefix) - key0;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const int key = 16 * (e >> 2) + 4 * lg + (e & 3);
@@ -269,10 +371,10 @@ __device__ __forceinline__ void narrow_tile(const PagedTile &t, char *smem,
       }
     }
     if (more) {
-      block.place(p, t, lead, c + kPagedWaves);
+      block.place(pages, lead, c + kPagedWaves);
       load_k();
       if (c + 2 * kPagedWaves < c_end)
-        block.find(p, t, lead, c + 2 * kPagedWaves);
+        block.find(pages, lead, c + 2 * kPagedWaves);
     }
 
     float top = s[0][0];
@@ -411,11 +513,12 @@ __device__ __forceinline__ int wide_v_swizzle(int key) {
   return DP == 128 ? 4 * (key & 3) : 4 * ((key >> 1) & 1);
 }
 
-template <int DP>
-__device__ __forceinline__ void wide_tile(const PagedTile &t, char *smem) {
+template <int DP, int DX>
+__device__ __forceinline__ void wide_tile(const PagedTile &t,
+                                          const Requests &all, char *smem) {
   const PagedAttention &p = arguments();
-  constexpr int DS = DP / 16;         // 16-wide d steps of S^T = K Q^T
-  constexpr int DT = DP / 32;         // 32-row d tiles of O^T
+  constexpr int DS = DX / 16;         // 16-wide d steps of S^T = K Q^T
+  constexpr int DT = DX / 32;         // 32-row d tiles of O^T
   constexpr int ROW = DP * 2;         // bytes of a staged row
   constexpr int CH = ROW / 16;        // its 16-byte chunks
   constexpr int BLK = kStepKeys * ROW;
@@ -437,8 +540,7 @@ __device__ __forceinline__ void wide_tile(const PagedTile &t, char *smem) {
   const int all_own = sees(p, t, r_wave < t.r_end ? r_wave : t.r_end - 1);
   i32x4 qf[DS];
   {
-    const f16 *qp = p.q + (int64_t)(r_mine / p.group) * p.q_row +
-                    (int64_t)(t.kv_head * p.group + r_mine % p.group) * p.q_head;
+    const f16 *qp = query_row(p, t, all, r_mine);
 #pragma unroll
     for (int s = 0; s < DS; ++s) {
       const int c = 16 * s + 8 * g;
@@ -446,6 +548,11 @@ __device__ __forceinline__ void wide_tile(const PagedTile &t, char *smem) {
       if (c < p.dqk)
         qf[s] = *(const i32x4 *)(qp + c);
     }
+    // Waited for here, or the compiler would at their use in every step.
+    wait_vmcnt<0>();
+#pragma unroll
+    for (int s = 0; s < DS; ++s)
+      lgkm_tie(qf[s]);
   }
 
   // Copy side: an instruction moves ROWS rows of CH chunks, lane -> (row,
@@ -453,38 +560,48 @@ __device__ __forceinline__ void wide_tile(const PagedTile &t, char *smem) {
   // within the head dim (the LDS past it is zeroed once and never written).
   // The swizzles repeat every 16 rows, so the chunk is the same in all passes.
   // Where pages are multiples of ROWS tokens an instruction's rows follow one
-  // another in a page: their base is scalar, a lane's offset the same for all
-  // of them, and a copy takes no vector instruction. Otherwise every lane's
-  // place comes from the lane that has the key: 90 instead of 16 vector and
-  // LDS instructions a block of 8 copies a wave.
+  // another in a page; with a head's rows within 4 GiB their place is then one
+  // scalar offset, and a lane's own the same for all copies: 28 instructions a
+  // block, which a wave issues one by one, instead of 100.
   const int c_row = lane / CH, c_phys = lane % CH;
   const int k_chunk = c_phys ^ wide_k_swizzle<DP>(wave * ROWS + c_row);
   const int v_chunk = c_phys ^ wide_v_swizzle<DP>(wave * ROWS + c_row);
   const bool k_in = 8 * k_chunk < p.dqk, v_in = 8 * v_chunk < p.dv;
-  const bool grouped = p.page_size % ROWS == 0 &&
-                       p.k_row16 < (1u << 24) && p.v_row16 < (1u << 24);
+  const Pages pages(p, t);
+  const bool grouped = pages.near && pages.page_size % ROWS == 0;
+  const bool alike =
+      pages.k_page == pages.v_page && pages.k_row == pages.v_row;
   const int group = grouped ? ROWS : 1;
-  const uint32_t k_lane = ((uint32_t)c_row * p.k_row16 + k_chunk) * 16;
-  const uint32_t v_lane = ((uint32_t)c_row * p.v_row16 + v_chunk) * 16;
+  const uint32_t k_lane = ((uint32_t)c_row * pages.k_row + k_chunk) * 16;
+  const uint32_t v_lane = ((uint32_t)c_row * pages.v_row + v_chunk) * 16;
+  const i32x4 k_rows = rows_from(Kp), v_rows = rows_from(Vp);
   IHP_LDS char *lds = (IHP_LDS char *)smem;
   PagedBlock<kStepKeys> block;
   auto copy = [&](int slot) {
     IHP_LDS char *kd = lds + slot * BLK + wave * (ROWS * ROW);
     IHP_LDS char *vd = kd + 2 * BLK;
+    constexpr int NEXT = kPagedWaves * ROWS * ROW;
     if (grouped) {
-      auto rows = [&](const char *base, uint32_t at, uint32_t mine, bool in,
-                      IHP_LDS char *to) {
+      uint32_t at[PASSES];
 #pragma unroll
-        for (int i = 0; i < PASSES; ++i) {
-          const uint32_t row0 = (uint32_t)__builtin_amdgcn_readlane(
-              (int)at, (i * kPagedWaves + wave) * ROWS);
-          if (in)
-            global_to_lds_16s(base + (uint64_t)row0 * 16, mine,
-                              to + i * kPagedWaves * ROWS * ROW);
-        }
-      };
-      rows(Kp, block.k, k_lane, k_in, kd);
-      rows(Vp, block.v, v_lane, v_in, vd);
+      for (int i = 0; i < PASSES; ++i)
+        at[i] = (uint32_t)__builtin_amdgcn_readlane(
+                    (int)block.k, (i * kPagedWaves + wave) * ROWS) *
+                16;
+      if (k_in)
+#pragma unroll
+        for (int i = 0; i < PASSES; ++i)
+          buffer_to_lds_16(k_rows, k_lane, at[i], kd + i * NEXT);
+      if (!alike)
+#pragma unroll
+        for (int i = 0; i < PASSES; ++i)
+          at[i] = (uint32_t)__builtin_amdgcn_readlane(
+                      (int)block.v, (i * kPagedWaves + wave) * ROWS) *
+                  16;
+      if (v_in)
+#pragma unroll
+        for (int i = 0; i < PASSES; ++i)
+          buffer_to_lds_16(v_rows, v_lane, at[i], vd + i * NEXT);
     } else {
       uint32_t at[2 * PASSES];
 #pragma unroll
@@ -497,11 +614,11 @@ __device__ __forceinline__ void wide_tile(const PagedTile &t, char *smem) {
       for (int i = 0; i < PASSES; ++i) {
         if (k_in)
           global_to_lds_16(Kp + ((uint64_t)at[i] + (uint32_t)k_chunk) * 16,
-                           kd + i * kPagedWaves * ROWS * ROW);
+                           kd + i * NEXT);
         if (v_in)
           global_to_lds_16(
               Vp + ((uint64_t)at[PASSES + i] + (uint32_t)v_chunk) * 16,
-              vd + i * kPagedWaves * ROWS * ROW);
+              vd + i * NEXT);
       }
     }
   };
@@ -545,11 +662,11 @@ __device__ __forceinline__ void wide_tile(const PagedTile &t, char *smem) {
     block_barrier();
   }
   if (c < c_end) {
-    block.find(p, t, lead, c, group);
-    block.place(p, t, lead, c);
+    block.find(pages, lead, c, group);
+    block.place(pages, lead, c);
     copy(0);
     if (c + 1 < c_end)
-      block.find(p, t, lead, c + 1, group);
+      block.find(pages, lead, c + 1, group);
   }
   for (int slot = 0; c < c_end; ++c, slot ^= 1) {
     const bool own = c >= lead;
@@ -568,10 +685,10 @@ __device__ __forceinline__ void wide_tile(const PagedTile &t, char *smem) {
       block_barrier();
     }
     if (c + 1 < c_end) {
-      block.place(p, t, lead, c + 1);
+      block.place(pages, lead, c + 1);
       copy(slot ^ 1);
       if (c + 2 < c_end)
-        block.find(p, t, lead, c + 2, group);
+        block.find(pages, lead, c + 2, group);
     }
 
     if (idle)
@@ -604,19 +721,21 @@ __device__ __forceinline__ void wide_tile(const PagedTile &t, char *smem) {
 
     __builtin_amdgcn_s_setprio(0);
 
-    // Softmax. Element (t, r) of S^T is key 32 t + 8 (r / 4) + 4 g + r % 4.
+    // Softmax. Element (h, r) of S^T is key 32 h + 8 (r / 4) + 4 g + r % 4.
     float sc = scale;
     if (live != ~0ull || (own && key0 + kStepKeys > all_own) || scale <= 0.0f) {
-      const int end = (own ? limit : p.prefix) - key0 - 4 * g;
-      const uint64_t mine = live >> (4 * g);
+      const int sees_to = (own ? limit : pages.prefix) - key0;
+      const uint64_t seen = sees_to >= kStepKeys ? live
+                            : sees_to > 0 ? live & ((1ull << sees_to) - 1)
+                                          : 0;
 #pragma unroll
-      for (int tt = 0; tt < 2; ++tt)
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t mine = (uint32_t)(seen >> (32 * h)) >> (4 * g);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int key = 32 * tt + 8 * (r >> 2) + (r & 3);
-          st[tt][r] = key < end && (mine >> key & 1) ? st[tt][r] * scale
-                                                     : kNegInf;
-        }
+        for (int r = 0; r < 16; ++r)
+          st[h][r] = mine >> (8 * (r >> 2) + (r & 3)) & 1 ? st[h][r] * scale
+                                                         : kNegInf;
+      }
       sc = 1.0f;
     }
     float top[4];
@@ -736,17 +855,11 @@ __device__ __forceinline__ void wide_tile(const PagedTile &t, char *smem) {
 
 namespace {
 
-// Rows of a tile where `rows` of them belong together.
-template <int DP>
-__device__ __forceinline__ int tile_rows(int64_t rows) {
-  return DP >= 256 || rows <= kNarrowRows ? kNarrowRows : kWideRows;
-}
-
 // Request b's tiles on the line: tile i takes a + i * step units, near the keys
 // that it walks and what a tile costs besides, so that their sums have a
 // closed form. A unit is 2^unit keys, which keeps the line below 2^31.
 struct Request {
-  int begin, end, tile, tiles;  // rows' tokens, rows a tile
+  int begin, end, shift, tiles;  // rows' tokens, log2 of a tile's rows
   int own_end, base;
   uint32_t a, step;
   __device__ __forceinline__ uint32_t before(uint32_t i) const {
@@ -757,27 +870,37 @@ struct Request {
 struct Line {
   uint32_t x, x_end, start, per;
   float inv_per;
-  int packed, kv_head, way, b, i;
+  int kv_head, way, b, i, small_rows;
+  bool shared;
   Request q;
 };
 
+__device__ __forceinline__ int rows_of(const PagedAttention &p, int begin,
+                                       int end) {
+  return end > begin ? (end - begin) * p.group : 0;
+}
+
+// `shared`: small requests leave the prefix to tiles of their own.
 template <int DP>
 __device__ __forceinline__ Request request(const PagedAttention &p, int begin,
-                                           int end, int length, int lead) {
+                                           int end, int length, bool shared,
+                                           int prefix_keys) {
   Request q;
+  const int rows = rows_of(p, begin, end);
   const int added = end > begin ? end - begin : 0;
+  const bool small = rows <= kSmallRows;
   q.begin = begin;
   q.end = begin + added;
-  const int rows = added * p.group;
-  q.tile = tile_rows<DP>(rows);
-  q.tiles = (rows + q.tile - 1) / q.tile;
+  q.shift = DP >= 256 || small ? 4 : 7;
+  q.tiles = (rows + (1 << q.shift) - 1) >> q.shift;
   length = length > 0 ? length : 0;
   q.own_end = length < p.capacity ? length : p.capacity;
   q.base = length - added;
-  const int tokens = rows <= q.tile ? added : q.tile / p.group;
+  const int tokens =
+      small ? added : DP >= 256 ? p.narrow_tokens : p.wide_tokens;
   const bool whole = q.base >= 0 && length <= p.capacity && tokens > 0;
-  const uint32_t keys =
-      (uint32_t)lead + (uint32_t)(whole ? q.base + tokens : q.own_end);
+  const uint32_t keys = (uint32_t)(small && shared ? 0 : prefix_keys) +
+                        (uint32_t)(whole ? q.base + tokens : q.own_end);
   q.a = (keys >> p.unit) + p.tile_units;
   q.step = whole && q.tiles > 1 ? (uint32_t)tokens >> p.unit : 0;
   return q;
@@ -785,7 +908,7 @@ __device__ __forceinline__ Request request(const PagedAttention &p, int begin,
 
 }  // namespace
 
-template <int DP>
+template <int DP, int DX>
 __global__ __launch_bounds__(kPagedThreads, DP >= 256 ? 1 : 2) void
 attention_paged_kernel(PagedAttention) {
   constexpr int VBYTES = kBlockKeys * DP * 2;
@@ -797,17 +920,15 @@ attention_paged_kernel(PagedAttention) {
   __shared__ __attribute__((aligned(1024))) char smem[SMEM];
   __shared__ float wave_m[kPagedWaves][kNarrowRows],
       wave_l[kPagedWaves][kNarrowRows];
-  // Where each wave is on the line, and the requests' row starts and lengths
-  // where every lane has one: kept here, out of the tiles' registers.
+  // Where each wave is on the line, kept here, out of the tiles' registers.
+  // (Every wave finds the same; the requests' are written by all alike.)
   __shared__ Line line_at[kPagedWaves];
-  __shared__ int request_of[kPagedWaves][3][64];
+  __shared__ Requests all;
 
   const PagedAttention &p = arguments();
-  // Lane l sums requests l * each .. + each - 1; its first one's row starts
-  // and length stay in registers.
-  const int lane = threadIdx.x & 63;
-  const int each = (p.batch + 63) / 64;
-  const int rows_end = row_start(p, p.batch);
+  // Lane l has requests l * each .. + each - 1.
+  const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6);
+  const int each = (p.batch + 63) >> 6;
   int begin = 0, end = 0, length = 0;
   if (lane * each < p.batch) {
     begin = row_start(p, lane * each);
@@ -819,60 +940,73 @@ attention_paged_kernel(PagedAttention) {
   xcd_tile_order((int)blockIdx.x, (int)gridDim.x, (int)gridDim.x, 1, 1, &item,
                  &unused);
   PagedTile t;
-  t.kv_head = item / p.ways;
-  int way = item % p.ways;
+  t.kv_head = p.ways == 1 ? item
+                          : (int)__umulhi((uint32_t)item, p.ways_magic);
+  int way = item - t.kv_head * p.ways;
 
-  // The line: the prefix's tiles (rows of the whole batch), then the
-  // requests'.
+  // The small requests' rows, and whether the prefix gets tiles of them.
+  auto rest_of_lane = [&](auto f) {  // the lane's requests after its first
+    for (int i = 1; i < each && lane * each + i < p.batch; ++i) {
+      const int b = lane * each + i;
+      f(row_start(p, b), row_start(p, b + 1), p.lengths[b]);
+    }
+  };
+  auto small_of = [&](int from, int to) {
+    const int rows = rows_of(p, from, to);
+    return (uint32_t)(rows <= kSmallRows ? rows : 0);
+  };
+  uint32_t small = small_of(begin, end);
+  rest_of_lane([&](int from, int to, int) { small += small_of(from, to); });
+  const uint32_t small_upto = lane_sums(small);
+  int small_rows = __builtin_amdgcn_readlane((int)small_upto, 63);
+  all.of[0][lane] = begin;
+  all.of[1][lane] = end;
+  all.of[2][lane] = length;
+  all.small[lane] = (int)(small_upto - small);
+  bool shared = p.shared && small_rows > 0 &&
+                !__any(small == (uint32_t)small_rows);
+
+  // The line: the prefix's tiles, then the requests'.
   const int prefix_steps = (p.prefix + kStepKeys - 1) / kStepKeys;
-  const int lead_keys = p.shared ? 0 : prefix_steps * kStepKeys;
-  uint32_t mine = 0;
-  for (int i = 0; i < each && lane * each + i < p.batch; ++i) {
-    const int b = lane * each + i;
-    const Request q =
-        i == 0 ? request<DP>(p, begin, end, length, lead_keys)
-               : request<DP>(p, row_start(p, b), row_start(p, b + 1),
-                             p.lengths[b], lead_keys);
+  const int prefix_keys = prefix_steps * kStepKeys;
+  uint32_t mine;
+  {
+    const Request q = request<DP>(p, begin, end, length, shared, prefix_keys);
+    mine = q.before(q.tiles);
+  }
+  rest_of_lane([&](int from, int to, int n) {
+    const Request q = request<DP>(p, from, to, n, shared, prefix_keys);
     mine += q.before(q.tiles);
-  }
-  uint32_t upto = mine;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const uint32_t y = __shfl_up(upto, d);
-    if (lane >= d)
-      upto += y;
-  }
+  });
+  const uint32_t upto = lane_sums(mine);
   Request q = {};
-  int packed = uniform(rows_end) * p.group;
-  q.tile = tile_rows<DP>(p.packed);
-  q.tiles = p.shared ? (packed + q.tile - 1) / q.tile : 0;
-  q.a = ((uint32_t)(prefix_steps * kStepKeys) >> p.unit) + p.tile_units;
+  q.shift = DP >= 256 || small_rows <= kNarrowRows ? 4 : 7;
+  q.tiles = shared ? (small_rows + (1 << q.shift) - 1) >> q.shift : 0;
+  q.a = ((uint32_t)prefix_keys >> p.unit) + p.tile_units;
   const uint32_t shared_units = q.before(q.tiles);
-  const uint32_t total = shared_units + (uint32_t)uniform((int)__shfl(upto, 63));
-  uint32_t per = (total + (uint32_t)p.ways - 1) / (uint32_t)p.ways;
+  const uint32_t total =
+      shared_units + (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
+  // enough for `ways` of them to reach the end
+  uint32_t per = p.ways == 1 ? total : __umulhi(total, p.ways_magic) + 1;
   per = per < (uint32_t)p.least ? p.least : per;
   float inv_per = 1.0f / (float)per;
-  uint32_t x = (uint32_t)way * per;  // below 2^31 + 2^31
+  uint32_t x = (uint32_t)way * per;  // below 2^32: `ways` is at most 2^24
   if (x >= total)
     return;
   uint32_t x_end = x + per < total ? x + per : total;
 
-  const int wave = uniform((int)threadIdx.x >> 6);
-  request_of[wave][0][lane] = begin;
-  request_of[wave][1][lane] = end;
-  request_of[wave][2][lane] = length;
   auto request_at = [&](int b) {
     int of[3];
     if (p.batch <= 64) {
 #pragma unroll
       for (int k = 0; k < 3; ++k)
-        of[k] = uniform(request_of[wave][k][b]);
+        of[k] = uniform(all.of[k][b]);
     } else {
       of[0] = uniform(row_start(p, b));
       of[1] = uniform(row_start(p, b + 1));
       of[2] = uniform(p.lengths[b]);
     }
-    return request<DP>(p, of[0], of[1], of[2], p.shared ? 0 : prefix_steps * kStepKeys);
+    return request<DP>(p, of[0], of[1], of[2], shared, prefix_keys);
   };
 
   // Where the stretch begins: among the prefix's tiles, or in the request that
@@ -884,7 +1018,8 @@ attention_paged_kernel(PagedAttention) {
     const int lane_of = uniform(
         63 - __builtin_clzll(
                  __ballot(shared_units + upto - mine <= x) | 1));
-    start = shared_units + (uint32_t)uniform((int)__shfl(upto - mine, lane_of));
+    start = shared_units +
+            (uint32_t)__builtin_amdgcn_readlane((int)(upto - mine), lane_of);
     b = lane_of * each;
     q = request_at(b);
     while (start + q.before(q.tiles) <= x && b + 1 < p.batch) {
@@ -915,14 +1050,18 @@ attention_paged_kernel(PagedAttention) {
     const uint32_t from = x - at;
     uint32_t to = x_end - at < units ? x_end - at : units;
     x = at + to;
-    t.r0 = q.begin * p.group + i * q.tile;
-    t.r_end = lead ? packed : q.end * p.group;
-    t.r_end = t.r_end - t.r0 < q.tile ? t.r_end : t.r0 + q.tile;
+    t.compact = lead;
+    t.r0 = q.begin * p.group + (i << q.shift);
+    t.r_end = lead ? small_rows : q.end * p.group;
+    t.r_end = t.r_end - t.r0 < 1 << q.shift ? t.r_end : t.r0 + (1 << q.shift);
     t.first = q.begin;
     t.base = q.base;
-    t.own_end = lead ? 0 : q.own_end;
+    t.own_end = q.own_end;
     t.table = p.table + (int64_t)(lead ? 0 : b) * p.table_stride;
-    t.lead = lead || !p.shared ? prefix_steps : 0;
+    // Whether the tile has all of its rows' keys.
+    const bool all_keys =
+        !lead && !(shared && (q.end - q.begin) * p.group <= kSmallRows);
+    t.lead = lead || all_keys ? (p.prefix + kStepKeys - 1) / kStepKeys : 0;
     t.seen = lead ? 0 : uniform(sees(p, t, t.r_end - 1));
     const int steps = t.lead + (t.seen + kStepKeys - 1) / kStepKeys;
     ++i;
@@ -951,34 +1090,41 @@ attention_paged_kernel(PagedAttention) {
     };
     t.s_begin = step_at(from);
     t.s_end = step_at(to);
-    const bool whole = count == 1 && !p.shared;
-    const int64_t line = p.shared && !lead ? p.packed : 0;
+    const bool whole = count == 1 && all_keys;
+    const int64_t line = lead ? 0 : p.packed;
     t.part = whole ? -1 : line + (int64_t)kWideRows * way;
     if (p.partials && from == 0 && t.kv_head == 0)
-      for (int r = t.r0 + (int)threadIdx.x; r < t.r_end; r += kPagedThreads)
-        p.part_of[line + r] = i32x2{first, whole ? 0 : count};
-    const int tile = q.tile;
-    line_at[wave] = {x, x_end, start, per, inv_per, packed, t.kv_head, way,
-                     b, i, q};
-    if (tile == kNarrowRows)
-      narrow_tile<DP>(t, smem, wave_m, wave_l);
+      for (int r = t.r0 + (int)threadIdx.x; r < t.r_end; r += kPagedThreads) {
+        const i32x2 parts = {(int)(line + r) + kWideRows * first,
+                             whole ? 0 : count};
+        p.part_of[line + (lead ? packed_row(p, all, r) : r)] = parts;
+        if (all_keys)
+          p.part_of[r] = i32x2{0, 0};
+      }
+    const int shift = q.shift;
+    line_at[wave] = {x,  x_end, start, per,        inv_per, t.kv_head,
+                     way, b,    i,     small_rows, shared,  q};
+    if (shift == 4)
+      narrow_tile<DP, DX>(t, all, smem, wave_m, wave_l);
     else if constexpr (DP < 256)
-      wide_tile<DP>(t, smem);
+      wide_tile<DP, DX>(t, all, smem);
     asm volatile("" ::: "memory");
     const Line &l = line_at[wave];
     x = (uint32_t)uniform((int)l.x);
     x_end = (uint32_t)uniform((int)l.x_end);
     start = (uint32_t)uniform((int)l.start);
     per = (uint32_t)uniform((int)l.per);
-    inv_per = __builtin_bit_cast(float, uniform(__builtin_bit_cast(int, l.inv_per)));
-    packed = uniform(l.packed);
+    inv_per =
+        __builtin_bit_cast(float, uniform(__builtin_bit_cast(int, l.inv_per)));
     t.kv_head = uniform(l.kv_head);
     way = uniform(l.way);
     b = uniform(l.b);
     i = uniform(l.i);
+    small_rows = uniform(l.small_rows);
+    shared = uniform((int)l.shared);
     q.begin = uniform(l.q.begin);
     q.end = uniform(l.q.end);
-    q.tile = uniform(l.q.tile);
+    q.shift = uniform(l.q.shift);
     q.tiles = uniform(l.q.tiles);
     q.own_end = uniform(l.q.own_end);
     q.base = uniform(l.q.base);
@@ -989,8 +1135,8 @@ attention_paged_kernel(PagedAttention) {
 
 // Joins the parts of every row that has some: DP / 4 threads, 4 columns each,
 // for every GROUPS-th four of a row's parts, then the GROUPS sums through LDS.
-// A row's parts of one kind (the prefix's and its own, or both at once) are
-// kWideRows rows apart, part_of telling the first and how many.
+// A row's parts of one kind (the prefix's of a small request, its own or both
+// at once) are kWideRows rows apart; part_of tells the first and how many.
 template <int DP, int GROUPS>
 __global__ __launch_bounds__(kPagedThreads) void attention_paged_join_kernel(
     PagedAttention p) {
@@ -1004,14 +1150,14 @@ __global__ __launch_bounds__(kPagedThreads) void attention_paged_join_kernel(
   float top = kNegInf, sum = 0.0f;
   f32x4 acc = {0, 0, 0, 0};
   int parts = 0;
-  for (int kind = 0; real && kind <= p.shared; ++kind) {
-    const int64_t line = kind * p.packed + row;
-    const i32x2 of = p.part_of[line];
-    // within the workgroups of the line, whatever it holds
-    const int first = of[0] < 0 ? 0 : of[0] < p.ways ? of[0] : p.ways - 1;
-    const int count = of[1] < p.ways - first ? of[1] : p.ways - first;
-    const int64_t at0 = (int64_t)kv_head * p.part_rows + line +
-                        (int64_t)kWideRows * first;
+  for (int kind = 0; real && kind < 2; ++kind) {
+    const i32x2 of = p.part_of[kind * p.packed + row];
+    // within the head's part rows, whatever it holds
+    const int64_t first =
+        of[0] < 0 ? 0 : of[0] < p.part_rows ? of[0] : p.part_rows - 1;
+    const int most = (int)((p.part_rows - 1 - first) / kWideRows) + 1;
+    const int count = of[1] < most ? of[1] : most;
+    const int64_t at0 = (int64_t)kv_head * p.part_rows + first;
     // 4 parts' loads in flight; a part past the last repeats it with weight 0
     for (int s0 = 4 * g; s0 < count; s0 += 4 * GROUPS) {
       f32x2 ml[4];
@@ -1083,17 +1229,20 @@ namespace {
 
 struct PagedKernel {
   const char *name;
-  int dp, groups;  // groups: of a joined row's parts
+  int dp, dx, groups;  // groups: of a joined row's parts
   const void *fn;
 };
 const PagedKernel kPagedKernels[] = {
-    {"attention_paged_d64", 64, 0, (const void *)&attention_paged_kernel<64>},
-    {"attention_paged_d128", 128, 0,
-     (const void *)&attention_paged_kernel<128>},
-    {"attention_paged_d256", 256, 0,
-     (const void *)&attention_paged_kernel<256>},
+    {"attention_paged_d64", 64, 64, 0,
+     (const void *)&attention_paged_kernel<64, 64>},
+    {"attention_paged_d96", 128, 96, 0,
+     (const void *)&attention_paged_kernel<128, 96>},
+    {"attention_paged_d128", 128, 128, 0,
+     (const void *)&attention_paged_kernel<128, 128>},
+    {"attention_paged_d256", 256, 256, 0,
+     (const void *)&attention_paged_kernel<256, 256>},
 #define IHP_JOIN(DP, GROUPS)                                                   \
-  {"attention_paged_join_d" #DP "_g" #GROUPS, DP, GROUPS,                      \
+  {"attention_paged_join_d" #DP "_g" #GROUPS, DP, DP, GROUPS,                  \
    (const void *)&attention_paged_join_kernel<DP, GROUPS>}
     IHP_JOIN(64, 1),
     IHP_JOIN(64, 8),
@@ -1115,9 +1264,10 @@ PagedPlan plan_attention_paged(int64_t rows, int64_t batch, int64_t kv_heads,
   PagedPlan p = {};
   const int64_t d = head_dim > head_dim_v ? head_dim : head_dim_v;
   p.dp = d <= 64 ? 64 : d <= 128 ? 128 : 256;
+  p.dx = d > 64 && d <= 96 ? 96 : p.dp;
   const int64_t packed = rows * group;
   // Requests that fill wide tiles walk the prefix themselves, as one alone.
-  p.shared = prefix > 0 && batch > 1 && packed < kWideRows * batch;
+  p.shared = prefix > 0 && batch > 1;
   const int64_t wgs = p.dp < 256 ? kPagedTargetWgs : kPagedTargetWgs / 2;
   p.ways = wgs / kv_heads > 1 ? wgs / kv_heads : 1;
   // The line in 32 bits, also where row_starts do not ascend and every request
@@ -1156,6 +1306,9 @@ hipError_t launch_attention_paged(const PagedAttention &attention,
   a.unit = (int)plan.unit;
   a.tile_units = (int)plan.tile_units;
   a.shared = plan.shared ? 1 : 0;
+  // item / ways of items below 2^24 with at most 2^8 ways or one head, and
+  // the ways' share of a line of less than 2^31 units, rounded down or not.
+  a.ways_magic = (uint32_t)(((uint64_t)1 << 32) / (uint64_t)plan.ways + 1);
   a.part_rows = plan.part_rows;
   a.part_of = nullptr;
   a.partials = a.part_ml = nullptr;
@@ -1170,9 +1323,9 @@ hipError_t launch_attention_paged(const PagedAttention &attention,
   const PagedKernel *kernel = nullptr, *join = nullptr;
   for (const PagedKernel &k : kPagedKernels)
     if (k.dp == plan.dp) {
-      if (k.groups == 0)
+      if (k.groups == 0 && k.dx == plan.dx)
         kernel = &k;
-      else if ((k.groups > 1) == few)
+      else if (k.groups > 0 && (k.groups > 1) == few)
         join = &k;
     }
   if (!kernel || !join)

@@ -106,6 +106,27 @@ __device__ __forceinline__ void global_to_lds_16s(const char *sbase,
       : "memory", "m0");
 }
 
+// The same from rows_from(base) + a scalar offset + a lane's, in bytes: no
+// address is computed for a copy.
+__device__ __forceinline__ i32x4 rows_from(const void *base) {
+  const uint64_t at = (uint64_t)base;
+  return i32x4{__builtin_amdgcn_readfirstlane((int)at),
+               __builtin_amdgcn_readfirstlane((int)(at >> 32)), -1,
+               0x00027000};
+}
+__device__ __forceinline__ void buffer_to_lds_16(i32x4 rows, uint32_t voff,
+                                                 uint32_t soff,
+                                                 IHP_LDS void *lds_wave_base) {
+  const uint32_t m0 = (uint32_t)(uintptr_t)lds_wave_base;
+  asm volatile(
+      "s_mov_b32 m0, %3\n\t"
+      "s_nop 0\n\t"
+      "buffer_load_dwordx4 %0, %1, %2 offen lds"
+      :
+      : "v"(voff), "s"(rows), "s"(soff), "s"(m0)
+      : "memory", "m0");
+}
+
 // s_waitcnt vmcnt(N) (gfx9 encoding: vmcnt[3:0] | vmcnt[5:4] << 14, other
 // counters left at their maximum so they are not waited on).
 template <int N>

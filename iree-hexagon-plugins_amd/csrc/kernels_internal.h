@@ -381,23 +381,31 @@ struct PagedAttention {
   const int32_t *row_starts, *lengths, *table, *prefix_pages;
   int64_t q_row, q_head, o_row, o_head, k_head, v_head, table_stride;
   int64_t packed;             // rows of a KV head: rows * group
-  uint64_t page_magic;        // key / page_size = key * magic >> shift
+  uint32_t page_magic;        // key / page_size = (key * magic >> 32) >> shift
   uint32_t k_page16, k_row16, v_page16, v_row16;
   int page_shift, page_size, pages;
+  // A head's rows lie within 4 GiB, and page numbers, places and the strides
+  // in 16 bytes are below 2^24.
+  int near;
+  uint32_t group_magic;       // row / group (above 1), as of a page
+  int group_shift;
+  int narrow_tokens, wide_tokens;  // whole tokens that a tile's rows hold
+  uint32_t ways_magic;        // item / ways
   int batch, rows, kv_heads, group, dqk, dv;
   int prefix, capacity;       // prefix keys, keys that a table row can name
   float scale;
   // Workgroups that share a KV head's tiles, the units of 2^unit keys that one
   // takes at least, the units that a tile counts for besides its keys, and
-  // whether the prefix has tiles of its own.
+  // whether the prefix may have tiles of its own.
   int ways, least, unit, tile_units, shared;
-  // Parts (no workspace: null): a row's f32 part of workgroup w at row
-  // line + 128 w of its KV head's part_rows, line = its row, plus `packed`
-  // for its own keys where the prefix has tiles of its own; their (max, sum);
-  // and per line the first workgroup and how many (0: none, the result is
-  // stored). Distinct on the line of tiles: from one tile to the next the row
-  // moves on by the tile's at most 128 rows, from one workgroup to the next w
-  // does.
+  // Parts (no workspace: null): workgroup w's f32 part of a tile's row at
+  // row line + 128 w of its KV head's part_rows, and its (max, sum). line is
+  // the row's number among the small requests' for the prefix's tiles, its
+  // packed row plus `packed` for the others. They are distinct: along the
+  // tiles the line moves on by a tile's at most 128 rows from one to the next,
+  // and w does from one workgroup to the next. part_of has, for either kind
+  // and packed row, the first part and how many (0: none, the result is
+  // stored).
   int64_t part_rows;
   float *partials, *part_ml;
   int __attribute__((ext_vector_type(2))) *part_of;
@@ -412,7 +420,7 @@ constexpr int64_t kPagedWholeKeys = 512;
 // Rows (of all heads) up to which a row's parts are joined by several groups.
 constexpr int64_t kPagedFewRows = 8192;
 struct PagedPlan {
-  int dp;  // head-dim bucket
+  int dp, dx;  // head-dim bucket: a staged key's row, what is computed
   bool shared;
   int64_t ways, least, unit, tile_units, part_rows, workspace;
 };

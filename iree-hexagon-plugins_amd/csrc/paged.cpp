@@ -66,6 +66,19 @@ static int check_cache(const char *who, const iree_mi355x_kv_cache_t &c) {
   return st ? st : check_cache_strides(who, "v", c, c.v_strides, c.head_dim_v);
 }
 
+// n / d = (n * magic >> 32) >> shift for n below 2^31, d > 1: with 2^(l-1) < d
+// <= 2^l and magic = floor(2^(31+l) / d) + 1 (below 2^32), the product is over
+// the true quotient by less than 2^-l, which does not reach the next multiple
+// of 1 / d.
+static void divider(int64_t d, uint32_t *magic, int *shift) {
+  int l = 1;
+  while (((int64_t)1 << l) < d)
+    ++l;
+  *magic = (uint32_t)((((uint64_t)1 << (31 + l)) / (uint64_t)(d > 1 ? d : 2)) +
+                      1);
+  *shift = l - 1;
+}
+
 // A call's extents, as far as its plan goes by them.
 static bool plannable(const iree_mi355x_paged_attention_t &a) {
   const iree_mi355x_kv_cache_t &c = a.cache;
@@ -278,21 +291,26 @@ int iree_mi355x_shared_prefix_attention_f16(
   p.k_row16 = (uint32_t)(c.k_strides[2] / 8);
   p.v_page16 = (uint32_t)(c.v_strides[0] / 8);
   p.v_row16 = (uint32_t)(c.v_strides[2] / 8);
-  // key / d for keys below 2^31: with 2^(l-1) < d <= 2^l and magic =
-  // floor(2^(31+l) / d) + 1, the product is over the true quotient by less
-  // than 2^-l, which does not reach the next multiple of 1 / d.
-  int l = 0;
-  while (((int64_t)1 << l) < c.page_size)
-    ++l;
-  p.page_magic = (((uint64_t)1 << (31 + l)) / (uint64_t)c.page_size) + 1;
-  p.page_shift = 31 + l;
+  divider(c.page_size, &p.page_magic, &p.page_shift);
   p.page_size = (int)c.page_size;
   p.pages = (int)c.pages;
+  const int64_t small = (int64_t)1 << 24;
+  auto reach = [&](const int64_t *st, int64_t dim) {  // bytes, head 0's rows
+    return ((c.pages > 0 ? c.pages - 1 : 0) * st[0] +
+            (c.page_size - 1) * st[2] + dim) * 2;
+  };
+  p.near = c.pages <= small && c.page_size <= small &&
+           p.k_page16 < small && p.k_row16 < small && p.v_page16 < small &&
+           p.v_row16 < small && reach(c.k_strides, 256) < UINT32_MAX &&
+           reach(c.v_strides, 256) < UINT32_MAX;
   p.batch = (int)a->batch;
   p.rows = (int)a->rows;
   p.kv_heads = (int)c.kv_heads;
   p.group = (int)(a->heads / c.kv_heads);
   p.packed = a->rows * p.group;
+  divider(p.group, &p.group_magic, &p.group_shift);
+  p.narrow_tokens = 16 / p.group;
+  p.wide_tokens = 128 / p.group;
   p.dqk = (int)c.head_dim;
   p.dv = (int)c.head_dim_v;
   // A cache without pages has no keys.

@@ -331,6 +331,10 @@ SHAPES = [
     ([0, 1], [64, 64], 2, 1, 40, 24, 5, 65),
     ([1000], [1], 8, 1, 64, 64, 16, 2000),
     ([700, 3, 0], [1, 1, 1], 4, 2, 128, 128, 1, 40),
+    # small requests around ones of more than 16 rows, behind a prefix
+    ([30, 5, 200, 9], [1, 60, 2, 1], 8, 2, 96, 96, 16, 150),
+    ([0, 3, 40, 0, 7, 90, 1], [40, 1, 0, 33, 1, 16, 17], 4, 4, 80, 64, 24, 70),
+    ([5, 600, 0, 2], [1, 1, 20, 1], 24, 3, 192, 128, 32, 513),
 ]
 
 
@@ -354,6 +358,10 @@ def test_attention_batches(pkg, dev, batch):
     for prefix in (0, 50):
         a = Attention(cached, added, 2, 1, 64, 64, 16, prefix, seed=batch)
         a.check(a.call(pkg))
+    # a table wide enough for parts, and every tenth request of 30 rows or so
+    added[::10] = [n + 14 for n in added[::10]]
+    a = Attention(cached, added, 2, 1, 64, 64, 16, 130, seed=batch, spare=40)
+    a.check(a.call(pkg))
 
 
 def test_attention_empty(pkg, dev):
