@@ -855,6 +855,15 @@ __device__ __forceinline__ void wide_tile(const PagedTile &t,
 
 namespace {
 
+// What keys cost a tile, and back: a wide tile's step is the longer one.
+__device__ __forceinline__ uint32_t cost_of(uint32_t keys, int shift) {
+  return shift > 4 ? keys + (keys * (kWideCost - 8) >> 3) : keys;
+}
+__device__ __forceinline__ uint32_t keys_of(uint32_t cost, int shift) {
+  return shift > 4 ? cost / kWideCost * 8 + cost % kWideCost * 8 / kWideCost
+                   : cost;
+}
+
 // Request b's tiles on the line: tile i takes a + i * step units, near the keys
 // that it walks and what a tile costs besides, so that their sums have a
 // closed form. A unit is 2^unit keys, which keeps the line below 2^31.
@@ -901,8 +910,9 @@ __device__ __forceinline__ Request request(const PagedAttention &p, int begin,
   const bool whole = q.base >= 0 && length <= p.capacity && tokens > 0;
   const uint32_t keys = (uint32_t)(small && shared ? 0 : prefix_keys) +
                         (uint32_t)(whole ? q.base + tokens : q.own_end);
-  q.a = (keys >> p.unit) + p.tile_units;
-  q.step = whole && q.tiles > 1 ? (uint32_t)tokens >> p.unit : 0;
+  q.a = cost_of(keys >> p.unit, q.shift) + p.tile_units;
+  q.step =
+      whole && q.tiles > 1 ? cost_of((uint32_t)tokens >> p.unit, q.shift) : 0;
   return q;
 }
 
@@ -982,7 +992,7 @@ attention_paged_kernel(PagedAttention) {
   Request q = {};
   q.shift = DP >= 256 || small_rows <= kNarrowRows ? 4 : 7;
   q.tiles = shared ? (small_rows + (1 << q.shift) - 1) >> q.shift : 0;
-  q.a = ((uint32_t)prefix_keys >> p.unit) + p.tile_units;
+  q.a = cost_of((uint32_t)prefix_keys >> p.unit, q.shift) + p.tile_units;
   const uint32_t shared_units = q.before(q.tiles);
   const uint32_t total =
       shared_units + (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
@@ -1084,7 +1094,8 @@ attention_paged_kernel(PagedAttention) {
     }
     // A tile's own units come first, before its keys.
     auto step_at = [&](uint32_t u) {
-      const uint32_t n = u > (uint32_t)p.tile_units ? u - p.tile_units : 0;
+      const uint32_t n = keys_of(
+          u > (uint32_t)p.tile_units ? u - p.tile_units : 0, q.shift);
       const uint64_t s = (((uint64_t)n << p.unit) + kStepKeys - 1) / kStepKeys;
       return u >= units || s > (uint64_t)steps ? steps : (int)s;
     };
@@ -1273,7 +1284,7 @@ PagedPlan plan_attention_paged(int64_t rows, int64_t batch, int64_t kv_heads,
   // The line in 32 bits, also where row_starts do not ascend and every request
   // has all rows.
   const int64_t each = packed / (p.dp < 256 ? kWideRows : kNarrowRows) + 2;
-  const double line = (double)(batch * each + packed) *
+  const double line = (double)(batch * each + packed) * (kWideCost / 8.0) *
                       (double)(prefix + capacity + rows + 512);
   while (line / (double)((int64_t)1 << p.unit) >= 1e9)
     ++p.unit;

@@ -415,6 +415,8 @@ struct PagedAttention {
 constexpr int64_t kPagedTargetWgs = 512;
 constexpr int64_t kPagedLeastKeys = 128;
 constexpr int64_t kPagedTileKeys = 256;
+// A wide tile's keys in eighths of a narrow one's cost.
+constexpr uint32_t kWideCost = 10;
 // Keys up to which a tile is not split: its parts would take longer to join.
 constexpr int64_t kPagedWholeKeys = 512;
 // Rows (of all heads) up to which a row's parts are joined by several groups.
