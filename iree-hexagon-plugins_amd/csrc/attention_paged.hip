@@ -936,6 +936,9 @@ attention_paged_kernel(PagedAttention) {
   __shared__ Requests all;
 
   const PagedAttention &p = arguments();
+  // All of the arguments' cache lines at once, not one after the other.
+  asm volatile("" ::"s"(p.batch), "s"(p.items), "s"(p.table_stride),
+               "s"(p.q_row), "s"(p.k_head));
   // Lane l has requests l * each .. + each - 1.
   const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6);
   const int each = (p.batch + 63) >> 6;
@@ -947,8 +950,7 @@ attention_paged_kernel(PagedAttention) {
   }
   // Consecutive stretches of one head's line read the same prefix: one XCD's.
   int item, unused;
-  xcd_tile_order((int)blockIdx.x, (int)gridDim.x, (int)gridDim.x, 1, 1, &item,
-                 &unused);
+  xcd_tile_order((int)blockIdx.x, p.items, p.items, 1, 1, &item, &unused);
   PagedTile t;
   t.kv_head = p.ways == 1 ? item
                           : (int)__umulhi((uint32_t)item, p.ways_magic);
@@ -1313,6 +1315,7 @@ hipError_t launch_attention_paged(const PagedAttention &attention,
                                   void *stream) {
   PagedAttention a = attention;
   a.ways = (int)plan.ways;
+  a.items = (int)(plan.ways * a.kv_heads);
   a.least = (int)plan.least;
   a.unit = (int)plan.unit;
   a.tile_units = (int)plan.tile_units;
@@ -1343,7 +1346,7 @@ hipError_t launch_attention_paged(const PagedAttention &attention,
     return hipErrorInvalidValue;
   void *args[] = {&a};
   hipError_t e =
-      hipLaunchKernel(kernel->fn, dim3((unsigned)(plan.ways * a.kv_heads)),
+      hipLaunchKernel(kernel->fn, dim3((unsigned)a.items),
                       dim3(kPagedThreads), args, 0, (hipStream_t)stream);
   if (e != hipSuccess || !plan.workspace)
     return e;

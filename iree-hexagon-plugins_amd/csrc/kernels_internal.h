@@ -375,29 +375,35 @@ const KernelEntry *paged_cache_kernels(int *count);
 // Attention over the paged cache (attention_paged.hip). Strides in elements;
 // a cache row's place within its head is counted in 16 bytes, in 32 bits
 // (checked on the host).
+// In the order of use, 64 bytes at a time.
 struct PagedAttention {
-  const _Float16 *q, *k_cache, *v_cache;
-  _Float16 *o;
-  const int32_t *row_starts, *lengths, *table, *prefix_pages;
-  int64_t q_row, q_head, o_row, o_head, k_head, v_head, table_stride;
-  int64_t packed;             // rows of a KV head: rows * group
-  uint32_t page_magic;        // key / page_size = (key * magic >> 32) >> shift
-  uint32_t k_page16, k_row16, v_page16, v_row16;
-  int page_shift, page_size, pages;
+  // What a workgroup finds its place by.
+  const int32_t *row_starts, *lengths;
+  int batch, rows, group;
+  int prefix, capacity;       // prefix keys, keys that a table row can name
+  // Workgroups that share a KV head's tiles (item / ways by its magic), the
+  // units of 2^unit keys that one takes at least, the units that a tile counts
+  // for besides its keys, and whether the prefix may have tiles of its own.
+  int ways;
+  uint32_t ways_magic;
+  int least, unit, tile_units, shared;
+  int wide_tokens;            // whole tokens that a wide tile's rows hold
+
+  int items;                  // the grid: ways * kv_heads
+  int narrow_tokens;          // and a narrow one's
+  uint32_t group_magic;       // row / group (above 1): (n * magic >> 32) >> shift
+  int group_shift;
+  int kv_heads, dqk, dv, pages;
+  uint32_t page_magic;        // key / page_size, alike
+  int page_shift, page_size;
   // A head's rows lie within 4 GiB, and page numbers, places and the strides
   // in 16 bytes are below 2^24.
   int near;
-  uint32_t group_magic;       // row / group (above 1), as of a page
-  int group_shift;
-  int narrow_tokens, wide_tokens;  // whole tokens that a tile's rows hold
-  uint32_t ways_magic;        // item / ways
-  int batch, rows, kv_heads, group, dqk, dv;
-  int prefix, capacity;       // prefix keys, keys that a table row can name
-  float scale;
-  // Workgroups that share a KV head's tiles, the units of 2^unit keys that one
-  // takes at least, the units that a tile counts for besides its keys, and
-  // whether the prefix may have tiles of its own.
-  int ways, least, unit, tile_units, shared;
+  uint32_t k_page16, k_row16, v_page16, v_row16;
+
+  const int32_t *table, *prefix_pages;
+  int64_t table_stride;
+  int64_t packed;             // rows of a KV head: rows * group
   // Parts (no workspace: null): workgroup w's f32 part of a tile's row at
   // row line + 128 w of its KV head's part_rows, and its (max, sum). line is
   // the row's number among the small requests' for the prefix's tiles, its
@@ -409,6 +415,13 @@ struct PagedAttention {
   int64_t part_rows;
   float *partials, *part_ml;
   int __attribute__((ext_vector_type(2))) *part_of;
+
+  const _Float16 *q, *k_cache, *v_cache;
+  _Float16 *o;
+  int64_t q_row, q_head, o_row, o_head;
+
+  int64_t k_head, v_head;
+  float scale;
 };
 // Workgroups wanted (two a CU where head dims allow it), the keys that one
 // takes at least, and the keys that a tile's start and end cost as much as.
