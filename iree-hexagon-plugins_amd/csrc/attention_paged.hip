@@ -1059,11 +1059,43 @@ attention_paged_kernel(PagedAttention) {
     // Units from .. to - 1 of the `units` that the tile has on the line.
     const bool lead = b < 0;
     const uint32_t at = start + q.before(i), units = q.a + q.step * i;
-    const uint32_t from = x - at;
+    uint32_t from = x - at;
     uint32_t to = x_end - at < units ? x_end - at : units;
     x = at + to;
+    ++i;
+    int first = 0, count = 1;
+    if (p.partials) {
+      // An end less than `snap` from a tile's first key or from its last one
+      // moves there: what a part costs is more than it takes off another.
+      const uint32_t early = (uint32_t)(p.tile_units + p.snap);
+      const uint32_t late = units - (uint32_t)p.snap;
+      auto snapped = [&](uint32_t u) {
+        return u < early ? 0 : u > late ? units : u;
+      };
+      // The workgroups of the tile's first and last keys: quotients that the
+      // float is off by one of at most.
+      auto way_of = [&](uint32_t u) {
+        int w = (int)((float)u * inv_per);
+        w -= (uint64_t)w * per > u;
+        return w + ((uint64_t)(w + 1) * per <= u);
+      };
+      const uint32_t lead_in = (early < units ? early : units) - 1;
+      first = uniform(way_of(at + lead_in));
+      count =
+          uniform(way_of(at + (late > lead_in ? late : lead_in))) - first + 1;
+      from = snapped(from);
+      to = to < units ? snapped(to) : units;
+      if (from >= to)
+        continue;
+    } else {
+      // without a workspace a workgroup takes the tiles that start in its
+      // stretch, whole
+      if (from > 0)
+        continue;
+      to = units;
+    }
     t.compact = lead;
-    t.r0 = q.begin * p.group + (i << q.shift);
+    t.r0 = q.begin * p.group + ((i - 1) << q.shift);
     t.r_end = lead ? small_rows : q.end * p.group;
     t.r_end = t.r_end - t.r0 < 1 << q.shift ? t.r_end : t.r0 + (1 << q.shift);
     t.first = q.begin;
@@ -1076,24 +1108,6 @@ attention_paged_kernel(PagedAttention) {
     t.lead = lead || all_keys ? (p.prefix + kStepKeys - 1) / kStepKeys : 0;
     t.seen = lead ? 0 : uniform(sees(p, t, t.r_end - 1));
     const int steps = t.lead + (t.seen + kStepKeys - 1) / kStepKeys;
-    ++i;
-    int first = 0, count = 1;
-    if (p.partials) {
-      // quotients that the float is off by one of at most
-      auto way_of = [&](uint32_t u) {
-        int w = (int)((float)u * inv_per);
-        w -= (uint64_t)w * per > u;
-        return w + ((uint64_t)(w + 1) * per <= u);
-      };
-      first = uniform(way_of(at));
-      count = uniform(way_of(at + units - 1)) - first + 1;
-    } else {
-      // without a workspace a workgroup takes the tiles that start in its
-      // stretch, whole
-      if (from > 0)
-        continue;
-      to = units;
-    }
     // A tile's own units come first, before its keys.
     auto step_at = [&](uint32_t u) {
       const uint32_t n = keys_of(
@@ -1106,7 +1120,7 @@ attention_paged_kernel(PagedAttention) {
     const bool whole = count == 1 && all_keys;
     const int64_t line = lead ? 0 : p.packed;
     t.part = whole ? -1 : line + (int64_t)kWideRows * way;
-    if (p.partials && from == 0 && t.kv_head == 0)
+    if (p.partials && way == first && t.kv_head == 0)
       for (int r = t.r0 + (int)threadIdx.x; r < t.r_end; r += kPagedThreads) {
         const i32x2 parts = {(int)(line + r) + kWideRows * first,
                              whole ? 0 : count};
@@ -1293,6 +1307,7 @@ PagedPlan plan_attention_paged(int64_t rows, int64_t batch, int64_t kv_heads,
   auto units = [&](int64_t keys) { return (keys >> p.unit) + 1; };
   p.least = units(kPagedLeastKeys + kPagedTileKeys);
   p.tile_units = units(kPagedTileKeys);
+  p.snap = units(kPagedSnapKeys);
   p.part_rows = 2 * packed + kWideRows * p.ways;
   p.workspace = (int64_t)kWorkspaceCounterBytes + 2 * packed * 8 +
                 kv_heads * p.part_rows * (p.dp + 2) * 4;
@@ -1319,6 +1334,7 @@ hipError_t launch_attention_paged(const PagedAttention &attention,
   a.least = (int)plan.least;
   a.unit = (int)plan.unit;
   a.tile_units = (int)plan.tile_units;
+  a.snap = (int)plan.snap;
   a.shared = plan.shared ? 1 : 0;
   // item / ways of items below 2^24 with at most 2^8 ways or one head, and
   // the ways' share of a line of less than 2^31 units, rounded down or not.

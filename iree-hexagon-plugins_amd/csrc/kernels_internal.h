@@ -383,10 +383,11 @@ struct PagedAttention {
   int prefix, capacity;       // prefix keys, keys that a table row can name
   // Workgroups that share a KV head's tiles (item / ways by its magic), the
   // units of 2^unit keys that one takes at least, the units that a tile counts
-  // for besides its keys, and whether the prefix may have tiles of its own.
+  // for besides its keys, those next to a tile's first and last key that stay
+  // in one part, and whether the prefix may have tiles of its own.
   int ways;
   uint32_t ways_magic;
-  int least, unit, tile_units, shared;
+  int least, unit, tile_units, snap, shared;
   int wide_tokens;            // whole tokens that a wide tile's rows hold
 
   int items;                  // the grid: ways * kv_heads
@@ -428,6 +429,11 @@ struct PagedAttention {
 constexpr int64_t kPagedTargetWgs = 512;
 constexpr int64_t kPagedLeastKeys = 128;
 constexpr int64_t kPagedTileKeys = 256;
+// A part is not begun or ended within so many keys of its tile's ends (38
+// requests of a token and at most 21 keys, 3 heads: 18.0 us at 0, 14.8 at 64;
+// 771 rows of a prompt: 36.1, 28.9; drafts of 12 requests 21.1, 20.8, but 22.7
+// at 128 and 23.8 at 256, which leave workgroups without work).
+constexpr int64_t kPagedSnapKeys = 64;
 // A wide tile's keys in eighths of a narrow one's cost.
 constexpr uint32_t kWideCost = 10;
 // Keys up to which a tile is not split: its parts would take longer to join.
@@ -437,7 +443,7 @@ constexpr int64_t kPagedFewRows = 8192;
 struct PagedPlan {
   int dp, dx;  // head-dim bucket: a staged key's row, what is computed
   bool shared;
-  int64_t ways, least, unit, tile_units, part_rows, workspace;
+  int64_t ways, least, unit, tile_units, snap, part_rows, workspace;
 };
 PagedPlan plan_attention_paged(int64_t rows, int64_t batch, int64_t kv_heads,
                                int64_t group, int64_t prefix, int64_t capacity,
