@@ -245,15 +245,15 @@ __device__ __forceinline__ int64_t part_row(const PagedAttention &p,
 
 }  // namespace
 
-// A tile of up to 16 rows. DP: the row of a staged key (64, 128 or 256); DX:
-// a multiple of 32 up to it, at least both head dims.
-template <int DP, int DX>
+// A tile of up to 16 rows. DP: the row of a staged V (64, 128 or 256); DX: a
+// multiple of 32 up to it, at least V's head dim; DK: alike of Q's and K's.
+template <int DP, int DX, int DK>
 __device__ __forceinline__ void narrow_tile(const PagedTile &t,
                                             const Requests &all, char *smem,
                                             float (*wave_m)[kNarrowRows],
                                             float (*wave_l)[kNarrowRows]) {
   const PagedAttention &p = arguments();
-  constexpr int KS = DX / 32;           // head-dim steps of S
+  constexpr int KS = DK / 32;           // head-dim steps of S
   constexpr int DB = DX / 16;           // 16-wide d blocks of O
   constexpr int NCH = DP / 8;           // 16-byte chunks of a V row
   constexpr int VROWS = 64 / NCH;       // V rows per load
@@ -285,7 +285,7 @@ __device__ __forceinline__ void narrow_tile(const PagedTile &t,
 
   // Chunks of a row past the head dim: K's are zeroed before use, V's reach
   // columns that are not stored; both are loaded from inside the row.
-  const bool pad_k = p.dqk != DX;
+  const bool pad_k = p.dqk != DK;
   int koff[KS];
 #pragma unroll
   for (int ks = 0; ks < KS; ++ks) {
@@ -890,7 +890,7 @@ __device__ __forceinline__ int rows_of(const PagedAttention &p, int begin,
 }
 
 // `shared`: small requests leave the prefix to tiles of their own.
-template <int DP>
+template <bool WIDE>
 __device__ __forceinline__ Request request(const PagedAttention &p, int begin,
                                            int end, int length, bool shared,
                                            int prefix_keys) {
@@ -900,13 +900,13 @@ __device__ __forceinline__ Request request(const PagedAttention &p, int begin,
   const bool small = rows <= kSmallRows;
   q.begin = begin;
   q.end = begin + added;
-  q.shift = DP >= 256 || small ? 4 : 7;
+  q.shift = !WIDE || small ? 4 : 7;
   q.tiles = (rows + (1 << q.shift) - 1) >> q.shift;
   length = length > 0 ? length : 0;
   q.own_end = length < p.capacity ? length : p.capacity;
   q.base = length - added;
   const int tokens =
-      small ? added : DP >= 256 ? p.narrow_tokens : p.wide_tokens;
+      small ? added : WIDE ? p.wide_tokens : p.narrow_tokens;
   const bool whole = q.base >= 0 && length <= p.capacity && tokens > 0;
   const uint32_t keys = (uint32_t)(small && shared ? 0 : prefix_keys) +
                         (uint32_t)(whole ? q.base + tokens : q.own_end);
@@ -918,15 +918,16 @@ __device__ __forceinline__ Request request(const PagedAttention &p, int begin,
 
 }  // namespace
 
-template <int DP, int DX>
+// WIDE: requests of more than 16 rows have wide tiles.
+template <int DP, int DX, int DK, bool WIDE>
 __global__ __launch_bounds__(kPagedThreads, DP >= 256 ? 1 : 2) void
 attention_paged_kernel(PagedAttention) {
   constexpr int VBYTES = kBlockKeys * DP * 2;
   constexpr int MERGE = kPagedWaves * 16 * (DP + 4) * 4;
-  constexpr int WIDE = DP >= 256 ? 0 : 4 * kStepKeys * DP * 2;
+  constexpr int RING = WIDE ? 4 * kStepKeys * DP * 2 : 0;
   constexpr int NARROW =
       kPagedWaves * VBYTES > MERGE ? kPagedWaves * VBYTES : MERGE;
-  constexpr int SMEM = NARROW > WIDE ? NARROW : WIDE;
+  constexpr int SMEM = NARROW > RING ? NARROW : RING;
   __shared__ __attribute__((aligned(1024))) char smem[SMEM];
   __shared__ float wave_m[kPagedWaves][kNarrowRows],
       wave_l[kPagedWaves][kNarrowRows];
@@ -983,16 +984,16 @@ attention_paged_kernel(PagedAttention) {
   const int prefix_keys = prefix_steps * kStepKeys;
   uint32_t mine;
   {
-    const Request q = request<DP>(p, begin, end, length, shared, prefix_keys);
+    const Request q = request<WIDE>(p, begin, end, length, shared, prefix_keys);
     mine = q.before(q.tiles);
   }
   rest_of_lane([&](int from, int to, int n) {
-    const Request q = request<DP>(p, from, to, n, shared, prefix_keys);
+    const Request q = request<WIDE>(p, from, to, n, shared, prefix_keys);
     mine += q.before(q.tiles);
   });
   const uint32_t upto = lane_sums(mine);
   Request q = {};
-  q.shift = DP >= 256 || small_rows <= kNarrowRows ? 4 : 7;
+  q.shift = !WIDE || small_rows <= kNarrowRows ? 4 : 7;
   q.tiles = shared ? (small_rows + (1 << q.shift) - 1) >> q.shift : 0;
   q.a = cost_of((uint32_t)prefix_keys >> p.unit, q.shift) + p.tile_units;
   const uint32_t shared_units = q.before(q.tiles);
@@ -1018,7 +1019,7 @@ attention_paged_kernel(PagedAttention) {
       of[1] = uniform(row_start(p, b + 1));
       of[2] = uniform(p.lengths[b]);
     }
-    return request<DP>(p, of[0], of[1], of[2], shared, prefix_keys);
+    return request<WIDE>(p, of[0], of[1], of[2], shared, prefix_keys);
   };
 
   // Where the stretch begins: among the prefix's tiles, or in the request that
@@ -1132,8 +1133,8 @@ attention_paged_kernel(PagedAttention) {
     line_at[wave] = {x,  x_end, start, per,        inv_per, t.kv_head,
                      way, b,    i,     small_rows, shared,  q};
     if (shift == 4)
-      narrow_tile<DP, DX>(t, all, smem, wave_m, wave_l);
-    else if constexpr (DP < 256)
+      narrow_tile<DP, DX, DK>(t, all, smem, wave_m, wave_l);
+    else if constexpr (WIDE)
       wide_tile<DP, DX>(t, all, smem);
     asm volatile("" ::: "memory");
     const Line &l = line_at[wave];
@@ -1256,20 +1257,21 @@ namespace {
 
 struct PagedKernel {
   const char *name;
-  int dp, dx, groups;  // groups: of a joined row's parts
+  int dp, dx, dk, groups;  // groups: of a joined row's parts
   const void *fn;
 };
 const PagedKernel kPagedKernels[] = {
-    {"attention_paged_d64", 64, 64, 0,
-     (const void *)&attention_paged_kernel<64, 64>},
-    {"attention_paged_d96", 128, 96, 0,
-     (const void *)&attention_paged_kernel<128, 96>},
-    {"attention_paged_d128", 128, 128, 0,
-     (const void *)&attention_paged_kernel<128, 128>},
-    {"attention_paged_d256", 256, 256, 0,
-     (const void *)&attention_paged_kernel<256, 256>},
+#define IHP_PAGED(NAME, DP, DX, DK, WIDE)                                      \
+  {"attention_paged_" NAME, DP, DX, DK, 0,                                     \
+   (const void *)&attention_paged_kernel<DP, DX, DK, WIDE>}
+    IHP_PAGED("d64", 64, 64, 64, true),
+    IHP_PAGED("d96", 128, 96, 96, true),
+    IHP_PAGED("d128", 128, 128, 128, true),
+    IHP_PAGED("d192_128", 128, 128, 192, false),
+    IHP_PAGED("d256", 256, 256, 256, false),
+#undef IHP_PAGED
 #define IHP_JOIN(DP, GROUPS)                                                   \
-  {"attention_paged_join_d" #DP "_g" #GROUPS, DP, DP, GROUPS,                  \
+  {"attention_paged_join_d" #DP "_g" #GROUPS, DP, DP, DP, GROUPS,                  \
    (const void *)&attention_paged_join_kernel<DP, GROUPS>}
     IHP_JOIN(64, 1),
     IHP_JOIN(64, 8),
@@ -1290,8 +1292,11 @@ PagedPlan plan_attention_paged(int64_t rows, int64_t batch, int64_t kv_heads,
                                size_t workspace_limit) {
   PagedPlan p = {};
   const int64_t d = head_dim > head_dim_v ? head_dim : head_dim_v;
-  p.dp = d <= 64 ? 64 : d <= 128 ? 128 : 256;
+  p.wide = d <= 128;
+  const bool longer_k = !p.wide && head_dim <= 192 && head_dim_v <= 128;
+  p.dp = d <= 64 ? 64 : d <= 128 || longer_k ? 128 : 256;
   p.dx = d > 64 && d <= 96 ? 96 : p.dp;
+  p.dk = longer_k ? 192 : p.dx;
   const int64_t packed = rows * group;
   // Requests that fill wide tiles walk the prefix themselves, as one alone.
   p.shared = prefix > 0 && batch > 1;
@@ -1299,7 +1304,7 @@ PagedPlan plan_attention_paged(int64_t rows, int64_t batch, int64_t kv_heads,
   p.ways = wgs / kv_heads > 1 ? wgs / kv_heads : 1;
   // The line in 32 bits, also where row_starts do not ascend and every request
   // has all rows.
-  const int64_t each = packed / (p.dp < 256 ? kWideRows : kNarrowRows) + 2;
+  const int64_t each = packed / (p.wide ? kWideRows : kNarrowRows) + 2;
   const double line = (double)(batch * each + packed) * (kWideCost / 8.0) *
                       (double)(prefix + capacity + rows + 512);
   while (line / (double)((int64_t)1 << p.unit) >= 1e9)
@@ -1319,7 +1324,7 @@ PagedPlan plan_attention_paged(int64_t rows, int64_t batch, int64_t kv_heads,
     p.workspace = p.part_rows = 0;
     p.least = p.tile_units;
     const int64_t tiles =
-        batch + packed / (p.dp < 256 ? kWideRows : kNarrowRows);
+        batch + packed / (p.wide ? kWideRows : kNarrowRows);
     p.ways = 4 * p.ways < 3 * tiles + 1 ? 4 * p.ways : 3 * tiles + 1;
   }
   return p;
@@ -1353,7 +1358,7 @@ hipError_t launch_attention_paged(const PagedAttention &attention,
   const PagedKernel *kernel = nullptr, *join = nullptr;
   for (const PagedKernel &k : kPagedKernels)
     if (k.dp == plan.dp) {
-      if (k.groups == 0 && k.dx == plan.dx)
+      if (k.groups == 0 && k.dx == plan.dx && k.dk == plan.dk)
         kernel = &k;
       else if (k.groups > 0 && (k.groups > 1) == few)
         join = &k;

@@ -441,8 +441,9 @@ constexpr int64_t kPagedWholeKeys = 512;
 // Rows (of all heads) up to which a row's parts are joined by several groups.
 constexpr int64_t kPagedFewRows = 8192;
 struct PagedPlan {
-  int dp, dx;  // head-dim bucket: a staged key's row, what is computed
-  bool shared;
+  // Head-dim buckets: a staged V's row, what is computed of V, and of Q and K.
+  int dp, dx, dk;
+  bool wide, shared;  // wide tiles there are, and the prefix's own
   int64_t ways, least, unit, tile_units, snap, part_rows, workspace;
 };
 PagedPlan plan_attention_paged(int64_t rows, int64_t batch, int64_t kv_heads,
