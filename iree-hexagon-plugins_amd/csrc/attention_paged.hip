@@ -1171,52 +1171,62 @@ __global__ __launch_bounds__(kPagedThreads) void attention_paged_join_kernel(
   constexpr int TPR = DP / 4, ROWS = kPagedThreads / TPR / GROUPS;
   const int tid = threadIdx.x;
   const int g = tid / TPR % GROUPS, dq = 4 * (tid % TPR);
-  const int64_t at = (int64_t)blockIdx.x * ROWS + tid / (TPR * GROUPS);
-  const int kv_head = (int)(at / p.packed), row = (int)(at % p.packed);
-  const bool real =
-      kv_head < p.kv_heads && row < row_start(p, p.batch) * p.group;
+  const uint32_t per_head = ((uint32_t)p.packed + ROWS - 1) / ROWS;
+  const int kv_head = (int)(blockIdx.x / per_head);
+  const int row =
+      (int)(blockIdx.x - kv_head * per_head) * ROWS + tid / (TPR * GROUPS);
+  // What part_of holds for a row past the last one is not used, but loaded
+  // with the rest.
+  const int at = row < (int)p.packed ? row : 0;
+  i32x2 of[2] = {p.part_of[at], p.part_of[p.packed + at]};
+  const int rows = row_start(p, p.batch);
+  asm volatile("" : "+v"(of[0]), "+v"(of[1]));
+  const bool real = row < (int)p.packed && row < rows * p.group;
+  int from[2], counts[2];
+#pragma unroll
+  for (int kind = 0; kind < 2; ++kind) {
+    // within the head's part rows, whatever it holds
+    const int last = (int)p.part_rows - 1;
+    from[kind] = of[kind][0] < 0        ? 0
+                 : of[kind][0] < last ? of[kind][0]
+                                        : last;
+    const int most = (last - from[kind]) / kWideRows + 1;
+    counts[kind] = of[kind][1] < most ? of[kind][1] : most;
+    counts[kind] = real && counts[kind] > 0 ? counts[kind] : 0;
+  }
+  const int parts = counts[0] + counts[1];
+  const int64_t head_at = (int64_t)kv_head * p.part_rows;
   float top = kNegInf, sum = 0.0f;
   f32x4 acc = {0, 0, 0, 0};
-  int parts = 0;
-  for (int kind = 0; real && kind < 2; ++kind) {
-    const i32x2 of = p.part_of[kind * p.packed + row];
-    // within the head's part rows, whatever it holds
-    const int64_t first =
-        of[0] < 0 ? 0 : of[0] < p.part_rows ? of[0] : p.part_rows - 1;
-    const int most = (int)((p.part_rows - 1 - first) / kWideRows) + 1;
-    const int count = of[1] < most ? of[1] : most;
-    const int64_t at0 = (int64_t)kv_head * p.part_rows + first;
-    // 4 parts' loads in flight; a part past the last repeats it with weight 0
-    for (int s0 = 4 * g; s0 < count; s0 += 4 * GROUPS) {
-      f32x2 ml[4];
-      f32x4 v[4];
+  // 4 parts' loads in flight; a part past the last repeats it with weight 0
+  for (int s0 = 4 * g; s0 < parts; s0 += 4 * GROUPS) {
+    f32x2 ml[4];
+    f32x4 v[4];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int64_t i =
-            at0 + (int64_t)kWideRows * (s0 + u < count ? s0 + u : count - 1);
-        ml[u] = *(const f32x2 *)(p.part_ml + 2 * i);
-        v[u] = *(const f32x4 *)(p.partials + i * DP + dq);
-      }
-      float x = top;
-#pragma unroll
-      for (int u = 0; u < 4; ++u)
-        x = fmaxf(x, ml[u][0]);
-      const float keep =
-          top == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(top - x);
-      top = x;
-      sum *= keep;
-      acc *= keep;
-#pragma unroll
-      for (int u = 0; u < 4; ++u)
-        if (s0 + u < count) {
-          const float f = ml[u][0] == kNegInf
-                              ? 0.0f
-                              : __builtin_amdgcn_exp2f(ml[u][0] - x);
-          sum += f * ml[u][1];
-          acc += f * v[u];
-        }
+    for (int u = 0; u < 4; ++u) {
+      const int s = s0 + u < parts ? s0 + u : parts - 1;
+      const int64_t i =
+          head_at + (s < counts[0] ? from[0] + kWideRows * s
+                                   : from[1] + kWideRows * (s - counts[0]));
+      ml[u] = *(const f32x2 *)(p.part_ml + 2 * i);
+      v[u] = *(const f32x4 *)(p.partials + i * DP + dq);
     }
-    parts += count > 0 ? count : 0;
+    asm volatile("" ::"v"(v[1]), "v"(v[2]), "v"(v[3]));
+    float x = top;
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      x = fmaxf(x, ml[u][0]);
+    const float keep = top == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(top - x);
+    top = x;
+    sum *= keep;
+    acc *= keep;
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (s0 + u < parts && ml[u][0] != kNegInf) {
+        const float f = __builtin_amdgcn_exp2f(ml[u][0] - x);
+        sum += f * ml[u][1];
+        acc += f * v[u];
+      }
   }
   if constexpr (GROUPS > 1) {
     __shared__ f32x4 group_acc[kPagedThreads];
@@ -1317,7 +1327,7 @@ PagedPlan plan_attention_paged(int64_t rows, int64_t batch, int64_t kv_heads,
   p.workspace = (int64_t)kWorkspaceCounterBytes + 2 * packed * 8 +
                 kv_heads * p.part_rows * (p.dp + 2) * 4;
   if (prefix + capacity <= kPagedWholeKeys ||
-      (uint64_t)p.workspace > workspace_limit) {
+      (uint64_t)p.workspace > workspace_limit || p.part_rows > INT32_MAX) {
     // every tile whole, at most one a workgroup as far as they go: a stretch
     // is no longer than the shortest tile's units
     p.shared = false;
@@ -1371,8 +1381,9 @@ hipError_t launch_attention_paged(const PagedAttention &attention,
                       dim3(kPagedThreads), args, 0, (hipStream_t)stream);
   if (e != hipSuccess || !plan.workspace)
     return e;
-  const int per = kPagedThreads / (plan.dp / 4) / join->groups;
-  return hipLaunchKernel(join->fn, dim3((unsigned)((all + per - 1) / per)),
+  const int64_t per = kPagedThreads / (plan.dp / 4) / join->groups;
+  const int64_t blocks = (a.packed + per - 1) / per * a.kv_heads;
+  return hipLaunchKernel(join->fn, dim3((unsigned)blocks),
                          dim3(kPagedThreads), args, 0, (hipStream_t)stream);
 }
 

@@ -427,7 +427,9 @@ struct PagedAttention {
 // Workgroups wanted (two a CU where head dims allow it), the keys that one
 // takes at least, and the keys that a tile's start and end cost as much as.
 constexpr int64_t kPagedTargetWgs = 512;
-constexpr int64_t kPagedLeastKeys = 128;
+// (64 least: 283 rows of 6 prompts 27.4 -> 24.7 us against 128, 5 requests of
+// a 5024 key prefix 16.1 -> 16.2; 256 least: 31.5 and 17.7.)
+constexpr int64_t kPagedLeastKeys = 64;
 constexpr int64_t kPagedTileKeys = 256;
 // A part is not begun or ended within so many keys of its tile's ends (38
 // requests of a token and at most 21 keys, 3 heads: 18.0 us at 0, 14.8 at 64;
