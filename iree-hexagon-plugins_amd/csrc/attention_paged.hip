@@ -253,6 +253,13 @@ __device__ __forceinline__ void narrow_tile(const PagedTile &t,
                                             float (*wave_m)[kNarrowRows],
                                             float (*wave_l)[kNarrowRows]) {
   const PagedAttention &p = arguments();
+  asm volatile("" ::"s"(p.q), "s"(p.q_row), "s"(p.q_head), "s"(p.k_cache),
+               "s"(p.v_cache), "s"(p.k_head), "s"(p.v_head), "s"(p.group),
+               "s"(p.group_magic), "s"(p.group_shift), "s"(p.dqk), "s"(p.dv),
+               "s"(p.scale), "s"(p.prefix_pages), "s"(p.prefix), "s"(p.pages),
+               "s"(p.page_size), "s"(p.page_shift), "s"(p.page_magic),
+               "s"(p.near), "s"(p.k_page16), "s"(p.k_row16), "s"(p.v_page16),
+               "s"(p.v_row16));
   constexpr int KS = DK / 32;           // head-dim steps of S
   constexpr int DB = DX / 16;           // 16-wide d blocks of O
   constexpr int NCH = DP / 8;           // 16-byte chunks of a V row
@@ -937,9 +944,13 @@ attention_paged_kernel(PagedAttention) {
   __shared__ Requests all;
 
   const PagedAttention &p = arguments();
-  // All of the arguments' cache lines at once, not one after the other.
-  asm volatile("" ::"s"(p.batch), "s"(p.items), "s"(p.table_stride),
-               "s"(p.q_row), "s"(p.k_head));
+  // What the place on the line takes, in one go instead of each where it is
+  // used, a wait apiece (of the other cache lines, a word).
+  asm volatile("" ::"s"(p.row_starts), "s"(p.lengths), "s"(p.batch),
+               "s"(p.rows), "s"(p.group), "s"(p.prefix), "s"(p.capacity),
+               "s"(p.ways), "s"(p.ways_magic), "s"(p.least), "s"(p.unit),
+               "s"(p.tile_units), "s"(p.shared), "s"(p.wide_tokens),
+               "s"(p.items), "s"(p.table_stride), "s"(p.q_row), "s"(p.k_head));
   // Lane l has requests l * each .. + each - 1.
   const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6);
   const int each = (p.batch + 63) >> 6;
@@ -1008,7 +1019,7 @@ attention_paged_kernel(PagedAttention) {
     return;
   uint32_t x_end = x + per < total ? x + per : total;
 
-  auto request_at = [&](int b) {
+  auto request_at = [&](const PagedAttention &p, int b) {
     int of[3];
     if (p.batch <= 64) {
 #pragma unroll
@@ -1034,10 +1045,10 @@ attention_paged_kernel(PagedAttention) {
     start = shared_units +
             (uint32_t)__builtin_amdgcn_readlane((int)(upto - mine), lane_of);
     b = lane_of * each;
-    q = request_at(b);
+    q = request_at(p, b);
     while (start + q.before(q.tiles) <= x && b + 1 < p.batch) {
       start += q.before(q.tiles);
-      q = request_at(++b);
+      q = request_at(p, ++b);
     }
   }
   for (int span = q.tiles; span > 1;) {
@@ -1049,11 +1060,16 @@ attention_paged_kernel(PagedAttention) {
 
   while (x < x_end) {
     const PagedAttention &p = arguments();
+    asm volatile("" ::"s"(p.batch), "s"(p.rows), "s"(p.group), "s"(p.prefix),
+                 "s"(p.capacity), "s"(p.unit), "s"(p.tile_units), "s"(p.snap),
+                 "s"(p.wide_tokens), "s"(p.group_magic), "s"(p.group_shift),
+                 "s"(p.table), "s"(p.table_stride), "s"(p.packed),
+                 "s"(p.partials), "s"(p.part_of));
     if (i >= q.tiles) {  // on to the next request
       start += q.before(q.tiles);
       if (++b >= p.batch)
         return;
-      q = request_at(b);
+      q = request_at(p, b);
       i = 0;
       continue;
     }
