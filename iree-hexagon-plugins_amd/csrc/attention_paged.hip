@@ -1010,8 +1010,8 @@ attention_paged_kernel(PagedAttention) {
   const uint32_t shared_units = q.before(q.tiles);
   const uint32_t total =
       shared_units + (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
-  // enough for `ways` of them to reach the end
-  uint32_t per = p.ways == 1 ? total : __umulhi(total, p.ways_magic) + 1;
+  // enough for `ways` of them to reach the end (without tiles x is not below)
+  uint32_t per = p.ways == 1 ? total : __umulhi(total - 1, p.ways_magic) + 1;
   per = per < (uint32_t)p.least ? p.least : per;
   float inv_per = 1.0f / (float)per;
   uint32_t x = (uint32_t)way * per;  // below 2^32: `ways` is at most 2^24
@@ -1342,16 +1342,17 @@ PagedPlan plan_attention_paged(int64_t rows, int64_t batch, int64_t kv_heads,
   p.part_rows = 2 * packed + kWideRows * p.ways;
   p.workspace = (int64_t)kWorkspaceCounterBytes + 2 * packed * 8 +
                 kv_heads * p.part_rows * (p.dp + 2) * 4;
-  if (prefix + capacity <= kPagedWholeKeys ||
+  const int64_t tiles = batch + packed / (p.wide ? kWideRows : kNarrowRows);
+  const int64_t most =
+      tiles * kv_heads <= wgs ? kPagedWholeKeysFew : kPagedWholeKeys;
+  if (prefix + capacity <= most ||
       (uint64_t)p.workspace > workspace_limit || p.part_rows > INT32_MAX) {
-    // every tile whole, at most one a workgroup as far as they go: a stretch
-    // is no longer than the shortest tile's units
+    // every tile whole and one unit, so each workgroup takes as many
     p.shared = false;
     p.workspace = p.part_rows = 0;
-    p.least = p.tile_units;
-    const int64_t tiles =
-        batch + packed / (p.wide ? kWideRows : kNarrowRows);
-    p.ways = 4 * p.ways < 3 * tiles + 1 ? 4 * p.ways : 3 * tiles + 1;
+    p.unit = 31;
+    p.least = p.tile_units = p.snap = 1;
+    p.ways = 4 * p.ways < tiles ? 4 * p.ways : tiles;
   }
   return p;
 }

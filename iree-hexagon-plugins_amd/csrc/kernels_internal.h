@@ -438,8 +438,15 @@ constexpr int64_t kPagedTileKeys = 256;
 constexpr int64_t kPagedSnapKeys = 64;
 // A wide tile's keys in eighths of a narrow one's cost.
 constexpr uint32_t kWideCost = 10;
-// Keys up to which a tile is not split: its parts would take longer to join.
+// Keys up to which no tile is split: a second launch to join the parts costs
+// 4 us, a tile 0.8 us for 128 keys. More of them where the tiles that there
+// can be run at once (38 requests of 21 keys, 768 possible: 14.1 -> 9.4 us
+// whole; 28 of 42 keys and a prefix of 157, 925 possible: 15.0 -> 10.3; 75
+// requests that then read a prefix of 514 each 20.5 -> 22.6; at most 1529
+// possible: 17 -> 31, at worst), fewer where they are not (808 tiles, 745
+// keys: 23.3 -> 25.7).
 constexpr int64_t kPagedWholeKeys = 512;
+constexpr int64_t kPagedWholeKeysFew = 1024;
 // Rows (of all heads) up to which a row's parts are joined by several groups.
 constexpr int64_t kPagedFewRows = 8192;
 struct PagedPlan {
