@@ -561,6 +561,217 @@ def test_two_streams_and_capture(pkg, dev):
     batches[0].check(outs[0])
 
 
+# Tables that could name more than 1024 keys, so that tiles are shared out and
+# their parts joined, whatever the lengths are in the end.
+
+def columns(page, keys=1100):
+    return up(keys, page)
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+def test_attention_parts(pkg, dev, shape):
+    cached, added, heads, hk, d, dv, page, prefix = shape
+    print(f"parts {shape}", flush=True)
+    a = Attention(cached, added, heads, hk, d, dv, page, prefix, pad=3,
+                  spare=columns(page), seed=len(cached) + d)
+    a.check(a.call(pkg))
+
+
+@pytest.mark.parametrize("seed", range(12))
+def test_attention_drawn(pkg, dev, seed):
+    """Small and large requests in any order, lengths around a part's ends."""
+    g = torch.Generator().manual_seed(seed)
+
+    def one(*of):
+        return of[int(torch.randint(0, len(of), (1,), generator=g))]
+
+    batch = one(1, 2, 5, 9)
+    cached = [one(0, 1, 63, 64, 65, 200, 321, 700) for _ in range(batch)]
+    added = [one(0, 1, 1, 2, 5, 16, 17, 40, 130) for _ in range(batch)]
+    hk = one(1, 2, 3)
+    heads, d = hk * one(1, 3, 4, 8), one(8, 40, 64, 80, 128, 192)
+    page, prefix = one(1, 5, 16, 64, 100), one(0, 0, 1, 64, 127, 450, 1300)
+    print(f"drawn {cached} {added} {heads} {hk} {d} {page} {prefix}",
+          flush=True)
+    a = Attention(cached, added, heads, hk, d, min(d, 128), page, prefix,
+                  pad=one(0, 1, 7), spare=one(0, 1, columns(page)),
+                  token_major=one(False, True), seed=seed)
+    a.check(a.call(pkg))
+
+
+@pytest.mark.parametrize("batch", [33, 65, 200])
+def test_attention_batches_parts(pkg, dev, batch):
+    g = torch.Generator().manual_seed(batch + 1)
+    cached = torch.randint(0, 70, (batch,), generator=g).tolist()
+    added = torch.randint(0, 4, (batch,), generator=g).tolist()
+    print(f"batch {batch}", flush=True)
+    for prefix in (0, 50, 700):
+        a = Attention(cached, added, 4, 2, 64, 64, 16, prefix, seed=batch,
+                      spare=columns(16), pad=2)
+        a.check(a.call(pkg))
+        added[::10] = [n + 14 for n in added[::10]]
+
+
+@pytest.mark.parametrize("added", [[1, 1, 1], [60, 2, 33], [0, 0, 0]])
+def test_attention_pages_outside_the_cache_parts(pkg, dev, added):
+    """Pages that the cache does not have, lengths below 0, requests without
+    rows, where there are parts."""
+    a = Attention([40, 1000, 70], added, 4, 2, 64, 64, 16, 1500, pad=1,
+                  spare=columns(16))
+    pages = a.kc.shape[0]
+    a.table[0][1], a.table[1][0] = -1, pages
+    a.table[1][30:50] = [2 ** 31 - 1] * 20
+    a.prefix_pages[20:60] = [-2 ** 31] * 40
+    a.check(a.call(pkg))
+    a.prefix_pages = [pages + 5] * len(a.prefix_pages)
+    a.table = [[-1] * a.width] * 3
+    rows = sum(added)
+    assert bool((a.call(pkg)[:rows] == 0).all())
+    a.prefix, a.prefix_pages = 0, []
+    a.lengths = [-1, -2 ** 31, 0]
+    o = a.call(pkg)
+    assert bool((o[:rows] == 0).all()) and bool((o[rows:] == 9).all())
+
+
+def test_attention_row_starts(pkg, dev):
+    """Starts below 0, past the rows or out of order: rows stay within the
+    tensors, and requests in order get their rows."""
+    a = Attention([40, 9, 30, 4], [2, 3, 20, 1], 4, 2, 64, 64, 16, 70, pad=3)
+    for spare in (0, columns(16)):
+        a.table = [r + [-1] * spare for r in a.table]
+        a.width += spare
+        a.starts = [0, 2, 5, 25, 26]
+        a.check(a.call(pkg))
+        want, bound = a.expected()
+        # request 3's end lies past the rows: the padding is its. The others'
+        # rows have their keys (the parts' ends move with all requests' rows,
+        # so not the same roundings).
+        a.starts[4] = 2 ** 31 - 1
+        o = a.call(pkg)
+        assert bool(((o.double().cpu() - want).abs() <= bound)[:25].all())
+        assert not bool((o == 9).all(-1).any())
+        for starts in ([-5, -1, 5, 25, 26], [7, 2, 25, 5, 26],
+                       [-2 ** 31, 2 ** 31 - 1, 0, 2 ** 31 - 1, 3]):
+            a.starts = starts
+            a.call(pkg)
+    torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("added", [2, 40])
+def test_attention_long_lines(pkg, dev, added):
+    """A table that could name 2^26 keys a request: keys are shared out in
+    larger units, with few and with many rows."""
+    page, batch = 1 << 16, 40
+    cached = [9000, 70, 3000] + [7 * i % 40 for i in range(batch - 3)]
+    a = Attention(cached, [added, 1, 0, added] + [1] * (batch - 4), 2, 1, 8,
+                  8, page, 100, spare=1023)
+    a.check(a.call(pkg))
+
+
+@pytest.mark.parametrize("added", [1, 40])
+def test_attention_far_pages(pkg, dev, added):
+    """Pages of a cache past 2^32 elements, for narrow and wide tiles."""
+    a = Attention([20, 9], [added, 2], 2, 1, 8, 8, 16, 20, spare=columns(16))
+    want = a.call(pkg).clone()
+    pages = a.kc.shape[0]
+    buf = torch.zeros((1 << 30) * (pages - 1) + 128, dtype=H, device="cuda")
+    far = buf.as_strided(a.kc.shape, (1 << 30, 128, 8, 1))
+    far.copy_(a.kc)
+    a.kc = far
+    assert torch.equal(a.call(pkg), want)
+    a.check(want)
+
+
+def test_stream_argument(pkg, dev):
+    """Each call on the stream that it names, behind that stream's work."""
+    a = Attention([900, 40], [1, 30], 4, 2, 64, 64, 16, 1500)
+    want = a.call(pkg).clone()
+    table, page = ints([[3, -1, -1], [5, 6, -1]]), 16
+    k = torch.randn(4, 2, 64, device="cuda").half()
+    caches = [torch.zeros(9, 2, page, 64, dtype=H, device="cuda")
+              for _ in range(2)]
+    free, cached, added = ints([1, 2, 7]), ints([15, 30]), ints([2, 2])
+    o = torch.empty_like(want)
+    lengths = torch.zeros(2, dtype=I32, device="cuda")
+    t = [ints(a.starts), lengths, ints(a.table), ints(a.prefix_pages)]
+    late = ints(a.lengths)
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    big = torch.randn(4096, 4096, device="cuda")
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s):  # the lengths arrive behind some work
+        for _ in range(10):
+            big = big @ big * 1e-3
+        lengths.copy_(late)
+    pkg.shared_prefix_attention(a.q, a.kc, a.vc, *t, a.prefix, o, stream=s)
+    starts, total, slots, needed = pkg.page_tables(
+        cached, added, free, table, page, 4, stream=s)
+    pkg.append_kv(k, k, *caches, slots, stream=s)
+    s.synchronize()
+    assert torch.equal(o, want)
+    assert table.tolist() == [[3, 1, -1], [5, 6, -1]]
+    assert slots.tolist() == [3 * 16 + 15, 16, 6 * 16 + 14, 6 * 16 + 15]
+    assert needed.tolist() == [1] and total.tolist() == [17, 32]
+    for c in caches:
+        flat = c.transpose(1, 2).reshape(-1, 2, 64)
+        assert torch.equal(flat[slots.long()], k)
+
+
+def test_captured_step(pkg, dev):
+    """Tables, rows and attention of a step in one graph, whose replays read
+    what its inputs hold then; eager steps between give the same."""
+    page, pages, width, heads, hk, d = 16, 40, 80, 4, 2, 64
+    g = torch.Generator().manual_seed(3)
+    start = ints([[0, 1] + [-1] * (width - 2), [2] + [-1] * (width - 1)])
+
+    def state():
+        return {"cached": ints([20, 9]), "added": ints([1, 3]),
+                "free": ints(range(10, 20)), "table": start.clone(),
+                "kc": torch.zeros(pages, hk, page, d, dtype=H, device="cuda"),
+                "vc": torch.zeros(pages, hk, page, d, dtype=H, device="cuda"),
+                "kv": torch.zeros(6, hk, d, dtype=H, device="cuda"),
+                "q": torch.zeros(6, heads, d, dtype=H, device="cuda"),
+                "o": torch.zeros(6, heads, d, dtype=H, device="cuda")}
+
+    def step(t):
+        starts, lengths, slots, needed = pkg.page_tables(
+            t["cached"], t["added"], t["free"], t["table"], page, 6)
+        pkg.append_kv(t["kv"], t["kv"], t["kc"], t["vc"], slots)
+        pkg.shared_prefix_attention(
+            t["q"], t["kc"], t["vc"], starts, lengths, t["table"],
+            ints_none, 0, t["o"])
+        return lengths, needed
+
+    ints_none = torch.empty(0, dtype=I32, device="cuda")
+    captured, eager = state(), state()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step(state())
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        lengths, needed = step(captured)
+    for added in ([1, 3], [4, 0], [2, 4], [0, 0], [1, 1]):
+        q, kv = (torch.randn(6, n, d, generator=g).half().cuda()
+                 for n in (heads, hk))
+        for t in (captured, eager):
+            t["added"].copy_(ints(added))
+            t["q"].copy_(q)
+            t["kv"].copy_(kv)
+        graph.replay()
+        their_lengths, their_need = step(eager)
+        torch.cuda.synchronize()
+        for n in ("table", "kc", "vc", "o"):
+            assert torch.equal(captured[n], eager[n]), n
+        assert torch.equal(lengths, their_lengths)
+        assert torch.equal(needed, their_need)
+        used = int(needed)
+        for t, n in ((captured, lengths), (eager, their_lengths)):
+            t["cached"].copy_(n)
+            t["free"].copy_(t["free"].roll(-used))
+
+
 # ------------------------------------------------------------- all together --
 
 def test_steps(pkg, dev):
