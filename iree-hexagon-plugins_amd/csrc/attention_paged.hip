@@ -1336,7 +1336,7 @@ PagedPlan plan_attention_paged(int64_t rows, int64_t batch, int64_t kv_heads,
   while (line / (double)((int64_t)1 << p.unit) >= 1e9)
     ++p.unit;
   auto units = [&](int64_t keys) { return (keys >> p.unit) + 1; };
-  p.least = units(kPagedLeastKeys + kPagedTileKeys);
+  p.least = units(kPagedLeastKeys);
   p.tile_units = units(kPagedTileKeys);
   p.snap = units(kPagedSnapKeys);
   p.part_rows = 2 * packed + kWideRows * p.ways;

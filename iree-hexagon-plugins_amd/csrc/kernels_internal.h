@@ -424,13 +424,19 @@ struct PagedAttention {
   int64_t k_head, v_head;
   float scale;
 };
-// Workgroups wanted (two a CU where head dims allow it), the keys that one
-// takes at least, and the keys that a tile's start and end cost as much as.
+// Workgroups wanted: two a CU where head dims allow it (768 and 1024 instead
+// of 512: 64 requests' tokens behind a prefix 48.5 -> 59 us and more, prompts
+// of 4 x 1000 rows 240 -> 272).
 constexpr int64_t kPagedTargetWgs = 512;
-// (64 least: 283 rows of 6 prompts 27.4 -> 24.7 us against 128, 5 requests of
-// a 5024 key prefix 16.1 -> 16.2; 256 least: 31.5 and 17.7.)
-constexpr int64_t kPagedLeastKeys = 64;
+// The keys that a tile's start and end cost as much as: 256 balances many
+// tiles (160: tokens 48.5 -> 49.7, 101 tiles a head 23.2 -> 25.8 us; 384: 49.9,
+// 26.5).
 constexpr int64_t kPagedTileKeys = 256;
+// What one takes at least, keys and tiles' shares. Where all the work is short
+// fewer keys each end sooner, down to a step or two (5 requests of a 5024 key
+// prefix: 15.9 us at 320, 13.3 at 224, 14.4 at 160; one request of 1001 keys,
+// 192-wide: 15.9, 12.7, 12.8).
+constexpr int64_t kPagedLeastKeys = 224;
 // A part is not begun or ended within so many keys of its tile's ends (38
 // requests of a token and at most 21 keys, 3 heads: 18.0 us at 0, 14.8 at 64;
 // 771 rows of a prompt: 36.1, 28.9; drafts of 12 requests 21.1, 20.8, but 22.7
