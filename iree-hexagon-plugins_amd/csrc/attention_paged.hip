@@ -511,26 +511,33 @@ __device__ __forceinline__ void narrow_tile(const PagedTile &t,
 // ring, rows of 16-byte chunks swizzled on the copy side (as attention.hip's):
 // K is read 16 lanes = 16 keys at one chunk, V transposed, 32 lanes = 4 keys
 // x 32 columns.
+// Elements of a staged K row: V's, or the next power of two.
+constexpr int staged_k(int dp, int dk) { return dk > dp ? 2 * dp : dp; }
 template <int DP>
 __device__ __forceinline__ int wide_k_swizzle(int key) {
-  return DP == 128 ? (key & 15) : ((key >> 1) & 7);
+  return DP >= 128 ? (key & 15) : ((key >> 1) & 7);
 }
 template <int DP>
 __device__ __forceinline__ int wide_v_swizzle(int key) {
   return DP == 128 ? 4 * (key & 3) : 4 * ((key >> 1) & 1);
 }
 
-template <int DP, int DX>
+template <int DP, int DX, int DK>
 __device__ __forceinline__ void wide_tile(const PagedTile &t,
                                           const Requests &all, char *smem) {
   const PagedAttention &p = arguments();
-  constexpr int DS = DX / 16;         // 16-wide d steps of S^T = K Q^T
+  constexpr int DS = DK / 16;         // 16-wide d steps of S^T = K Q^T
   constexpr int DT = DX / 32;         // 32-row d tiles of O^T
-  constexpr int ROW = DP * 2;         // bytes of a staged row
-  constexpr int CH = ROW / 16;        // its 16-byte chunks
-  constexpr int BLK = kStepKeys * ROW;
-  constexpr int ROWS = 64 / CH;       // rows a copy instruction moves
+  // Of K, then V: bytes of a staged row, its 16-byte chunks, rows that a copy
+  // instruction moves.
+  constexpr int KP = staged_k(DP, DK), KROW = KP * 2, ROW = DP * 2;
+  constexpr int KCH = KROW / 16, CH = ROW / 16;
+  constexpr int KBLK = kStepKeys * KROW, BLK = kStepKeys * ROW;
+  constexpr int KROWS = 64 / KCH, ROWS = 64 / CH;
+  constexpr int KPASSES = kStepKeys / (kPagedWaves * KROWS);
   constexpr int PASSES = kStepKeys / (kPagedWaves * ROWS);
+  // Passes of K after which its swizzle, of 16 rows, is the same again.
+  constexpr int TURN = kPagedWaves * KROWS < 16 ? 16 / (kPagedWaves * KROWS) : 1;
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -565,40 +572,54 @@ __device__ __forceinline__ void wide_tile(const PagedTile &t,
   // Copy side: an instruction moves ROWS rows of CH chunks, lane -> (row,
   // physical chunk), fetching the logical chunk that belongs there if it lies
   // within the head dim (the LDS past it is zeroed once and never written).
-  // The swizzles repeat every 16 rows, so the chunk is the same in all passes.
+  // The swizzles repeat every 16 rows, so V's chunk is the same in all passes.
   // Where pages are multiples of ROWS tokens an instruction's rows follow one
   // another in a page; with a head's rows within 4 GiB their place is then one
-  // scalar offset, and a lane's own the same for all copies: 28 instructions a
-  // block, which a wave issues one by one, instead of 100.
-  const int c_row = lane / CH, c_phys = lane % CH;
-  const int k_chunk = c_phys ^ wide_k_swizzle<DP>(wave * ROWS + c_row);
-  const int v_chunk = c_phys ^ wide_v_swizzle<DP>(wave * ROWS + c_row);
-  const bool k_in = 8 * k_chunk < p.dqk, v_in = 8 * v_chunk < p.dv;
+  // scalar offset, and a lane's own the same for all copies: fewer
+  // instructions to issue, though within a run's noise of the other form.
+  static_assert(ROWS % KROWS == 0, "a group of V's rows holds K's");
+  const int k_at = lane / KCH, v_at = lane / CH;
+  int k_chunk[TURN];
+  bool k_in[TURN];
+#pragma unroll
+  for (int i = 0; i < TURN; ++i) {
+    k_chunk[i] = lane % KCH ^ wide_k_swizzle<KP>(
+                                  (i * kPagedWaves + wave) * KROWS + k_at);
+    k_in[i] = 8 * k_chunk[i] < p.dqk;
+  }
+  const int v_chunk = lane % CH ^ wide_v_swizzle<DP>(wave * ROWS + v_at);
+  const bool v_in = 8 * v_chunk < p.dv;
   const Pages pages(p, t);
   const bool grouped = pages.near && pages.page_size % ROWS == 0;
-  const bool alike =
-      pages.k_page == pages.v_page && pages.k_row == pages.v_row;
+  const bool alike = KPASSES == PASSES && pages.k_page == pages.v_page &&
+                     pages.k_row == pages.v_row;
   const int group = grouped ? ROWS : 1;
-  const uint32_t k_lane = ((uint32_t)c_row * pages.k_row + k_chunk) * 16;
-  const uint32_t v_lane = ((uint32_t)c_row * pages.v_row + v_chunk) * 16;
+  uint32_t k_lane[TURN];
+#pragma unroll
+  for (int i = 0; i < TURN; ++i)
+    k_lane[i] = ((uint32_t)k_at * pages.k_row + k_chunk[i]) * 16;
+  const uint32_t v_lane = ((uint32_t)v_at * pages.v_row + v_chunk) * 16;
   const i32x4 k_rows = rows_from(Kp), v_rows = rows_from(Vp);
   IHP_LDS char *lds = (IHP_LDS char *)smem;
   PagedBlock<kStepKeys> block;
   auto copy = [&](int slot) {
-    IHP_LDS char *kd = lds + slot * BLK + wave * (ROWS * ROW);
-    IHP_LDS char *vd = kd + 2 * BLK;
+    IHP_LDS char *kd = lds + slot * KBLK + wave * (KROWS * KROW);
+    IHP_LDS char *vd = lds + 2 * KBLK + slot * BLK + wave * (ROWS * ROW);
+    constexpr int KNEXT = kPagedWaves * KROWS * KROW;
     constexpr int NEXT = kPagedWaves * ROWS * ROW;
     if (grouped) {
-      uint32_t at[PASSES];
+      uint32_t at[KPASSES];
 #pragma unroll
-      for (int i = 0; i < PASSES; ++i)
+      for (int i = 0; i < KPASSES; ++i)
         at[i] = (uint32_t)__builtin_amdgcn_readlane(
-                    (int)block.k, (i * kPagedWaves + wave) * ROWS) *
+                    (int)block.k, (i * kPagedWaves + wave) * KROWS) *
                 16;
-      if (k_in)
 #pragma unroll
-        for (int i = 0; i < PASSES; ++i)
-          buffer_to_lds_16(k_rows, k_lane, at[i], kd + i * NEXT);
+      for (int turn = 0; turn < TURN; ++turn)
+        if (k_in[turn])
+#pragma unroll
+          for (int i = turn; i < KPASSES; i += TURN)
+            buffer_to_lds_16(k_rows, k_lane[turn], at[i], kd + i * KNEXT);
       if (!alike)
 #pragma unroll
         for (int i = 0; i < PASSES; ++i)
@@ -610,23 +631,28 @@ __device__ __forceinline__ void wide_tile(const PagedTile &t,
         for (int i = 0; i < PASSES; ++i)
           buffer_to_lds_16(v_rows, v_lane, at[i], vd + i * NEXT);
     } else {
-      uint32_t at[2 * PASSES];
+      uint32_t k_of[KPASSES], v_of[PASSES];
 #pragma unroll
-      for (int i = 0; i < PASSES; ++i) {
-        const int row = (i * kPagedWaves + wave) * ROWS + c_row;
-        at[i] = (uint32_t)__shfl((int)block.k, row);
-        at[PASSES + i] = (uint32_t)__shfl((int)block.v, row);
-      }
+      for (int i = 0; i < KPASSES; ++i)
+        k_of[i] = (uint32_t)__shfl(
+            (int)block.k, (i * kPagedWaves + wave) * KROWS + k_at);
 #pragma unroll
-      for (int i = 0; i < PASSES; ++i) {
-        if (k_in)
-          global_to_lds_16(Kp + ((uint64_t)at[i] + (uint32_t)k_chunk) * 16,
-                           kd + i * NEXT);
-        if (v_in)
-          global_to_lds_16(
-              Vp + ((uint64_t)at[PASSES + i] + (uint32_t)v_chunk) * 16,
-              vd + i * NEXT);
-      }
+      for (int i = 0; i < PASSES; ++i)
+        v_of[i] = (uint32_t)__shfl(
+            (int)block.v, (i * kPagedWaves + wave) * ROWS + v_at);
+#pragma unroll
+      for (int turn = 0; turn < TURN; ++turn)
+        if (k_in[turn])
+#pragma unroll
+          for (int i = turn; i < KPASSES; i += TURN)
+            global_to_lds_16(
+                Kp + ((uint64_t)k_of[i] + (uint32_t)k_chunk[turn]) * 16,
+                kd + i * KNEXT);
+      if (v_in)
+#pragma unroll
+        for (int i = 0; i < PASSES; ++i)
+          global_to_lds_16(Vp + ((uint64_t)v_of[i] + (uint32_t)v_chunk) * 16,
+                           vd + i * NEXT);
     }
   };
 
@@ -634,10 +660,10 @@ __device__ __forceinline__ void wide_tile(const PagedTile &t,
   // ring is aligned, and the swizzle flips chunk bits only). V^T reads: load
   // lane j = lane % 16 of block b = lane / 16 reads row kstart + j / 4,
   // columns 32 dt + 16 (b % 2) + 4 (j % 4) .. + 3.
-  const int k_sw = wide_k_swizzle<DP>(l32);
+  const int k_sw = wide_k_swizzle<KP>(l32);
   const uint32_t ka =
       (uint32_t)(uintptr_t)lds +
-      (uint32_t)(l32 * ROW + 16 * (g ^ (k_sw & 1)) + 32 * (k_sw >> 1));
+      (uint32_t)(l32 * KROW + 16 * (g ^ (k_sw & 1)) + 32 * (k_sw >> 1));
   const int vj = lane & 15, vb = lane >> 4;
   int v_off[DT];
 #pragma unroll
@@ -662,8 +688,8 @@ __device__ __forceinline__ void wide_tile(const PagedTile &t,
   // Every wave has finished with the LDS of the tile before.
   wait_lgkmcnt0();
   block_barrier();
-  if (p.dqk != DP || p.dv != DP) {
-    for (int i = tid * 16; i < 4 * BLK; i += kPagedThreads * 16)
+  if (p.dqk != DK || p.dv != DX) {
+    for (int i = tid * 16; i < 2 * (KBLK + BLK); i += kPagedThreads * 16)
       *(IHP_LDS i32x4 *)(lds + i) = i32x4{0, 0, 0, 0};
     wait_lgkmcnt0();
     block_barrier();
@@ -686,7 +712,7 @@ __device__ __forceinline__ void wide_tile(const PagedTile &t,
     if (live != ~0ull) {  // keys that are not there: their V rows are zeros
       for (int i = tid; i < kStepKeys * CH; i += kPagedThreads)
         if (!(live >> (i / CH) & 1))
-          *(IHP_LDS i32x4 *)(lds + (2 + slot) * BLK + i * 16) =
+          *(IHP_LDS i32x4 *)(lds + 2 * KBLK + slot * BLK + i * 16) =
               i32x4{0, 0, 0, 0};
       wait_lgkmcnt0();
       block_barrier();
@@ -705,12 +731,12 @@ __device__ __forceinline__ void wide_tile(const PagedTile &t,
     // workgroup's wave on the SIMD leaves its softmax for these.
     __builtin_amdgcn_s_setprio(1);
     {
-      const uint32_t kbase = ka + (uint32_t)(slot * BLK);
+      const uint32_t kbase = ka + (uint32_t)(slot * KBLK);
       constexpr int NR = 2 * DS, KW = 3, NB = KW + 1;
       i32x4 kb[NB];
       auto issue = [&](auto r_c) {
         constexpr int R = decltype(r_c)::value;
-        kb[R % NB] = lds_read_16_async<32 * (R % 2) * ROW>(
+        kb[R % NB] = lds_read_16_async<32 * (R % 2) * KROW>(
             (const IHP_LDS char *)(uintptr_t)(kbase ^ (32u * (R / 2))));
       };
       static_for<KW>(issue);
@@ -785,7 +811,7 @@ __device__ __forceinline__ void wide_tile(const PagedTile &t,
     __builtin_amdgcn_s_setprio(1);
     {
       float psum[4];
-      const IHP_LDS char *vs = lds + (2 + slot) * BLK;
+      const IHP_LDS char *vs = lds + 2 * KBLK + slot * BLK;
       i32x2 vr[2][DT][2];
       auto read_v = [&](auto step_c) {
         constexpr int ST = decltype(step_c)::value;
@@ -927,11 +953,12 @@ __device__ __forceinline__ Request request(const PagedAttention &p, int begin,
 
 // WIDE: requests of more than 16 rows have wide tiles.
 template <int DP, int DX, int DK, bool WIDE>
-__global__ __launch_bounds__(kPagedThreads, DP >= 256 ? 1 : 2) void
+__global__ __launch_bounds__(kPagedThreads,
+                             DP >= 256 || (WIDE && DK > 128) ? 1 : 2) void
 attention_paged_kernel(PagedAttention) {
   constexpr int VBYTES = kBlockKeys * DP * 2;
   constexpr int MERGE = kPagedWaves * 16 * (DP + 4) * 4;
-  constexpr int RING = WIDE ? 4 * kStepKeys * DP * 2 : 0;
+  constexpr int RING = WIDE ? 4 * kStepKeys * (DP + staged_k(DP, DK)) : 0;
   constexpr int NARROW =
       kPagedWaves * VBYTES > MERGE ? kPagedWaves * VBYTES : MERGE;
   constexpr int SMEM = NARROW > RING ? NARROW : RING;
@@ -1151,7 +1178,7 @@ attention_paged_kernel(PagedAttention) {
     if (shift == 4)
       narrow_tile<DP, DX, DK>(t, all, smem, wave_m, wave_l);
     else if constexpr (WIDE)
-      wide_tile<DP, DX>(t, all, smem);
+      wide_tile<DP, DX, DK>(t, all, smem);
     asm volatile("" ::: "memory");
     const Line &l = line_at[wave];
     x = (uint32_t)uniform((int)l.x);
@@ -1284,20 +1311,22 @@ namespace {
 struct PagedKernel {
   const char *name;
   int dp, dx, dk, groups;  // groups: of a joined row's parts
+  bool wide;
   const void *fn;
 };
 const PagedKernel kPagedKernels[] = {
 #define IHP_PAGED(NAME, DP, DX, DK, WIDE)                                      \
-  {"attention_paged_" NAME, DP, DX, DK, 0,                                     \
+  {"attention_paged_" NAME, DP, DX, DK, 0, WIDE,                               \
    (const void *)&attention_paged_kernel<DP, DX, DK, WIDE>}
     IHP_PAGED("d64", 64, 64, 64, true),
     IHP_PAGED("d96", 128, 96, 96, true),
     IHP_PAGED("d128", 128, 128, 128, true),
     IHP_PAGED("d192_128", 128, 128, 192, false),
+    IHP_PAGED("d192_128_rows", 128, 128, 192, true),
     IHP_PAGED("d256", 256, 256, 256, false),
 #undef IHP_PAGED
 #define IHP_JOIN(DP, GROUPS)                                                   \
-  {"attention_paged_join_d" #DP "_g" #GROUPS, DP, DP, DP, GROUPS,                  \
+  {"attention_paged_join_d" #DP "_g" #GROUPS, DP, DP, DP, GROUPS, false,      \
    (const void *)&attention_paged_join_kernel<DP, GROUPS>}
     IHP_JOIN(64, 1),
     IHP_JOIN(64, 8),
@@ -1318,15 +1347,19 @@ PagedPlan plan_attention_paged(int64_t rows, int64_t batch, int64_t kv_heads,
                                size_t workspace_limit) {
   PagedPlan p = {};
   const int64_t d = head_dim > head_dim_v ? head_dim : head_dim_v;
-  p.wide = d <= 128;
-  const bool longer_k = !p.wide && head_dim <= 192 && head_dim_v <= 128;
+  const int64_t packed = rows * group;
+  const bool longer_k = d > 128 && head_dim <= 192 && head_dim_v <= 128;
+  // Wide tiles of longer keys fill a CU's LDS alone: only where some request
+  // must have more than 16 rows (653 of two, 3 heads each, 3947 keys ahead:
+  // 72.3 -> 38.3 us; 181 rows of 4 heads, 696 ahead: 18.2 -> 21.0).
+  p.wide = d <= 128 || (longer_k && packed > batch * kSmallRows);
   p.dp = d <= 64 ? 64 : d <= 128 || longer_k ? 128 : 256;
   p.dx = d > 64 && d <= 96 ? 96 : p.dp;
   p.dk = longer_k ? 192 : p.dx;
-  const int64_t packed = rows * group;
   // Requests that fill wide tiles walk the prefix themselves, as one alone.
   p.shared = prefix > 0 && batch > 1;
-  const int64_t wgs = p.dp < 256 ? kPagedTargetWgs : kPagedTargetWgs / 2;
+  const bool two = p.dp < 256 && !(p.wide && p.dk > 128);  // a CU holds
+  const int64_t wgs = two ? kPagedTargetWgs : kPagedTargetWgs / 2;
   p.ways = wgs / kv_heads > 1 ? wgs / kv_heads : 1;
   // The line in 32 bits, also where row_starts do not ascend and every request
   // has all rows.
@@ -1343,8 +1376,10 @@ PagedPlan plan_attention_paged(int64_t rows, int64_t batch, int64_t kv_heads,
   p.workspace = (int64_t)kWorkspaceCounterBytes + 2 * packed * 8 +
                 kv_heads * p.part_rows * (p.dp + 2) * 4;
   const int64_t tiles = batch + packed / (p.wide ? kWideRows : kNarrowRows);
-  const int64_t most =
-      tiles * kv_heads <= wgs ? kPagedWholeKeysFew : kPagedWholeKeys;
+  const bool rows_many = p.wide && packed > batch * kSmallRows;
+  const int64_t most = tiles * kv_heads > wgs ? kPagedWholeKeys
+                       : rows_many            ? kPagedWholeKeysWide
+                                              : kPagedWholeKeysFew;
   if (prefix + capacity <= most ||
       (uint64_t)p.workspace > workspace_limit || p.part_rows > INT32_MAX) {
     // every tile whole and one unit, so each workgroup takes as many
@@ -1385,7 +1420,8 @@ hipError_t launch_attention_paged(const PagedAttention &attention,
   const PagedKernel *kernel = nullptr, *join = nullptr;
   for (const PagedKernel &k : kPagedKernels)
     if (k.dp == plan.dp) {
-      if (k.groups == 0 && k.dx == plan.dx && k.dk == plan.dk)
+      if (k.groups == 0 && k.dx == plan.dx && k.dk == plan.dk &&
+          k.wide == plan.wide)
         kernel = &k;
       else if (k.groups > 0 && (k.groups > 1) == few)
         join = &k;

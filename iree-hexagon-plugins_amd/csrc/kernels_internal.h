@@ -450,9 +450,11 @@ constexpr uint32_t kWideCost = 10;
 // whole; 28 of 42 keys and a prefix of 157, 925 possible: 15.0 -> 10.3; 75
 // requests that then read a prefix of 514 each 20.5 -> 22.6; at most 1529
 // possible: 17 -> 31, at worst), fewer where they are not (808 tiles, 745
-// keys: 23.3 -> 25.7).
+// keys: 23.3 -> 25.7) or wide, whose keys take twice as long (494 rows, 578
+// possible: 27.1 -> 23.2; 181 rows of 192-wide heads, 952: 21.0 -> 36.0).
 constexpr int64_t kPagedWholeKeys = 512;
 constexpr int64_t kPagedWholeKeysFew = 1024;
+constexpr int64_t kPagedWholeKeysWide = 768;
 // Rows (of all heads) up to which a row's parts are joined by several groups.
 constexpr int64_t kPagedFewRows = 8192;
 struct PagedPlan {

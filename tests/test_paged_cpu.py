@@ -236,9 +236,14 @@ def test_attention_workspace(pkg):
     full = (256 << 10) + rows * (64 + 2) * 4 + 2 * 6 * 4 * 8
     assert need(prefix_length=8192) == need(table_width=99) == full
     assert need(rows=5000, prefix_length=8192) > full + 2 * 8 * 4994 * 66 * 4
-    # up to 512 keys no row has parts
-    assert need() == need(prefix_length=512 - 32) == 0
-    assert need(prefix_length=513 - 32) == full
+    # up to 1024 keys no row has parts; up to 768 where a request must have
+    # more than 16 rows, 512 where there can be more tiles than run at once
+    assert need() == need(prefix_length=1024 - 32) == 0
+    assert need(prefix_length=1025 - 32) == full
+    assert need(rows=50, prefix_length=768 - 32) == 0
+    assert need(rows=50, prefix_length=769 - 32) > full
+    assert need(rows=50000, prefix_length=512 - 32) == 0
+    assert need(rows=50000, prefix_length=513 - 32) > full
     for kw in (dict(rows=0), dict(heads=7), dict(batch=0), dict(rows=1 << 40),
                dict(prefix_length=-1)):
         assert need(**kw) == 0

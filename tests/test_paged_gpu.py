@@ -577,6 +577,17 @@ def test_attention_parts(pkg, dev, shape):
     a.check(a.call(pkg))
 
 
+@pytest.mark.parametrize("spare", [0, 80])
+@pytest.mark.parametrize("added", [[1, 1, 1, 1], [150, 1, 40, 3]])
+@pytest.mark.parametrize("d, dv", [(192, 128), (160, 96), (136, 128),
+                                   (128, 192), (200, 128)])
+def test_attention_unequal_head_dims(pkg, dev, d, dv, added, spare):
+    print(f"unequal {d} {dv} {added} {spare}", flush=True)
+    a = Attention([70, 9, 0, 300], added, 6, 2, d, dv, 16, 100, pad=1,
+                  spare=spare, seed=d)
+    a.check(a.call(pkg))
+
+
 @pytest.mark.parametrize("seed", range(12))
 def test_attention_drawn(pkg, dev, seed):
     """Small and large requests in any order, lengths around a part's ends."""
