@@ -351,11 +351,15 @@ int iree_mi355x_append_kv_f16(const iree_mi355x_kv_cache_t *cache,
 // pages. Rows from row_starts[batch] on are left as they were. A NaN or
 // infinity in the V of a token that a row does not see may reach it where
 // another row of its tile does (0 times it).
-// The prefix's keys are read once for tiles of rows of the whole batch where
-// requests bring few rows each, which takes a workspace; without one every
-// request reads them. A call runs with any workspace or none. Unlike the
-// matmuls' it needs no zero-filled contents; its first 256 KiB (their
-// counters) are left alone. row_starts must ascend from 0.
+// Requests of up to 16 rows (tokens * heads / kv_heads) have the prefix's keys
+// read once for tiles of rows of them all, where there are two of them and
+// prefix and table can name more than some hundred keys; that takes a
+// workspace, and without one (or with a shorter one) every request reads them
+// itself. A call runs with any workspace or none, and gives the same bits each
+// time for the same extents, lengths and workspace. Unlike the matmuls' it
+// needs no zero-filled contents; its first 256 KiB (their counters) are left
+// alone. row_starts must ascend from 0: where it does not, rows hold anything,
+// but nothing outside the tensors is read or written.
 typedef struct iree_mi355x_paged_attention_t {
   iree_mi355x_kv_cache_t cache;
   const void *q;               // [rows, heads, head_dim]

@@ -426,7 +426,7 @@ struct PagedAttention {
 };
 // Workgroups wanted: two a CU where head dims allow it (768 and 1024 instead
 // of 512: 64 requests' tokens behind a prefix 48.5 -> 59 us and more, prompts
-// of 4 x 1000 rows 240 -> 272).
+// of 2243 rows 240 -> 272).
 constexpr int64_t kPagedTargetWgs = 512;
 // The keys that a tile's start and end cost as much as: 256 balances many
 // tiles (160: tokens 48.5 -> 49.7, 101 tiles a head 23.2 -> 25.8 us; 384: 49.9,
@@ -442,10 +442,12 @@ constexpr int64_t kPagedLeastKeys = 224;
 // 771 rows of a prompt: 36.1, 28.9; drafts of 12 requests 21.1, 20.8, but 22.7
 // at 128 and 23.8 at 256, which leave workgroups without work).
 constexpr int64_t kPagedSnapKeys = 64;
-// A wide tile's keys in eighths of a narrow one's cost.
+// A wide tile's keys in eighths of a narrow one's cost (8: drafts of 12
+// requests 23.3 us, one prompt among tokens 39.0; 10: 21.5, 37.0; 12 within a
+// run's noise of 10).
 constexpr uint32_t kWideCost = 10;
 // Keys up to which no tile is split: a second launch to join the parts costs
-// 4 us, a tile 0.8 us for 128 keys. More of them where the tiles that there
+// 4 us, 128 more keys of a narrow tile 1.3. More of them where the tiles that there
 // can be run at once (38 requests of 21 keys, 768 possible: 14.1 -> 9.4 us
 // whole; 28 of 42 keys and a prefix of 157, 925 possible: 15.0 -> 10.3; 75
 // requests that then read a prefix of 514 each 20.5 -> 22.6; at most 1529
@@ -455,7 +457,9 @@ constexpr uint32_t kWideCost = 10;
 constexpr int64_t kPagedWholeKeys = 512;
 constexpr int64_t kPagedWholeKeysFew = 1024;
 constexpr int64_t kPagedWholeKeysWide = 768;
-// Rows (of all heads) up to which a row's parts are joined by several groups.
+// Rows (of all heads) up to which a row's parts are joined by several groups
+// (768 rows of 32749 keys: 52.6 -> 47.8 us; 12960 rows of a prompt and tokens
+// 32.9, with groups 39.1; 71776 rows of prompts 241, with groups 281).
 constexpr int64_t kPagedFewRows = 8192;
 struct PagedPlan {
   // Head-dim buckets: a staged V's row, what is computed of V, and of Q and K.

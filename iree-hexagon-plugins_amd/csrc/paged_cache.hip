@@ -13,10 +13,12 @@
 // (both prefix sums in one pass over the waves), and writes the rows and
 // table entries that fall to it, finding their request by bisection in LDS.
 // Nothing is exchanged between workgroups, so there is no second launch and
-// no counter.
+// no counter. Bound by its chain of loads and barriers: 3.7 us for one
+// request, 4.8 for 256, 7.6 for 48 with 55832 new rows.
 //
 // append_kv_kernel: rows of K and V into the pages that the slots name,
-// 16 bytes a lane. A row whose slot lies outside the cache is skipped.
+// 16 bytes a lane. A row whose slot lies outside the cache is skipped. Bound
+// by memory: 8191 rows of 8 heads (67 MB) in 11.5 us, 5.8 TB/s; 64 rows 3.4.
 #include "device_common.h"
 #include "kernels_internal.h"
 
@@ -190,6 +192,7 @@ __global__ __launch_bounds__(kAppendThreads) void append_kv_kernel(
 hipError_t launch_page_tables(const PageTables &tables, void *stream) {
   PageTables t = tables;
   const int64_t most = t.rows > t.batch ? t.rows : t.batch;
+  // 4 rows a thread (55832 rows: 8.9 us a call, with 1 the same, 16 16.6).
   int64_t wgs = (most + kTableThreads * 4 - 1) / (kTableThreads * 4);
   wgs = wgs < 1 ? 1 : wgs > 256 ? 256 : wgs;
   void *args[] = {&t};
@@ -201,7 +204,7 @@ hipError_t launch_page_tables(const PageTables &tables, void *stream) {
 hipError_t launch_append_kv(const AppendKv &append, void *stream) {
   AppendKv a = append;
   int64_t wgs = (a.rows + kAppendThreads / 64 - 1) / (kAppendThreads / 64);
-  wgs = wgs > 2048 ? 2048 : wgs;
+  wgs = wgs > 2048 ? 2048 : wgs;  // 1024 and 8192: the same within 4 %
   void *args[] = {&a};
   return hipLaunchKernel((const void *)&append_kv_kernel, dim3((unsigned)wgs),
                          dim3(kAppendThreads), args, 0, (hipStream_t)stream);
