@@ -1207,45 +1207,38 @@ _PAIR = struct.Struct("@2q")
 _PAGED_ATTENTION = struct.Struct("@2P11q6P10qfI")
 
 
+# A small call is bound by the host: shapes and strides are asked for once.
+
 def _ints(t, name, dims=1):
-    """A device table: int32, its rows contiguous."""
+    """Shape of a device table: int32, its rows contiguous."""
     import torch
     if not isinstance(t, torch.Tensor) or t.dtype is not torch.int32:
         raise TypeError(f"{name} must be an int32 tensor")
-    if t.dim() != dims or (t.stride(-1) != 1 and t.shape[-1] != 1
-                           and t.numel()):
+    st = t.stride()
+    if len(st) != dims or (st[-1] != 1 and t.shape[-1] != 1 and t.numel()):
         raise ValueError(f"{name} must be {dims}-D with unit column stride")
+    return t.shape
 
 
 def _rows_of(t, name, dims):
-    """Shape of f16 rows, the head dim contiguous."""
+    """Shape and strides of f16 rows, the head dim contiguous."""
     import torch
-    if (not isinstance(t, torch.Tensor) or t.dtype is not torch.float16
-            or t.dim() != dims or (t.stride(-1) != 1 and t.shape[-1] != 1)):
-        raise TypeError(f"{name} must be a {dims}-D f16 tensor with unit "
-                        "stride along head_dim")
-    return t.shape
+    if isinstance(t, torch.Tensor) and t.dtype is torch.float16:
+        st = t.stride()
+        if len(st) == dims and (st[-1] == 1 or t.shape[-1] == 1):
+            return t.shape, st
+    raise TypeError(f"{name} must be a {dims}-D f16 tensor with unit stride "
+                    "along head_dim")
 
 
 def _cache_fields(k_cache, v_cache):
     """The fields of iree_mi355x_kv_cache_t after its pointers, of checked
     caches."""
-    pages, heads, page, d = _rows_of(k_cache, "k_cache", 4)
-    *rest, dv = _rows_of(v_cache, "v_cache", 4)
+    (pages, heads, page, d), (k0, k1, k2, _) = _rows_of(k_cache, "k_cache", 4)
+    (*rest, dv), (v0, v1, v2, _) = _rows_of(v_cache, "v_cache", 4)
     if rest != [pages, heads, page]:
         _shape(v_cache, (pages, heads, page, dv), "v_cache")
-    return (pages, page, heads, d, dv, *k_cache.stride()[:3],
-            *v_cache.stride()[:3])
-
-
-def _one_device(first, name, *named):
-    """_on_device, and the index of the device; nothing is looked up where all
-    is well."""
-    index = first.get_device()
-    for t, _ in named:
-        if t is not None and (t.get_device() != index or index < 0):
-            _on_device((first, name), *named)
-    return index
+    return pages, page, heads, d, dv, k0, k1, k2, v0, v1, v2
 
 
 def _stream_on(index, stream):
@@ -1263,7 +1256,7 @@ def _other_device(index) -> bool:
     """Whether device `index` is not the current one: the call is then made
     again with it current, on its current stream unless one is given."""
     import torch
-    return index != torch.cuda.current_device()
+    return index != torch._C._cuda_getDevice()
 
 
 def page_tables(cached, added, free_pages, block_table, page_size, rows, *,
@@ -1277,22 +1270,22 @@ def page_tables(cached, added, free_pages, block_table, page_size, rows, *,
     row's page * page_size + place (-1: none, or a row past the last), and
     how many pages were taken (more than F: the list was too short, and the
     pages past it are -1). All tables are int32."""
-    _ints(cached, "cached")
-    _ints(added, "added")
-    _ints(free_pages, "free_pages")
-    _ints(block_table, "block_table", 2)
-    batch = cached.shape[0]
-    if added.shape[0] != batch:
+    batch, = _ints(cached, "cached")
+    many, = _ints(added, "added")
+    free, = _ints(free_pages, "free_pages")
+    have, width = _ints(block_table, "block_table", 2)
+    if many != batch:
         _shape(added, (batch,), "added")
-    have, width = block_table.shape
     if have != batch:
         _shape(block_table, (batch, width), "block_table")
     if page_size < 1 or rows < 0:
         raise ValueError(f"page_size {page_size} and rows {rows} must be at "
                          "least 1 and 0")
-    index = _one_device(cached, "cached", (added, "added"),
-                        (free_pages, "free_pages"),
-                        (block_table, "block_table"))
+    index = cached.get_device()
+    if not (index >= 0 and index == added.get_device()
+            == free_pages.get_device() == block_table.get_device()):
+        _on_device((cached, "cached"), (added, "added"),
+                   (free_pages, "free_pages"), (block_table, "block_table"))
     if _other_device(index):
         import torch
         with torch.cuda.device(index):
@@ -1306,7 +1299,7 @@ def page_tables(cached, added, free_pages, block_table, page_size, rows, *,
         cached.data_ptr(), added.data_ptr(), free_pages.data_ptr(),
         block_table.data_ptr(), at, at + 4 * (batch + 1),
         at + 4 * (2 * batch + 2), at + 4 * (2 * batch + 1), batch,
-        free_pages.shape[0], page_size, width, block_table.stride(0), rows),
+        free, page_size, width, block_table.stride(0), rows),
         _stream_on(index, stream))
     if st != OK:
         _check(st)
@@ -1322,24 +1315,27 @@ def append_kv(k, v, k_cache, v_cache, slots, *, stream=None):
     a permuted view."""
     fields = _cache_fields(k_cache, v_cache)
     _, _, heads, d, dv = fields[:5]
-    rows, *of_k = _rows_of(k, "k", 3)
+    (rows, *of_k), k_strides = _rows_of(k, "k", 3)
     if of_k != [heads, d]:
         _shape(k, (rows, heads, d), "k")
-    if tuple(_rows_of(v, "v", 3)) != (rows, heads, dv):
+    of_v, v_strides = _rows_of(v, "v", 3)
+    if of_v != (rows, heads, dv):
         _shape(v, (rows, heads, dv), "v")
-    _ints(slots, "slots")
-    if slots.shape[0] != rows:
+    if _ints(slots, "slots") != (rows,):
         _shape(slots, (rows,), "slots")
-    index = _one_device(k, "k", (v, "v"), (k_cache, "k_cache"),
-                        (v_cache, "v_cache"), (slots, "slots"))
+    index = k.get_device()
+    if not (index >= 0 and index == v.get_device() == k_cache.get_device()
+            == v_cache.get_device() == slots.get_device()):
+        _on_device((k, "k"), (v, "v"), (k_cache, "k_cache"),
+                   (v_cache, "v_cache"), (slots, "slots"))
     if _other_device(index):
         import torch
         with torch.cuda.device(index):
             return append_kv(k, v, k_cache, v_cache, slots, stream=stream)
     st = library().iree_mi355x_append_kv_f16(
         _KV_CACHE.pack(k_cache.data_ptr(), v_cache.data_ptr(), *fields),
-        k.data_ptr(), v.data_ptr(), rows, _PAIR.pack(*k.stride()[:2]),
-        _PAIR.pack(*v.stride()[:2]), slots.data_ptr(),
+        k.data_ptr(), v.data_ptr(), rows, _PAIR.pack(*k_strides[:2]),
+        _PAIR.pack(*v_strides[:2]), slots.data_ptr(),
         _stream_on(index, stream))
     if st != OK:
         _check(st)
@@ -1371,21 +1367,20 @@ def shared_prefix_attention(q, k_cache, v_cache, row_starts, lengths,
     prefix_length 0 this is paged attention."""
     fields = _cache_fields(k_cache, v_cache)
     _, page, hkv, d, dv = fields[:5]
-    rows, h, of_q = _rows_of(q, "q", 3)
+    (rows, h, of_q), (q0, q1, _) = _rows_of(q, "q", 3)
     if of_q != d:
         _shape(q, (rows, h, d), "q")
     if hkv < 1 or h % hkv:
         raise ValueError(f"{h} query heads are not a multiple of {hkv} KV "
                          "heads")
-    if o is not None and tuple(_rows_of(o, "o", 3)) != (rows, h, dv):
-        _shape(o, (rows, h, dv), "o")
-    _ints(lengths, "lengths")
-    _ints(row_starts, "row_starts")
-    _ints(block_table, "block_table", 2)
-    batch = lengths.shape[0]
-    if row_starts.shape[0] != batch + 1:
+    if o is not None:
+        of_o, (o0, o1, _) = _rows_of(o, "o", 3)
+        if of_o != (rows, h, dv):
+            _shape(o, (rows, h, dv), "o")
+    batch, = _ints(lengths, "lengths")
+    if _ints(row_starts, "row_starts") != (batch + 1,):
         _shape(row_starts, (batch + 1,), "row_starts")
-    have, width = block_table.shape
+    have, width = _ints(block_table, "block_table", 2)
     if have != batch:
         _shape(block_table, (batch, width), "block_table")
     if prefix_length < 0:
@@ -1393,17 +1388,23 @@ def shared_prefix_attention(q, k_cache, v_cache, row_starts, lengths,
     if prefix_length:
         if prefix_pages is None:
             raise ValueError("prefix_length needs prefix_pages")
-        _ints(prefix_pages, "prefix_pages")
-        if prefix_pages.shape[0] * page < prefix_length:
+        have, = _ints(prefix_pages, "prefix_pages")
+        if have * page < prefix_length:
             raise ValueError(f"prefix_pages hold {prefix_pages.shape[0]} "
                              f"pages of {page}, fewer than {prefix_length} "
                              "tokens")
     else:
         prefix_pages = None
-    index = _one_device(q, "q", (k_cache, "k_cache"), (v_cache, "v_cache"),
-                        (row_starts, "row_starts"), (lengths, "lengths"),
-                        (block_table, "block_table"),
-                        (prefix_pages, "prefix_pages"), (o, "o"))
+    index = q.get_device()
+    if not (index >= 0 and index == k_cache.get_device()
+            == v_cache.get_device() == row_starts.get_device()
+            == lengths.get_device() == block_table.get_device()
+            and (prefix_pages is None or index == prefix_pages.get_device())
+            and (o is None or index == o.get_device())):
+        _on_device((q, "q"), (k_cache, "k_cache"), (v_cache, "v_cache"),
+                   (row_starts, "row_starts"), (lengths, "lengths"),
+                   (block_table, "block_table"),
+                   (prefix_pages, "prefix_pages"), (o, "o"))
     if _other_device(index):
         import torch
         with torch.cuda.device(index):
@@ -1412,14 +1413,14 @@ def shared_prefix_attention(q, k_cache, v_cache, row_starts, lengths,
                 prefix_pages, prefix_length, o, scale=scale, stream=stream)
     if o is None:
         o = q.new_empty((rows, h, dv))
-    qs, os_ = q.stride(), o.stride()
+        o0, o1 = h * dv, dv
     args = _PAGED_ATTENTION.pack(
         k_cache.data_ptr(), v_cache.data_ptr(), *fields, q.data_ptr(),
         o.data_ptr(), row_starts.data_ptr(), lengths.data_ptr(),
         block_table.data_ptr(),
         0 if prefix_pages is None else prefix_pages.data_ptr(), rows, h,
-        batch, width, block_table.stride(0), prefix_length, qs[0], qs[1],
-        os_[0], os_[1], d ** -0.5 if scale is None else scale, 0)
+        batch, width, block_table.stride(0), prefix_length, q0, q1, o0, o1,
+        d ** -0.5 if scale is None else scale, 0)
     s = _stream_on(index, stream)
     need = _paged_workspace_need(rows, batch, h, hkv, d, dv, page, width,
                                  prefix_length)
