@@ -588,6 +588,29 @@ def test_attention_unequal_head_dims(pkg, dev, d, dv, added, spare):
     a.check(a.call(pkg))
 
 
+@pytest.mark.parametrize("spare", [0, 80])
+@pytest.mark.parametrize("heads, hk", [(200, 200), (600, 600), (130, 1),
+                                       (260, 2), (17, 1)])
+def test_attention_many_heads(pkg, dev, heads, hk, spare):
+    """More KV heads than workgroups; a token's rows past a tile."""
+    print(f"heads {heads} {hk} {spare}", flush=True)
+    a = Attention([70, 0, 9], [1, 3, 2], heads, hk, 16, 16, 16, 40, pad=1,
+                  spare=spare)
+    a.check(a.call(pkg))
+
+
+@pytest.mark.parametrize("prefix", [0, 30])
+def test_attention_large_batch(pkg, dev, prefix):
+    g = torch.Generator().manual_seed(prefix)
+    cached = torch.randint(0, 30, (1500,), generator=g).tolist()
+    added = torch.randint(0, 3, (1500,), generator=g).tolist()
+    for spare in (0, columns(16)):
+        print(f"large batch {prefix} {spare}", flush=True)
+        a = Attention(cached, added, 1, 1, 8, 8, 16, prefix, pad=1,
+                      spare=spare)
+        a.check(a.call(pkg))
+
+
 @pytest.mark.parametrize("seed", range(12))
 def test_attention_drawn(pkg, dev, seed):
     """Small and large requests in any order, lengths around a part's ends."""
