@@ -1207,12 +1207,20 @@ _PAIR = struct.Struct("@2q")
 _PAGED_ATTENTION = struct.Struct("@2P11q6P10qfI")
 
 
-# A small call is bound by the host: shapes and strides are asked for once.
+# A small call is bound by the host: shapes and strides are asked for once, and
+# torch's types once at all.
+_F16 = _I32 = None
+
+
+def _load_types():
+    global _F16, _I32
+    import torch
+    _F16, _I32 = torch.float16, torch.int32
+
 
 def _ints(t, name, dims=1):
     """Shape of a device table: int32, its rows contiguous."""
-    import torch
-    if not isinstance(t, torch.Tensor) or t.dtype is not torch.int32:
+    if getattr(t, "dtype", None) is not _I32:
         raise TypeError(f"{name} must be an int32 tensor")
     st = t.stride()
     if len(st) != dims or (st[-1] != 1 and t.shape[-1] != 1 and t.numel()):
@@ -1222,8 +1230,7 @@ def _ints(t, name, dims=1):
 
 def _rows_of(t, name, dims):
     """Shape and strides of f16 rows, the head dim contiguous."""
-    import torch
-    if isinstance(t, torch.Tensor) and t.dtype is torch.float16:
+    if getattr(t, "dtype", None) is _F16:
         st = t.stride()
         if len(st) == dims and (st[-1] == 1 or t.shape[-1] == 1):
             return t.shape, st
@@ -1270,6 +1277,8 @@ def page_tables(cached, added, free_pages, block_table, page_size, rows, *,
     row's page * page_size + place (-1: none, or a row past the last), and
     how many pages were taken (more than F: the list was too short, and the
     pages past it are -1). All tables are int32."""
+    if _I32 is None:
+        _load_types()
     batch, = _ints(cached, "cached")
     many, = _ints(added, "added")
     free, = _ints(free_pages, "free_pages")
@@ -1313,6 +1322,8 @@ def append_kv(k, v, k_cache, v_cache, slots, *, stream=None):
     // S. Rows whose slot is negative or past the cache are skipped; two rows
     must not name one slot. A cache in [page, token, head] order is passed as
     a permuted view."""
+    if _F16 is None:
+        _load_types()
     fields = _cache_fields(k_cache, v_cache)
     _, _, heads, d, dv = fields[:5]
     (rows, *of_k), k_strides = _rows_of(k, "k", 3)
@@ -1365,6 +1376,8 @@ def shared_prefix_attention(q, k_cache, v_cache, row_starts, lengths,
     and v_cache [P, Hkv, S, Dv] as in append_kv; o [T, H, Dv] f16 keeps the
     rows past row_starts[B]. Tables are int32, from page_tables. With
     prefix_length 0 this is paged attention."""
+    if _F16 is None:
+        _load_types()
     fields = _cache_fields(k_cache, v_cache)
     _, page, hkv, d, dv = fields[:5]
     (rows, h, of_q), (q0, q1, _) = _rows_of(q, "q", 3)
