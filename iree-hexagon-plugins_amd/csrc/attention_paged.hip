@@ -1361,15 +1361,21 @@ PagedPlan plan_attention_paged(int64_t rows, int64_t batch, int64_t kv_heads,
   const int64_t d = head_dim > head_dim_v ? head_dim : head_dim_v;
   const int64_t packed = rows * group;
   const bool longer_k = d > 128 && head_dim <= 192 && head_dim_v <= 128;
+  // Requests that fill wide tiles walk the prefix themselves, as one alone.
+  p.shared = prefix > 0 && batch > 1;
   // Wide tiles of longer keys fill a CU's LDS alone: only where some request
   // must have more than 16 rows (653 of two, 3 heads each, 3947 keys ahead:
-  // 72.3 -> 38.3 us; 181 rows of 4 heads, 696 ahead: 18.2 -> 21.0).
-  p.wide = d <= 128 || (longer_k && packed > batch * kSmallRows);
+  // 72.3 -> 38.3 us; 181 rows of 4 heads, 696 ahead: 18.2 -> 21.0), or where
+  // narrow tiles of the prefix would read more keys than all requests can have
+  // (676 rows of 68 requests, 11936 keys ahead, 740 each at most: 297.8 ->
+  // 213.4 us).
+  const bool rows_many = packed > batch * kSmallRows;
+  const bool prefix_more = p.shared && prefix + capacity > kPagedWholeKeysFew &&
+                           packed / kNarrowRows * prefix > batch * capacity;
+  p.wide = d <= 128 || (longer_k && (rows_many || prefix_more));
   p.dp = d <= 64 ? 64 : d <= 128 || longer_k ? 128 : 256;
   p.dx = d > 64 && d <= 96 ? 96 : p.dp;
   p.dk = longer_k ? 192 : p.dx;
-  // Requests that fill wide tiles walk the prefix themselves, as one alone.
-  p.shared = prefix > 0 && batch > 1;
   const bool two = p.dp < 256 && !(p.wide && p.dk > 128);  // a CU holds
   const int64_t wgs = two ? kPagedTargetWgs : kPagedTargetWgs / 2;
   p.ways = wgs / kv_heads > 1 ? wgs / kv_heads : 1;
@@ -1388,9 +1394,8 @@ PagedPlan plan_attention_paged(int64_t rows, int64_t batch, int64_t kv_heads,
   p.workspace = (int64_t)kWorkspaceCounterBytes + 2 * packed * 8 +
                 kv_heads * p.part_rows * (p.dp + 2) * 4;
   const int64_t tiles = batch + packed / (p.wide ? kWideRows : kNarrowRows);
-  const bool rows_many = p.wide && packed > batch * kSmallRows;
   const int64_t most = tiles * kv_heads > wgs ? kPagedWholeKeys
-                       : rows_many            ? kPagedWholeKeysWide
+                       : p.wide && rows_many  ? kPagedWholeKeysWide
                                               : kPagedWholeKeysFew;
   if (prefix + capacity <= most ||
       (uint64_t)p.workspace > workspace_limit || p.part_rows > INT32_MAX) {

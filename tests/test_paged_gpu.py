@@ -611,6 +611,14 @@ def test_attention_large_batch(pkg, dev, prefix):
         a.check(a.call(pkg))
 
 
+def test_attention_long_prefix_of_longer_keys(pkg, dev):
+    """192-wide keys whose prefix has wide tiles though every request is
+    small."""
+    a = Attention([9, 0, 33, 70] * 6, [1, 2, 0, 3] * 6, 4, 1, 192, 128, 16,
+                  1300, pad=1, seed=6)
+    a.check(a.call(pkg))
+
+
 @pytest.mark.parametrize("seed", range(12))
 def test_attention_drawn(pkg, dev, seed):
     """Small and large requests in any order, lengths around a part's ends."""
