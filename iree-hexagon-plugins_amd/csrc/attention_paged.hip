@@ -99,7 +99,7 @@ __device__ __forceinline__ int token_of(const PagedAttention &p, int r) {
 // requests before them.
 struct Requests {
   int of[3][64];
-  int small[64];
+  uint32_t small[64];
 };
 
 // Requests of up to 16 rows share tiles of the prefix.
@@ -128,15 +128,16 @@ __device__ __forceinline__ int sees(const PagedAttention &p,
 }
 
 // The packed row of the small requests' row r: the last lane whose small rows
-// start at or before it, then its requests one after the other.
+// start at or before it, then its requests one after the other. Unsigned, and
+// a packed row whatever row_starts hold (the lanes' sums may have wrapped).
 __device__ __forceinline__ int packed_row(const PagedAttention &p,
-                                          const Requests &all, int r) {
+                                          const Requests &all, uint32_t r) {
   int l = 0;
 #pragma unroll
   for (int step = 32; step > 0; step >>= 1)
     if (all.small[l + step] <= r)
       l += step;
-  int rest = r - all.small[l];
+  uint32_t rest = r - all.small[l];
   const int each = (p.batch + 63) >> 6;
   int begin = all.of[0][l];
   if (each > 1) {
@@ -145,15 +146,15 @@ __device__ __forceinline__ int packed_row(const PagedAttention &p,
     for (;; ++b) {
       begin = row_start(p, b);
       const int rows = (row_start(p, b + 1) - begin) * p.group;
-      const int mine = rows > 0 && rows <= kSmallRows ? rows : 0;
+      const uint32_t mine = rows > 0 && rows <= kSmallRows ? rows : 0;
       if (rest < mine || b >= last)
         break;
       rest -= mine;
     }
   }
-  r = begin * p.group + rest;
-  const int end = p.rows * p.group;
-  return r < end ? r : end - 1;
+  r = (uint32_t)(begin * p.group) + rest;
+  const uint32_t end = (uint32_t)(p.rows * p.group);
+  return (int)(r < end ? r : end - 1);
 }
 
 // The lane's query row of a tile.
@@ -161,7 +162,7 @@ __device__ __forceinline__ const f16 *query_row(const PagedAttention &p,
                                                 const PagedTile &t,
                                                 const Requests &all, int r) {
   if (t.compact)
-    r = packed_row(p, all, r);
+    r = packed_row(p, all, (uint32_t)r);
   const int token = token_of(p, r);
   return p.q + (int64_t)token * p.q_row +
          (int64_t)(t.kv_head * p.group + r - token * p.group) * p.q_head;
@@ -1021,13 +1022,17 @@ attention_paged_kernel(PagedAttention) {
   uint32_t small = small_of(begin, end);
   rest_of_lane([&](int from, int to, int) { small += small_of(from, to); });
   const uint32_t small_upto = lane_sums(small);
-  int small_rows = __builtin_amdgcn_readlane((int)small_upto, 63);
+  // At most the packed rows, which the parts have room for: requests whose
+  // starts do not ascend may count a row several times.
+  const uint32_t small_all =
+      (uint32_t)__builtin_amdgcn_readlane((int)small_upto, 63);
+  const uint32_t rows_all = (uint32_t)(p.rows * p.group);
+  int small_rows = (int)(small_all < rows_all ? small_all : rows_all);
   all.of[0][lane] = begin;
   all.of[1][lane] = end;
   all.of[2][lane] = length;
-  all.small[lane] = (int)(small_upto - small);
-  bool shared = p.shared && small_rows > 0 &&
-                !__any(small == (uint32_t)small_rows);
+  all.small[lane] = small_upto - small;
+  bool shared = p.shared && small_rows > 0 && !__any(small == small_all);
 
   // The line: the prefix's tiles, then the requests'.
   const int prefix_steps = (p.prefix + kStepKeys - 1) / kStepKeys;
@@ -1180,7 +1185,8 @@ attention_paged_kernel(PagedAttention) {
       for (int r = t.r0 + (int)threadIdx.x; r < t.r_end; r += kPagedThreads) {
         const i32x2 parts = {(int)(line + r) + kWideRows * first,
                              whole ? 0 : count};
-        p.part_of[line + (lead ? packed_row(p, all, r) : r)] = parts;
+        const int at_row = lead ? packed_row(p, all, (uint32_t)r) : r;
+        p.part_of[line + at_row] = parts;
         if (all_keys)
           p.part_of[r] = i32x2{0, 0};
       }

@@ -814,6 +814,79 @@ def test_captured_step(pkg, dev):
             t["free"].copy_(t["free"].roll(-used))
 
 
+def abi(pkg, a, o):
+    """The C-ABI's arguments of a call, and the tables to keep."""
+    args = pkg.PagedAttentionArgs(
+        q=a.q.data_ptr(), o=o.data_ptr(), rows=a.rows, heads=a.heads,
+        batch=len(a.added), table_width=a.width, table_stride=a.width,
+        prefix_length=a.prefix, scale=a.scale)
+    keep = [ints(x) for x in (a.starts, a.lengths, a.table, a.prefix_pages)]
+    for n, t in zip(("row_starts", "lengths", "block_table", "prefix_pages"),
+                    keep):
+        setattr(args, n, t.data_ptr())
+    c = args.cache
+    c.k, c.v = a.kc.data_ptr(), a.vc.data_ptr()
+    c.pages, c.kv_heads, c.page_size, c.head_dim = a.kc.shape
+    c.head_dim_v = a.dv
+    c.k_strides[:], c.v_strides[:] = a.kc.stride()[:3], a.vc.stride()[:3]
+    args.q_strides[:], args.o_strides[:] = a.q.stride()[:2], o.stride()[:2]
+    return args, keep
+
+
+# row starts (a pattern and how often), heads, kv heads, d, dv, prefix
+STARTS = [([0, 1], 500, 16, 1, 64, 64, 32768),
+          ([0, 4], 128, 32, 8, 64, 64, 32768),
+          ([0, 4], 2048, 32, 8, 64, 64, 4096),
+          ([0, 1], 500, 16, 1, 256, 256, 32768),
+          ([0, 4], 128, 32, 8, 192, 128, 32768),
+          ([0, 3, 1, 2, 0, 4], 300, 32, 8, 96, 96, 9000)]
+
+
+@pytest.mark.parametrize("starts,times,heads,hk,d,dv,prefix", STARTS)
+def test_attention_row_starts_guarded(pkg, dev, starts, times, heads, hk, d,
+                                      dv, prefix):
+    """Many requests whose starts do not ascend count the rows again and again:
+    nothing outside o and the workspace is written, and the parts hold a batch
+    of requests in order afterwards."""
+    page, rows = 16, max(starts)
+    a = Attention([5, 40, 9, 2], [rows, 0, 0, 0], heads, hk, d, dv, page, 64,
+                  spare=3)
+    a.prefix_pages = (a.prefix_pages * up(prefix, 64))[:up(prefix, page)]
+    a.prefix = prefix
+    in_order = a.starts, a.table, a.lengths, a.added
+    batch = len(starts) * times
+    a.starts = starts * times + [0]
+    a.table = [a.table[0]] * batch
+    a.lengths = [7] * batch
+    a.added = [0] * batch
+    out = torch.full((3 * rows, heads, dv), 9.0, dtype=H, device="cuda")
+    o = out[rows:2 * rows]
+    lib, s = pkg.library(), torch.cuda.current_stream().cuda_stream
+    args, keep = abi(pkg, a, o)
+    need = lib.iree_mi355x_shared_prefix_attention_workspace_bytes(
+        ctypes.byref(args))
+    head, guard = 256 << 10, 64 << 20
+    assert need > head
+    ws = torch.full((need + guard,), 0xA5, dtype=torch.uint8, device="cuda")
+    print(f"starts {starts} x {times}, {heads} {hk} {d} {prefix}", flush=True)
+    for size in (need, 0):
+        assert lib.iree_mi355x_shared_prefix_attention_f16(
+            ctypes.byref(args), ws.data_ptr() if size else None, size,
+            s) == pkg.OK
+        torch.cuda.synchronize()
+        assert bool((ws[need:] == 0xA5).all()) and bool(
+            (ws[:head] == 0xA5).all())
+        assert bool((out[:rows] == 9).all()) and bool(
+            (out[2 * rows:] == 9).all())
+    a.starts, a.table, a.lengths, a.added = in_order
+    args, keep = abi(pkg, a, o)
+    assert lib.iree_mi355x_shared_prefix_attention_workspace_bytes(
+        ctypes.byref(args)) <= need
+    assert lib.iree_mi355x_shared_prefix_attention_f16(
+        ctypes.byref(args), ws.data_ptr(), need, s) == pkg.OK
+    a.check(o)
+
+
 # ------------------------------------------------------------- all together --
 
 def test_steps(pkg, dev):
