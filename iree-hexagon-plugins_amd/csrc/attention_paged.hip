@@ -1281,10 +1281,15 @@ __global__ __launch_bounds__(kPagedThreads) void attention_paged_join_kernel(
     top = x;
     sum *= keep;
     acc *= keep;
+    // A part without a maximum is one whose keys the row does not see (sum 0:
+    // left out, an infinite value of a key that others see is none of it) or
+    // gives it NaN scores alone (sum NaN: 0 times it stays NaN).
 #pragma unroll
     for (int u = 0; u < 4; ++u)
-      if (s0 + u < parts && ml[u][0] != kNegInf) {
-        const float f = __builtin_amdgcn_exp2f(ml[u][0] - x);
+      if (s0 + u < parts && !(ml[u][0] == kNegInf && ml[u][1] == 0.0f)) {
+        const float f = ml[u][0] == kNegInf
+                            ? 0.0f
+                            : __builtin_amdgcn_exp2f(ml[u][0] - x);
         sum += f * ml[u][1];
         acc += f * v[u];
       }

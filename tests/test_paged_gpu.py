@@ -814,6 +814,41 @@ def test_captured_step(pkg, dev):
             t["free"].copy_(t["free"].roll(-used))
 
 
+# Every head-dim bucket, narrow and wide tiles, rows joined by one group and
+# by several (up to 8192 rows of all heads).
+@pytest.mark.parametrize("added,heads,hk,d,dv", [
+    ([1, 2, 1], 4, 2, 64, 64), ([1, 2, 40], 4, 2, 64, 64),
+    ([1, 2, 40], 8, 2, 96, 96), ([300, 1, 20], 32, 4, 128, 128),
+    ([1, 2, 40], 4, 2, 192, 128), ([1, 2, 1], 4, 2, 256, 256),
+    ([300, 1, 20], 32, 4, 256, 256)])
+@pytest.mark.parametrize("prefix", [0, 1500])
+def test_attention_nan_parts(pkg, dev, added, heads, hk, d, dv, prefix):
+    """A row whose scores are all NaN, in every part or in one kind's, is NaN
+    where its tiles are split as well, and does nothing to other rows."""
+    print(f"nan {added} {heads} {hk} {d} {prefix}", flush=True)
+    a = Attention([1040, 9, 300], added, heads, hk, d, dv, 16, prefix, pad=1,
+                  spare=columns(16))
+    want = a.call(pkg).clone()
+    assert bool(want.isfinite().all())
+    q = a.q.clone()
+    rows = sum(added)
+    ill = torch.zeros(a.rows, heads, dtype=torch.bool, device="cuda")
+    for row, head in ((0, 1), (added[0], heads - 1), (rows - 1, 0)):
+        a.q[row, head] = NAN
+        ill[row, head] = True
+    o = a.call(pkg)
+    assert bool(o[ill].isnan().all()) and torch.equal(o[~ill], want[~ill])
+    # every key of the last KV head's prefix, or of request 0's own
+    a.q = q
+    group = heads // hk
+    pages = a.prefix_pages if prefix else a.table[0][:up(a.lengths[0], 16)]
+    a.kc[torch.tensor(pages, device="cuda"), hk - 1] = NAN
+    ill[:] = False
+    ill[:rows if prefix else added[0], heads - group:] = True
+    o = a.call(pkg)
+    assert bool(o[ill].isnan().all()) and torch.equal(o[~ill], want[~ill])
+
+
 def abi(pkg, a, o):
     """The C-ABI's arguments of a call, and the tables to keep."""
     args = pkg.PagedAttentionArgs(
