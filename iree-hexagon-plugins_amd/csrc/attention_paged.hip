@@ -1019,8 +1019,12 @@ attention_paged_kernel(PagedAttention) {
     const int rows = rows_of(p, from, to);
     return (uint32_t)(rows <= kSmallRows ? rows : 0);
   };
-  uint32_t small = small_of(begin, end);
-  rest_of_lane([&](int from, int to, int) { small += small_of(from, to); });
+  uint32_t small = small_of(begin, end), largest = small;
+  rest_of_lane([&](int from, int to, int) {
+    const uint32_t n = small_of(from, to);
+    small += n;
+    largest = n > largest ? n : largest;
+  });
   const uint32_t small_upto = lane_sums(small);
   // At most the packed rows, which the parts have room for: requests whose
   // starts do not ascend may count a row several times.
@@ -1032,7 +1036,8 @@ attention_paged_kernel(PagedAttention) {
   all.of[1][lane] = end;
   all.of[2][lane] = length;
   all.small[lane] = small_upto - small;
-  bool shared = p.shared && small_rows > 0 && !__any(small == small_all);
+  // shared by two at least: no request has all the small ones' rows
+  bool shared = p.shared && small_rows > 0 && !__any(largest == small_all);
 
   // The line: the prefix's tiles, then the requests'.
   const int prefix_steps = (p.prefix + kStepKeys - 1) / kStepKeys;

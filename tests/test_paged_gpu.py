@@ -611,6 +611,25 @@ def test_attention_large_batch(pkg, dev, prefix):
         a.check(a.call(pkg))
 
 
+@pytest.mark.parametrize("first", [0, 40, 1008])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_attention_padded_batch(pkg, dev, d, first):
+    """A step padded to 1024 requests, of which 16 that follow one another have
+    rows: they share the prefix as a batch of 16 does, to the last bit."""
+    print(f"padded {d} {first}", flush=True)
+    cached = [9, 0, 33, 70] * 4
+    a = Attention(cached, [1, 2, 1, 3] * 4, 8, 2, d, d, 16, 3000, pad=1,
+                  spare=columns(16), seed=d)
+    want = a.call(pkg).clone()
+    a.check(want)
+    rest = 1024 - first - 16
+    a.added = [0] * first + a.added + [0] * rest
+    a.starts = [0] * first + a.starts + [a.starts[-1]] * rest
+    a.lengths = [5] * first + a.lengths + [0] * rest
+    a.table = ([a.table[0]] * first + a.table + [[-1] * a.width] * rest)
+    assert torch.equal(a.call(pkg), want)
+
+
 def test_attention_long_prefix_of_longer_keys(pkg, dev):
     """192-wide keys whose prefix has wide tiles though every request is
     small."""
