@@ -358,7 +358,9 @@ int iree_mi355x_append_kv_f16(const iree_mi355x_kv_cache_t *cache,
 // itself. A call runs with any workspace or none, and gives the same bits each
 // time for the same extents, lengths and workspace. Unlike the matmuls' it
 // needs no zero-filled contents; its first 256 KiB (their counters) are left
-// alone. row_starts must ascend from 0: where it does not, rows hold anything,
+// alone. With a workspace a call is up to two launches, so what other threads
+// enqueue on the same stream must not use the same workspace meanwhile.
+// row_starts must ascend from 0: where it does not, rows hold anything,
 // but nothing outside the tensors is read or written.
 typedef struct iree_mi355x_paged_attention_t {
   iree_mi355x_kv_cache_t cache;

@@ -15,6 +15,7 @@ import ctypes
 import functools
 import os
 import struct
+import threading
 from dataclasses import dataclass
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -1352,6 +1353,31 @@ def append_kv(k, v, k_cache, v_cache, slots, *, stream=None):
         _check(st)
 
 
+# Attention with parts is two launches, tiles and the join: what another thread
+# enqueued between them on the same workspace would be joined. So it has a
+# buffer of its own for each (device index, stream), [pointer, bytes, lock]
+# here, which no other operator or captured graph writes, and its calls on it
+# are made one at a time (by one thread nested at most, as from a finalizer,
+# which cannot come between the launches: they are in one library call).
+_PAGED_WORKSPACES: dict = {}
+
+
+def _paged_call(args, need, index, stream):
+    """One attention call on the stream's own workspace of at least `need`
+    bytes: its status."""
+    held = _PAGED_WORKSPACES.get((index, stream))
+    if held is None:
+        held = _PAGED_WORKSPACES.setdefault((index, stream),
+                                            [None, 0, threading.RLock()])
+    with held[2]:
+        if held[1] < need:
+            import torch
+            held[:2] = stream_workspace(need, torch.device("cuda", index),
+                                        stream, "paged attention")
+        return library().iree_mi355x_shared_prefix_attention_f16(
+            args, held[0], held[1], stream)
+
+
 @functools.lru_cache(maxsize=4096)
 def _paged_workspace_need(rows, batch, h, hkv, d, dv, page, width,
                           prefix) -> int:
@@ -1437,16 +1463,17 @@ def shared_prefix_attention(q, k_cache, v_cache, row_starts, lengths,
     s = _stream_on(index, stream)
     need = _paged_workspace_need(rows, batch, h, hkv, d, dv, page, width,
                                  prefix_length)
-    ws, wsb = None, 0
-    if need > 0:
-        if s and _capturing(s):
+    if need > 0 and not (s and _capturing(s)):
+        st = _paged_call(args, need, index, s)
+    else:
+        ws = None
+        if need > 0:
             # the graph's own: no other graph's replays share it
             import torch
             held = torch.empty(need, dtype=torch.uint8, device=q.device)
-            ws, wsb = held.data_ptr(), need
-        else:
-            ws, wsb = _call_workspace(need, index, s)
-    st = library().iree_mi355x_shared_prefix_attention_f16(args, ws, wsb, s)
+            ws = held.data_ptr()
+        st = library().iree_mi355x_shared_prefix_attention_f16(args, ws, need,
+                                                               s)
     if st != OK:
         _check(st)
     return o

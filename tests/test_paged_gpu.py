@@ -6,6 +6,8 @@ compared with the definition in 64 bits (`Attention`, which also says how far
 a result may be off, from the roundings that the kernel makes).
 """
 import ctypes
+import threading
+import time
 
 import pytest
 import torch
@@ -776,6 +778,66 @@ def test_stream_argument(pkg, dev):
     for c in caches:
         flat = c.transpose(1, 2).reshape(-1, 2, 64)
         assert torch.equal(flat[slots.long()], k)
+
+
+def test_threads_on_one_stream(pkg, dev, monkeypatch):
+    """Calls that two threads make on one stream take turns from the first of
+    their launches to the last, on a buffer that no other operator has."""
+    batches = [Attention([900, 40, 300 + s], [1, 2, 1], 8, 2, 64, 64, 16,
+                         1500 + 900 * s, seed=s) for s in range(2)]
+    want = [a.call(pkg).clone() for a in batches]
+    x = torch.randn(64, 8192, device="cuda").half()
+    w = torch.randn(8192, 256, device="cuda").half()
+    product = pkg.matmul(x, w)
+    torch.cuda.synchronize()
+    real, inside, used, met = pkg.library(), [], [], []
+
+    class Slow:
+        """The library, with time for others before a call's launches."""
+
+        def __getattr__(self, name):
+            return getattr(real, name)
+
+        def iree_mi355x_shared_prefix_attention_f16(self, args, ws, wsb, s):
+            used.append((ws, wsb))
+            inside.append(s)
+            met.append(len(inside))
+            time.sleep(0.01)
+            st = real.iree_mi355x_shared_prefix_attention_f16(args, ws, wsb,
+                                                              s)
+            inside.pop()
+            return st
+
+    monkeypatch.setattr(pkg, "library", Slow)
+    got, products, start = [[], []], [], threading.Barrier(3)
+
+    def attend(t):
+        start.wait()
+        for _ in range(5):
+            got[t].append(batches[t].call(pkg))
+
+    def multiply():
+        start.wait()
+        for _ in range(50):
+            products.append(pkg.matmul(x, w))
+
+    threads = [threading.Thread(target=attend, args=(t,)) for t in range(2)]
+    threads.append(threading.Thread(target=multiply))
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert len(used) == 10 and met == [1] * 10, met
+    for g, o in zip(got, want):
+        assert len(g) == 5 and all(torch.equal(x, o) for x in g)
+    assert len(products) == 50
+    assert all(torch.equal(p, product) for p in products)
+    flat = [b for (_, _, layout), bufs in pkg._STREAM_WORKSPACES.items()
+            if layout is None for b in bufs]
+    for ws, wsb in used:
+        assert all(ws + wsb <= b.data_ptr() or b.data_ptr() + b.numel() <= ws
+                   for b in flat)
 
 
 def test_captured_step(pkg, dev):
