@@ -324,6 +324,7 @@ def library():
     lib.iree_mi355x_last_error.restype = ctypes.c_char_p
     # the HIP runtime's, through the library that links it
     lib.hipStreamIsCapturing.argtypes = [p, p]
+    lib.hipStreamGetCaptureInfo.argtypes = [p, p, p]
     lib.iree_mi355x_version.restype = ctypes.c_char_p
     lib.iree_mi355x_matmul_desc_init.restype = None
     lib.iree_mi355x_matmul_desc_init.argtypes = [
@@ -1378,6 +1379,36 @@ def _paged_call(args, need, index, stream):
             args, held[0], held[1], stream)
 
 
+def _capture_of(stream) -> int:
+    """The number of the capture that a raw stream takes part in, 0: none."""
+    status, number = ctypes.c_int(), ctypes.c_ulonglong()
+    if not stream or library().hipStreamGetCaptureInfo(
+            stream, ctypes.byref(status), ctypes.byref(number)):
+        return 0
+    return number.value if status.value else 0
+
+
+def _graph_workspace(need, index, stream):
+    """A workspace for a call on a raw stream that is being captured: memory of
+    torch's for that graph, in that stream's order, so that once dropped it
+    serves later calls captured on the same stream, and no other work of this
+    graph or another. None where the capture is not torch's: its memory would
+    be anyone's as soon as it is dropped."""
+    import torch
+    which = _capture_of(stream)
+    if not which or which != _capture_of(_current_stream_ptr()):
+        return None
+    device = torch.device("cuda", index)
+    with torch.cuda.stream(_torch_stream(stream, device)):
+        held = torch.empty(need, dtype=torch.uint8, device=device)
+    at = held.data_ptr()
+    for s in torch.cuda.memory_snapshot():
+        if (s["device"] == index
+                and s["address"] <= at < s["address"] + s["total_size"]):
+            return held if tuple(s["segment_pool_id"]) != (0, 0) else None
+    return None
+
+
 @functools.lru_cache(maxsize=4096)
 def _paged_workspace_need(rows, batch, h, hkv, d, dv, page, width,
                           prefix) -> int:
@@ -1466,13 +1497,9 @@ def shared_prefix_attention(q, k_cache, v_cache, row_starts, lengths,
     if need > 0 and not (s and _capturing(s)):
         st = _paged_call(args, need, index, s)
     else:
-        ws = None
-        if need > 0:
-            # the graph's own: no other graph's replays share it
-            import torch
-            held = torch.empty(need, dtype=torch.uint8, device=q.device)
-            ws = held.data_ptr()
-        st = library().iree_mi355x_shared_prefix_attention_f16(args, ws, need,
+        held = _graph_workspace(need, index, s) if need > 0 else None
+        ws, wsb = (None, 0) if held is None else (held.data_ptr(), need)
+        st = library().iree_mi355x_shared_prefix_attention_f16(args, ws, wsb,
                                                                s)
     if st != OK:
         _check(st)

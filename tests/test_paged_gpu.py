@@ -840,6 +840,99 @@ def test_threads_on_one_stream(pkg, dev, monkeypatch):
                    for b in flat)
 
 
+class Seen:
+    """The library, which keeps the workspaces of attention calls."""
+
+    def __init__(self, pkg):
+        self.real, self.used = pkg.library(), []
+
+    def __getattr__(self, name):
+        return getattr(self.real, name)
+
+    def iree_mi355x_shared_prefix_attention_f16(self, args, ws, wsb, s):
+        self.used.append((ws, wsb))
+        return self.real.iree_mi355x_shared_prefix_attention_f16(args, ws,
+                                                                 wsb, s)
+
+
+def test_capture_on_another_stream(pkg, dev, monkeypatch):
+    """A call on a stream forked from the capture, with other work captured
+    beside it: what torch hands out then is not the call's workspace."""
+    a = Attention([900, 40, 300], [1, 2, 1], 8, 2, 64, 64, 16, 1500)
+    want = a.call(pkg).clone()
+    t = [ints(x) for x in (a.starts, a.lengths, a.table, a.prefix_pages)]
+    outs = [torch.empty_like(want) for _ in range(2)]
+    main, side = torch.cuda.Stream(), torch.cuda.Stream()
+    seen = Seen(pkg)
+    monkeypatch.setattr(pkg, "library", lambda: seen)
+    torch.cuda.synchronize()
+    graph, beside = torch.cuda.CUDAGraph(), []
+    with torch.cuda.graph(graph, stream=main):
+        side.wait_stream(main)
+        for o, stream in zip(outs, (side, side.cuda_stream)):
+            pkg.shared_prefix_attention(a.q, a.kc, a.vc, *t, a.prefix, o,
+                                        stream=stream)
+            (ws, wsb) = seen.used[-1]
+            for _ in range(3):
+                x = torch.empty(wsb, dtype=torch.uint8, device="cuda")
+                x.fill_(0x7f)
+                beside.append(x)
+        main.wait_stream(side)
+    assert len(seen.used) == 2
+    for ws, wsb in seen.used:
+        assert ws and wsb and all(
+            ws + wsb <= x.data_ptr() or x.data_ptr() + x.numel() <= ws
+            for x in beside)
+    for turn in range(4):
+        for o in outs:
+            o.fill_(3.0)
+        torch.cuda.synchronize()
+        graph.replay()
+        eager = a.call(pkg)
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, want) for o in outs + [eager]), turn
+        assert all(bool((x == 0x7f).all()) for x in beside)
+
+
+def hip(status):
+    assert status == 0, status
+
+
+@pytest.mark.parametrize("current", [False, True])
+def test_capture_not_torch(pkg, dev, monkeypatch, current):
+    """A stream captured through the HIP API, torch's current one or another:
+    the call keeps no memory that torch gives to later tensors."""
+    a = Attention([900, 40, 300], [1, 2, 1], 8, 2, 64, 64, 16, 1500)
+    a.check(a.call(pkg))
+    t = [ints(x) for x in (a.starts, a.lengths, a.table, a.prefix_pages)]
+    o = torch.full((a.rows, 8, 64), 9.0, dtype=H, device="cuda")
+    stream = torch.cuda.Stream()
+    seen, lib = Seen(pkg), pkg.library()
+    monkeypatch.setattr(pkg, "library", lambda: seen)
+    graph, run = ctypes.c_void_p(), ctypes.c_void_p()
+    s = ctypes.c_void_p(stream.cuda_stream)
+    held = torch.empty(64 << 20, dtype=torch.uint8, device="cuda")
+    with torch.cuda.stream(stream):  # memory of this stream to hand out
+        mine = torch.empty(64 << 20, dtype=torch.uint8, device="cuda")
+    del held, mine
+    torch.cuda.synchronize()
+    hip(lib.hipStreamBeginCapture(s, 2))  # relaxed
+    with torch.cuda.stream(stream if current else None):
+        pkg.shared_prefix_attention(a.q, a.kc, a.vc, *t, a.prefix, o,
+                                    stream=stream)
+    hip(lib.hipStreamEndCapture(s, ctypes.byref(graph)))
+    hip(lib.hipGraphInstantiate(ctypes.byref(run), graph, None, None, 0))
+    assert seen.used == [(None, 0)]
+    with torch.cuda.stream(stream):
+        for turn in range(3):
+            o.fill_(9.0)
+            hip(lib.hipGraphLaunch(run, s))
+            stream.synchronize()
+            a.check(o)
+    hip(lib.hipGraphExecDestroy(run))
+    hip(lib.hipGraphDestroy(graph))
+
+
 def test_captured_step(pkg, dev):
     """Tables, rows and attention of a step in one graph, whose replays read
     what its inputs hold then; eager steps between give the same."""
