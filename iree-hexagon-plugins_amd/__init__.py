@@ -1261,6 +1261,23 @@ def _stream_on(index, stream):
     return _stream_ptr(stream)
 
 
+def _empty_on(like, shape, stream):
+    """like.new_empty(shape) for a call on `stream` (None: the current one): in
+    that stream's order, so that no other work still reads or writes the
+    memory, and kept until the current stream's work with it is done too."""
+    if stream is None:
+        return like.new_empty(shape)
+    import torch
+    here = torch.cuda.current_stream(like.device)
+    there = _torch_stream(stream, like.device)
+    if there.cuda_stream == here.cuda_stream:
+        return like.new_empty(shape)
+    with torch.cuda.stream(there):
+        t = like.new_empty(shape)
+    t.record_stream(here)
+    return t
+
+
 def _other_device(index) -> bool:
     """Whether device `index` is not the current one: the call is then made
     again with it current, on its current stream unless one is given."""
@@ -1302,7 +1319,7 @@ def page_tables(cached, added, free_pages, block_table, page_size, rows, *,
         with torch.cuda.device(index):
             return page_tables(cached, added, free_pages, block_table,
                                page_size, rows, stream=stream)
-    out = cached.new_empty(2 * batch + 2 + rows)
+    out = _empty_on(cached, 2 * batch + 2 + rows, stream)
     at = out.data_ptr()
     starts, lengths, needed, slots = out.split_with_sizes(
         (batch + 1, batch, 1, rows))
@@ -1482,7 +1499,7 @@ def shared_prefix_attention(q, k_cache, v_cache, row_starts, lengths,
                 q, k_cache, v_cache, row_starts, lengths, block_table,
                 prefix_pages, prefix_length, o, scale=scale, stream=stream)
     if o is None:
-        o = q.new_empty((rows, h, dv))
+        o = _empty_on(q, (rows, h, dv), stream)
         o0, o1 = h * dv, dv
     args = _PAGED_ATTENTION.pack(
         k_cache.data_ptr(), v_cache.data_ptr(), *fields, q.data_ptr(),

@@ -780,6 +780,72 @@ def test_stream_argument(pkg, dev):
         assert torch.equal(flat[slots.long()], k)
 
 
+@pytest.mark.parametrize("raw", [False, True])
+@pytest.mark.parametrize("operator", ["page_tables", "attention"])
+def test_results_on_another_stream(pkg, dev, operator, raw):
+    """The results of a call on another stream than the current one: memory
+    that neither stream's work still uses."""
+    a = Attention([40, 9], [1, 30], 4, 2, 64, 64, 16, 70)
+    t = [ints(x) for x in (a.starts, a.lengths, a.table, a.prefix_pages)]
+    free, table = ints([1, 2, 7]), ints([[3, -1, -1], [5, 6, -1]])
+    cached, added = ints([15, 30]), ints([2, 2])
+    stream = torch.cuda.Stream()
+    on = stream.cuda_stream if raw else stream
+    tables = [table.clone() for _ in range(9)]  # a call's, kept to the end
+    each = iter(tables)
+
+    def call():
+        if operator == "attention":
+            return pkg.shared_prefix_attention(a.q, a.kc, a.vc, *t, a.prefix,
+                                               stream=on)
+        return pkg.page_tables(cached, added, free, next(each), 16, 1000,
+                               stream=on)[0]
+
+    def work(big):
+        for _ in range(10):
+            big = big @ big * 1e-3
+
+    torch.cuda.synchronize()
+    want = call()
+    torch.cuda.synchronize()
+    want = want.clone()
+    size = call().untyped_storage().nbytes()
+    big = torch.randn(4096, 4096, device="cuda")
+    torch.cuda.synchronize()
+    # dropped before the call has run: not the next tensor's
+    with torch.cuda.stream(stream):
+        work(big)
+    at = call().data_ptr()
+    others = [torch.full((size,), 7, dtype=torch.uint8, device="cuda")
+              for _ in range(3)]
+    assert at not in [x.data_ptr() for x in others]
+    torch.cuda.synchronize()
+    assert all(bool((x == 7).all()) for x in others)
+    # memory that the current stream's work still reads: not the call's
+    del others
+    last = torch.full((size,), 7, dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    work(big)
+    copy, at = last.clone(), last.data_ptr()
+    del last
+    got = call()
+    assert got.data_ptr() != at
+    torch.cuda.synchronize()
+    assert bool((copy == 7).all()) and torch.equal(got, want)
+    # the current stream's work with results that are dropped meanwhile
+    got = call()
+    torch.cuda.current_stream().wait_stream(stream)
+    work(big)
+    copy, at = got.clone(), got.data_ptr()
+    del got
+    with torch.cuda.stream(stream):
+        others = [torch.full((size,), 7, dtype=torch.uint8, device="cuda")
+                  for _ in range(3)]
+    assert at not in [x.data_ptr() for x in others]
+    torch.cuda.synchronize()
+    assert torch.equal(copy, want)
+
+
 def test_threads_on_one_stream(pkg, dev, monkeypatch):
     """Calls that two threads make on one stream take turns from the first of
     their launches to the last, on a buffer that no other operator has."""
