@@ -1436,8 +1436,11 @@ hipError_t launch_attention_paged(const PagedAttention &attention,
   a.tile_units = (int)plan.tile_units;
   a.snap = (int)plan.snap;
   a.shared = plan.shared ? 1 : 0;
-  // item / ways of items below 2^24 with at most 2^8 ways or one head, and
-  // the ways' share of a line of less than 2^31 units, rounded down or not.
+  // item / ways, exact while item * ways is below 2^32: at most 4 ways to each
+  // of 65535 heads, or 2048 workgroups in all; and the ways' share of a line of
+  // less than 2^31 units, at most one unit over. (One way's is not used.)
+  if ((uint64_t)a.items * (uint64_t)a.ways >> 32)
+    return hipErrorInvalidValue;
   a.ways_magic = (uint32_t)(((uint64_t)1 << 32) / (uint64_t)plan.ways + 1);
   a.part_rows = plan.part_rows;
   a.part_of = nullptr;

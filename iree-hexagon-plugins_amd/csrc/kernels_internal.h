@@ -408,11 +408,12 @@ struct PagedAttention {
   // Parts (no workspace: null): workgroup w's f32 part of a tile's row at
   // row line + 128 w of its KV head's part_rows, and its (max, sum). line is
   // the row's number among the small requests' for the prefix's tiles, its
-  // packed row plus `packed` for the others. They are distinct: along the
-  // tiles the line moves on by a tile's at most 128 rows from one to the next,
-  // and w does from one workgroup to the next. part_of has, for either kind
-  // and packed row, the first part and how many (0: none, the result is
-  // stored).
+  // packed row plus `packed` for the others. Where row_starts ascend they are
+  // distinct: along the tiles the line moves on by a tile's at most 128 rows
+  // from one to the next, and w does from one workgroup to the next. Where they
+  // do not, parts may overwrite one another, within part_rows: a line's number
+  // is below 2 * packed. part_of has, for either kind and packed row, the first
+  // part and how many (0: none, the result is stored).
   int64_t part_rows;
   float *partials, *part_ml;
   int __attribute__((ext_vector_type(2))) *part_of;
