@@ -712,7 +712,8 @@ def stream_workspace(need: int, device=None, stream=None, layout=None,
     current one; an int: a raw hipStream_t) on `device`, holding at least
     `need` bytes; (None, 0) when `need` is 0. `layout` keeps apart buffers
     whose arrival counters sit at different offsets (a command buffer's lane
-    slices): None for flat calls, whose counters open the buffer. Under graph
+    slices) or that no other call may write (paged attention's): None for flat
+    calls, whose counters open the buffer. Under graph
     capture a buffer that is too small is not grown:
     MI355XError(WORKSPACE_TOO_SMALL), or with `partial` what there is of it
     (a general matmul then splits K less, or not at all; a call that cannot
@@ -1390,8 +1391,9 @@ def _paged_call(args, need, index, stream):
     with held[2]:
         if held[1] < need:
             import torch
+            # while the current stream is capturing: what there is
             held[:2] = stream_workspace(need, torch.device("cuda", index),
-                                        stream, "paged attention")
+                                        stream, "paged attention", True)
         return library().iree_mi355x_shared_prefix_attention_f16(
             args, held[0], held[1], stream)
 
@@ -1413,8 +1415,9 @@ def _graph_workspace(need, index, stream):
     be anyone's as soon as it is dropped."""
     import torch
     which = _capture_of(stream)
-    if not which or which != _capture_of(_current_stream_ptr()):
-        return None
+    if (not which or which != _capture_of(_current_stream_ptr())
+            or torch.cuda.get_allocator_backend() != "native"):
+        return None  # (other allocators do not tell whose memory is)
     device = torch.device("cuda", index)
     with torch.cuda.stream(_torch_stream(stream, device)):
         held = torch.empty(need, dtype=torch.uint8, device=device)

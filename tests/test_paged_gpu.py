@@ -960,6 +960,31 @@ def test_capture_on_another_stream(pkg, dev, monkeypatch):
         assert all(bool((x == 0x7f).all()) for x in beside)
 
 
+def test_eager_call_beside_a_capture(pkg, dev, monkeypatch):
+    """A call on a stream that is not captured while the current one is: the
+    stream has no buffer yet and gets none, the call runs."""
+    a = Attention([900, 40, 300], [1, 2, 1], 8, 2, 64, 64, 16, 1500)
+    t = [ints(x) for x in (a.starts, a.lengths, a.table, a.prefix_pages)]
+    o = torch.full((a.rows, 8, 64), 9.0, dtype=H, device="cuda")
+    main, other = torch.cuda.Stream(), torch.cuda.Stream()
+    monkeypatch.setattr(pkg, "_PAGED_WORKSPACES", {})
+    monkeypatch.setattr(pkg, "_STREAM_WORKSPACES", {})
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=main,
+                          capture_error_mode="thread_local"):
+        x = torch.full((1000,), 3.0, device="cuda")
+        pkg.shared_prefix_attention(a.q, a.kc, a.vc, *t, a.prefix, o,
+                                    stream=other)
+    torch.cuda.synchronize()
+    a.check(o)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert bool((x == 3).all())
+    want = a.call(pkg)  # with a buffer: the same within the roundings
+    a.check(want)
+
+
 def hip(status):
     assert status == 0, status
 
