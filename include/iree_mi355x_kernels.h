@@ -346,7 +346,7 @@ int iree_mi355x_append_kv_f16(const iree_mi355x_kv_cache_t *cache,
 // the prefix and own tokens 0 .. lengths[b] - added[b] + i, added[b] =
 // row_starts[b + 1] - row_starts[b]: the new tokens are its last ones.
 //   o[row, h] = softmax(q[row, h] k^T * scale) v, KV head h / (heads /
-//   kv_heads); 0 for a row that sees no key
+//   kv_heads); 0 for a row that sees no key, NaN for one with a NaN score
 // Tokens in pages outside the cache are not seen, nor those past table_width
 // pages. Rows from row_starts[batch] on are left as they were. A NaN or
 // infinity in the V of a token that a row does not see may reach it where

@@ -1443,9 +1443,10 @@ def _paged_workspace_need(rows, batch, h, hkv, d, dv, page, width,
 def shared_prefix_attention(q, k_cache, v_cache, row_starts, lengths,
                             block_table, prefix_pages=None, prefix_length=0,
                             o=None, *, scale=None, stream=None):
-    """Attention of a batch's new tokens over a paged KV cache, the keys of a
-    prefix that all requests share read once for all of them. q [T, H, D]
-    holds the requests' rows one after the other, request b's at row_starts[b]
+    """Attention of a batch's new tokens over a paged KV cache, behind a prefix
+    that all requests share. Its keys are read once for all requests of up to
+    16 rows (tokens * H // Hkv); a longer request reads them in tiles of its
+    own rows. q [T, H, D] holds the requests' rows one after the other, request b's at row_starts[b]
     .. row_starts[b + 1] - 1; its own tokens are the first lengths[b] of the
     pages block_table[b] (the new ones included, appended before), and the
     prefix the first prefix_length tokens of prefix_pages. A row sees the

@@ -30,9 +30,9 @@
 // into a two-slot LDS ring that all waves read, one barrier a block; two such
 // workgroups share a CU, so one's softmax runs beside the other's MFMAs. They
 // are bound by issuing: of a step's 4100 cycles the matrix cores are busy for
-// 45 % (four prompts, 2243 rows of 32 heads behind 4096 keys: 193 GFLOP in 221
-// us and 17 to join, 870 TFLOP/s without the joining). Two barriers a step
-// with copies further ahead took 263 us for the 239 of then, copies between
+// 45 % (four prompts, 2243 rows of 32 heads behind 4096 keys: 193 GFLOP in 234
+// to 244 us by box, 790 to 820 TFLOP/s, of which 17 us to join). Two barriers a
+// step with copies further ahead took 263 us for the 239 of then, copies between
 // the MFMAs 247.
 // A call costs 7 us at least (launch 2, finding its place 2, a tile 3), and 4
 // more where parts are joined.
@@ -102,7 +102,8 @@ struct Requests {
   uint32_t small[64];
 };
 
-// Requests of up to 16 rows share tiles of the prefix.
+// Requests of up to 16 rows share tiles of the prefix (a request of 17 has a tile
+// of its own and walks the prefix in it).
 constexpr int kSmallRows = kNarrowRows;
 
 // One tile's work: rows r0 .. r_end - 1 (of a KV head; `compact`: the small
