@@ -1446,14 +1446,14 @@ def shared_prefix_attention(q, k_cache, v_cache, row_starts, lengths,
     """Attention of a batch's new tokens over a paged KV cache, behind a prefix
     that all requests share. Its keys are read once for all requests of up to
     16 rows (tokens * H // Hkv); a longer request reads them in tiles of its
-    own rows. q [T, H, D] holds the requests' rows one after the other, request b's at row_starts[b]
-    .. row_starts[b + 1] - 1; its own tokens are the first lengths[b] of the
-    pages block_table[b] (the new ones included, appended before), and the
-    prefix the first prefix_length tokens of prefix_pages. A row sees the
-    prefix and its request's own tokens up to itself. k_cache [P, Hkv, S, D]
-    and v_cache [P, Hkv, S, Dv] as in append_kv; o [T, H, Dv] f16 keeps the
-    rows past row_starts[B]. Tables are int32, from page_tables. With
-    prefix_length 0 this is paged attention."""
+    own rows. q [T, H, D] holds the requests' rows one after the other, request
+    b's at row_starts[b] .. row_starts[b + 1] - 1; its own tokens are the first
+    lengths[b] of the pages block_table[b] (the new ones included, appended
+    before), and the prefix the first prefix_length tokens of prefix_pages. A
+    row sees the prefix and its request's own tokens up to itself. k_cache
+    [P, Hkv, S, D] and v_cache [P, Hkv, S, Dv] as in append_kv; o [T, H, Dv]
+    f16 keeps the rows past row_starts[B]. Tables are int32, from page_tables.
+    With prefix_length 0 this is paged attention."""
     if _F16 is None:
         _load_types()
     fields = _cache_fields(k_cache, v_cache)

@@ -31,7 +31,7 @@
 // workgroups share a CU, so one's softmax runs beside the other's MFMAs. They
 // are bound by issuing: of a step's 4100 cycles the matrix cores are busy for
 // 45 % (four prompts, 2243 rows of 32 heads behind 4096 keys: 193 GFLOP in 234
-// to 244 us by box, 790 to 820 TFLOP/s, of which 17 us to join). Two barriers a
+// to 244 us by card, 790 to 820 TFLOP/s, of which 17 us to join). Two barriers a
 // step with copies further ahead took 263 us for the 239 of then, copies between
 // the MFMAs 247.
 // A call costs 7 us at least (launch 2, finding its place 2, a tile 3), and 4
@@ -590,7 +590,7 @@ __device__ __forceinline__ void wide_tile(const PagedTile &t,
   // another in a page; with a head's rows within 4 GiB their place is then one
   // scalar offset, and a lane's own the same for all copies: 28 instructions a
   // block instead of 100 (four prompts of 2243 rows 255.7 -> 247.3 us on one
-  // box, others the same).
+  // card, others the same).
   static_assert(ROWS % KROWS == 0, "a group of V's rows holds K's");
   const int k_at = lane / KCH, v_at = lane / CH;
   int k_chunk[TURN];
