@@ -387,6 +387,100 @@ int iree_mi355x_shared_prefix_attention_f16(
 size_t iree_mi355x_shared_prefix_attention_workspace_bytes(
     const iree_mi355x_paged_attention_t *args);
 
+// Trees of drafted tokens: a request's new rows are the nodes of a tree (or of
+// several), each after its parent, and a node sees its ancestors and itself
+// instead of all rows before it.
+
+// From the nodes' parents (numbers within their request; -1, or any that is not
+// an earlier node of it: a root), for row i of a request:
+//   masks[row], `words` words: bit j % 32 of word j / 32 is set where node j is
+//     i or an ancestor of it, j < 32 * words
+//   depths[row]: how many ancestors it has
+// Rows from row_starts[batch] on get 0 in both.
+typedef struct iree_mi355x_tree_masks_t {
+  const int32_t *parents;     // [rows]
+  const int32_t *row_starts;  // [batch + 1]
+  int32_t *masks;             // [rows, words]
+  int32_t *depths;            // [rows]
+  int64_t rows, batch, words;
+} iree_mi355x_tree_masks_t;
+int iree_mi355x_tree_masks(const iree_mi355x_tree_masks_t *args, void *stream);
+
+// iree_mi355x_shared_prefix_attention_f16 of trees: row i of a request sees the
+// prefix, the request's cached tokens, and of the new ones those j <= i whose
+// bit is set in masks[row] (`words` words, row pitch mask_stride in words).
+// Tokens from the 32 * words'th new one on have no bit and are seen by every
+// row from themselves on, as without masks, so a prompt beside trees needs no
+// more words than they do. Its workspace is that call's.
+int iree_mi355x_tree_attention_f16(const iree_mi355x_paged_attention_t *args,
+                                   const int32_t *masks, int64_t words,
+                                   int64_t mask_stride, void *workspace,
+                                   size_t workspace_bytes, void *stream);
+
+// ------------------------------------------------------------- packed rows
+//
+// Whole sequences of different lengths as packed rows, without a cache.
+
+// Attention of packed sequences, f16 in, f16 or f32 (OUT_F32) out, f32 scores
+// and softmax. Sequence b's queries are rows row_starts[b] .. row_starts[b + 1]
+// - 1 of q and o, its keys rows key_starts[b] .. key_starts[b + 1] - 1 of k and
+// v (the same array where they are the same rows). With n queries and m keys,
+// query i sees all keys, or with CAUSAL keys 0 .. m - n + i: the queries are
+// its last tokens.
+//   o[row, h] = softmax(q[row, h] k^T * scale) v, KV head h / (heads /
+//   kv_heads); 0 for a row that sees no key, NaN for one with a NaN score
+// Rows from row_starts[batch] on are left as they were. A NaN or infinity in the V
+// of a key that a row does not see may reach it where another row of its tile
+// sees the key (0 times it). Head dims are multiples of 8 up to 256. The starts
+// must ascend from 0: where they do not, rows hold anything, but nothing
+// outside the tensors is read or written. The workspace is as
+// iree_mi355x_shared_prefix_attention_f16's.
+typedef struct iree_mi355x_packed_attention_t {
+  const void *q;              // [rows, heads, head_dim]
+  const void *k;              // [key_rows, kv_heads, head_dim]
+  const void *v;              // [key_rows, kv_heads, head_dim_v]
+  void *o;                    // [rows, heads, head_dim_v]
+  const int32_t *row_starts;  // [batch + 1]
+  const int32_t *key_starts;  // [batch + 1]
+  int64_t rows, key_rows, batch, heads, kv_heads, head_dim, head_dim_v;
+  // (row, head), in elements: multiples of 8 and 16-byte aligned, o's of 4 and
+  // 8-byte (f32: 16-byte) aligned
+  int64_t q_strides[2], k_strides[2], v_strides[2], o_strides[2];
+  float scale;
+  uint32_t flags;  // IREE_MI355X_ATTENTION_CAUSAL | _OUT_F32
+} iree_mi355x_packed_attention_t;
+int iree_mi355x_packed_attention_f16(const iree_mi355x_packed_attention_t *args,
+                                     void *workspace, size_t workspace_bytes,
+                                     void *stream);
+
+// The workspace a call of these extents can use (0: none); pointers and
+// strides are not looked at.
+size_t iree_mi355x_packed_attention_workspace_bytes(
+    const iree_mi355x_packed_attention_t *args);
+
+// Rotary positions with several axes (a token's time, height and width), f16.
+// The first 2 * half dims of every head are half = sum of sections pairs, (i,
+// half + i) or with INTERLEAVED (2 i, 2 i + 1); the first sections[0] pairs turn
+// by positions of axis 0, the next sections[1] by those of axis 1, and so on:
+//   t = positions[axis, row] * frequencies[i], the product in 64 bits
+//   y1 = x1 cos t - x2 sin t, y2 = x2 cos t + x1 sin t
+// The dims past them are copied. Outputs may be their inputs, with the same
+// strides (in place); otherwise they do not overlap them. kv_heads 0: q alone.
+#define IREE_MI355X_ROTARY_INTERLEAVED 0x1u
+typedef struct iree_mi355x_rotary_t {
+  const void *q, *k;  // [rows, heads, head_dim], [rows, kv_heads, head_dim]
+  void *q_out, *k_out;
+  const int32_t *positions;  // [axes, rows], axis pitch position_stride
+  const float *frequencies;  // [half]
+  int64_t rows, heads, kv_heads, head_dim;  // head_dim up to 256
+  int64_t axes, sections[4];                // 1 to 4
+  int64_t position_stride;
+  int64_t q_strides[2], k_strides[2];  // (row, head), in elements; 16-byte
+  int64_t q_out_strides[2], k_out_strides[2];  // accesses where all allow it
+  uint32_t flags;
+} iree_mi355x_rotary_t;
+int iree_mi355x_rotary_f16(const iree_mi355x_rotary_t *args, void *stream);
+
 // Workspace a matmul_f16 / matmul_i8 / w8a16_matmul call of this shape
 // needs (split-K
 // partials and arrival counters), 0 if none. Mirrors the scratch query of the

@@ -44,6 +44,7 @@ SPLITS_STREAM_K = -1  # matmul_mfma_config: stream-K runs of (tile, K stage)
 CAUSAL = 0x1
 ATTENTION_OUT_F32 = 0x2
 ATTENTION_MASK = 0x4
+ROTARY_INTERLEAVED = 0x1
 
 # Element kinds (iree_mi355x_elem_t) and kernel families.
 ELEM_F16, ELEM_I8, ELEM_I32, ELEM_F32 = 0, 1, 2, 3
@@ -90,6 +91,9 @@ EXPORTED_SYMBOLS = (
     "iree_mi355x_page_tables", "iree_mi355x_append_kv_f16",
     "iree_mi355x_shared_prefix_attention_f16",
     "iree_mi355x_shared_prefix_attention_workspace_bytes",
+    "iree_mi355x_tree_masks", "iree_mi355x_tree_attention_f16",
+    "iree_mi355x_packed_attention_f16",
+    "iree_mi355x_packed_attention_workspace_bytes", "iree_mi355x_rotary_f16",
 )
 
 # Activations of the fused matmul epilogue (include/iree_mi355x_kernels.h).
@@ -313,6 +317,12 @@ def library():
     lib.iree_mi355x_shared_prefix_attention_f16.argtypes = [p, p, sz, p]
     lib.iree_mi355x_shared_prefix_attention_workspace_bytes.restype = sz
     lib.iree_mi355x_shared_prefix_attention_workspace_bytes.argtypes = [p]
+    lib.iree_mi355x_tree_masks.argtypes = [p, p]
+    lib.iree_mi355x_tree_attention_f16.argtypes = [p, p, i64, i64, p, sz, p]
+    lib.iree_mi355x_packed_attention_f16.argtypes = [p, p, sz, p]
+    lib.iree_mi355x_packed_attention_workspace_bytes.restype = sz
+    lib.iree_mi355x_packed_attention_workspace_bytes.argtypes = [p]
+    lib.iree_mi355x_rotary_f16.argtypes = [p, p]
     lib.iree_mi355x_matmul_workspace_bytes.restype = sz
     lib.iree_mi355x_matmul_workspace_bytes.argtypes = [i64, i64, i64, u32]
     lib.iree_mi355x_batch_matmul_f16.argtypes = [
@@ -1203,7 +1213,40 @@ class PagedAttentionArgs(ctypes.Structure):
         ("scale", ctypes.c_float), ("flags", ctypes.c_uint32)]
 
 
+class TreeMasksArgs(ctypes.Structure):
+    """iree_mi355x_tree_masks_t."""
+    _fields_ = [(n, ctypes.c_void_p) for n in (
+        "parents", "row_starts", "masks", "depths")] + [
+        (n, ctypes.c_int64) for n in ("rows", "batch", "words")]
+
+
+class PackedAttentionArgs(ctypes.Structure):
+    """iree_mi355x_packed_attention_t."""
+    _fields_ = [(n, ctypes.c_void_p) for n in (
+        "q", "k", "v", "o", "row_starts", "key_starts")] + [
+        (n, ctypes.c_int64) for n in (
+            "rows", "key_rows", "batch", "heads", "kv_heads", "head_dim",
+            "head_dim_v")] + [(n + "_strides", ctypes.c_int64 * 2)
+                              for n in "qkvo"] + [
+        ("scale", ctypes.c_float), ("flags", ctypes.c_uint32)]
+
+
+class RotaryArgs(ctypes.Structure):
+    """iree_mi355x_rotary_t."""
+    _fields_ = [(n, ctypes.c_void_p) for n in (
+        "q", "k", "q_out", "k_out", "positions", "frequencies")] + [
+        (n, ctypes.c_int64) for n in (
+            "rows", "heads", "kv_heads", "head_dim", "axes")] + [
+        ("sections", ctypes.c_int64 * 4),
+        ("position_stride", ctypes.c_int64)] + [
+        (n + "_strides", ctypes.c_int64 * 2)
+        for n in ("q", "k", "q_out", "k_out")] + [("flags", ctypes.c_uint32)]
+
+
 # The structures above as bytes.
+_TREE_MASKS = struct.Struct("@4P3q")
+_PACKED_ATTENTION = struct.Struct("@6P15qfI")
+_ROTARY = struct.Struct("@6P18qI4x")
 _PAGE_TABLES = struct.Struct("@8P6q")
 _KV_CACHE = struct.Struct("@2P11q")
 _PAIR = struct.Struct("@2q")
@@ -1262,19 +1305,19 @@ def _stream_on(index, stream):
     return _stream_ptr(stream)
 
 
-def _empty_on(like, shape, stream):
+def _empty_on(like, shape, stream, dtype=None):
     """like.new_empty(shape) for a call on `stream` (None: the current one): in
     that stream's order, so that no other work still reads or writes the
     memory, and kept until the current stream's work with it is done too."""
     if stream is None:
-        return like.new_empty(shape)
+        return like.new_empty(shape, dtype=dtype)
     import torch
     here = torch.cuda.current_stream(like.device)
     there = _torch_stream(stream, like.device)
     if there.cuda_stream == here.cuda_stream:
-        return like.new_empty(shape)
+        return like.new_empty(shape, dtype=dtype)
     with torch.cuda.stream(there):
-        t = like.new_empty(shape)
+        t = like.new_empty(shape, dtype=dtype)
     t.record_stream(here)
     return t
 
@@ -1381,9 +1424,16 @@ def append_kv(k, v, k_cache, v_cache, slots, *, stream=None):
 _PAGED_WORKSPACES: dict = {}
 
 
-def _paged_call(args, need, index, stream):
-    """One attention call on the stream's own workspace of at least `need`
-    bytes: its status."""
+def _paged_call(fn, args, need, index, stream):
+    """One attention call of the library on a raw stream: its status. With
+    `need` bytes of the stream's own workspace, or of the graph's that is being
+    captured."""
+    if need == 0:
+        return fn(*args, None, 0, stream)
+    if stream and _capturing(stream):
+        held = _graph_workspace(need, index, stream)
+        return (fn(*args, None, 0, stream) if held is None
+                else fn(*args, held.data_ptr(), need, stream))
     held = _PAGED_WORKSPACES.get((index, stream))
     if held is None:
         held = _PAGED_WORKSPACES.setdefault((index, stream),
@@ -1394,8 +1444,7 @@ def _paged_call(args, need, index, stream):
             # while the current stream is capturing: what there is
             held[:2] = stream_workspace(need, torch.device("cuda", index),
                                         stream, "paged attention", True)
-        return library().iree_mi355x_shared_prefix_attention_f16(
-            args, held[0], held[1], stream)
+        return fn(*args, held[0], held[1], stream)
 
 
 def _capture_of(stream) -> int:
@@ -1454,6 +1503,13 @@ def shared_prefix_attention(q, k_cache, v_cache, row_starts, lengths,
     [P, Hkv, S, D] and v_cache [P, Hkv, S, Dv] as in append_kv; o [T, H, Dv]
     f16 keeps the rows past row_starts[B]. Tables are int32, from page_tables.
     With prefix_length 0 this is paged attention."""
+    return _cache_attention(q, k_cache, v_cache, row_starts, lengths,
+                            block_table, None, prefix_pages, prefix_length, o,
+                            scale, stream)
+
+
+def _cache_attention(q, k_cache, v_cache, row_starts, lengths, block_table,
+                     masks, prefix_pages, prefix_length, o, scale, stream):
     if _F16 is None:
         _load_types()
     fields = _cache_fields(k_cache, v_cache)
@@ -1486,22 +1542,28 @@ def shared_prefix_attention(q, k_cache, v_cache, row_starts, lengths,
                              "tokens")
     else:
         prefix_pages = None
+    if masks is not None:
+        have, words = _ints(masks, "masks", 2)
+        if have != rows or words < 1:
+            raise ValueError(f"masks must be [{rows}, at least 1], got "
+                             f"{list(masks.shape)}")
     index = q.get_device()
     if not (index >= 0 and index == k_cache.get_device()
             == v_cache.get_device() == row_starts.get_device()
             == lengths.get_device() == block_table.get_device()
             and (prefix_pages is None or index == prefix_pages.get_device())
+            and (masks is None or index == masks.get_device())
             and (o is None or index == o.get_device())):
         _on_device((q, "q"), (k_cache, "k_cache"), (v_cache, "v_cache"),
                    (row_starts, "row_starts"), (lengths, "lengths"),
                    (block_table, "block_table"),
-                   (prefix_pages, "prefix_pages"), (o, "o"))
+                   (masks, "masks"), (prefix_pages, "prefix_pages"), (o, "o"))
     if _other_device(index):
         import torch
         with torch.cuda.device(index):
-            return shared_prefix_attention(
-                q, k_cache, v_cache, row_starts, lengths, block_table,
-                prefix_pages, prefix_length, o, scale=scale, stream=stream)
+            return _cache_attention(
+                q, k_cache, v_cache, row_starts, lengths, block_table, masks,
+                prefix_pages, prefix_length, o, scale, stream)
     if o is None:
         o = _empty_on(q, (rows, h, dv), stream)
         o0, o1 = h * dv, dv
@@ -1512,19 +1574,233 @@ def shared_prefix_attention(q, k_cache, v_cache, row_starts, lengths,
         0 if prefix_pages is None else prefix_pages.data_ptr(), rows, h,
         batch, width, block_table.stride(0), prefix_length, q0, q1, o0, o1,
         d ** -0.5 if scale is None else scale, 0)
-    s = _stream_on(index, stream)
     need = _paged_workspace_need(rows, batch, h, hkv, d, dv, page, width,
                                  prefix_length)
-    if need > 0 and not (s and _capturing(s)):
-        st = _paged_call(args, need, index, s)
+    lib = library()
+    if masks is None:
+        st = _paged_call(lib.iree_mi355x_shared_prefix_attention_f16, (args,),
+                         need, index, _stream_on(index, stream))
     else:
-        held = _graph_workspace(need, index, s) if need > 0 else None
-        ws, wsb = (None, 0) if held is None else (held.data_ptr(), need)
-        st = library().iree_mi355x_shared_prefix_attention_f16(args, ws, wsb,
-                                                               s)
+        st = _paged_call(lib.iree_mi355x_tree_attention_f16,
+                         (args, masks.data_ptr(), words, masks.stride(0)),
+                         need, index, _stream_on(index, stream))
     if st != OK:
         _check(st)
     return o
+
+
+def tree_masks(parents, row_starts, words=1, *, stream=None):
+    """What the nodes of drafted trees see, for tree_attention. The new rows of
+    request b, row_starts[b] .. row_starts[b + 1] - 1, are nodes 0, 1, ... of a
+    tree (or several), each after its parent: parents [T] holds every node's
+    parent as a number within its request (-1, or any that is not an earlier
+    node of it: a root). Returns (masks [T, words], depths [T]): bit j % 32 of
+    masks[row, j // 32] is set where node j is the row's or an ancestor of it,
+    j < 32 * words, and depths counts a node's ancestors (its position is the
+    cached tokens' number plus that). Rows past row_starts[B] get 0. All int32;
+    one call a step serves every layer."""
+    if _I32 is None:
+        _load_types()
+    rows, = _ints(parents, "parents")
+    starts, = _ints(row_starts, "row_starts")
+    if starts < 1:
+        raise ValueError("row_starts must be [requests + 1], got [0]")
+    if words < 1:
+        raise ValueError(f"words {words} must be at least 1")
+    index = parents.get_device()
+    if not (index >= 0 and index == row_starts.get_device()):
+        _on_device((parents, "parents"), (row_starts, "row_starts"))
+    if _other_device(index):
+        import torch
+        with torch.cuda.device(index):
+            return tree_masks(parents, row_starts, words, stream=stream)
+    out = _empty_on(parents, rows * (words + 1), stream)
+    masks, depths = out.split_with_sizes((rows * words, rows))
+    st = library().iree_mi355x_tree_masks(_TREE_MASKS.pack(
+        parents.data_ptr(), row_starts.data_ptr(), out.data_ptr(),
+        out.data_ptr() + 4 * rows * words, rows, starts - 1, words),
+        _stream_on(index, stream))
+    if st != OK:
+        _check(st)
+    return masks.view(rows, words), depths
+
+
+def tree_attention(q, k_cache, v_cache, row_starts, lengths, block_table,
+                   masks, prefix_pages=None, prefix_length=0, o=None, *,
+                   scale=None, stream=None):
+    """shared_prefix_attention of drafted trees: of its request's new tokens a
+    row sees those before it and itself whose bit is set in masks [T, W] (int32,
+    from tree_masks), instead of all of them; the prefix and the cached tokens
+    it sees whole. New tokens from the 32 * W'th on have no bit and are seen as
+    without masks, so a prompt beside trees needs no more words than they do.
+    A row that sees nothing is 0."""
+    if masks is None:
+        raise TypeError("masks must be an int32 tensor")
+    return _cache_attention(q, k_cache, v_cache, row_starts, lengths,
+                            block_table, masks, prefix_pages, prefix_length, o,
+                            scale, stream)
+
+
+@functools.lru_cache(maxsize=4096)
+def _packed_workspace_need(rows, keys, batch, h, hkv, d, dv) -> int:
+    return library().iree_mi355x_packed_attention_workspace_bytes(
+        ctypes.byref(PackedAttentionArgs(
+            rows=rows, key_rows=keys, batch=batch, heads=h, kv_heads=hkv,
+            head_dim=d, head_dim_v=dv)))
+
+
+def packed_attention(q, k, v, row_starts, key_starts=None, o=None, *,
+                     causal=True, scale=None, out_dtype=None, stream=None):
+    """Attention of whole sequences of different lengths, packed one after the
+    other: q [T, H, D], k [N, Hkv, D], v [N, Hkv, Dv], f16 with any row and head
+    strides that are multiples of 8. Sequence b's queries are rows
+    row_starts[b] .. row_starts[b + 1] - 1 (int32 [B + 1], ascending from 0), its
+    keys rows key_starts[b] .. key_starts[b + 1] - 1 (None: the same rows). Every
+    query sees all of its sequence's keys, or with `causal` those up to itself,
+    the queries being the sequence's last tokens: query i of n sees keys
+    0 .. m - n + i of m. One that sees none is 0. o [T, H, Dv], f16 or f32
+    (out_dtype), keeps the rows past row_starts[B]."""
+    if _F16 is None:
+        _load_types()
+    (rows, h, d), (q0, q1, _) = _rows_of(q, "q", 3)
+    (keys, hkv, of_k), (k0, k1, _) = _rows_of(k, "k", 3)
+    (*rest, dv), (v0, v1, _) = _rows_of(v, "v", 3)
+    if of_k != d:
+        _shape(k, (keys, hkv, d), "k")
+    if rest != [keys, hkv]:
+        _shape(v, (keys, hkv, dv), "v")
+    if hkv < 1 or h % hkv:
+        raise ValueError(f"{h} query heads are not a multiple of {hkv} KV "
+                         "heads")
+    flags = CAUSAL if causal else 0
+    if o is None and out_dtype in (None, _F16):
+        pass
+    else:
+        import torch
+        want = out_dtype or o.dtype
+        if want not in (torch.float16, torch.float32):
+            raise TypeError("packed_attention writes float16 or float32")
+        if o is not None:
+            _require(o, want, "o", (3,))
+            _shape(o, (rows, h, dv), "o")
+            o0, o1, _ = o.stride()
+        if want == torch.float32:
+            flags |= ATTENTION_OUT_F32
+    starts, = _ints(row_starts, "row_starts")
+    if starts < 1:
+        raise ValueError("row_starts must be [sequences + 1], got [0]")
+    if key_starts is None:
+        if keys != rows:
+            raise ValueError(f"{rows} queries and {keys} keys need key_starts")
+        key_starts = row_starts
+    elif _ints(key_starts, "key_starts") != (starts,):
+        _shape(key_starts, (starts,), "key_starts")
+    index = q.get_device()
+    if not (index >= 0 and index == k.get_device() == v.get_device()
+            == row_starts.get_device() == key_starts.get_device()
+            and (o is None or index == o.get_device())):
+        _on_device((q, "q"), (k, "k"), (v, "v"), (row_starts, "row_starts"),
+                   (key_starts, "key_starts"), (o, "o"))
+    if _other_device(index):
+        import torch
+        with torch.cuda.device(index):
+            return packed_attention(
+                q, k, v, row_starts, key_starts, o, causal=causal,
+                scale=scale, out_dtype=out_dtype, stream=stream)
+    if o is None:
+        o = _empty_on(q, (rows, h, dv), stream,
+                      None if not flags & ATTENTION_OUT_F32 else want)
+        o0, o1 = h * dv, dv
+    batch = starts - 1
+    st = _paged_call(
+        library().iree_mi355x_packed_attention_f16,
+        (_PACKED_ATTENTION.pack(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
+            row_starts.data_ptr(), key_starts.data_ptr(), rows, keys, batch, h,
+            hkv, d, dv, q0, q1, k0, k1, v0, v1, o0, o1,
+            d ** -0.5 if scale is None else scale, flags),),
+        _packed_workspace_need(rows, keys, batch, h, hkv, d, dv), index,
+        _stream_on(index, stream))
+    if st != OK:
+        _check(st)
+    return o
+
+
+def rotary(q, k, positions, frequencies, sections=None, *, interleaved=False,
+           q_out=None, k_out=None, stream=None):
+    """Rotary positions of packed rows: turns the first 2 * P dims of every
+    head of q [T, H, D] and k [T, Hkv, D] (f16; k None: q alone) and copies the
+    others. positions [T] or [A, T] (int32) has 1 to 4 axes (a token's time,
+    height and width), frequencies [P] (f32) the angle per position of every
+    pair, and sections how many pairs turn by each axis, in their order (None:
+    one axis). Pair i is dims i and P + i, or with `interleaved` 2 i and 2 i + 1.
+    Angles are made in 64 bits, so far positions keep theirs. Returns (q_out,
+    k_out); q_out=q and k_out=k rotate in place (they may not overlap
+    otherwise)."""
+    if _F16 is None:
+        _load_types()
+    import torch
+    (rows, h, d), (q0, q1, _) = _rows_of(q, "q", 3)
+    hk = k0 = k1 = 0
+    if k is not None:
+        (of_t, hk, of_d), (k0, k1, _) = _rows_of(k, "k", 3)
+        if (of_t, of_d) != (rows, d):
+            _shape(k, (rows, hk, d), "k")
+    elif k_out is not None:
+        raise ValueError("k_out without k")
+    dims = positions.dim() if isinstance(positions, torch.Tensor) else 1
+    *axes, of_t = _ints(positions, "positions", 2 if dims == 2 else 1)
+    axes = axes[0] if axes else 1
+    if of_t != rows:
+        raise ValueError(f"positions must be [{rows}] or [axes, {rows}], got "
+                         f"{list(positions.shape)}")
+    _require(frequencies, torch.float32, "frequencies", (1,))
+    half, = frequencies.shape
+    if half > 1 and frequencies.stride(0) != 1:
+        raise ValueError("frequencies must be contiguous")
+    sections = (half,) if sections is None else tuple(sections)
+    if not 1 <= axes <= 4 or len(sections) != axes:
+        raise ValueError(f"{len(sections)} sections for {axes} axes (1 to 4)")
+    if min(sections) < 0 or sum(sections) != half or 2 * half > d:
+        raise ValueError(f"sections {sections} must be the {half} "
+                         f"frequencies, and twice them at most head_dim {d}")
+    qo, ko = (h * d, d), (hk * d, d)
+    if q_out is not None:
+        of_q, (*qo, _) = _rows_of(q_out, "q_out", 3)
+        if of_q != (rows, h, d):
+            _shape(q_out, (rows, h, d), "q_out")
+    if k_out is not None:
+        of_k, (*ko, _) = _rows_of(k_out, "k_out", 3)
+        if of_k != (rows, hk, d):
+            _shape(k_out, (rows, hk, d), "k_out")
+    index = q.get_device()
+    if not (index >= 0 and index == positions.get_device()
+            == frequencies.get_device()
+            and (k is None or index == k.get_device())
+            and (q_out is None or index == q_out.get_device())
+            and (k_out is None or index == k_out.get_device())):
+        _on_device((q, "q"), (k, "k"), (positions, "positions"),
+                   (frequencies, "frequencies"), (q_out, "q_out"),
+                   (k_out, "k_out"))
+    if _other_device(index):
+        with torch.cuda.device(index):
+            return rotary(q, k, positions, frequencies, sections,
+                          interleaved=interleaved, q_out=q_out, k_out=k_out,
+                          stream=stream)
+    if q_out is None:
+        q_out = _empty_on(q, (rows, h, d), stream)
+    if k_out is None and k is not None:
+        k_out = _empty_on(k, (rows, hk, d), stream)
+    st = library().iree_mi355x_rotary_f16(_ROTARY.pack(
+        q.data_ptr(), 0 if k is None else k.data_ptr(), q_out.data_ptr(),
+        0 if k is None else k_out.data_ptr(), positions.data_ptr(),
+        frequencies.data_ptr(), rows, h, hk, d, axes,
+        *sections, *(0,) * (4 - axes), positions.stride(0) if axes > 1 else 0,
+        q0, q1, k0, k1, *qo, *ko, ROTARY_INTERLEAVED if interleaved else 0),
+        _stream_on(index, stream))
+    if st != OK:
+        _check(st)
+    return q_out, k_out
 
 
 def matmul_mfma_config(index, a, b, c, *, scale=None, splits=0, accumulate=False,

@@ -110,6 +110,7 @@ constexpr int kSmallRows = kNarrowRows;
 // requests' rows alone) against steps s_begin .. s_end - 1 of 64 keys, the
 // first `lead` of them the prefix's.
 struct PagedTile {
+  int64_t key0;  // kRows: the row of the request's first key
   int kv_head, r0, r_end;
   bool compact;
   int lead;
@@ -126,6 +127,34 @@ __device__ __forceinline__ int sees(const PagedAttention &p,
                                     const PagedTile &t, int r) {
   const int64_t n = (int64_t)t.base + token_of(p, r) - t.first + 1;
   return n < 0 ? 0 : n > t.own_end ? t.own_end : (int)n;
+}
+
+// What a row's mask says of the KEYS own keys from key0, bit i of key key0 + i.
+// New token j of the request is key t.base + j: those below 0 are cached, those
+// from 32 * words on have no bit, and neither are hidden here.
+struct TreeWords {
+  uint32_t w[3];
+};
+template <int KEYS>
+__device__ __forceinline__ TreeWords tree_words(const PagedAttention &p,
+                                                const PagedTile &t, int token,
+                                                int key0) {
+  const int32_t *mine = p.masks + (int64_t)token * p.mask_stride;
+  const int first = (key0 - t.base) >> 5;
+  TreeWords x;
+#pragma unroll
+  for (int i = 0; i <= KEYS / 32; ++i) {
+    const int at = first + i, last = p.words - 1;
+    const uint32_t word = (uint32_t)mine[at < 0 ? 0 : at < last ? at : last];
+    x.w[i] = at < 0 || at > last ? ~0u : word;
+  }
+  return x;
+}
+__device__ __forceinline__ uint32_t tree_bits(const PagedTile &t,
+                                              const TreeWords &x, int key0,
+                                              int half) {
+  return __builtin_amdgcn_alignbit(x.w[half + 1], x.w[half],
+                                   (uint32_t)(key0 - t.base) & 31);
 }
 
 // The packed row of the small requests' row r: the last lane whose small rows
@@ -188,7 +217,7 @@ struct Pages {
   const int32_t *prefix_pages, *table;
   int prefix, own_end;  // keys
   int pages, page_size, shift, near;
-  uint32_t magic, k_page, k_row, v_page, v_row;
+  uint32_t magic, k_page, k_row, v_page, v_row, key0;
 
   __device__ __forceinline__ Pages(const PagedAttention &p, const PagedTile &t)
       : prefix_pages(held(p.prefix_pages)), table(held(t.table)),
@@ -196,14 +225,15 @@ struct Pages {
         page_size(held(p.page_size)), shift(held(p.page_shift)),
         near(held(p.near)), magic(held(p.page_magic)),
         k_page(held(p.k_page16)), k_row(held(p.k_row16)),
-        v_page(held(p.v_page16)), v_row(held(p.v_row16)) {}
+        v_page(held(p.v_page16)), v_row(held(p.v_row16)),
+        key0((uint32_t)t.key0) {}
 };
 
 // Pages of the KEYS keys of a block: a lane's key, its table's page number
 // (find, a block ahead of the rows) and the places in the caches that `place`
 // makes of it, in 16 bytes. A page that the cache does not have hides its
 // keys.
-template <int KEYS>
+template <int KEYS, PagedKeys KIND>
 struct PagedBlock {
   typedef typename std::conditional<KEYS == 64, uint64_t, uint32_t>::type Mask;
   int found = 0, inside = 0;
@@ -215,6 +245,11 @@ struct PagedBlock {
   // multiple of them holds whole).
   __device__ __forceinline__ void find(const Pages &p, int lead, int c,
                                        int group = 1) {
+    if constexpr (KIND == PagedKeys::kRows) {
+      const int key = c * KEYS + ((int)threadIdx.x & (KEYS - 1));
+      inside = key < p.own_end ? key : p.own_end - 1;
+      return;
+    }
     const bool own = c >= lead;
     const int end = own ? p.own_end : p.prefix;
     const int32_t *table = own ? p.table : p.prefix_pages;
@@ -229,6 +264,12 @@ struct PagedBlock {
   __device__ __forceinline__ void place(const Pages &p, int lead, int c) {
     const bool own = c >= lead;
     const int left = own ? p.own_end - (c - lead) * KEYS : p.prefix - c * KEYS;
+    if constexpr (KIND == PagedKeys::kRows) {
+      k = (p.key0 + (uint32_t)inside) * p.k_row;
+      v = (p.key0 + (uint32_t)inside) * p.v_row;
+      there = left < KEYS ? ((Mask)1 << left) - 1 : ~(Mask)0;
+      return;
+    }
     const bool has = (uint32_t)found < (uint32_t)p.pages;
     const uint32_t page = has ? (uint32_t)found : 0u;
     if (p.near) {  // every factor below 2^24
@@ -245,11 +286,20 @@ struct PagedBlock {
 };
 
 // Where a row's result or part goes.
-__device__ __forceinline__ f16 *result_row(const PagedAttention &p, int kv_head,
-                                           int row) {
+__device__ __forceinline__ int64_t result_row(const PagedAttention &p,
+                                              int kv_head, int row) {
   const int token = token_of(p, row);
-  return p.o + (int64_t)token * p.o_row +
+  return (int64_t)token * p.o_row +
          (int64_t)(kv_head * p.group + row - token * p.group) * p.o_head;
+}
+// Four columns of it.
+template <PagedKeys KIND>
+__device__ __forceinline__ void store_result(const PagedAttention &p,
+                                             int64_t at, f32x4 x) {
+  if (KIND == PagedKeys::kRows && p.out_f32)
+    *(f32x4 *)((float *)p.o + at) = x;
+  else
+    *(f16x4 *)(p.o + at) = f16x4{(f16)x[0], (f16)x[1], (f16)x[2], (f16)x[3]};
 }
 __device__ __forceinline__ int64_t part_row(const PagedAttention &p,
                                             const PagedTile &t, int row) {
@@ -260,7 +310,7 @@ __device__ __forceinline__ int64_t part_row(const PagedAttention &p,
 
 // A tile of up to 16 rows. DP: the row of a staged V (64, 128 or 256); DX: a
 // multiple of 32 up to it, at least V's head dim; DK: alike of Q's and K's.
-template <int DP, int DX, int DK>
+template <int DP, int DX, int DK, PagedKeys KIND>
 __device__ __forceinline__ void narrow_tile(const PagedTile &t,
                                             const Requests &all, char *smem,
                                             float (*wave_m)[kNarrowRows],
@@ -290,7 +340,9 @@ __device__ __forceinline__ void narrow_tile(const PagedTile &t,
   // This lane's query row (rows past the end repeat the last one), the own
   // keys that it sees, and those that every row sees.
   const int r_mine = t.r0 + l15 < t.r_end ? t.r0 + l15 : t.r_end - 1;
-  const int limit = sees(p, t, r_mine), all_own = sees(p, t, t.r0);
+  const int limit = sees(p, t, r_mine);
+  const int all_own = KIND == PagedKeys::kTree ? t.base : sees(p, t, t.r0);
+  const int token = token_of(p, r_mine);
   i32x4 qf[KS];
   {
     const f16 *qp = query_row(p, t, all, r_mine);
@@ -321,7 +373,14 @@ __device__ __forceinline__ void narrow_tile(const PagedTile &t,
   if (c_end > t.s_end * (kStepKeys / kBlockKeys))
     c_end = t.s_end * (kStepKeys / kBlockKeys);
   const Pages pages(p, t);
-  PagedBlock<kBlockKeys> block;
+  PagedBlock<kBlockKeys, KIND> block;
+  // The mask's words of a block, read with its rows.
+  TreeWords tree = {{~0u, ~0u, ~0u}}, tree_next = tree;
+  auto load_tree = [&](int c) __attribute__((always_inline)) {
+    const int key0 = (c - lead) * kBlockKeys;
+    if (KIND == PagedKeys::kTree && c >= lead && key0 + kBlockKeys > t.base)
+      tree_next = tree_words<kBlockKeys>(p, t, token, key0);
+  };
   i32x4 kf[2][KS], vf[VP];
   auto load_k = [&]() __attribute__((always_inline)) {
 #pragma unroll
@@ -358,6 +417,7 @@ __device__ __forceinline__ void narrow_tile(const PagedTile &t,
     block.place(pages, lead, c);
     load_k();
     load_v();
+    load_tree(c);
     if (c + kPagedWaves < c_end)
       block.find(pages, lead, c + kPagedWaves);
   }
@@ -366,6 +426,7 @@ __device__ __forceinline__ void narrow_tile(const PagedTile &t,
     const bool own = c >= lead;
     const int key0 = (own ? c - lead : c) * kBlockKeys;
     const uint32_t live = block.there;
+    tree = tree_next;
     if (pad_k) {
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks)
@@ -383,16 +444,20 @@ __device__ __forceinline__ void narrow_tile(const PagedTile &t,
     }
     if (live != 0xffffffffu || (own && key0 + kBlockKeys > all_own)) {
       const int end = (own ? limit : pages.prefix) - key0;
+      uint32_t seen = live;
+      if (KIND == PagedKeys::kTree && own && key0 + kBlockKeys > t.base)
+        seen &= tree_bits(t, tree, key0, 0);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const int key = 16 * (e >> 2) + 4 * lg + (e & 3);
-        if (key >= end || !(live >> key & 1))
+        if (key >= end || !(seen >> key & 1))
           s[e >> 2][e & 3] = kNegInf;
       }
     }
     if (more) {
       block.place(pages, lead, c + kPagedWaves);
       load_k();
+      load_tree(c + kPagedWaves);
       if (c + 2 * kPagedWaves < c_end)
         block.find(pages, lead, c + 2 * kPagedWaves);
     }
@@ -503,13 +568,11 @@ __device__ __forceinline__ void narrow_tile(const PagedTile &t,
   }
   if (t.part < 0) {
     const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
-    f16 *dst = result_row(p, t.kv_head, row) + dq;
+    const int64_t dst = result_row(p, t.kv_head, row) + dq;
 #pragma unroll
     for (int e = 0; e < CPT / 4; ++e)
       if (dq + 4 * e < p.dv)  // dv is a multiple of 8
-        *(f16x4 *)(dst + 4 * e) =
-            f16x4{(f16)(acc[e][0] * inv), (f16)(acc[e][1] * inv),
-                  (f16)(acc[e][2] * inv), (f16)(acc[e][3] * inv)};
+        store_result<KIND>(p, dst + 4 * e, acc[e] * inv);
   } else {
     const int64_t at = part_row(p, t, row);
 #pragma unroll
@@ -532,10 +595,10 @@ __device__ __forceinline__ int wide_k_swizzle(int key) {
 }
 template <int DP>
 __device__ __forceinline__ int wide_v_swizzle(int key) {
-  return DP == 128 ? 4 * (key & 3) : 4 * ((key >> 1) & 1);
+  return DP >= 128 ? 4 * (key & 3) : 4 * ((key >> 1) & 1);
 }
 
-template <int DP, int DX, int DK>
+template <int DP, int DX, int DK, PagedKeys KIND>
 __device__ __forceinline__ void wide_tile(const PagedTile &t,
                                           const Requests &all, char *smem) {
   const PagedAttention &p = arguments();
@@ -551,6 +614,10 @@ __device__ __forceinline__ void wide_tile(const PagedTile &t,
   constexpr int PASSES = kStepKeys / (kPagedWaves * ROWS);
   // Passes of K after which its swizzle, of 16 rows, is the same again.
   constexpr int TURN = kPagedWaves * KROWS < 16 ? 16 / (kPagedWaves * KROWS) : 1;
+  // LDS reads whose waits are counted here, not by the compiler. A read that is
+  // still on its way must stay in its registers, so not where there are too few
+  // of them.
+  constexpr bool OWN_WAITS = DP < 256;
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -564,7 +631,11 @@ __device__ __forceinline__ void wide_tile(const PagedTile &t,
   const int r_mine = r_wave + l32 < t.r_end ? r_wave + l32 : t.r_end - 1;
   const bool idle = r_wave >= t.r_end;  // no rows: the wave only copies
   const int limit = sees(p, t, r_mine);
-  const int all_own = sees(p, t, r_wave < t.r_end ? r_wave : t.r_end - 1);
+  const int all_own =
+      KIND == PagedKeys::kTree
+          ? t.base
+          : sees(p, t, r_wave < t.r_end ? r_wave : t.r_end - 1);
+  const int token = token_of(p, r_mine);
   i32x4 qf[DS];
   {
     const f16 *qp = query_row(p, t, all, r_mine);
@@ -604,7 +675,8 @@ __device__ __forceinline__ void wide_tile(const PagedTile &t,
   const int v_chunk = lane % CH ^ wide_v_swizzle<DP>(wave * ROWS + v_at);
   const bool v_in = 8 * v_chunk < p.dv;
   const Pages pages(p, t);
-  const bool grouped = pages.near && pages.page_size % ROWS == 0;
+  const bool grouped = KIND != PagedKeys::kRows && pages.near &&
+                       pages.page_size % ROWS == 0;
   const bool alike = KPASSES == PASSES && pages.k_page == pages.v_page &&
                      pages.k_row == pages.v_row;
   const int group = grouped ? ROWS : 1;
@@ -615,7 +687,36 @@ __device__ __forceinline__ void wide_tile(const PagedTile &t,
   const uint32_t v_lane = ((uint32_t)v_at * pages.v_row + v_chunk) * 16;
   const i32x4 k_rows = rows_from(Kp), v_rows = rows_from(Vp);
   IHP_LDS char *lds = (IHP_LDS char *)smem;
-  PagedBlock<kStepKeys> block;
+  PagedBlock<kStepKeys, KIND> block;
+  // kRows: a whole block's rows follow one another, so its place is the
+  // descriptor's base, a pass of the copy a scalar offset and a lane's own the
+  // same for all. The last keys, fewer than a block, take the others' way.
+  const char *Kq = Kp + t.key0 * pages.k_row * 16;
+  const char *Vq = Vp + t.key0 * pages.v_row * 16;
+  auto copy_rows = [&](int slot, int key0) {
+    IHP_LDS char *kd = lds + slot * KBLK + wave * (KROWS * KROW);
+    IHP_LDS char *vd = lds + 2 * KBLK + slot * BLK + wave * (ROWS * ROW);
+    constexpr int KNEXT = kPagedWaves * KROWS * KROW;
+    constexpr int NEXT = kPagedWaves * ROWS * ROW;
+    const i32x4 kr = rows_from(Kq + (int64_t)key0 * (pages.k_row * 16));
+    const i32x4 vr = rows_from(Vq + (int64_t)key0 * (pages.v_row * 16));
+#pragma unroll
+    for (int turn = 0; turn < TURN; ++turn)
+      if (k_in[turn])
+#pragma unroll
+        for (int i = turn; i < KPASSES; i += TURN)
+          buffer_to_lds_16(kr, k_lane[turn],
+                           (uint32_t)(i * kPagedWaves + wave) *
+                               (KROWS * 16 * pages.k_row),
+                           kd + i * KNEXT);
+    if (v_in)
+#pragma unroll
+      for (int i = 0; i < PASSES; ++i)
+        buffer_to_lds_16(vr, v_lane,
+                         (uint32_t)(i * kPagedWaves + wave) *
+                             (ROWS * 16 * pages.v_row),
+                         vd + i * NEXT);
+  };
   auto copy = [&](int slot) {
     IHP_LDS char *kd = lds + slot * KBLK + wave * (KROWS * KROW);
     IHP_LDS char *vd = lds + 2 * KBLK + slot * BLK + wave * (ROWS * ROW);
@@ -708,11 +809,23 @@ __device__ __forceinline__ void wide_tile(const PagedTile &t,
     wait_lgkmcnt0();
     block_barrier();
   }
+  // Block n's rows into a slot.
+  auto fetch = [&](int n, int slot) {
+    if (KIND == PagedKeys::kRows && (n + 1) * kStepKeys <= pages.own_end) {
+      block.there = ~0ull;
+      copy_rows(slot, n * kStepKeys);
+      return;
+    }
+    if (KIND == PagedKeys::kRows)
+      block.find(pages, lead, n);
+    block.place(pages, lead, n);
+    copy(slot);
+  };
   if (c < c_end) {
-    block.find(pages, lead, c, group);
-    block.place(pages, lead, c);
-    copy(0);
-    if (c + 1 < c_end)
+    if (KIND != PagedKeys::kRows)
+      block.find(pages, lead, c, group);
+    fetch(c, 0);
+    if (KIND != PagedKeys::kRows && c + 1 < c_end)
       block.find(pages, lead, c + 1, group);
   }
   for (int slot = 0; c < c_end; ++c, slot ^= 1) {
@@ -732,9 +845,8 @@ __device__ __forceinline__ void wide_tile(const PagedTile &t,
       block_barrier();
     }
     if (c + 1 < c_end) {
-      block.place(pages, lead, c + 1);
-      copy(slot ^ 1);
-      if (c + 2 < c_end)
+      fetch(c + 1, slot ^ 1);
+      if (KIND != PagedKeys::kRows && c + 2 < c_end)
         block.find(pages, lead, c + 2, group);
     }
 
@@ -750,16 +862,22 @@ __device__ __forceinline__ void wide_tile(const PagedTile &t,
       i32x4 kb[NB];
       auto issue = [&](auto r_c) {
         constexpr int R = decltype(r_c)::value;
-        kb[R % NB] = lds_read_16_async<32 * (R % 2) * KROW>(
-            (const IHP_LDS char *)(uintptr_t)(kbase ^ (32u * (R / 2))));
+        const IHP_LDS char *at =
+            (const IHP_LDS char *)(uintptr_t)(kbase ^ (32u * (R / 2)));
+        if constexpr (OWN_WAITS)
+          kb[R % NB] = lds_read_16_async<32 * (R % 2) * KROW>(at);
+        else
+          kb[R % NB] = lds_read_16(at + 32 * (R % 2) * KROW);
       };
       static_for<KW>(issue);
       static_for<NR>([&](auto r_c) {
         constexpr int R = decltype(r_c)::value;
         constexpr int S = R / 2, T = R % 2;
         constexpr int AHEAD = (R + KW < NR ? R + KW : NR) - R - 1;
-        lgkm_wait<AHEAD>();
-        lgkm_tie(kb[R % NB]);
+        if constexpr (OWN_WAITS) {
+          lgkm_wait<AHEAD>();
+          lgkm_tie(kb[R % NB]);
+        }
         st[T] = Mfma32<f16>::mma(kb[R % NB], qf[S], S == 0 ? f32x16{} : st[T]);
         if constexpr (R + KW < NR)
           issue(std::integral_constant<int, R + KW>());
@@ -772,9 +890,14 @@ __device__ __forceinline__ void wide_tile(const PagedTile &t,
     float sc = scale;
     if (live != ~0ull || (own && key0 + kStepKeys > all_own) || scale <= 0.0f) {
       const int sees_to = (own ? limit : pages.prefix) - key0;
-      const uint64_t seen = sees_to >= kStepKeys ? live
-                            : sees_to > 0 ? live & ((1ull << sees_to) - 1)
-                                          : 0;
+      uint64_t seen = sees_to >= kStepKeys ? live
+                      : sees_to > 0 ? live & ((1ull << sees_to) - 1)
+                                    : 0;
+      if (KIND == PagedKeys::kTree && own && key0 + kStepKeys > t.base) {
+        const TreeWords x = tree_words<kStepKeys>(p, t, token, key0);
+        seen &= tree_bits(t, x, key0, 0) |
+                (uint64_t)tree_bits(t, x, key0, 1) << 32;
+      }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const uint32_t mine = (uint32_t)(seen >> (32 * h)) >> (4 * g);
@@ -832,8 +955,18 @@ __device__ __forceinline__ void wide_tile(const PagedTile &t,
         constexpr int KOFF = 16 * ST * ROW;
         static_for<DT>([&](auto dt) {
           constexpr int DTI = decltype(dt)::value;
-          vr[ST % 2][DTI][0] = lds_read_tr16_at<KOFF>(vs + v_off[DTI]);
-          vr[ST % 2][DTI][1] = lds_read_tr16_at<KOFF + 8 * ROW>(vs + v_off[DTI]);
+          if constexpr (OWN_WAITS) {
+            vr[ST % 2][DTI][0] = lds_read_tr16_at<KOFF>(vs + v_off[DTI]);
+            vr[ST % 2][DTI][1] =
+                lds_read_tr16_at<KOFF + 8 * ROW>(vs + v_off[DTI]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+              vr[ST % 2][DTI][i] = __builtin_bit_cast(
+                  i32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                             (IHP_LDS i16x4 *)(vs + v_off[DTI] + KOFF +
+                                               i * 8 * ROW)));
+          }
         });
       };
       read_v(std::integral_constant<int, 0>());
@@ -841,11 +974,14 @@ __device__ __forceinline__ void wide_tile(const PagedTile &t,
         constexpr int ST = decltype(step_c)::value;
         if constexpr (ST < 3)
           read_v(std::integral_constant<int, ST + 1>());
-        lgkm_wait<ST < 3 ? 2 * DT : 0>();
+        if constexpr (OWN_WAITS)
+          lgkm_wait<ST < 3 ? 2 * DT : 0>();
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
-          tie2(vr[ST % 2][dt][0]);
-          tie2(vr[ST % 2][dt][1]);
+          if constexpr (OWN_WAITS) {
+            tie2(vr[ST % 2][dt][0]);
+            tie2(vr[ST % 2][dt][1]);
+          }
           const i32x4 vf = i32x4{vr[ST % 2][dt][0][0], vr[ST % 2][dt][0][1],
                                  vr[ST % 2][dt][1][0], vr[ST % 2][dt][1][1]};
           o[dt] = Mfma32<f16>::mma(vf, pw[ST], o[dt]);
@@ -871,16 +1007,16 @@ __device__ __forceinline__ void wide_tile(const PagedTile &t,
     return;
   if (t.part < 0) {
     const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
-    f16 *dst = result_row(p, t.kv_head, row) + 4 * g;
+    const int64_t dst = result_row(p, t.kv_head, row) + 4 * g;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
       for (int q = 0; q < 4; ++q)
         if (32 * dt + 8 * q < p.dv)  // dv is a multiple of 8
-          *(f16x4 *)(dst + 32 * dt + 8 * q) =
-              f16x4{(f16)(o[dt][4 * q] * inv), (f16)(o[dt][4 * q + 1] * inv),
-                    (f16)(o[dt][4 * q + 2] * inv),
-                    (f16)(o[dt][4 * q + 3] * inv)};
+          store_result<KIND>(
+              p, dst + 32 * dt + 8 * q,
+              f32x4{o[dt][4 * q] * inv, o[dt][4 * q + 1] * inv,
+                    o[dt][4 * q + 2] * inv, o[dt][4 * q + 3] * inv});
   } else {
     const int64_t at = part_row(p, t, row);
     float *dst = p.partials + at * DP + 4 * g;
@@ -936,8 +1072,23 @@ __device__ __forceinline__ int rows_of(const PagedAttention &p, int begin,
   return end > begin ? (end - begin) * p.group : 0;
 }
 
+// kRows: the row of request b's first key, and its keys, within the rows that
+// there are whatever the starts hold; otherwise its length.
+__device__ __forceinline__ int key_start(const PagedAttention &p, int b) {
+  const int r = p.lengths[b];
+  return r < 0 ? 0 : r > p.key_rows ? p.key_rows : r;
+}
+template <PagedKeys KIND>
+__device__ __forceinline__ int length_of(const PagedAttention &p, int b) {
+  if constexpr (KIND == PagedKeys::kRows) {
+    const int n = key_start(p, b + 1) - key_start(p, b);
+    return n > 0 ? n : 0;
+  }
+  return p.lengths[b];
+}
+
 // `shared`: small requests leave the prefix to tiles of their own.
-template <bool WIDE>
+template <bool WIDE, PagedKeys KIND>
 __device__ __forceinline__ Request request(const PagedAttention &p, int begin,
                                            int end, int length, bool shared,
                                            int prefix_keys) {
@@ -952,12 +1103,19 @@ __device__ __forceinline__ Request request(const PagedAttention &p, int begin,
   length = length > 0 ? length : 0;
   q.own_end = length < p.capacity ? length : p.capacity;
   q.base = length - added;
+  if (KIND == PagedKeys::kRows && !p.causal)
+    q.base = length;  // every row sees them all
   const int tokens =
       small ? added : WIDE ? p.wide_tokens : p.narrow_tokens;
   const bool whole = q.base >= 0 && length <= p.capacity && tokens > 0;
   const uint32_t keys = (uint32_t)(small && shared ? 0 : prefix_keys) +
                         (uint32_t)(whole ? q.base + tokens : q.own_end);
   q.a = cost_of(keys >> p.unit, q.shift) + p.tile_units;
+  if (KIND == PagedKeys::kRows && !p.causal) {
+    q.a = cost_of((uint32_t)q.own_end >> p.unit, q.shift) + p.tile_units;
+    q.step = 0;
+    return q;
+  }
   q.step =
       whole && q.tiles > 1 ? cost_of((uint32_t)tokens >> p.unit, q.shift) : 0;
   return q;
@@ -966,7 +1124,7 @@ __device__ __forceinline__ Request request(const PagedAttention &p, int begin,
 }  // namespace
 
 // WIDE: requests of more than 16 rows have wide tiles.
-template <int DP, int DX, int DK, bool WIDE>
+template <int DP, int DX, int DK, bool WIDE, PagedKeys KIND>
 __global__ __launch_bounds__(kPagedThreads,
                              DP >= 256 || (WIDE && DK > 128) ? 1 : 2) void
 attention_paged_kernel(PagedAttention) {
@@ -999,21 +1157,29 @@ attention_paged_kernel(PagedAttention) {
   if (lane * each < p.batch) {
     begin = row_start(p, lane * each);
     end = row_start(p, lane * each + 1);
-    length = p.lengths[lane * each];
+    length = length_of<KIND>(p, lane * each);
   }
   // Consecutive stretches of one head's line read the same prefix: one XCD's.
   int item, unused;
   xcd_tile_order((int)blockIdx.x, p.items, p.items, 1, 1, &item, &unused);
   PagedTile t;
-  t.kv_head = p.ways == 1 ? item
-                          : (int)__umulhi((uint32_t)item, p.ways_magic);
+  t.kv_head = KIND == PagedKeys::kRows
+                  ? item / p.ways
+              : p.ways == 1 ? item
+                            : (int)__umulhi((uint32_t)item, p.ways_magic);
   int way = item - t.kv_head * p.ways;
+  // Whole tiles of heads that do not fall to the XCDs evenly: all heads' tiles
+  // of the most keys first.
+  if (KIND == PagedKeys::kRows && !p.partials && p.kv_heads % 8 != 0) {
+    way = (int)blockIdx.x / p.kv_heads;
+    t.kv_head = (int)blockIdx.x - way * p.kv_heads;
+  }
 
   // The small requests' rows, and whether the prefix gets tiles of them.
   auto rest_of_lane = [&](auto f) {  // the lane's requests after its first
     for (int i = 1; i < each && lane * each + i < p.batch; ++i) {
       const int b = lane * each + i;
-      f(row_start(p, b), row_start(p, b + 1), p.lengths[b]);
+      f(row_start(p, b), row_start(p, b + 1), length_of<KIND>(p, b));
     }
   };
   auto small_of = [&](int from, int to) {
@@ -1045,11 +1211,11 @@ attention_paged_kernel(PagedAttention) {
   const int prefix_keys = prefix_steps * kStepKeys;
   uint32_t mine;
   {
-    const Request q = request<WIDE>(p, begin, end, length, shared, prefix_keys);
+    const Request q = request<WIDE, KIND>(p, begin, end, length, shared, prefix_keys);
     mine = q.before(q.tiles);
   }
   rest_of_lane([&](int from, int to, int n) {
-    const Request q = request<WIDE>(p, from, to, n, shared, prefix_keys);
+    const Request q = request<WIDE, KIND>(p, from, to, n, shared, prefix_keys);
     mine += q.before(q.tiles);
   });
   const uint32_t upto = lane_sums(mine);
@@ -1064,6 +1230,12 @@ attention_paged_kernel(PagedAttention) {
   uint32_t per = p.ways == 1 ? total : __umulhi(total - 1, p.ways_magic) + 1;
   per = per < (uint32_t)p.least ? p.least : per;
   float inv_per = 1.0f / (float)per;
+  // The tiles of a request's last tokens have the most keys: they come first.
+  if (KIND == PagedKeys::kRows && !p.partials) {
+    way = (int)((total + per - 1) / per) - 1 - way;
+    if (way < 0)
+      return;
+  }
   uint32_t x = (uint32_t)way * per;  // below 2^32: `ways` is at most 2^24
   if (x >= total)
     return;
@@ -1078,9 +1250,9 @@ attention_paged_kernel(PagedAttention) {
     } else {
       of[0] = uniform(row_start(p, b));
       of[1] = uniform(row_start(p, b + 1));
-      of[2] = uniform(p.lengths[b]);
+      of[2] = uniform(length_of<KIND>(p, b));
     }
-    return request<WIDE>(p, of[0], of[1], of[2], shared, prefix_keys);
+    return request<WIDE, KIND>(p, of[0], of[1], of[2], shared, prefix_keys);
   };
 
   // Where the stretch begins: among the prefix's tiles, or in the request that
@@ -1169,6 +1341,7 @@ attention_paged_kernel(PagedAttention) {
     t.base = q.base;
     t.own_end = q.own_end;
     t.table = p.table + (int64_t)(lead ? 0 : b) * p.table_stride;
+    t.key0 = KIND == PagedKeys::kRows ? uniform(key_start(p, b)) : 0;
     // Whether the tile has all of its rows' keys.
     const bool all_keys =
         !lead && !(shared && (q.end - q.begin) * p.group <= kSmallRows);
@@ -1185,7 +1358,8 @@ attention_paged_kernel(PagedAttention) {
     t.s_begin = step_at(from);
     t.s_end = step_at(to);
     const bool whole = count == 1 && all_keys;
-    const int64_t line = lead ? 0 : p.packed;
+    // kRows has parts of one kind alone.
+    const int64_t line = lead || KIND == PagedKeys::kRows ? 0 : p.packed;
     t.part = whole ? -1 : line + (int64_t)kWideRows * way;
     if (p.partials && way == first && t.kv_head == 0)
       for (int r = t.r0 + (int)threadIdx.x; r < t.r_end; r += kPagedThreads) {
@@ -1194,15 +1368,15 @@ attention_paged_kernel(PagedAttention) {
         const int at_row = lead ? packed_row(p, all, (uint32_t)r) : r;
         p.part_of[line + at_row] = parts;
         if (all_keys)
-          p.part_of[r] = i32x2{0, 0};
+          p.part_of[p.packed - line + r] = i32x2{0, 0};
       }
     const int shift = q.shift;
     line_at[wave] = {x,  x_end, start, per,        inv_per, t.kv_head,
                      way, b,    i,     small_rows, shared,  q};
     if (shift == 4)
-      narrow_tile<DP, DX, DK>(t, all, smem, wave_m, wave_l);
+      narrow_tile<DP, DX, DK, KIND>(t, all, smem, wave_m, wave_l);
     else if constexpr (WIDE)
-      wide_tile<DP, DX, DK>(t, all, smem);
+      wide_tile<DP, DX, DK, KIND>(t, all, smem);
     asm volatile("" ::: "memory");
     const Line &l = line_at[wave];
     x = (uint32_t)uniform((int)l.x);
@@ -1232,7 +1406,7 @@ attention_paged_kernel(PagedAttention) {
 // for every GROUPS-th four of a row's parts, then the GROUPS sums through LDS.
 // A row's parts of one kind (the prefix's of a small request, its own or both
 // at once) are kWideRows rows apart; part_of tells the first and how many.
-template <int DP, int GROUPS>
+template <int DP, int GROUPS, PagedKeys KIND>
 __global__ __launch_bounds__(kPagedThreads) void attention_paged_join_kernel(
     PagedAttention p) {
   constexpr int TPR = DP / 4, ROWS = kPagedThreads / TPR / GROUPS;
@@ -1326,9 +1500,7 @@ __global__ __launch_bounds__(kPagedThreads) void attention_paged_join_kernel(
   if (!real || parts == 0 || dq >= p.dv)
     return;
   const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
-  *(f16x4 *)(result_row(p, kv_head, row) + dq) =
-      f16x4{(f16)(acc[0] * inv), (f16)(acc[1] * inv), (f16)(acc[2] * inv),
-            (f16)(acc[3] * inv)};
+  store_result<KIND>(p, result_row(p, kv_head, row) + dq, acc * inv);
 }
 
 // ----------------------------------------------------------------------------
@@ -1339,30 +1511,40 @@ namespace {
 
 struct PagedKernel {
   const char *name;
+  PagedKeys keys;
   int dp, dx, dk, groups;  // groups: of a joined row's parts
   bool wide;
   const void *fn;
 };
+// A join of kPages is also kTree's.
 const PagedKernel kPagedKernels[] = {
-#define IHP_PAGED(NAME, DP, DX, DK, WIDE)                                      \
-  {"attention_paged_" NAME, DP, DX, DK, 0, WIDE,                               \
-   (const void *)&attention_paged_kernel<DP, DX, DK, WIDE>}
-    IHP_PAGED("d64", 64, 64, 64, true),
-    IHP_PAGED("d96", 128, 96, 96, true),
-    IHP_PAGED("d128", 128, 128, 128, true),
-    IHP_PAGED("d192_128", 128, 128, 192, false),
-    IHP_PAGED("d192_128_rows", 128, 128, 192, true),
-    IHP_PAGED("d256", 256, 256, 256, false),
+#define IHP_PAGED(NAME, KIND, DP, DX, DK, WIDE)                                \
+  {"attention_" NAME, PagedKeys::KIND, DP, DX, DK, 0, WIDE,                    \
+   (const void *)&attention_paged_kernel<DP, DX, DK, WIDE, PagedKeys::KIND>}
+#define IHP_PAGED_ALL(NAME, KIND)                                              \
+  IHP_PAGED(NAME "_d64", KIND, 64, 64, 64, true),                              \
+      IHP_PAGED(NAME "_d96", KIND, 128, 96, 96, true),                         \
+      IHP_PAGED(NAME "_d128", KIND, 128, 128, 128, true),                      \
+      IHP_PAGED(NAME "_d192_128", KIND, 128, 128, 192, false),                 \
+      IHP_PAGED(NAME "_d192_128_rows", KIND, 128, 128, 192, true),             \
+      IHP_PAGED(NAME "_d256", KIND, 256, 256, 256, false)
+    IHP_PAGED_ALL("paged", kPages),
+    IHP_PAGED_ALL("tree", kTree),
+    IHP_PAGED_ALL("packed", kRows),
+    IHP_PAGED("packed_d256_rows", kRows, 256, 256, 256, true),
+#undef IHP_PAGED_ALL
 #undef IHP_PAGED
-#define IHP_JOIN(DP, GROUPS)                                                   \
-  {"attention_paged_join_d" #DP "_g" #GROUPS, DP, DP, DP, GROUPS, false,      \
-   (const void *)&attention_paged_join_kernel<DP, GROUPS>}
-    IHP_JOIN(64, 1),
-    IHP_JOIN(64, 8),
-    IHP_JOIN(128, 1),
-    IHP_JOIN(128, 8),
-    IHP_JOIN(256, 1),
-    IHP_JOIN(256, 4),
+#define IHP_JOIN(NAME, KIND, DP, GROUPS)                                       \
+  {"attention_" NAME "_join_d" #DP "_g" #GROUPS, PagedKeys::KIND, DP, DP, DP,  \
+   GROUPS, false,                                                              \
+   (const void *)&attention_paged_join_kernel<DP, GROUPS, PagedKeys::KIND>}
+#define IHP_JOIN_ALL(NAME, KIND)                                               \
+  IHP_JOIN(NAME, KIND, 64, 1), IHP_JOIN(NAME, KIND, 64, 8),                    \
+      IHP_JOIN(NAME, KIND, 128, 1), IHP_JOIN(NAME, KIND, 128, 8),              \
+      IHP_JOIN(NAME, KIND, 256, 1), IHP_JOIN(NAME, KIND, 256, 4)
+    IHP_JOIN_ALL("paged", kPages),
+    IHP_JOIN_ALL("packed", kRows),
+#undef IHP_JOIN_ALL
 #undef IHP_JOIN
 };
 constexpr int kPagedKernelCount =
@@ -1370,10 +1552,10 @@ constexpr int kPagedKernelCount =
 
 }  // namespace
 
-PagedPlan plan_attention_paged(int64_t rows, int64_t batch, int64_t kv_heads,
-                               int64_t group, int64_t prefix, int64_t capacity,
-                               int64_t head_dim, int64_t head_dim_v,
-                               size_t workspace_limit) {
+PagedPlan plan_attention_paged(PagedKeys keys, int64_t rows, int64_t batch,
+                               int64_t kv_heads, int64_t group, int64_t prefix,
+                               int64_t capacity, int64_t head_dim,
+                               int64_t head_dim_v, size_t workspace_limit) {
   PagedPlan p = {};
   const int64_t d = head_dim > head_dim_v ? head_dim : head_dim_v;
   const int64_t packed = rows * group;
@@ -1389,7 +1571,9 @@ PagedPlan plan_attention_paged(int64_t rows, int64_t batch, int64_t kv_heads,
   const bool rows_many = packed > batch * kSmallRows;
   const bool prefix_more = p.shared && prefix + capacity > kPagedWholeKeysFew &&
                            packed / kNarrowRows * prefix > batch * capacity;
-  p.wide = d <= 128 || (longer_k && (rows_many || prefix_more));
+  const bool packed_keys = keys == PagedKeys::kRows;
+  p.wide = d <= 128 || (longer_k && (rows_many || prefix_more)) ||
+           (packed_keys && rows_many);
   p.dp = d <= 64 ? 64 : d <= 128 || longer_k ? 128 : 256;
   p.dx = d > 64 && d <= 96 ? 96 : p.dp;
   p.dk = longer_k ? 192 : p.dx;
@@ -1407,26 +1591,29 @@ PagedPlan plan_attention_paged(int64_t rows, int64_t batch, int64_t kv_heads,
   p.least = units(kPagedLeastKeys);
   p.tile_units = units(kPagedTileKeys);
   p.snap = units(kPagedSnapKeys);
-  p.part_rows = 2 * packed + kWideRows * p.ways;
+  p.part_rows = (packed_keys ? 1 : 2) * packed + kWideRows * p.ways;
   p.workspace = (int64_t)kWorkspaceCounterBytes + 2 * packed * 8 +
                 kv_heads * p.part_rows * (p.dp + 2) * 4;
   const int64_t tiles = batch + packed / (p.wide ? kWideRows : kNarrowRows);
   const int64_t most = tiles * kv_heads > wgs ? kPagedWholeKeys
                        : p.wide && rows_many  ? kPagedWholeKeysWide
                                               : kPagedWholeKeysFew;
-  if (prefix + capacity <= most ||
+  // Packed rows: tiles that keep every CU busy without being split.
+  const bool many = packed_keys && tiles * kv_heads >= 2 * wgs;
+  if (prefix + capacity <= most || many ||
       (uint64_t)p.workspace > workspace_limit || p.part_rows > INT32_MAX) {
     // every tile whole and one unit, so each workgroup takes as many
     p.shared = false;
     p.workspace = p.part_rows = 0;
     p.unit = 31;
     p.least = p.tile_units = p.snap = 1;
-    p.ways = 4 * p.ways < tiles ? 4 * p.ways : tiles;
+    p.ways = 4 * p.ways < tiles && !packed_keys ? 4 * p.ways : tiles;
   }
   return p;
 }
 
-hipError_t launch_attention_paged(const PagedAttention &attention,
+hipError_t launch_attention_paged(PagedKeys keys,
+                                  const PagedAttention &attention,
                                   const PagedPlan &plan, void *workspace,
                                   void *stream) {
   PagedAttention a = attention;
@@ -1438,9 +1625,10 @@ hipError_t launch_attention_paged(const PagedAttention &attention,
   a.snap = (int)plan.snap;
   a.shared = plan.shared ? 1 : 0;
   // item / ways, exact while item * ways is below 2^32: at most 4 ways to each
-  // of 65535 heads, or 2048 workgroups in all; and the ways' share of a line of
-  // less than 2^31 units, at most one unit over. (One way's is not used.)
-  if ((uint64_t)a.items * (uint64_t)a.ways >> 32)
+  // of 65535 heads, or 2048 workgroups in all (kRows divides: its whole tiles
+  // may be more); and the ways' share of a line of less than 2^31 units, at
+  // most one unit over. (One way's is not used.)
+  if (keys != PagedKeys::kRows && (uint64_t)a.items * (uint64_t)a.ways >> 32)
     return hipErrorInvalidValue;
   a.ways_magic = (uint32_t)(((uint64_t)1 << 32) / (uint64_t)plan.ways + 1);
   a.part_rows = plan.part_rows;
@@ -1457,10 +1645,11 @@ hipError_t launch_attention_paged(const PagedAttention &attention,
   const PagedKernel *kernel = nullptr, *join = nullptr;
   for (const PagedKernel &k : kPagedKernels)
     if (k.dp == plan.dp) {
-      if (k.groups == 0 && k.dx == plan.dx && k.dk == plan.dk &&
-          k.wide == plan.wide)
+      if (k.groups == 0 && k.keys == keys && k.dx == plan.dx &&
+          k.dk == plan.dk && k.wide == plan.wide)
         kernel = &k;
-      else if (k.groups > 0 && (k.groups > 1) == few)
+      else if (k.groups > 0 && (k.groups > 1) == few &&
+               (k.keys == PagedKeys::kRows) == (keys == PagedKeys::kRows))
         join = &k;
     }
   if (!kernel || !join)

@@ -372,9 +372,41 @@ struct AppendKv {
 hipError_t launch_append_kv(const AppendKv &append, void *stream);
 const KernelEntry *paged_cache_kernels(int *count);
 
-// Attention over the paged cache (attention_paged.hip). Strides in elements;
-// a cache row's place within its head is counted in 16 bytes, in 32 bits
-// (checked on the host).
+// Which of its request's new rows each one of a tree sees: see
+// iree_mi355x_tree_masks_t.
+struct TreeMasks {
+  const int32_t *parents, *row_starts;
+  int32_t *masks, *depths;
+  int batch, rows, words;
+};
+hipError_t launch_tree_masks(const TreeMasks &masks, void *stream);
+
+// Rotated rows of q, then of k (rotary.hip): element strides (row, head).
+// A thread takes `pairs` pairs at a time: 8 of halves or 4 of neighbours, where
+// 16-byte loads can (checked on the host), or 1; then the dims past the rotated
+// ones, 8 or 1 at a time. A head's pieces are `pieces`, the first `rotated` of
+// them rotated ones.
+struct Rotary {
+  const _Float16 *in[2];
+  _Float16 *out[2];
+  const int32_t *positions;
+  const float *frequencies;
+  int64_t in_strides[2][2], out_strides[2][2], position_stride;
+  int rows, heads[2], half, dim, ends[3], axes;
+  int tokens, pieces, rotated, interleaved, wide;
+};
+hipError_t launch_rotary(const Rotary &rotary, void *stream);
+const KernelEntry *rotary_kernels(int *count);
+
+// Attention of packed rows (attention_paged.hip): where a request's keys are
+// and which of its new ones a row sees.
+enum class PagedKeys {
+  kPages,  // in pages; every row sees those up to itself
+  kTree,   // in pages; of the new ones a row sees those that its mask names
+  kRows,   // in packed rows of their own
+};
+// Strides in elements; a key's place within its head is counted in 16 bytes,
+// in 32 bits (checked on the host).
 // In the order of use, 64 bytes at a time.
 struct PagedAttention {
   // What a workgroup finds its place by.
@@ -424,6 +456,13 @@ struct PagedAttention {
 
   int64_t k_head, v_head;
   float scale;
+
+  // kTree: W = `words` words a row, row pitch mask_stride.
+  int words;
+  const int32_t *masks;
+  int64_t mask_stride;
+  // kRows: `lengths` are the keys' starts, among key_rows rows.
+  int key_rows, causal, out_f32;
 };
 // Workgroups wanted: two a CU where head dims allow it (768 and 1024 instead
 // of 512: 64 requests' tokens behind a prefix 48.5 -> 59 us and more, prompts
@@ -468,11 +507,12 @@ struct PagedPlan {
   bool wide, shared;  // wide tiles there are, and the prefix's own
   int64_t ways, least, unit, tile_units, snap, part_rows, workspace;
 };
-PagedPlan plan_attention_paged(int64_t rows, int64_t batch, int64_t kv_heads,
-                               int64_t group, int64_t prefix, int64_t capacity,
-                               int64_t head_dim, int64_t head_dim_v,
-                               size_t workspace_limit);
-hipError_t launch_attention_paged(const PagedAttention &attention,
+PagedPlan plan_attention_paged(PagedKeys keys, int64_t rows, int64_t batch,
+                               int64_t kv_heads, int64_t group, int64_t prefix,
+                               int64_t capacity, int64_t head_dim,
+                               int64_t head_dim_v, size_t workspace_limit);
+hipError_t launch_attention_paged(PagedKeys keys,
+                                  const PagedAttention &attention,
                                   const PagedPlan &plan, void *workspace,
                                   void *stream);
 const KernelEntry *attention_paged_kernels(int *count);

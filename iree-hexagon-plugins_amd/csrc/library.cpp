@@ -373,7 +373,7 @@ const ihp::KernelEntry *kernel_at(int index) {
       ihp::gemm_kernels, ihp::gemv_kernels, ihp::attention_kernels,
       ihp::attention_general_kernels, ihp::attention_rows_kernels,
       ihp::paged_cache_kernels, ihp::attention_paged_kernels,
-      ihp::runtime_kernels};
+      ihp::rotary_kernels,      ihp::runtime_kernels};
   for (auto list : lists) {
     int n = 0;
     const ihp::KernelEntry *e = list(&n);
@@ -401,6 +401,8 @@ extern "C" int iree_mi355x_kernel_count(void) {
   ihp::paged_cache_kernels(&n);
   total += n;
   ihp::attention_paged_kernels(&n);
+  total += n;
+  ihp::rotary_kernels(&n);
   total += n;
   ihp::runtime_kernels(&n);
   return total + n;

@@ -102,15 +102,177 @@ static int64_t own_capacity(const iree_mi355x_paged_attention_t &a) {
 static PagedPlan plan_of(const iree_mi355x_paged_attention_t &a,
                          size_t workspace_limit) {
   const iree_mi355x_kv_cache_t &c = a.cache;
-  return plan_attention_paged(a.rows, a.batch, c.kv_heads,
+  return plan_attention_paged(PagedKeys::kPages, a.rows, a.batch, c.kv_heads,
                               a.heads / c.kv_heads, a.prefix_length,
                               own_capacity(a), c.head_dim, c.head_dim_v,
                               workspace_limit);
 }
 
+// The fields that go by the rows and heads alone.
+static void set_rows(PagedAttention *p, int64_t rows, int64_t batch,
+                     int64_t heads, int64_t kv_heads, int64_t head_dim,
+                     int64_t head_dim_v) {
+  p->batch = (int)batch;
+  p->rows = (int)rows;
+  p->kv_heads = (int)kv_heads;
+  p->group = (int)(heads / kv_heads);
+  p->packed = rows * p->group;
+  divider(p->group, &p->group_magic, &p->group_shift);
+  p->narrow_tokens = 16 / p->group;
+  p->wide_tokens = 128 / p->group;
+  p->dqk = (int)head_dim;
+  p->dv = (int)head_dim_v;
+}
+
+// A launch has fewer than 2^32 threads.
+static bool launchable(const PagedPlan &plan, const PagedAttention &p) {
+  const int64_t most = (int64_t)1 << 24;
+  return plan.ways * p.kv_heads < most &&
+         !(plan.workspace &&
+           p.packed * p.kv_heads / (1024 / plan.dp) >= most - 1);
+}
+
+static bool plannable(const iree_mi355x_packed_attention_t &a) {
+  return a.rows > 0 && a.batch > 0 && a.heads > 0 && a.kv_heads > 0 &&
+         a.heads % a.kv_heads == 0 && a.heads <= 65535 && a.head_dim >= 8 &&
+         a.head_dim <= 256 && a.head_dim_v >= 8 && a.head_dim_v <= 256 &&
+         a.key_rows >= 0 && a.key_rows < kMaxExtent / 2 &&
+         a.batch < kMaxExtent / 2 &&
+         a.rows < kMaxExtent / 2 / (a.heads / a.kv_heads);
+}
+
+static PagedPlan plan_of(const iree_mi355x_packed_attention_t &a,
+                         size_t workspace_limit) {
+  return plan_attention_paged(PagedKeys::kRows, a.rows, a.batch, a.kv_heads,
+                              a.heads / a.kv_heads, 0, a.key_rows, a.head_dim,
+                              a.head_dim_v, workspace_limit);
+}
+
 }  // namespace ihp
 
 using namespace ihp;
+
+static int paged_attention(const char *who, PagedKeys keys,
+                           const iree_mi355x_paged_attention_t *a,
+                           const int32_t *masks, int64_t words,
+                           int64_t mask_stride, void *workspace,
+                           size_t workspace_bytes, void *stream) {
+  if (!a)
+    return fail(IREE_MI355X_INVALID_ARGUMENT, "%s: null arguments", who);
+  if (a->flags)
+    return fail(IREE_MI355X_INVALID_ARGUMENT, "%s: unknown flag bits 0x%x",
+                who, a->flags);
+  const iree_mi355x_kv_cache_t &c = a->cache;
+  int st = check_cache(who, c);
+  if (st)
+    return st;
+  if (a->rows < 0 || a->heads < 0 || a->batch < 0 || a->table_width < 0 ||
+      a->table_stride < 0 || a->prefix_length < 0)
+    return fail(IREE_MI355X_INVALID_ARGUMENT, "%s: negative extent", who);
+  if (!std::isfinite(a->scale))
+    return fail(IREE_MI355X_INVALID_ARGUMENT, "%s: scale not finite", who);
+  for (int i = 0; i < 2; ++i)
+    if (a->q_strides[i] < 0 || a->o_strides[i] < 0)
+      return fail(IREE_MI355X_INVALID_ARGUMENT, "%s: negative stride", who);
+  if (a->rows == 0 || a->heads == 0 || a->batch == 0)
+    return ok();
+  if (c.kv_heads == 0 || a->heads % c.kv_heads != 0)
+    return fail(IREE_MI355X_INVALID_ARGUMENT,
+                "%s: %lld query heads are not a multiple of %lld KV heads",
+                who, (long long)a->heads, (long long)c.kv_heads);
+  if (!plannable(*a) ||
+      (a->table_stride > 0 && a->batch > INT64_MAX / 8 / a->table_stride))
+    return fail(IREE_MI355X_UNSUPPORTED, "%s: problem too large", who);
+  if (a->batch > 1 && a->table_stride < a->table_width)
+    return fail(IREE_MI355X_INVALID_ARGUMENT,
+                "%s: table pitch %lld overlaps its rows", who,
+                (long long)a->table_stride);
+  if (!a->q || !a->o || !a->row_starts || !a->lengths ||
+      (a->table_width > 0 && !a->block_table) ||
+      (a->prefix_length > 0 && !a->prefix_pages))
+    return fail(IREE_MI355X_INVALID_ARGUMENT, "%s: null pointer", who);
+  if ((a->heads > 1 && a->o_strides[1] < c.head_dim_v) ||
+      (a->rows > 1 && a->o_strides[0] < c.head_dim_v))
+    return fail(IREE_MI355X_INVALID_ARGUMENT,
+                "%s: o strides %lld, %lld overlap its rows", who,
+                (long long)a->o_strides[0], (long long)a->o_strides[1]);
+  for (int i = 0; i < 2; ++i)
+    if (a->q_strides[i] % 8 != 0 || a->o_strides[i] % 4 != 0)
+      return fail(IREE_MI355X_MISALIGNED,
+                  "%s: strides must be multiples of 8 elements (q), 4 (o)",
+                  who);
+  if (!aligned_to(a->q, 16) || !aligned_to(a->o, 8) ||
+      !aligned_to(workspace, 16))
+    return fail(IREE_MI355X_MISALIGNED,
+                "%s: q and the workspace must be 16-byte aligned, o 8", who);
+  if (!aligned_to(a->row_starts, 4) || !aligned_to(a->lengths, 4) ||
+      !aligned_to(a->block_table, 4) || !aligned_to(a->prefix_pages, 4))
+    return fail(IREE_MI355X_MISALIGNED,
+                "%s: tables must be aligned to their element size", who);
+
+  const bool tree = keys == PagedKeys::kTree;
+  if (tree && (!masks || words < 1))
+    return fail(IREE_MI355X_INVALID_ARGUMENT, "%s: no masks", who);
+  if (tree && (words >= kMaxExtent / 64 || mask_stride >= kMaxExtent))
+    return fail(IREE_MI355X_UNSUPPORTED, "%s: problem too large", who);
+  if (tree && (mask_stride < 0 || (a->rows > 1 && mask_stride < words)))
+    return fail(IREE_MI355X_INVALID_ARGUMENT,
+                "%s: mask pitch %lld overlaps its rows", who,
+                (long long)mask_stride);
+  if (tree && !aligned_to(masks, 4))
+    return fail(IREE_MI355X_MISALIGNED,
+                "%s: tables must be aligned to their element size", who);
+
+  PagedAttention p = {};
+  p.q = (const _Float16 *)a->q;
+  p.o = (_Float16 *)a->o;
+  p.k_cache = (const _Float16 *)c.k;
+  p.v_cache = (const _Float16 *)c.v;
+  p.row_starts = a->row_starts;
+  p.lengths = a->lengths;
+  p.table = a->block_table;
+  p.prefix_pages = a->prefix_pages;
+  p.q_row = a->q_strides[0];
+  p.q_head = a->q_strides[1];
+  p.o_row = a->o_strides[0];
+  p.o_head = a->o_strides[1];
+  p.k_head = c.k_strides[1];
+  p.v_head = c.v_strides[1];
+  p.table_stride = a->table_stride;
+  p.k_page16 = (uint32_t)(c.k_strides[0] / 8);
+  p.k_row16 = (uint32_t)(c.k_strides[2] / 8);
+  p.v_page16 = (uint32_t)(c.v_strides[0] / 8);
+  p.v_row16 = (uint32_t)(c.v_strides[2] / 8);
+  divider(c.page_size, &p.page_magic, &p.page_shift);
+  p.page_size = (int)c.page_size;
+  p.pages = (int)c.pages;
+  const int64_t small = (int64_t)1 << 24;
+  auto reach = [&](const int64_t *st, int64_t dim) {  // bytes, head 0's rows
+    return ((c.pages > 0 ? c.pages - 1 : 0) * st[0] +
+            (c.page_size - 1) * st[2] + dim) * 2;
+  };
+  p.near = c.pages <= small && c.page_size <= small &&
+           p.k_page16 < small && p.k_row16 < small && p.v_page16 < small &&
+           p.v_row16 < small && reach(c.k_strides, 256) < UINT32_MAX &&
+           reach(c.v_strides, 256) < UINT32_MAX;
+  set_rows(&p, a->rows, a->batch, a->heads, c.kv_heads, c.head_dim,
+           c.head_dim_v);
+  p.masks = masks;
+  p.words = (int)words;
+  p.mask_stride = mask_stride;
+  // A cache without pages has no keys.
+  p.prefix = c.pages > 0 ? (int)a->prefix_length : 0;
+  p.capacity = c.pages > 0 ? (int)own_capacity(*a) : 0;
+  p.scale = a->scale;
+  iree_mi355x_paged_attention_t b = *a;
+  if (c.pages == 0)
+    b.prefix_length = b.table_width = 0;
+  const PagedPlan plan = plan_of(b, workspace ? workspace_bytes : 0);
+  if (!launchable(plan, p))
+    return fail(IREE_MI355X_UNSUPPORTED, "%s: problem too large", who);
+  return launch_status(
+      launch_attention_paged(keys, p, plan, workspace, stream), who);
+}
 
 extern "C" {
 
@@ -217,117 +379,237 @@ int iree_mi355x_append_kv_f16(const iree_mi355x_kv_cache_t *cache,
 int iree_mi355x_shared_prefix_attention_f16(
     const iree_mi355x_paged_attention_t *a, void *workspace,
     size_t workspace_bytes, void *stream) {
-  const char *who = "shared_prefix_attention";
+  return paged_attention("shared_prefix_attention", PagedKeys::kPages, a,
+                         nullptr, 0, 0, workspace, workspace_bytes, stream);
+}
+
+int iree_mi355x_tree_attention_f16(const iree_mi355x_paged_attention_t *a,
+                                   const int32_t *masks, int64_t words,
+                                   int64_t mask_stride, void *workspace,
+                                   size_t workspace_bytes, void *stream) {
+  return paged_attention("tree_attention", PagedKeys::kTree, a, masks, words,
+                         mask_stride, workspace, workspace_bytes, stream);
+}
+
+int iree_mi355x_tree_masks(const iree_mi355x_tree_masks_t *a, void *stream) {
+  const char *who = "tree_masks";
   if (!a)
     return fail(IREE_MI355X_INVALID_ARGUMENT, "%s: null arguments", who);
-  if (a->flags)
+  if (a->batch < 0 || a->rows < 0 || a->words < 0)
+    return fail(IREE_MI355X_INVALID_ARGUMENT, "%s: negative extent", who);
+  if (a->words < 1)
+    return fail(IREE_MI355X_INVALID_ARGUMENT, "%s: masks of no words", who);
+  if (a->rows >= kMaxExtent / 2 || a->words >= kMaxExtent / 64 ||
+      a->batch >= (int64_t)1 << 24)
+    return fail(IREE_MI355X_UNSUPPORTED, "%s: problem too large", who);
+  if (a->rows == 0)
+    return ok();
+  if (!a->parents || !a->row_starts || !a->masks || !a->depths)
+    return fail(IREE_MI355X_INVALID_ARGUMENT, "%s: null pointer", who);
+  if (!aligned_to(a->parents, 4) || !aligned_to(a->row_starts, 4) ||
+      !aligned_to(a->masks, 4) || !aligned_to(a->depths, 4))
+    return fail(IREE_MI355X_MISALIGNED,
+                "%s: operands must be aligned to their element size", who);
+  TreeMasks t = {};
+  t.parents = a->parents;
+  t.row_starts = a->row_starts;
+  t.masks = a->masks;
+  t.depths = a->depths;
+  t.batch = (int)a->batch;
+  t.rows = (int)a->rows;
+  t.words = (int)a->words;
+  return launch_status(launch_tree_masks(t, stream), who);
+}
+
+int iree_mi355x_rotary_f16(const iree_mi355x_rotary_t *a, void *stream) {
+  const char *who = "rotary";
+  if (!a)
+    return fail(IREE_MI355X_INVALID_ARGUMENT, "%s: null arguments", who);
+  if (a->rows < 0 || a->heads < 0 || a->kv_heads < 0 || a->head_dim < 0 ||
+      a->position_stride < 0)
+    return fail(IREE_MI355X_INVALID_ARGUMENT, "%s: negative extent", who);
+  if (a->flags & ~IREE_MI355X_ROTARY_INTERLEAVED)
     return fail(IREE_MI355X_INVALID_ARGUMENT, "%s: unknown flag bits 0x%x",
                 who, a->flags);
-  const iree_mi355x_kv_cache_t &c = a->cache;
-  int st = check_cache(who, c);
-  if (st)
-    return st;
-  if (a->rows < 0 || a->heads < 0 || a->batch < 0 || a->table_width < 0 ||
-      a->table_stride < 0 || a->prefix_length < 0)
+  if (a->axes < 1 || a->axes > 4)
+    return fail(IREE_MI355X_UNSUPPORTED, "%s: %lld axes (1 to 4 supported)",
+                who, (long long)a->axes);
+  int64_t half = 0;
+  for (int i = 0; i < a->axes; ++i) {
+    if (a->sections[i] < 0)
+      return fail(IREE_MI355X_INVALID_ARGUMENT, "%s: negative section", who);
+    if (a->sections[i] > 128 - half)
+      return fail(IREE_MI355X_UNSUPPORTED,
+                  "%s: more than 128 pairs of dims", who);
+    half += a->sections[i];
+  }
+  if (a->head_dim > 256)
+    return fail(IREE_MI355X_UNSUPPORTED, "%s: head dim %lld (up to 256)", who,
+                (long long)a->head_dim);
+  if (2 * half > a->head_dim)
+    return fail(IREE_MI355X_INVALID_ARGUMENT,
+                "%s: %lld pairs of a head dim of %lld", who, (long long)half,
+                (long long)a->head_dim);
+  if (a->rows >= kMaxExtent || a->heads > 65535 || a->kv_heads > 65535)
+    return fail(IREE_MI355X_UNSUPPORTED, "%s: problem too large", who);
+  if (a->rows == 0 || a->heads + a->kv_heads == 0 || a->head_dim == 0)
+    return ok();
+  const int64_t heads[2] = {a->heads, a->kv_heads};
+  const void *in[2] = {a->q, a->k};
+  void *out[2] = {a->q_out, a->k_out};
+  const int64_t *in_strides[2] = {a->q_strides, a->k_strides};
+  const int64_t *out_strides[2] = {a->q_out_strides, a->k_out_strides};
+  const bool interleaved = a->flags & IREE_MI355X_ROTARY_INTERLEAVED;
+  bool wide = a->head_dim % 8 == 0 && half % (interleaved ? 4 : 8) == 0;
+  Rotary r = {};
+  for (int i = 0; i < 2; ++i) {
+    if (heads[i] == 0)
+      continue;
+    if (!in[i] || !out[i])
+      return fail(IREE_MI355X_INVALID_ARGUMENT, "%s: null pointer", who);
+    for (int j = 0; j < 2; ++j) {
+      if (in_strides[i][j] < 0 || out_strides[i][j] < 0)
+        return fail(IREE_MI355X_INVALID_ARGUMENT, "%s: negative stride", who);
+      if ((j == 0 ? a->rows : heads[i]) > 1 && out_strides[i][j] < a->head_dim)
+        return fail(IREE_MI355X_INVALID_ARGUMENT,
+                    "%s: output stride %lld overlaps its rows", who,
+                    (long long)out_strides[i][j]);
+      wide = wide && in_strides[i][j] % 8 == 0 && out_strides[i][j] % 8 == 0;
+      r.in_strides[i][j] = in_strides[i][j];
+      r.out_strides[i][j] = out_strides[i][j];
+    }
+    if (!aligned_to(in[i], 2) || !aligned_to(out[i], 2))
+      return fail(IREE_MI355X_MISALIGNED,
+                  "%s: operands must be aligned to their element size", who);
+    wide = wide && aligned_to(in[i], 16) && aligned_to(out[i], 16);
+    r.in[i] = (const _Float16 *)in[i];
+    r.out[i] = (_Float16 *)out[i];
+    r.heads[i] = (int)heads[i];
+  }
+  if (half > 0 && (!a->positions || !a->frequencies))
+    return fail(IREE_MI355X_INVALID_ARGUMENT, "%s: null pointer", who);
+  if (!aligned_to(a->positions, 4) || !aligned_to(a->frequencies, 4))
+    return fail(IREE_MI355X_MISALIGNED,
+                "%s: operands must be aligned to their element size", who);
+  r.positions = a->positions;
+  r.frequencies = a->frequencies;
+  r.position_stride = a->position_stride;
+  r.rows = (int)a->rows;
+  r.half = (int)half;
+  r.dim = (int)a->head_dim;
+  int64_t end = 0;
+  for (int i = 0; i < 3; ++i) {  // axes that there are not begin past the pairs
+    end = i + 1 < a->axes ? end + a->sections[i] : half;
+    r.ends[i] = (int)end;
+  }
+  r.axes = (int)a->axes;
+  const int vec = wide ? 8 : 1;
+  r.rotated = (int)(interleaved && wide ? half / 4 : half / vec);
+  r.pieces = r.rotated + (int)((a->head_dim - 2 * half) / vec);
+  r.interleaved = interleaved;
+  r.wide = wide;
+  return launch_status(launch_rotary(r, stream), who);
+}
+
+int iree_mi355x_packed_attention_f16(const iree_mi355x_packed_attention_t *a,
+                                     void *workspace, size_t workspace_bytes,
+                                     void *stream) {
+  const char *who = "packed_attention";
+  if (!a)
+    return fail(IREE_MI355X_INVALID_ARGUMENT, "%s: null arguments", who);
+  if (a->flags & ~(IREE_MI355X_ATTENTION_CAUSAL | IREE_MI355X_ATTENTION_OUT_F32))
+    return fail(IREE_MI355X_INVALID_ARGUMENT, "%s: unknown flag bits 0x%x",
+                who, a->flags);
+  if (a->rows < 0 || a->key_rows < 0 || a->batch < 0 || a->heads < 0 ||
+      a->kv_heads < 0 || a->head_dim < 0 || a->head_dim_v < 0)
     return fail(IREE_MI355X_INVALID_ARGUMENT, "%s: negative extent", who);
   if (!std::isfinite(a->scale))
     return fail(IREE_MI355X_INVALID_ARGUMENT, "%s: scale not finite", who);
-  for (int i = 0; i < 2; ++i)
-    if (a->q_strides[i] < 0 || a->o_strides[i] < 0)
+  const int64_t *strides[4] = {a->q_strides, a->k_strides, a->v_strides,
+                               a->o_strides};
+  for (const int64_t *st : strides)
+    if (st[0] < 0 || st[1] < 0)
       return fail(IREE_MI355X_INVALID_ARGUMENT, "%s: negative stride", who);
+  if (a->head_dim < 8 || a->head_dim > 256 || a->head_dim % 8 != 0 ||
+      a->head_dim_v < 8 || a->head_dim_v > 256 || a->head_dim_v % 8 != 0)
+    return fail(IREE_MI355X_UNSUPPORTED,
+                "%s: head dims %lld / %lld (multiples of 8 up to 256 "
+                "supported)",
+                who, (long long)a->head_dim, (long long)a->head_dim_v);
   if (a->rows == 0 || a->heads == 0 || a->batch == 0)
     return ok();
-  if (c.kv_heads == 0 || a->heads % c.kv_heads != 0)
+  if (a->kv_heads == 0 || a->heads % a->kv_heads != 0)
     return fail(IREE_MI355X_INVALID_ARGUMENT,
                 "%s: %lld query heads are not a multiple of %lld KV heads",
-                who, (long long)a->heads, (long long)c.kv_heads);
-  if (!plannable(*a) ||
-      (a->table_stride > 0 && a->batch > INT64_MAX / 8 / a->table_stride))
+                who, (long long)a->heads, (long long)a->kv_heads);
+  // A head's keys are counted in 16 bytes, 64 of them in bytes, in 32 bits.
+  const int64_t most_row = (int64_t)1 << 24;
+  if (!plannable(*a) || a->k_strides[0] > most_row ||
+      a->v_strides[0] > most_row ||
+      a->key_rows * (a->k_strides[0] / 8) > UINT32_MAX ||
+      a->key_rows * (a->v_strides[0] / 8) > UINT32_MAX)
     return fail(IREE_MI355X_UNSUPPORTED, "%s: problem too large", who);
-  if (a->batch > 1 && a->table_stride < a->table_width)
-    return fail(IREE_MI355X_INVALID_ARGUMENT,
-                "%s: table pitch %lld overlaps its rows", who,
-                (long long)a->table_stride);
-  if (!a->q || !a->o || !a->row_starts || !a->lengths ||
-      (a->table_width > 0 && !a->block_table) ||
-      (a->prefix_length > 0 && !a->prefix_pages))
+  if (!a->q || !a->o || !a->row_starts || !a->key_starts ||
+      (a->key_rows > 0 && (!a->k || !a->v)))
     return fail(IREE_MI355X_INVALID_ARGUMENT, "%s: null pointer", who);
-  if ((a->heads > 1 && a->o_strides[1] < c.head_dim_v) ||
-      (a->rows > 1 && a->o_strides[0] < c.head_dim_v))
+  if ((a->heads > 1 && a->o_strides[1] < a->head_dim_v) ||
+      (a->rows > 1 && a->o_strides[0] < a->head_dim_v))
     return fail(IREE_MI355X_INVALID_ARGUMENT,
                 "%s: o strides %lld, %lld overlap its rows", who,
                 (long long)a->o_strides[0], (long long)a->o_strides[1]);
   for (int i = 0; i < 2; ++i)
-    if (a->q_strides[i] % 8 != 0 || a->o_strides[i] % 4 != 0)
+    if (a->q_strides[i] % 8 != 0 || a->k_strides[i] % 8 != 0 ||
+        a->v_strides[i] % 8 != 0 || a->o_strides[i] % 4 != 0)
       return fail(IREE_MI355X_MISALIGNED,
-                  "%s: strides must be multiples of 8 elements (q), 4 (o)",
+                  "%s: strides must be multiples of 8 elements (q, k, v), 4 "
+                  "(o)",
                   who);
-  if (!aligned_to(a->q, 16) || !aligned_to(a->o, 8) ||
-      !aligned_to(workspace, 16))
+  const bool f32 = a->flags & IREE_MI355X_ATTENTION_OUT_F32;
+  if (!aligned_to(a->q, 16) || !aligned_to(a->k, 16) || !aligned_to(a->v, 16) ||
+      !aligned_to(a->o, f32 ? 16 : 8) || !aligned_to(workspace, 16))
     return fail(IREE_MI355X_MISALIGNED,
-                "%s: q and the workspace must be 16-byte aligned, o 8", who);
-  if (!aligned_to(a->row_starts, 4) || !aligned_to(a->lengths, 4) ||
-      !aligned_to(a->block_table, 4) || !aligned_to(a->prefix_pages, 4))
+                "%s: q, k, v and the workspace must be 16-byte aligned, o 8 "
+                "(f32: 16)",
+                who);
+  if (!aligned_to(a->row_starts, 4) || !aligned_to(a->key_starts, 4))
     return fail(IREE_MI355X_MISALIGNED,
                 "%s: tables must be aligned to their element size", who);
 
   PagedAttention p = {};
   p.q = (const _Float16 *)a->q;
   p.o = (_Float16 *)a->o;
-  p.k_cache = (const _Float16 *)c.k;
-  p.v_cache = (const _Float16 *)c.v;
+  p.k_cache = (const _Float16 *)a->k;
+  p.v_cache = (const _Float16 *)a->v;
   p.row_starts = a->row_starts;
-  p.lengths = a->lengths;
-  p.table = a->block_table;
-  p.prefix_pages = a->prefix_pages;
+  p.lengths = a->key_starts;
   p.q_row = a->q_strides[0];
   p.q_head = a->q_strides[1];
   p.o_row = a->o_strides[0];
   p.o_head = a->o_strides[1];
-  p.k_head = c.k_strides[1];
-  p.v_head = c.v_strides[1];
-  p.table_stride = a->table_stride;
-  p.k_page16 = (uint32_t)(c.k_strides[0] / 8);
-  p.k_row16 = (uint32_t)(c.k_strides[2] / 8);
-  p.v_page16 = (uint32_t)(c.v_strides[0] / 8);
-  p.v_row16 = (uint32_t)(c.v_strides[2] / 8);
-  divider(c.page_size, &p.page_magic, &p.page_shift);
-  p.page_size = (int)c.page_size;
-  p.pages = (int)c.pages;
-  const int64_t small = (int64_t)1 << 24;
-  auto reach = [&](const int64_t *st, int64_t dim) {  // bytes, head 0's rows
-    return ((c.pages > 0 ? c.pages - 1 : 0) * st[0] +
-            (c.page_size - 1) * st[2] + dim) * 2;
-  };
-  p.near = c.pages <= small && c.page_size <= small &&
-           p.k_page16 < small && p.k_row16 < small && p.v_page16 < small &&
-           p.v_row16 < small && reach(c.k_strides, 256) < UINT32_MAX &&
-           reach(c.v_strides, 256) < UINT32_MAX;
-  p.batch = (int)a->batch;
-  p.rows = (int)a->rows;
-  p.kv_heads = (int)c.kv_heads;
-  p.group = (int)(a->heads / c.kv_heads);
-  p.packed = a->rows * p.group;
-  divider(p.group, &p.group_magic, &p.group_shift);
-  p.narrow_tokens = 16 / p.group;
-  p.wide_tokens = 128 / p.group;
-  p.dqk = (int)c.head_dim;
-  p.dv = (int)c.head_dim_v;
-  // A cache without pages has no keys.
-  p.prefix = c.pages > 0 ? (int)a->prefix_length : 0;
-  p.capacity = c.pages > 0 ? (int)own_capacity(*a) : 0;
+  p.k_head = a->k_strides[1];
+  p.v_head = a->v_strides[1];
+  p.k_row16 = (uint32_t)(a->k_strides[0] / 8);
+  p.v_row16 = (uint32_t)(a->v_strides[0] / 8);
+  p.page_size = 1;
+  set_rows(&p, a->rows, a->batch, a->heads, a->kv_heads, a->head_dim,
+           a->head_dim_v);
+  p.capacity = p.key_rows = (int)a->key_rows;
   p.scale = a->scale;
-  iree_mi355x_paged_attention_t b = *a;
-  if (c.pages == 0)
-    b.prefix_length = b.table_width = 0;
-  const PagedPlan plan = plan_of(b, workspace ? workspace_bytes : 0);
-  // A launch has fewer than 2^32 threads.
-  const int64_t most = (int64_t)1 << 24;
-  if (plan.ways * c.kv_heads >= most ||
-      (plan.workspace && p.packed * p.kv_heads / (1024 / plan.dp) >= most - 1))
+  p.causal = a->flags & IREE_MI355X_ATTENTION_CAUSAL ? 1 : 0;
+  p.out_f32 = f32 ? 1 : 0;
+  const PagedPlan plan = plan_of(*a, workspace ? workspace_bytes : 0);
+  if (!launchable(plan, p))
     return fail(IREE_MI355X_UNSUPPORTED, "%s: problem too large", who);
-  return launch_status(launch_attention_paged(p, plan, workspace, stream),
+  return launch_status(launch_attention_paged(PagedKeys::kRows, p, plan,
+                                              workspace, stream),
                        who);
+}
+
+size_t iree_mi355x_packed_attention_workspace_bytes(
+    const iree_mi355x_packed_attention_t *a) {
+  if (!a || !plannable(*a))
+    return 0;
+  return (size_t)plan_of(*a, (size_t)-1).workspace;
 }
 
 size_t iree_mi355x_shared_prefix_attention_workspace_bytes(

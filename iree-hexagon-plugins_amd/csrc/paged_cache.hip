@@ -19,6 +19,15 @@
 // append_kv_kernel: rows of K and V into the pages that the slots name,
 // 16 bytes a lane. A row whose slot lies outside the cache is skipped. Bound
 // by memory: 8191 rows of 8 heads (67 MB) in 11.5 us, 5.8 TB/s; 64 rows 3.4.
+//
+// tree_masks_kernel: which of its request's new rows each one of a tree sees,
+// from the rows' parents. A wave takes a request, 64 rows at a time: with p(i)
+// the parent of row i,
+//   seen(i) = {i} + seen(p(i)),  depth(i) = 1 + depth(p(i))
+// and within the 64 rows the ancestors of all come from six doublings,
+//   seen_k+1(i) = seen_k(i) + seen_k(p^(2^k)(i))
+// as a 64-bit set a lane. The first ancestor before the 64 rows is the parent
+// of the topmost one among them, and its mask and depth are known by then.
 #include "device_common.h"
 #include "kernels_internal.h"
 
@@ -29,6 +38,8 @@ namespace {
 constexpr int kTableThreads = 512;
 constexpr int kTableWaves = kTableThreads / 64;
 constexpr int kAppendThreads = 256;
+constexpr int kMaskThreads = 256;
+constexpr int kMaskWaves = kMaskThreads / 64;
 
 __device__ __forceinline__ int32_t saturated(int64_t v) {
   return v > INT32_MAX ? INT32_MAX : (int32_t)v;
@@ -189,6 +200,82 @@ __global__ __launch_bounds__(kAppendThreads) void append_kv_kernel(
   }
 }
 
+__global__ __launch_bounds__(kMaskThreads) void tree_masks_kernel(
+    TreeMasks t) {
+  const int lane = threadIdx.x & 63;
+  const int b = __builtin_amdgcn_readfirstlane(
+      (int)(blockIdx.x * kMaskWaves + (threadIdx.x >> 6)));
+  auto start = [&](int i) {  // within the rows that there are
+    const int r = t.row_starts[i];
+    return r < 0 ? 0 : r > t.rows ? t.rows : r;
+  };
+  if (b >= t.batch) {  // rows behind the last request
+    const int64_t first = start(t.batch), end = t.rows;
+    const int64_t step =
+        ((int64_t)gridDim.x * kMaskWaves - t.batch) * 64;
+    const int64_t mine = (int64_t)(b - t.batch) * 64 + lane;
+    for (int64_t i = first * t.words + mine; i < end * t.words; i += step)
+      t.masks[i] = 0;
+    for (int64_t r = first + mine; r < end; r += step)
+      t.depths[r] = 0;
+    return;
+  }
+  const int first = start(b), end = start(b + 1);
+  for (int r0 = first; r0 < end; r0 += 64) {
+    // node numbers within the request; a parent that is not an earlier one of
+    // it is none
+    const int i0 = r0 - first, i = i0 + lane;
+    const bool real = r0 + lane < end;
+    int parent = real ? t.parents[r0 + lane] : -1;
+    if (parent < 0 || parent >= i)
+      parent = -1;
+    uint64_t seen = 1ull << lane;
+    int jump = parent - i0;
+#pragma unroll
+    for (int k = 0; k < 6; ++k) {
+      const int from = jump < 0 ? lane : jump;
+      const uint64_t theirs =
+          (uint64_t)(uint32_t)__shfl((int)(seen >> 32), from) << 32 |
+          (uint32_t)__shfl((int)seen, from);
+      const int next = __shfl(jump, from);
+      if (jump >= 0) {
+        seen |= theirs;
+        jump = next;
+      }
+    }
+    const int above = __shfl(parent, __builtin_ctzll(seen));
+    // what this wave wrote of the rows before
+    __threadfence_block();
+    if (real) {
+      const int64_t row = r0 + lane, up = first + (above < 0 ? 0 : above);
+      const int depth = above < 0 ? -1 : t.depths[up];
+      t.depths[row] = depth + __popcll(seen);
+      for (int w = 0; w < t.words; ++w) {
+        // bits 32 w .. of the nodes i0 .. i0 + 63
+        const int shift = i0 - 32 * w;
+        uint32_t bits = above < 0 ? 0 : (uint32_t)t.masks[up * t.words + w];
+        if (shift == 0)
+          bits |= (uint32_t)seen;
+        else if (shift == -32)
+          bits |= (uint32_t)(seen >> 32);
+        t.masks[row * t.words + w] = (int32_t)bits;
+      }
+    }
+  }
+}
+
+hipError_t launch_tree_masks(const TreeMasks &masks, void *stream) {
+  TreeMasks t = masks;
+  // Waves for the rows behind the last request, were it all: 16 words a lane.
+  int64_t rest = ((int64_t)t.rows * t.words + 1023) / 1024;
+  rest = rest > 64 ? 64 : rest;
+  const int64_t wgs = (t.batch + rest + kMaskWaves - 1) / kMaskWaves;
+  void *args[] = {&t};
+  return hipLaunchKernel((const void *)&tree_masks_kernel,
+                         dim3((unsigned)wgs), dim3(kMaskThreads), args, 0,
+                         (hipStream_t)stream);
+}
+
 hipError_t launch_page_tables(const PageTables &tables, void *stream) {
   PageTables t = tables;
   const int64_t most = t.rows > t.batch ? t.rows : t.batch;
@@ -214,6 +301,7 @@ const KernelEntry *paged_cache_kernels(int *count) {
   static const KernelEntry all[] = {
       {"page_tables", (const void *)&page_tables_kernel, kTableThreads, 0},
       {"append_kv", (const void *)&append_kv_kernel, kAppendThreads, 0},
+      {"tree_masks", (const void *)&tree_masks_kernel, kMaskThreads, 0},
   };
   *count = (int)(sizeof(all) / sizeof(all[0]));
   return all;
