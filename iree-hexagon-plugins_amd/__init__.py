@@ -1255,13 +1255,14 @@ _PAGED_ATTENTION = struct.Struct("@2P11q6P10qfI")
 
 # A small call is bound by the host: shapes and strides are asked for once, and
 # torch's types once at all.
-_F16 = _I32 = None
+_F16 = _I32 = _F32 = None
+_PAD = [(0,) * (4 - n) for n in range(5)]  # sections of axes there are not
 
 
 def _load_types():
-    global _F16, _I32
+    global _F16, _I32, _F32
     import torch
-    _F16, _I32 = torch.float16, torch.int32
+    _F16, _I32, _F32 = torch.float16, torch.int32, torch.float32
 
 
 def _ints(t, name, dims=1):
@@ -1739,7 +1740,6 @@ def rotary(q, k, positions, frequencies, sections=None, *, interleaved=False,
     otherwise)."""
     if _F16 is None:
         _load_types()
-    import torch
     (rows, h, d), (q0, q1, _) = _rows_of(q, "q", 3)
     hk = k0 = k1 = 0
     if k is not None:
@@ -1748,20 +1748,24 @@ def rotary(q, k, positions, frequencies, sections=None, *, interleaved=False,
             _shape(k, (rows, hk, d), "k")
     elif k_out is not None:
         raise ValueError("k_out without k")
-    dims = positions.dim() if isinstance(positions, torch.Tensor) else 1
-    *axes, of_t = _ints(positions, "positions", 2 if dims == 2 else 1)
-    axes = axes[0] if axes else 1
+    axes, pitch = 1, 0
+    if getattr(positions, "ndim", 1) == 2:
+        axes, of_t = _ints(positions, "positions", 2)
+        pitch = positions.stride(0)
+    else:
+        of_t, = _ints(positions, "positions")
     if of_t != rows:
         raise ValueError(f"positions must be [{rows}] or [axes, {rows}], got "
                          f"{list(positions.shape)}")
-    _require(frequencies, torch.float32, "frequencies", (1,))
-    half, = frequencies.shape
-    if half > 1 and frequencies.stride(0) != 1:
-        raise ValueError("frequencies must be contiguous")
+    if getattr(frequencies, "dtype", None) is not _F32:
+        raise TypeError("frequencies must be a float32 tensor")
+    half = frequencies.numel()
+    if frequencies.stride() != (1,) and (frequencies.ndim != 1 or half > 1):
+        raise ValueError("frequencies must be 1-D with unit column stride")
     sections = (half,) if sections is None else tuple(sections)
     if not 1 <= axes <= 4 or len(sections) != axes:
         raise ValueError(f"{len(sections)} sections for {axes} axes (1 to 4)")
-    if min(sections) < 0 or sum(sections) != half or 2 * half > d:
+    if sum(sections) != half or 2 * half > d or min(sections) < 0:
         raise ValueError(f"sections {sections} must be the {half} "
                          f"frequencies, and twice them at most head_dim {d}")
     qo, ko = (h * d, d), (hk * d, d)
@@ -1783,6 +1787,7 @@ def rotary(q, k, positions, frequencies, sections=None, *, interleaved=False,
                    (frequencies, "frequencies"), (q_out, "q_out"),
                    (k_out, "k_out"))
     if _other_device(index):
+        import torch
         with torch.cuda.device(index):
             return rotary(q, k, positions, frequencies, sections,
                           interleaved=interleaved, q_out=q_out, k_out=k_out,
@@ -1795,8 +1800,7 @@ def rotary(q, k, positions, frequencies, sections=None, *, interleaved=False,
         q.data_ptr(), 0 if k is None else k.data_ptr(), q_out.data_ptr(),
         0 if k is None else k_out.data_ptr(), positions.data_ptr(),
         frequencies.data_ptr(), rows, h, hk, d, axes,
-        *sections, *(0,) * (4 - axes), positions.stride(0) if axes > 1 else 0,
-        q0, q1, k0, k1, *qo, *ko, ROTARY_INTERLEAVED if interleaved else 0),
+        *sections, *_PAD[axes], pitch, q0, q1, k0, k1, *qo, *ko, ROTARY_INTERLEAVED if interleaved else 0),
         _stream_on(index, stream))
     if st != OK:
         _check(st)

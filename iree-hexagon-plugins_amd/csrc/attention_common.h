@@ -44,6 +44,10 @@ __device__ __forceinline__ void half_swap(float x, float &lo, float &hi) {
   asm volatile("s_nop 1\n\tv_permlane32_swap_b32 %0, %1"
                : "+v"(lo), "+v"(hi));
 }
+// Lanes 32..63 of x and lanes 0..31 of y change places.
+__device__ __forceinline__ void half_exchange(int &x, int &y) {
+  asm volatile("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(x), "+v"(y));
+}
 __device__ __forceinline__ float pair_max(float x) {
   float a, b;
   half_swap(x, a, b);

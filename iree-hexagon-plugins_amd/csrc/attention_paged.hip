@@ -98,13 +98,17 @@ __device__ __forceinline__ int token_of(const PagedAttention &p, int r) {
 // requests the first one's row starts and length, and the rows of small
 // requests before them.
 struct Requests {
-  int of[3][64];
+  int of[4][64];  // kRows: the row of the first key last
   uint32_t small[64];
 };
 
-// Requests of up to 16 rows share tiles of the prefix (a request of 17 has a tile
-// of its own and walks the prefix in it).
+// Requests of up to so many rows share tiles of the prefix (one of more has tiles
+// of its own and walks the prefix in them): those of a narrow tile, and trees
+// that would leave much of a wide tile empty (24 trees of 3 to 114 rows a KV head
+// behind 2048 keys: 51.2 -> 45.4 us, 46.7 with 64).
 constexpr int kSmallRows = kNarrowRows;
+template <PagedKeys KIND>
+constexpr int kSharedRows = KIND == PagedKeys::kTree ? 96 : kSmallRows;
 
 // One tile's work: rows r0 .. r_end - 1 (of a KV head; `compact`: the small
 // requests' rows alone) against steps s_begin .. s_end - 1 of 64 keys, the
@@ -160,6 +164,7 @@ __device__ __forceinline__ uint32_t tree_bits(const PagedTile &t,
 // The packed row of the small requests' row r: the last lane whose small rows
 // start at or before it, then its requests one after the other. Unsigned, and
 // a packed row whatever row_starts hold (the lanes' sums may have wrapped).
+template <PagedKeys KIND>
 __device__ __forceinline__ int packed_row(const PagedAttention &p,
                                           const Requests &all, uint32_t r) {
   int l = 0;
@@ -176,7 +181,7 @@ __device__ __forceinline__ int packed_row(const PagedAttention &p,
     for (;; ++b) {
       begin = row_start(p, b);
       const int rows = (row_start(p, b + 1) - begin) * p.group;
-      const uint32_t mine = rows > 0 && rows <= kSmallRows ? rows : 0;
+      const uint32_t mine = rows > 0 && rows <= kSharedRows<KIND> ? rows : 0;
       if (rest < mine || b >= last)
         break;
       rest -= mine;
@@ -188,11 +193,12 @@ __device__ __forceinline__ int packed_row(const PagedAttention &p,
 }
 
 // The lane's query row of a tile.
+template <PagedKeys KIND>
 __device__ __forceinline__ const f16 *query_row(const PagedAttention &p,
                                                 const PagedTile &t,
                                                 const Requests &all, int r) {
   if (t.compact)
-    r = packed_row(p, all, (uint32_t)r);
+    r = packed_row<KIND>(p, all, (uint32_t)r);
   const int token = token_of(p, r);
   return p.q + (int64_t)token * p.q_row +
          (int64_t)(t.kv_head * p.group + r - token * p.group) * p.q_head;
@@ -345,7 +351,7 @@ __device__ __forceinline__ void narrow_tile(const PagedTile &t,
   const int token = token_of(p, r_mine);
   i32x4 qf[KS];
   {
-    const f16 *qp = query_row(p, t, all, r_mine);
+    const f16 *qp = query_row<KIND>(p, t, all, r_mine);
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
       const int c = 32 * ks + 8 * lg;
@@ -636,22 +642,6 @@ __device__ __forceinline__ void wide_tile(const PagedTile &t,
           ? t.base
           : sees(p, t, r_wave < t.r_end ? r_wave : t.r_end - 1);
   const int token = token_of(p, r_mine);
-  i32x4 qf[DS];
-  {
-    const f16 *qp = query_row(p, t, all, r_mine);
-#pragma unroll
-    for (int s = 0; s < DS; ++s) {
-      const int c = 16 * s + 8 * g;
-      qf[s] = i32x4{0, 0, 0, 0};
-      if (c < p.dqk)
-        qf[s] = *(const i32x4 *)(qp + c);
-    }
-    // Waited for here, or the compiler would at their use in every step.
-    wait_vmcnt<0>();
-#pragma unroll
-    for (int s = 0; s < DS; ++s)
-      lgkm_tie(qf[s]);
-  }
 
   // Copy side: an instruction moves ROWS rows of CH chunks, lane -> (row,
   // physical chunk), fetching the logical chunk that belongs there if it lies
@@ -828,6 +818,23 @@ __device__ __forceinline__ void wide_tile(const PagedTile &t,
     if (KIND != PagedKeys::kRows && c + 1 < c_end)
       block.find(pages, lead, c + 1, group);
   }
+  // The query rows, read while the first keys are.
+  i32x4 qf[DS];
+  {
+    const f16 *qp = query_row<KIND>(p, t, all, r_mine);
+#pragma unroll
+    for (int s = 0; s < DS; ++s) {
+      const int d = 16 * s + 8 * g;
+      qf[s] = i32x4{0, 0, 0, 0};
+      if (d < p.dqk)
+        qf[s] = *(const i32x4 *)(qp + d);
+    }
+    // Waited for here, or the compiler would at their use in every step.
+    wait_vmcnt<0>();
+#pragma unroll
+    for (int s = 0; s < DS; ++s)
+      lgkm_tie(qf[s]);
+  }
   for (int slot = 0; c < c_end; ++c, slot ^= 1) {
     const bool own = c >= lead;
     const int key0 = (own ? c - lead : c) * kStepKeys;
@@ -1003,6 +1010,33 @@ __device__ __forceinline__ void wide_tile(const PagedTile &t,
   // the lane's row.
   const float sum = pair_sum(l_run);
   const int row = r_wave + l32;
+  if (KIND != PagedKeys::kPages && t.part < 0 && p.o_wide) {
+    // The row's lanes exchange halves of two quarters, so that each stores 16
+    // bytes of one.
+    const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+    f16 *dst = p.o + result_row(p, t.kv_head, row < t.r_end ? row : t.r_end - 1);
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int q = 0; q < 4; q += 2) {
+        i32x4 mine;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int r = 4 * q + 2 * e;
+          const f16x2 lo = {(f16)(o[dt][r] * inv), (f16)(o[dt][r + 1] * inv)};
+          const f16x2 hi = {(f16)(o[dt][r + 4] * inv),
+                            (f16)(o[dt][r + 5] * inv)};
+          int a = __builtin_bit_cast(int, lo), b = __builtin_bit_cast(int, hi);
+          half_exchange(a, b);
+          mine[e] = a;
+          mine[2 + e] = b;
+        }
+        const int d = 32 * dt + 8 * (q + g);
+        if (row < t.r_end && d < p.dv)
+          *(i32x4 *)(dst + d) = mine;
+      }
+    return;
+  }
   if (row >= t.r_end)
     return;
   if (t.part < 0) {
@@ -1087,7 +1121,7 @@ __device__ __forceinline__ int length_of(const PagedAttention &p, int b) {
   return p.lengths[b];
 }
 
-// `shared`: small requests leave the prefix to tiles of their own.
+// `shared`: requests of few rows leave the prefix to tiles of their own.
 template <bool WIDE, PagedKeys KIND>
 __device__ __forceinline__ Request request(const PagedAttention &p, int begin,
                                            int end, int length, bool shared,
@@ -1095,7 +1129,7 @@ __device__ __forceinline__ Request request(const PagedAttention &p, int begin,
   Request q;
   const int rows = rows_of(p, begin, end);
   const int added = end > begin ? end - begin : 0;
-  const bool small = rows <= kSmallRows;
+  const bool small = rows <= kNarrowRows;
   q.begin = begin;
   q.end = begin + added;
   q.shift = !WIDE || small ? 4 : 7;
@@ -1108,7 +1142,8 @@ __device__ __forceinline__ Request request(const PagedAttention &p, int begin,
   const int tokens =
       small ? added : WIDE ? p.wide_tokens : p.narrow_tokens;
   const bool whole = q.base >= 0 && length <= p.capacity && tokens > 0;
-  const uint32_t keys = (uint32_t)(small && shared ? 0 : prefix_keys) +
+  const bool apart = shared && rows <= kSharedRows<KIND>;
+  const uint32_t keys = (uint32_t)(apart ? 0 : prefix_keys) +
                         (uint32_t)(whole ? q.base + tokens : q.own_end);
   q.a = cost_of(keys >> p.unit, q.shift) + p.tile_units;
   if (KIND == PagedKeys::kRows && !p.causal) {
@@ -1123,10 +1158,15 @@ __device__ __forceinline__ Request request(const PagedAttention &p, int begin,
 
 }  // namespace
 
-// WIDE: requests of more than 16 rows have wide tiles.
+// WIDE: requests of more than 16 rows have wide tiles. Three workgroups a CU of
+// packed rows of 64 dims, whose registers just allow it: a short sequence's tile
+// is mostly waiting for its place, its first keys and its stores (48 sequences
+// of 1 to 500 tokens, 12 heads: 44.7 -> 39.1 us).
 template <int DP, int DX, int DK, bool WIDE, PagedKeys KIND>
-__global__ __launch_bounds__(kPagedThreads,
-                             DP >= 256 || (WIDE && DK > 128) ? 1 : 2) void
+__global__ __launch_bounds__(
+    kPagedThreads, DP >= 256 || (WIDE && DK > 128)        ? 1
+                   : DP == 64 && KIND == PagedKeys::kRows ? 3
+                                                          : 2) void
 attention_paged_kernel(PagedAttention) {
   constexpr int VBYTES = kBlockKeys * DP * 2;
   constexpr int MERGE = kPagedWaves * 16 * (DP + 4) * 4;
@@ -1153,7 +1193,9 @@ attention_paged_kernel(PagedAttention) {
   // Lane l has requests l * each .. + each - 1.
   const int lane = threadIdx.x & 63, wave = uniform((int)threadIdx.x >> 6);
   const int each = (p.batch + 63) >> 6;
-  int begin = 0, end = 0, length = 0;
+  int begin = 0, end = 0, length = 0, key0 = 0;
+  if (KIND == PagedKeys::kRows && lane * each < p.batch)
+    key0 = key_start(p, lane * each);
   if (lane * each < p.batch) {
     begin = row_start(p, lane * each);
     end = row_start(p, lane * each + 1);
@@ -1184,7 +1226,7 @@ attention_paged_kernel(PagedAttention) {
   };
   auto small_of = [&](int from, int to) {
     const int rows = rows_of(p, from, to);
-    return (uint32_t)(rows <= kSmallRows ? rows : 0);
+    return (uint32_t)(rows <= kSharedRows<KIND> ? rows : 0);
   };
   uint32_t small = small_of(begin, end), largest = small;
   rest_of_lane([&](int from, int to, int) {
@@ -1202,6 +1244,8 @@ attention_paged_kernel(PagedAttention) {
   all.of[0][lane] = begin;
   all.of[1][lane] = end;
   all.of[2][lane] = length;
+  if (KIND == PagedKeys::kRows)
+    all.of[3][lane] = key0;
   all.small[lane] = small_upto - small;
   // shared by two at least: no request has all the small ones' rows
   bool shared = p.shared && small_rows > 0 && !__any(largest == small_all);
@@ -1341,10 +1385,12 @@ attention_paged_kernel(PagedAttention) {
     t.base = q.base;
     t.own_end = q.own_end;
     t.table = p.table + (int64_t)(lead ? 0 : b) * p.table_stride;
-    t.key0 = KIND == PagedKeys::kRows ? uniform(key_start(p, b)) : 0;
+    t.key0 = 0;
+    if (KIND == PagedKeys::kRows)
+      t.key0 = uniform(p.batch <= 64 ? all.of[3][b] : key_start(p, b));
     // Whether the tile has all of its rows' keys.
     const bool all_keys =
-        !lead && !(shared && (q.end - q.begin) * p.group <= kSmallRows);
+        !lead && !(shared && (q.end - q.begin) * p.group <= kSharedRows<KIND>);
     t.lead = lead || all_keys ? (p.prefix + kStepKeys - 1) / kStepKeys : 0;
     t.seen = lead ? 0 : uniform(sees(p, t, t.r_end - 1));
     const int steps = t.lead + (t.seen + kStepKeys - 1) / kStepKeys;
@@ -1365,7 +1411,7 @@ attention_paged_kernel(PagedAttention) {
       for (int r = t.r0 + (int)threadIdx.x; r < t.r_end; r += kPagedThreads) {
         const i32x2 parts = {(int)(line + r) + kWideRows * first,
                              whole ? 0 : count};
-        const int at_row = lead ? packed_row(p, all, (uint32_t)r) : r;
+        const int at_row = lead ? packed_row<KIND>(p, all, (uint32_t)r) : r;
         p.part_of[line + at_row] = parts;
         if (all_keys)
           p.part_of[p.packed - line + r] = i32x2{0, 0};

@@ -461,6 +461,7 @@ struct PagedAttention {
   int words;
   const int32_t *masks;
   int64_t mask_stride;
+  int o_wide;  // 16-byte stores of o (f16) can be made: not kPages
   // kRows: `lengths` are the keys' starts, among key_rows rows.
   int key_rows, causal, out_f32;
 };

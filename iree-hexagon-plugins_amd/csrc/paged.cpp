@@ -257,6 +257,8 @@ static int paged_attention(const char *who, PagedKeys keys,
            reach(c.v_strides, 256) < UINT32_MAX;
   set_rows(&p, a->rows, a->batch, a->heads, c.kv_heads, c.head_dim,
            c.head_dim_v);
+  p.o_wide = aligned_to(a->o, 16) && a->o_strides[0] % 8 == 0 &&
+             a->o_strides[1] % 8 == 0;
   p.masks = masks;
   p.words = (int)words;
   p.mask_stride = mask_stride;
@@ -597,6 +599,8 @@ int iree_mi355x_packed_attention_f16(const iree_mi355x_packed_attention_t *a,
   p.scale = a->scale;
   p.causal = a->flags & IREE_MI355X_ATTENTION_CAUSAL ? 1 : 0;
   p.out_f32 = f32 ? 1 : 0;
+  p.o_wide = !f32 && aligned_to(a->o, 16) && a->o_strides[0] % 8 == 0 &&
+             a->o_strides[1] % 8 == 0;
   const PagedPlan plan = plan_of(*a, workspace ? workspace_bytes : 0);
   if (!launchable(plan, p))
     return fail(IREE_MI355X_UNSUPPORTED, "%s: problem too large", who);

@@ -27,7 +27,9 @@
 // and within the 64 rows the ancestors of all come from six doublings,
 //   seen_k+1(i) = seen_k(i) + seen_k(p^(2^k)(i))
 // as a 64-bit set a lane. The first ancestor before the 64 rows is the parent
-// of the topmost one among them, and its mask and depth are known by then.
+// of the topmost one among them, and its mask and depth are known by then: in
+// LDS, as far as it holds a request's (4096 words), else in the output. Bound by
+// the chain of 64s in the longest request.
 #include "device_common.h"
 #include "kernels_internal.h"
 
@@ -40,6 +42,7 @@ constexpr int kTableWaves = kTableThreads / 64;
 constexpr int kAppendThreads = 256;
 constexpr int kMaskThreads = 256;
 constexpr int kMaskWaves = kMaskThreads / 64;
+constexpr int kMaskWords = 4096;
 
 __device__ __forceinline__ int32_t saturated(int64_t v) {
   return v > INT32_MAX ? INT32_MAX : (int32_t)v;
@@ -221,12 +224,18 @@ __global__ __launch_bounds__(kMaskThreads) void tree_masks_kernel(
     return;
   }
   const int first = start(b), end = start(b + 1);
+  // Rows whose masks, each with its depth behind it, LDS holds.
+  __shared__ int32_t held_all[kMaskWaves][kMaskWords];
+  int32_t *held = held_all[threadIdx.x >> 6];
+  const int pitch = t.words + 1, most = kMaskWords / pitch;
+  int next = first + lane < end ? t.parents[first + lane] : -1;
   for (int r0 = first; r0 < end; r0 += 64) {
     // node numbers within the request; a parent that is not an earlier one of
     // it is none
     const int i0 = r0 - first, i = i0 + lane;
     const bool real = r0 + lane < end;
-    int parent = real ? t.parents[r0 + lane] : -1;
+    int parent = next;
+    next = r0 + 64 + lane < end ? t.parents[r0 + 64 + lane] : -1;
     if (parent < 0 || parent >= i)
       parent = -1;
     uint64_t seen = 1ull << lane;
@@ -246,19 +255,40 @@ __global__ __launch_bounds__(kMaskThreads) void tree_masks_kernel(
     const int above = __shfl(parent, __builtin_ctzll(seen));
     // what this wave wrote of the rows before
     __threadfence_block();
-    if (real) {
-      const int64_t row = r0 + lane, up = first + (above < 0 ? 0 : above);
-      const int depth = above < 0 ? -1 : t.depths[up];
-      t.depths[row] = depth + __popcll(seen);
-      for (int w = 0; w < t.words; ++w) {
+    const int64_t row = r0 + lane, up = first + (int64_t)(above < 0 ? 0 : above);
+    const int at = above < most ? above * pitch : 0;
+    int depth = -1;
+    if (above >= 0)
+      depth = above < most ? held[at + t.words] : t.depths[up];
+    depth += __popcll(seen);
+    const bool hold = i < most;
+    if (real)
+      t.depths[row] = depth;
+    if (real && hold)
+      held[i * pitch + t.words] = depth;
+    for (int w0 = 0; w0 < t.words; w0 += 4) {
+      uint32_t bits[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int w = w0 + j < t.words ? w0 + j : t.words - 1;
+        bits[j] = 0;
+        if (above >= 0)
+          bits[j] = (uint32_t)(above < most ? held[at + w]
+                                            : t.masks[up * t.words + w]);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
         // bits 32 w .. of the nodes i0 .. i0 + 63
-        const int shift = i0 - 32 * w;
-        uint32_t bits = above < 0 ? 0 : (uint32_t)t.masks[up * t.words + w];
+        const int w = w0 + j, shift = i0 - 32 * w;
         if (shift == 0)
-          bits |= (uint32_t)seen;
+          bits[j] |= (uint32_t)seen;
         else if (shift == -32)
-          bits |= (uint32_t)(seen >> 32);
-        t.masks[row * t.words + w] = (int32_t)bits;
+          bits[j] |= (uint32_t)(seen >> 32);
+        if (real && w < t.words) {
+          t.masks[row * t.words + w] = (int32_t)bits[j];
+          if (hold)
+            held[i * pitch + w] = (int32_t)bits[j];
+        }
       }
     }
   }

@@ -40,7 +40,7 @@ def test_rotary_checks(pkg):
     bad("positions must be", positions=i(2, 3, 5))
     bad("unit column", positions=i(5, 3).t())
     bad("float32", TypeError, frequencies=z(6))
-    bad("frequencies must be", frequencies=z(2, 3, dtype=F))
+    bad("1-D", frequencies=z(2, 3, dtype=F))
     bad("unit column", frequencies=z(12, dtype=F)[::2])
     bad("sections for 3 axes", sections=None)
     bad("sections for 1 axes", positions=i(5))
