@@ -36,6 +36,8 @@
 // the MFMAs 247.
 // A call costs 7 us at least (launch 2, finding its place 2, a tile 3), and 4
 // more where parts are joined.
+#include <string>
+
 #include "attention_common.h"
 #include "device_common.h"
 #include "kernels_internal.h"
@@ -1158,23 +1160,20 @@ __device__ __forceinline__ Request request(const PagedAttention &p, int begin,
 
 }  // namespace
 
-// WIDE: requests of more than 16 rows have wide tiles. Three workgroups a CU of
-// packed rows of 64 dims, whose registers just allow it: a short sequence's tile
-// is mostly waiting for its place, its first keys and its stores (48 sequences
-// of 1 to 500 tokens, 12 heads: 44.7 -> 39.1 us).
+// LDS of a tile: a narrow one's V and the waves' merge, a wide one's ring.
+constexpr int tile_bytes(int dp, int dk, bool wide) {
+  const int v = kPagedWaves * kBlockKeys * dp * 2;
+  const int merge = kPagedWaves * 16 * (dp + 4) * 4;
+  const int ring = wide ? 4 * kStepKeys * (dp + staged_k(dp, dk)) : 0;
+  return ring > v && ring > merge ? ring : v > merge ? v : merge;
+}
+
+// WIDE: requests of more than 16 rows have wide tiles.
 template <int DP, int DX, int DK, bool WIDE, PagedKeys KIND>
 __global__ __launch_bounds__(
-    kPagedThreads, DP >= 256 || (WIDE && DK > 128)        ? 1
-                   : DP == 64 && KIND == PagedKeys::kRows ? 3
-                                                          : 2) void
+    kPagedThreads, DP >= 256 || (WIDE && DK > 128) ? 1 : 2) void
 attention_paged_kernel(PagedAttention) {
-  constexpr int VBYTES = kBlockKeys * DP * 2;
-  constexpr int MERGE = kPagedWaves * 16 * (DP + 4) * 4;
-  constexpr int RING = WIDE ? 4 * kStepKeys * (DP + staged_k(DP, DK)) : 0;
-  constexpr int NARROW =
-      kPagedWaves * VBYTES > MERGE ? kPagedWaves * VBYTES : MERGE;
-  constexpr int SMEM = NARROW > RING ? NARROW : RING;
-  __shared__ __attribute__((aligned(1024))) char smem[SMEM];
+  __shared__ __attribute__((aligned(1024))) char smem[tile_bytes(DP, DK, WIDE)];
   __shared__ float wave_m[kPagedWaves][kNarrowRows],
       wave_l[kPagedWaves][kNarrowRows];
   // Where each wave is on the line, kept here, out of the tiles' registers.
@@ -1205,17 +1204,9 @@ attention_paged_kernel(PagedAttention) {
   int item, unused;
   xcd_tile_order((int)blockIdx.x, p.items, p.items, 1, 1, &item, &unused);
   PagedTile t;
-  t.kv_head = KIND == PagedKeys::kRows
-                  ? item / p.ways
-              : p.ways == 1 ? item
-                            : (int)__umulhi((uint32_t)item, p.ways_magic);
+  t.kv_head = p.ways == 1 ? item
+                          : (int)__umulhi((uint32_t)item, p.ways_magic);
   int way = item - t.kv_head * p.ways;
-  // Whole tiles of heads that do not fall to the XCDs evenly: all heads' tiles
-  // of the most keys first.
-  if (KIND == PagedKeys::kRows && !p.partials && p.kv_heads % 8 != 0) {
-    way = (int)blockIdx.x / p.kv_heads;
-    t.kv_head = (int)blockIdx.x - way * p.kv_heads;
-  }
 
   // The small requests' rows, and whether the prefix gets tiles of them.
   auto rest_of_lane = [&](auto f) {  // the lane's requests after its first
@@ -1274,12 +1265,6 @@ attention_paged_kernel(PagedAttention) {
   uint32_t per = p.ways == 1 ? total : __umulhi(total - 1, p.ways_magic) + 1;
   per = per < (uint32_t)p.least ? p.least : per;
   float inv_per = 1.0f / (float)per;
-  // The tiles of a request's last tokens have the most keys: they come first.
-  if (KIND == PagedKeys::kRows && !p.partials) {
-    way = (int)((total + per - 1) / per) - 1 - way;
-    if (way < 0)
-      return;
-  }
   uint32_t x = (uint32_t)way * per;  // below 2^32: `ways` is at most 2^24
   if (x >= total)
     return;
@@ -1448,6 +1433,103 @@ attention_paged_kernel(PagedAttention) {
   }
 }
 
+// Packed rows whose tiles are all whole: a workgroup takes one, found by the
+// requests' numbers of tiles alone (as a line of them 1.5 us longer: 48
+// sequences of 1 to 500 tokens, 12 heads of 64, XXX -> XXX us; prompts of 7195
+// rows XXX -> XXX). The tiles of a request's last tokens, which have the most keys,
+// come first. Three workgroups a CU of 64 dims, whose registers just allow it: a
+// short sequence's tile is mostly waiting, for its place, its first keys and its
+// stores (the 48 sequences 44.7 -> 39.1 us).
+template <int DP, int DX, int DK, bool WIDE>
+__global__ __launch_bounds__(kPagedThreads, DP >= 256 || (WIDE && DK > 128) ? 1
+                                            : DP == 64                      ? 3
+                                                                            : 2)
+void attention_packed_kernel(PagedAttention) {
+  constexpr PagedKeys KIND = PagedKeys::kRows;
+  __shared__ __attribute__((aligned(1024))) char smem[tile_bytes(DP, DK, WIDE)];
+  __shared__ float wave_m[kPagedWaves][kNarrowRows],
+      wave_l[kPagedWaves][kNarrowRows];
+  __shared__ Requests all;  // not used: no tile is compact
+
+  const PagedAttention &p = arguments();
+  asm volatile("" ::"s"(p.row_starts), "s"(p.lengths), "s"(p.batch),
+               "s"(p.rows), "s"(p.group), "s"(p.ways), "s"(p.items),
+               "s"(p.q_row), "s"(p.causal), "s"(p.key_rows));
+  const int lane = threadIdx.x & 63;
+  const int each = (p.batch + 63) >> 6;
+  int begin = 0, end = 0, key0 = 0, key1 = 0;
+  if (lane * each < p.batch) {
+    begin = row_start(p, lane * each);
+    end = row_start(p, lane * each + 1);
+    key0 = key_start(p, lane * each);
+    key1 = key_start(p, lane * each + 1);
+  }
+  // Heads that fall to the XCDs evenly stay on one, for its L2; of others all
+  // heads' tiles of the most keys come first.
+  PagedTile t = {};
+  int way;
+  if (p.kv_heads % 8 == 0) {
+    int item, unused;
+    xcd_tile_order((int)blockIdx.x, p.items, p.items, 1, 1, &item, &unused);
+    t.kv_head = item / p.ways;
+    way = item - t.kv_head * p.ways;
+  } else {
+    way = (int)blockIdx.x / p.kv_heads;
+    t.kv_head = (int)blockIdx.x - way * p.kv_heads;
+  }
+  auto tiles_of = [&](int from, int to) {
+    const int rows = rows_of(p, from, to);
+    const int shift = !WIDE || rows <= kNarrowRows ? 4 : 7;
+    return (uint32_t)(rows + (1 << shift) - 1) >> shift;
+  };
+  uint32_t tiles = tiles_of(begin, end);
+  for (int i = 1; i < each && lane * each + i < p.batch; ++i)
+    tiles += tiles_of(row_start(p, lane * each + i),
+                      row_start(p, lane * each + i + 1));
+  const uint32_t upto = lane_sums(tiles);
+  const uint32_t total = (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
+  if ((uint32_t)way >= total)
+    return;
+  const uint32_t at = total - 1 - (uint32_t)way;
+  const int lane_of = uniform(
+      63 - __builtin_clzll(__ballot(upto - tiles <= at) | 1));
+  uint32_t i = at - (uint32_t)__builtin_amdgcn_readlane((int)(upto - tiles), lane_of);
+  begin = __builtin_amdgcn_readlane(begin, lane_of);
+  end = __builtin_amdgcn_readlane(end, lane_of);
+  key0 = __builtin_amdgcn_readlane(key0, lane_of);
+  key1 = __builtin_amdgcn_readlane(key1, lane_of);
+  for (int b = lane_of * each; i >= tiles_of(begin, end);) {
+    // (the sums may have wrapped: no further than the last request)
+    if (++b >= p.batch)
+      return;
+    i -= tiles_of(begin, end);
+    begin = uniform(row_start(p, b));
+    end = uniform(row_start(p, b + 1));
+    key0 = uniform(key_start(p, b));
+    key1 = uniform(key_start(p, b + 1));
+  }
+  const int rows = rows_of(p, begin, end);
+  const int shift = !WIDE || rows <= kNarrowRows ? 4 : 7;
+  const int length = key1 > key0 ? key1 - key0 : 0;
+  t.key0 = key0;
+  t.r0 = begin * p.group + ((int)i << shift);
+  t.r_end = begin * p.group + rows;
+  t.r_end = t.r_end - t.r0 < 1 << shift ? t.r_end : t.r0 + (1 << shift);
+  t.compact = false;
+  t.lead = 0;
+  t.own_end = length;
+  t.first = begin;
+  t.base = p.causal ? length - (end - begin) : length;
+  t.seen = uniform(sees(p, t, t.r_end - 1));
+  t.s_begin = 0;
+  t.s_end = (t.seen + kStepKeys - 1) / kStepKeys;
+  t.part = -1;
+  if (shift == 4)
+    narrow_tile<DP, DX, DK, KIND>(t, all, smem, wave_m, wave_l);
+  else if constexpr (WIDE)
+    wide_tile<DP, DX, DK, KIND>(t, all, smem);
+}
+
 // Joins the parts of every row that has some: DP / 4 threads, 4 columns each,
 // for every GROUPS-th four of a row's parts, then the GROUPS sums through LDS.
 // A row's parts of one kind (the prefix's of a small request, its own or both
@@ -1561,6 +1643,7 @@ struct PagedKernel {
   int dp, dx, dk, groups;  // groups: of a joined row's parts
   bool wide;
   const void *fn;
+  const void *whole = nullptr;  // where no tile is split
 };
 // A join of kPages is also kTree's.
 const PagedKernel kPagedKernels[] = {
@@ -1576,6 +1659,11 @@ const PagedKernel kPagedKernels[] = {
       IHP_PAGED(NAME "_d256", KIND, 256, 256, 256, false)
     IHP_PAGED_ALL("paged", kPages),
     IHP_PAGED_ALL("tree", kTree),
+#undef IHP_PAGED
+#define IHP_PAGED(NAME, KIND, DP, DX, DK, WIDE)                                \
+  {"attention_" NAME, PagedKeys::KIND, DP, DX, DK, 0, WIDE,                    \
+   (const void *)&attention_paged_kernel<DP, DX, DK, WIDE, PagedKeys::KIND>,   \
+   (const void *)&attention_packed_kernel<DP, DX, DK, WIDE>}
     IHP_PAGED_ALL("packed", kRows),
     IHP_PAGED("packed_d256_rows", kRows, 256, 256, 256, true),
 #undef IHP_PAGED_ALL
@@ -1671,8 +1759,8 @@ hipError_t launch_attention_paged(PagedKeys keys,
   a.snap = (int)plan.snap;
   a.shared = plan.shared ? 1 : 0;
   // item / ways, exact while item * ways is below 2^32: at most 4 ways to each
-  // of 65535 heads, or 2048 workgroups in all (kRows divides: its whole tiles
-  // may be more); and the ways' share of a line of less than 2^31 units, at
+  // of 65535 heads, or 2048 workgroups in all (whole tiles of packed rows may be
+  // more, and divide); and the ways' share of a line of less than 2^31 units, at
   // most one unit over. (One way's is not used.)
   if (keys != PagedKeys::kRows && (uint64_t)a.items * (uint64_t)a.ways >> 32)
     return hipErrorInvalidValue;
@@ -1701,8 +1789,9 @@ hipError_t launch_attention_paged(PagedKeys keys,
   if (!kernel || !join)
     return hipErrorInvalidValue;
   void *args[] = {&a};
+  const void *fn = !plan.workspace && kernel->whole ? kernel->whole : kernel->fn;
   hipError_t e =
-      hipLaunchKernel(kernel->fn, dim3((unsigned)a.items),
+      hipLaunchKernel(fn, dim3((unsigned)a.items),
                       dim3(kPagedThreads), args, 0, (hipStream_t)stream);
   if (e != hipSuccess || !plan.workspace)
     return e;
@@ -1713,14 +1802,21 @@ hipError_t launch_attention_paged(PagedKeys keys,
 }
 
 const KernelEntry *attention_paged_kernels(int *count) {
-  static KernelEntry all[kPagedKernelCount];
-  static const bool filled = [] {
-    for (int i = 0; i < kPagedKernelCount; ++i)
-      all[i] = {kPagedKernels[i].name, kPagedKernels[i].fn, kPagedThreads, 0};
-    return true;
+  static KernelEntry all[2 * kPagedKernelCount];
+  static std::string names[kPagedKernelCount];  // of the whole tiles' kernels
+  static const int filled = [] {
+    int n = 0;
+    for (const PagedKernel &k : kPagedKernels) {
+      all[n++] = {k.name, k.fn, kPagedThreads, 0};
+      if (k.whole) {
+        std::string &name = names[&k - kPagedKernels];
+        name = std::string(k.name) + "_whole";
+        all[n++] = {name.c_str(), k.whole, kPagedThreads, 0};
+      }
+    }
+    return n;
   }();
-  (void)filled;
-  *count = kPagedKernelCount;
+  *count = filled;
   return all;
 }
 
