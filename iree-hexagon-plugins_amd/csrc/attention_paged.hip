@@ -58,6 +58,7 @@ constexpr int kWideRows = 128;
 // bits than none (rounding N(0, 1) scores and values of 64 to 5000 keys).
 // (Four prompts of 2243 rows: 259.8 us with none, 241.3 with 4.)
 constexpr float kLag = 4.0f;
+constexpr uint32_t kLevelKeys = 128;  // by which whole tiles are ordered
 constexpr float kNegInf = -__builtin_inff();
 constexpr float kLog2e = 1.4426950408889634f;
 typedef float f32x2 __attribute__((ext_vector_type(2)));
@@ -1435,9 +1436,12 @@ attention_paged_kernel(PagedAttention) {
 
 // Packed rows whose tiles are all whole: a workgroup takes one, found by the
 // requests' numbers of tiles alone (as a line of them 1.5 us longer: 48
-// sequences of 1 to 500 tokens, 12 heads of 64, XXX -> XXX us; prompts of 7195
-// rows XXX -> XXX). The tiles of a request's last tokens, which have the most keys,
-// come first. Three workgroups a CU of 64 dims, whose registers just allow it: a
+// sequences of 1 to 500 tokens, 12 heads of 64, 37.7 -> 34.2 us; prompts of 7195
+// rows 119.8 -> 115). Tiles of the most keys come first, by 128 keys, among up to
+// 64 requests (16 of 10 to 1500 tokens, 9 / 3 heads of 64: 40.5 -> 34.4 us; 8 of
+// 100 to 1500, 24 / 8 heads of 96: 68.2 -> 63.6; of equal length the same; finding
+// them costs 0.8, so not where all are short); of more requests, those of each
+// one's last tokens. Three workgroups a CU of 64 dims, whose registers just allow it: a
 // short sequence's tile is mostly waiting, for its place, its first keys and its
 // stores (the 48 sequences 44.7 -> 39.1 us).
 template <int DP, int DX, int DK, bool WIDE>
@@ -1482,6 +1486,7 @@ void attention_packed_kernel(PagedAttention) {
     const int shift = !WIDE || rows <= kNarrowRows ? 4 : 7;
     return (uint32_t)(rows + (1 << shift) - 1) >> shift;
   };
+  const int tiles_rows = rows_of(p, begin, end);
   uint32_t tiles = tiles_of(begin, end);
   for (int i = 1; i < each && lane * each + i < p.batch; ++i)
     tiles += tiles_of(row_start(p, lane * each + i),
@@ -1490,10 +1495,44 @@ void attention_packed_kernel(PagedAttention) {
   const uint32_t total = (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
   if ((uint32_t)way >= total)
     return;
-  const uint32_t at = total - 1 - (uint32_t)way;
-  const int lane_of = uniform(
-      63 - __builtin_clzll(__ballot(upto - tiles <= at) | 1));
-  uint32_t i = at - (uint32_t)__builtin_amdgcn_readlane((int)(upto - tiles), lane_of);
+  auto lane_at = [&](uint32_t first, uint32_t x) {  // the last first <= x
+    return uniform(63 - __builtin_clzll(__ballot(first <= x) | 1));
+  };
+  auto of_lane = [&](uint32_t x, int l) {
+    return (uint32_t)__builtin_amdgcn_readlane((int)x, l);
+  };
+  int lane_of;
+  uint32_t i;
+  if (p.levels) {
+    // Tile `way` of all by their keys, most first: among those of kLevelKeys *
+    // level keys and more but not of the next level.
+    const uint32_t keys = key1 > key0 ? (uint32_t)(key1 - key0) : 0;
+    const int shift = !WIDE || tiles_rows <= kNarrowRows ? 4 : 7;
+    auto with = [&](uint32_t level) {  // the request's tiles of so many keys
+      const uint32_t least = level * kLevelKeys;
+      const uint32_t n =
+          p.causal ? (uint32_t)((uint64_t)(keys - least) * p.group >> shift) + 1
+                   : tiles;
+      return keys < least ? 0 : n < tiles ? n : tiles;
+    };
+    uint32_t level = 0;
+    for (uint32_t step = (uint32_t)p.levels; step > 0; step >>= 1)
+      if (of_lane(lane_sums(with(level + step)), 63) > (uint32_t)way)
+        level += step;
+    const uint32_t more = with(level + 1);
+    const uint32_t mine = (level == 0 ? tiles : with(level)) - more;
+    const uint32_t rank =
+        (uint32_t)way - of_lane(lane_sums(more), 63);
+    const uint32_t before = lane_sums(mine) - mine;
+    lane_of = lane_at(before, rank);
+    i = of_lane(tiles - 1 - more, lane_of) - (rank - of_lane(before, lane_of));
+    if (i >= of_lane(tiles, lane_of))
+      return;  // (the sums may have wrapped)
+  } else {
+    const uint32_t at = total - 1 - (uint32_t)way;
+    lane_of = lane_at(upto - tiles, at);
+    i = at - of_lane(upto - tiles, lane_of);
+  }
   begin = __builtin_amdgcn_readlane(begin, lane_of);
   end = __builtin_amdgcn_readlane(end, lane_of);
   key0 = __builtin_amdgcn_readlane(key0, lane_of);
@@ -1763,6 +1802,13 @@ hipError_t launch_attention_paged(PagedKeys keys,
   a.least = (int)plan.least;
   a.unit = (int)plan.unit;
   a.tile_units = (int)plan.tile_units;
+  // Requests of a lane each that may differ, and more tiles than run at once.
+  a.levels = a.batch > 1 && a.batch <= 64 && a.items > kPagedTargetWgs &&
+                     a.key_rows / a.batch >= 2 * (int)kLevelKeys
+                 ? 1
+                 : 0;
+  while (a.levels && (int64_t)a.levels * 2 * (int64_t)kLevelKeys <= a.key_rows)
+    a.levels *= 2;
   a.snap = (int)plan.snap;
   a.shared = plan.shared ? 1 : 0;
   // item / ways, exact while item * ways is below 2^32: at most 4 ways to each

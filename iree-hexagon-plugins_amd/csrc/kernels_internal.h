@@ -464,6 +464,9 @@ struct PagedAttention {
   int o_wide;  // 16-byte stores of o (f16) can be made: not kPages
   // kRows: `lengths` are the keys' starts, among key_rows rows.
   int key_rows, causal, out_f32;
+  // Whole tiles are ordered by their keys: a power of 2, twice which times
+  // kLevelKeys no request has. 0: they are not.
+  int levels;
 };
 // Workgroups wanted: two a CU where head dims allow it (768 and 1024 instead
 // of 512: 64 requests' tokens behind a prefix 48.5 -> 59 us and more, prompts

@@ -203,6 +203,88 @@ __global__ __launch_bounds__(kAppendThreads) void append_kv_kernel(
   }
 }
 
+// Words that a row takes in LDS: its mask and its depth, an odd number.
+__device__ __forceinline__ int mask_pitch(const TreeMasks &t) {
+  return (t.words + 1) | 1;
+}
+
+// A request's rows. HELD: `held` has room for their masks and depths.
+template <bool HELD>
+__device__ __forceinline__ void tree_masks_of(const TreeMasks &t, int first,
+                                              int end, int32_t *held) {
+  const int lane = threadIdx.x & 63, pitch = mask_pitch(t);
+  const bool fours =
+      t.words % 4 == 0 && (uintptr_t)t.masks % 16 == 0;  // of words
+  int next = first + lane < end ? t.parents[first + lane] : -1;
+  for (int r0 = first; r0 < end; r0 += 64) {
+    // node numbers within the request; a parent that is not an earlier one of
+    // it is none
+    const int i0 = r0 - first, i = i0 + lane;
+    const bool real = r0 + lane < end;
+    int parent = next;
+    next = r0 + 64 + lane < end ? t.parents[r0 + 64 + lane] : -1;
+    if (parent < 0 || parent >= i)
+      parent = -1;
+    uint64_t seen = 1ull << lane;
+    int jump = parent - i0;
+#pragma unroll
+    for (int k = 0; k < 6; ++k) {
+      const int from = jump < 0 ? lane : jump;
+      const uint64_t theirs =
+          (uint64_t)(uint32_t)__shfl((int)(seen >> 32), from) << 32 |
+          (uint32_t)__shfl((int)seen, from);
+      const int further = __shfl(jump, from);
+      if (jump >= 0) {
+        seen |= theirs;
+        jump = further;
+      }
+    }
+    const int above = __shfl(parent, __builtin_ctzll(seen));
+    // what this wave wrote of the rows before (LDS keeps a wave's order)
+    if (HELD)
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    else
+      __threadfence_block();
+    const int from = above < 0 ? 0 : above;
+    const int64_t row = r0 + lane;
+    const int32_t *theirs = HELD ? held + from * pitch
+                                 : t.masks + (int64_t)(first + from) * t.words;
+    int32_t *mine = HELD ? held + i * pitch : nullptr;
+    int depth = HELD ? theirs[t.words] : t.depths[first + from];
+    depth = (above < 0 ? -1 : depth) + __popcll(seen);
+    if (real) {
+      t.depths[row] = depth;
+      if (HELD)
+        mine[t.words] = depth;
+    }
+    for (int w0 = 0; w0 < t.words; w0 += 4) {
+      i32x4 bits;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int word = theirs[w0 + j < t.words ? w0 + j : t.words - 1];
+        // and bits 32 w .. of the nodes i0 .. i0 + 63
+        const int shift = i0 - 32 * (w0 + j);
+        bits[j] = (above < 0 ? 0 : word) | (shift == 0     ? (int)seen
+                                            : shift == -32 ? (int)(seen >> 32)
+                                                           : 0);
+      }
+      if (!real)
+        continue;
+      int32_t *out = t.masks + row * t.words + w0;
+      if (fours)
+        *(i32x4 *)out = bits;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (w0 + j < t.words) {
+          if (HELD)
+            mine[w0 + j] = bits[j];
+          if (!fours)
+            out[j] = bits[j];
+        }
+    }
+  }
+}
+
 __global__ __launch_bounds__(kMaskThreads) void tree_masks_kernel(
     TreeMasks t) {
   const int lane = threadIdx.x & 63;
@@ -223,75 +305,12 @@ __global__ __launch_bounds__(kMaskThreads) void tree_masks_kernel(
       t.depths[r] = 0;
     return;
   }
-  const int first = start(b), end = start(b + 1);
-  // Rows whose masks, each with its depth behind it, LDS holds.
   __shared__ int32_t held_all[kMaskWaves][kMaskWords];
-  int32_t *held = held_all[threadIdx.x >> 6];
-  const int pitch = t.words + 1, most = kMaskWords / pitch;
-  int next = first + lane < end ? t.parents[first + lane] : -1;
-  for (int r0 = first; r0 < end; r0 += 64) {
-    // node numbers within the request; a parent that is not an earlier one of
-    // it is none
-    const int i0 = r0 - first, i = i0 + lane;
-    const bool real = r0 + lane < end;
-    int parent = next;
-    next = r0 + 64 + lane < end ? t.parents[r0 + 64 + lane] : -1;
-    if (parent < 0 || parent >= i)
-      parent = -1;
-    uint64_t seen = 1ull << lane;
-    int jump = parent - i0;
-#pragma unroll
-    for (int k = 0; k < 6; ++k) {
-      const int from = jump < 0 ? lane : jump;
-      const uint64_t theirs =
-          (uint64_t)(uint32_t)__shfl((int)(seen >> 32), from) << 32 |
-          (uint32_t)__shfl((int)seen, from);
-      const int next = __shfl(jump, from);
-      if (jump >= 0) {
-        seen |= theirs;
-        jump = next;
-      }
-    }
-    const int above = __shfl(parent, __builtin_ctzll(seen));
-    // what this wave wrote of the rows before
-    __threadfence_block();
-    const int64_t row = r0 + lane, up = first + (int64_t)(above < 0 ? 0 : above);
-    const int at = above < most ? above * pitch : 0;
-    int depth = -1;
-    if (above >= 0)
-      depth = above < most ? held[at + t.words] : t.depths[up];
-    depth += __popcll(seen);
-    const bool hold = i < most;
-    if (real)
-      t.depths[row] = depth;
-    if (real && hold)
-      held[i * pitch + t.words] = depth;
-    for (int w0 = 0; w0 < t.words; w0 += 4) {
-      uint32_t bits[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int w = w0 + j < t.words ? w0 + j : t.words - 1;
-        bits[j] = 0;
-        if (above >= 0)
-          bits[j] = (uint32_t)(above < most ? held[at + w]
-                                            : t.masks[up * t.words + w]);
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        // bits 32 w .. of the nodes i0 .. i0 + 63
-        const int w = w0 + j, shift = i0 - 32 * w;
-        if (shift == 0)
-          bits[j] |= (uint32_t)seen;
-        else if (shift == -32)
-          bits[j] |= (uint32_t)(seen >> 32);
-        if (real && w < t.words) {
-          t.masks[row * t.words + w] = (int32_t)bits[j];
-          if (hold)
-            held[i * pitch + w] = (int32_t)bits[j];
-        }
-      }
-    }
-  }
+  const int first = start(b), end = start(b + 1);
+  if ((int64_t)(end - first) * mask_pitch(t) <= kMaskWords)
+    tree_masks_of<true>(t, first, end, held_all[threadIdx.x >> 6]);
+  else
+    tree_masks_of<false>(t, first, end, nullptr);
 }
 
 hipError_t launch_tree_masks(const TreeMasks &masks, void *stream) {
