@@ -58,6 +58,7 @@ constexpr int kWideRows = 128;
 // bits than none (rounding N(0, 1) scores and values of 64 to 5000 keys).
 // (Four prompts of 2243 rows: 259.8 us with none, 241.3 with 4.)
 constexpr float kLag = 4.0f;
+constexpr int kTurnWgs = 256;  // workgroups that give every CU one
 constexpr uint32_t kLevelKeys = 128;  // by which whole tiles are ordered
 constexpr float kNegInf = -__builtin_inff();
 constexpr float kLog2e = 1.4426950408889634f;
@@ -1450,6 +1451,8 @@ __global__ __launch_bounds__(kPagedThreads, DP >= 256 || (WIDE && DK > 128) ? 1
                                                                             : 2)
 void attention_packed_kernel(PagedAttention) {
   constexpr PagedKeys KIND = PagedKeys::kRows;
+  constexpr int RESIDENT =
+      DP >= 256 || (WIDE && DK > 128) ? 1 : DP == 64 ? 3 : 2;
   __shared__ __attribute__((aligned(1024))) char smem[tile_bytes(DP, DK, WIDE)];
   __shared__ float wave_m[kPagedWaves][kNarrowRows],
       wave_l[kPagedWaves][kNarrowRows];
@@ -1471,15 +1474,25 @@ void attention_packed_kernel(PagedAttention) {
   // Heads that fall to the XCDs evenly stay on one, for its L2; of others all
   // heads' tiles of the most keys come first.
   PagedTile t = {};
-  int way;
-  if (p.kv_heads % 8 == 0) {
+  int way, wg = (int)blockIdx.x;
+  const bool even = p.kv_heads % 8 == 0;
+  // Where all run at once the CUs' second workgroups come in the opposite order
+  // of the first ones: the CU with the most keys gets the fewest (a prompt of 2000
+  // tokens, 32 / 8 heads of 128: 53.3 -> 49.9 us).
+  const int turn = wg / kTurnWgs;
+  if (p.items <= kTurnWgs * RESIDENT && turn % 2 == 1) {
+    const int first = turn * kTurnWgs;
+    const int end = p.items < first + kTurnWgs ? p.items : first + kTurnWgs;
+    wg = even ? first + end - 8 - wg / 8 * 8 + wg % 8 : first + end - 1 - wg;
+  }
+  if (even) {
     int item, unused;
-    xcd_tile_order((int)blockIdx.x, p.items, p.items, 1, 1, &item, &unused);
+    xcd_tile_order(wg, p.items, p.items, 1, 1, &item, &unused);
     t.kv_head = item / p.ways;
     way = item - t.kv_head * p.ways;
   } else {
-    way = (int)blockIdx.x / p.kv_heads;
-    t.kv_head = (int)blockIdx.x - way * p.kv_heads;
+    way = wg / p.kv_heads;
+    t.kv_head = wg - way * p.kv_heads;
   }
   auto tiles_of = [&](int from, int to) {
     const int rows = rows_of(p, from, to);
@@ -1771,16 +1784,19 @@ PagedPlan plan_attention_paged(PagedKeys keys, int64_t rows, int64_t batch,
   const int64_t most = tiles * kv_heads > wgs ? kPagedWholeKeys
                        : p.wide && rows_many  ? kPagedWholeKeysWide
                                               : kPagedWholeKeysFew;
-  // Packed rows: as many tiles as can run at once are not split either (four
-  // prompts of 400 to 600 tokens, 32 / 8 heads of 128, 39.4 -> 25.7 us; 64
-  // sequences of up to 120, 8 heads, 20.9 -> 12.9; two of 2048, 16 heads, 65.2 ->
-  // 60.0; with half as many again wanted the first stays at 39.9). How long the
-  // longest sequence is is not known here: twice the mean is taken.
-  const bool many = packed_keys && tiles * kv_heads >= wgs;
+  // Packed rows: tiles are split where the longest would keep its workgroup
+  // busy for longer than a share of all the work and a second launch take:
+  // more than kPackedWholeKeys keys over that share, which grows with the tiles
+  // that there are (one prompt of 1024 tokens, 32 / 8 heads of 128, 35.3 -> 28.1
+  // us whole, of 2000 61.3 -> 50.0; of 4000, 9 / 3 of 64, 45.4 split, 63.6 whole;
+  // one of 2000, 16 heads, 42.2 and 46.3). How long the longest sequence is is not
+  // known here: twice the mean is taken.
   const int64_t longest =
-      packed_keys && 2 * (capacity / batch) < capacity ? 2 * (capacity / batch)
-                                                       : prefix + capacity;
-  if (longest <= most || many ||
+      batch > 2 ? 2 * (capacity / batch) : capacity;
+  const bool whole =
+      longest * (9 * kPagedTargetWgs - 8 * tiles * kv_heads) <=
+      kPackedWholeKeys * 9 * kPagedTargetWgs;
+  if ((packed_keys ? whole : prefix + capacity <= most) ||
       (uint64_t)p.workspace > workspace_limit || p.part_rows > INT32_MAX) {
     // every tile whole and one unit, so each workgroup takes as many
     p.shared = false;
@@ -1828,7 +1844,8 @@ hipError_t launch_attention_paged(PagedKeys keys,
     a.part_of = (i32x2 *)(a.part_ml + a.kv_heads * plan.part_rows * 2);
   }
   // Few rows, whose parts can be many: a row's are dealt to groups.
-  const bool few = all <= kPagedFewRows;
+  const bool few =
+      all <= (keys == PagedKeys::kPages ? kPagedFewRows : kTreeFewRows);
   const PagedKernel *kernel = nullptr, *join = nullptr;
   for (const PagedKernel &k : kPagedKernels)
     if (k.dp == plan.dp) {

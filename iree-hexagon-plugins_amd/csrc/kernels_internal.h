@@ -501,10 +501,14 @@ constexpr uint32_t kWideCost = 10;
 constexpr int64_t kPagedWholeKeys = 512;
 constexpr int64_t kPagedWholeKeysFew = 1024;
 constexpr int64_t kPagedWholeKeysWide = 768;
+constexpr int64_t kPackedWholeKeys = 768;
 // Rows (of all heads) up to which a row's parts are joined by several groups
 // (768 rows of 32749 keys: 52.6 -> 47.8 us; 12960 rows of a prompt and tokens
 // 32.9, with groups 39.1; 71776 rows of prompts 241, with groups 281).
 constexpr int64_t kPagedFewRows = 8192;
+// Of trees and packed rows, which have more rows of fewer parts (8192 rows of 8
+// parts 167.8 -> 163.5 us, 8192 of 1024 keys 29.7 -> 25.5; 1024 is no better).
+constexpr int64_t kTreeFewRows = 2048;
 struct PagedPlan {
   // Head-dim buckets: a staged V's row, what is computed of V, and of Q and K.
   int dp, dx, dk;

@@ -265,8 +265,8 @@ def test_packed_workspace(pkg):
     assert need(rows=2000, key_rows=2000, batch=1) > 0
     assert need(rows=200000, key_rows=200000, batch=1) == 0
     assert need(rows=0) == need(heads=3) == need(head_dim=300) == 0
-    most = 0
-    for rows in range(1, 40000, 501):
-        most = max(most, need(rows=rows, key_rows=rows, batch=1, heads=32,
-                              kv_heads=8, head_dim=128, head_dim_v=128))
-    assert 0 < most < 256 << 20
+    for heads, kv_heads in ((32, 8), (8, 2), (16, 16), (3, 1)):
+        most = max(need(rows=rows, key_rows=rows + more, batch=1, heads=heads,
+                        kv_heads=kv_heads, head_dim=128, head_dim_v=128)
+                   for rows in range(1, 40000, 501) for more in (0, 9000))
+        assert 0 < most < 256 << 20
