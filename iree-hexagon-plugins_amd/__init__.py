@@ -1674,19 +1674,19 @@ def packed_attention(q, k, v, row_starts, key_starts=None, o=None, *,
         raise ValueError(f"{h} query heads are not a multiple of {hkv} KV "
                          "heads")
     flags = CAUSAL if causal else 0
-    if o is None and out_dtype in (None, _F16):
-        pass
-    else:
-        import torch
-        want = out_dtype or o.dtype
-        if want not in (torch.float16, torch.float32):
-            raise TypeError("packed_attention writes float16 or float32")
-        if o is not None:
-            _require(o, want, "o", (3,))
+    want = getattr(o, "dtype", _F16) if out_dtype is None else out_dtype
+    if want is _F32:
+        flags |= ATTENTION_OUT_F32
+    elif want is not _F16:
+        raise TypeError("packed_attention writes float16 or float32")
+    if o is not None:
+        if getattr(o, "dtype", None) is not want:
+            raise TypeError(f"o must be a {want} tensor")
+        if o.shape != (rows, h, dv):
             _shape(o, (rows, h, dv), "o")
-            o0, o1, _ = o.stride()
-        if want == torch.float32:
-            flags |= ATTENTION_OUT_F32
+        o0, o1, last = o.stride()
+        if last != 1 and dv != 1:
+            raise ValueError("o must have unit stride along head_dim")
     starts, = _ints(row_starts, "row_starts")
     if starts < 1:
         raise ValueError("row_starts must be [sequences + 1], got [0]")
@@ -1709,8 +1709,7 @@ def packed_attention(q, k, v, row_starts, key_starts=None, o=None, *,
                 q, k, v, row_starts, key_starts, o, causal=causal,
                 scale=scale, out_dtype=out_dtype, stream=stream)
     if o is None:
-        o = _empty_on(q, (rows, h, dv), stream,
-                      None if not flags & ATTENTION_OUT_F32 else want)
+        o = _empty_on(q, (rows, h, dv), stream, want)
         o0, o1 = h * dv, dv
     batch = starts - 1
     st = _paged_call(

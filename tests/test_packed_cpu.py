@@ -100,6 +100,8 @@ def test_packed_attention_checks(pkg):
     bad("int32", TypeError, row_starts=torch.zeros(4, dtype=torch.int64))
     bad("o must be", o=z(5, 6, 16))
     bad("o must be", TypeError, o=z(5, 6, 24), out_dtype=F)
+    bad("o must be", TypeError, o=[1])
+    bad("unit stride", o=z(5, 24, 6).transpose(1, 2))
     bad("float16 or float32", TypeError, out_dtype=torch.bfloat16)
     bad("float16 or float32", TypeError, o=z(5, 6, 24, dtype=torch.float64))
     bad("device", TypeError)

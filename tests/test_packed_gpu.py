@@ -483,6 +483,89 @@ def test_packed_defaults(pkg, dev):
     assert bool((o == 0).all())
 
 
+def test_packed_output_views(pkg, dev):
+    """Outputs in the columns of a wider buffer, at 16 and at 8 bytes, whole
+    tiles and parts of f16 and f32: what lies beside them stays."""
+    for added, heads, hk, d in (([70, 3], 4, 2, 64), ([1500], 2, 2, 64),
+                                ([900], 2, 1, 128), ([9, 5], 2, 1, 40)):
+        p = Packed(added, heads, hk, d, d)
+        for dtype in (H, F):
+            for pad, at in ((8, 0), (8, 8), (4, 4), (12, 4)):
+                print(f"views {added} {dtype} {pad} {at}", flush=True)
+                buf = torch.full((p.rows, heads, d + pad), 9.0, dtype=dtype,
+                                 device="cuda")
+                view = buf[..., at:at + d]
+                p.check(p.call(pkg, view))
+                assert bool((buf[..., :at] == 9).all()
+                            and (buf[..., at + d:] == 9).all())
+        with pytest.raises(pkg.MI355XError, match="aligned|multiples"):
+            p.call(pkg, torch.zeros(p.rows, heads, d + 2, dtype=H,
+                                    device="cuda")[..., 2:])
+
+
+def test_packed_far_rows(pkg, dev):
+    """Keys whose bytes pass 32 bits, in narrow and wide tiles and in parts."""
+    stride, d, n = 1 << 24, 64, 140
+    buf = torch.empty(stride * (n - 1) + 2 * d, dtype=H, device="cuda")
+    k = buf.as_strided((n, 1, d), (stride, d, 1))
+    v = buf[d:].as_strided((n, 1, d), (stride, d, 1))
+    g = torch.Generator().manual_seed(3)
+    for x in (k, v):
+        x.copy_(torch.randn(n, 1, d, generator=g).half().cuda())
+    for added, keys in (([140], None), ([2, 1], [5, 135]), ([60, 3], [7, 133])):
+        print(f"far {added} {keys}", flush=True)
+        p = Packed(added, 1, 1, d, d, keys)
+        p.k, p.v = k, v
+        p.check(p.call(pkg))
+    # as the last of 6000 rows, in parts
+    k, v = (torch.randn(6000, 1, d, generator=g).half().cuda()
+            for _ in range(2))
+    p = Packed([1, 40], 1, 1, d, d, [100, 5900])
+    p.k, p.v = k, v
+    p.check(p.call(pkg))
+
+
+def test_packed_threads(pkg, dev):
+    """Calls of several threads on one stream, each of two launches, keep
+    their parts."""
+    import threading
+    calls = [Packed([1500 + 100 * i], 2, 2, 64, 64, seed=i) for i in range(4)]
+    want = [p.call(pkg) for p in calls]
+    got = [[] for _ in calls]
+
+    def run(i):
+        for _ in range(20):
+            got[i].append(calls[i].call(pkg))
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for i, p in enumerate(calls):
+        p.check(want[i])
+        assert len(got[i]) == 20
+        assert all(torch.equal(o, want[i]) for o in got[i])
+
+
+def test_packed_ordered_tiles(pkg, dev):
+    """More tiles than run at once, of requests of many lengths: ordered by
+    their keys, each found once; and of more requests than lanes."""
+    g = torch.Generator().manual_seed(11)
+    for batch, lo, hi, heads, hk, causal in (
+            (17, 200, 900, 24, 8, True), (64, 0, 700, 6, 6, True),
+            (30, 1, 1000, 9, 3, False), (65, 100, 500, 8, 8, True),
+            (2, 2000, 2600, 8, 8, True)):
+        added = torch.randint(lo, hi, (batch,), generator=g).tolist()
+        keys = [n + int(torch.randint(0, 300, (1,), generator=g))
+                for n in added]
+        keys[0] = 0
+        print(f"ordered {batch} {heads} {hk}", flush=True)
+        p = Packed(added, heads, hk, 64, 64, keys, causal, pad=2, seed=batch)
+        p.check(p.call(pkg))
+
+
 def test_packed_infinities(pkg, dev):
     """A NaN in a sequence's query or key stays in its rows; infinite scores of
     either sign are the formula's; other sequences' rows are not read."""
