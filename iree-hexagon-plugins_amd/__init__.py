@@ -1256,7 +1256,6 @@ _PAGED_ATTENTION = struct.Struct("@2P11q6P10qfI")
 # A small call is bound by the host: shapes and strides are asked for once, and
 # torch's types once at all.
 _F16 = _I32 = _F32 = None
-_PAD = [(0,) * (4 - n) for n in range(5)]  # sections of axes there are not
 
 
 def _load_types():
@@ -1615,15 +1614,15 @@ def tree_masks(parents, row_starts, words=1, *, stream=None):
         import torch
         with torch.cuda.device(index):
             return tree_masks(parents, row_starts, words, stream=stream)
-    out = _empty_on(parents, rows * (words + 1), stream)
-    masks, depths = out.split_with_sizes((rows * words, rows))
+    masks = _empty_on(parents, (rows, words), stream)
+    depths = _empty_on(parents, (rows,), stream)
     st = library().iree_mi355x_tree_masks(_TREE_MASKS.pack(
-        parents.data_ptr(), row_starts.data_ptr(), out.data_ptr(),
-        out.data_ptr() + 4 * rows * words, rows, starts - 1, words),
+        parents.data_ptr(), row_starts.data_ptr(), masks.data_ptr(),
+        depths.data_ptr(), rows, starts - 1, words),
         _stream_on(index, stream))
     if st != OK:
         _check(st)
-    return masks.view(rows, words), depths
+    return masks, depths
 
 
 def tree_attention(q, k_cache, v_cache, row_starts, lengths, block_table,
@@ -1726,6 +1725,17 @@ def packed_attention(q, k, v, row_starts, key_starts=None, o=None, *,
     return o
 
 
+@functools.lru_cache(maxsize=1024)
+def _sections(sections, axes, half, d) -> tuple:
+    """The four sections of iree_mi355x_rotary_t."""
+    if not 1 <= axes <= 4 or len(sections) != axes:
+        raise ValueError(f"{len(sections)} sections for {axes} axes (1 to 4)")
+    if sum(sections) != half or 2 * half > d or min(sections) < 0:
+        raise ValueError(f"sections {sections} must be the {half} "
+                         f"frequencies, and twice them at most head_dim {d}")
+    return sections + (0,) * (4 - axes)
+
+
 def rotary(q, k, positions, frequencies, sections=None, *, interleaved=False,
            q_out=None, k_out=None, stream=None):
     """Rotary positions of packed rows: turns the first 2 * P dims of every
@@ -1761,12 +1771,8 @@ def rotary(q, k, positions, frequencies, sections=None, *, interleaved=False,
     half = frequencies.numel()
     if frequencies.stride() != (1,) and (frequencies.ndim != 1 or half > 1):
         raise ValueError("frequencies must be 1-D with unit column stride")
-    sections = (half,) if sections is None else tuple(sections)
-    if not 1 <= axes <= 4 or len(sections) != axes:
-        raise ValueError(f"{len(sections)} sections for {axes} axes (1 to 4)")
-    if sum(sections) != half or 2 * half > d or min(sections) < 0:
-        raise ValueError(f"sections {sections} must be the {half} "
-                         f"frequencies, and twice them at most head_dim {d}")
+    pairs = _sections((half,) if sections is None else tuple(sections), axes,
+                      half, d)
     qo, ko = (h * d, d), (hk * d, d)
     if q_out is not None:
         of_q, (*qo, _) = _rows_of(q_out, "q_out", 3)
@@ -1799,7 +1805,7 @@ def rotary(q, k, positions, frequencies, sections=None, *, interleaved=False,
         q.data_ptr(), 0 if k is None else k.data_ptr(), q_out.data_ptr(),
         0 if k is None else k_out.data_ptr(), positions.data_ptr(),
         frequencies.data_ptr(), rows, h, hk, d, axes,
-        *sections, *_PAD[axes], pitch, q0, q1, k0, k1, *qo, *ko, ROTARY_INTERLEAVED if interleaved else 0),
+        *pairs, pitch, q0, q1, k0, k1, *qo, *ko, ROTARY_INTERLEAVED if interleaved else 0),
         _stream_on(index, stream))
     if st != OK:
         _check(st)

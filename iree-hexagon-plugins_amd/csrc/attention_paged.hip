@@ -55,7 +55,7 @@
 // matrix instructions (560 -> 623 us); 8 waves of 32 rows in alternating phases
 // on shared keys (3 % less from 3000 keys on, more below); K read 6 instructions
 // ahead, no wave priorities, priority for a tile's start, 4 workgroups a CU of 64
-// dims (all within 1 %).
+// dims or a third slot of their ring (none better; most within 1 %).
 #include <string>
 
 #include "attention_common.h"
