@@ -56,7 +56,7 @@
 // on shared keys (3 % less from 3000 keys on, more below); K read 6 instructions
 // ahead, no wave priorities, priority for a tile's start, 4 workgroups a CU of 64
 // dims or a third slot of their ring (none better; most within 1 %).
-#include <string>
+#include <cstdio>
 
 #include "attention_common.h"
 #include "device_common.h"
@@ -1893,15 +1893,15 @@ hipError_t launch_attention_paged(PagedKeys keys,
 
 const KernelEntry *attention_paged_kernels(int *count) {
   static KernelEntry all[2 * kPagedKernelCount];
-  static std::string names[kPagedKernelCount];  // of the whole tiles' kernels
+  static char names[kPagedKernelCount][48];  // of the whole tiles' kernels
   static const int filled = [] {
     int n = 0;
     for (const PagedKernel &k : kPagedKernels) {
       all[n++] = {k.name, k.fn, kPagedThreads, 0};
       if (k.whole) {
-        std::string &name = names[&k - kPagedKernels];
-        name = std::string(k.name) + "_whole";
-        all[n++] = {name.c_str(), k.whole, kPagedThreads, 0};
+        char *name = names[&k - kPagedKernels];
+        snprintf(name, sizeof(names[0]), "%s_whole", k.name);
+        all[n++] = {name, k.whole, kPagedThreads, 0};
       }
     }
     return n;

@@ -57,70 +57,73 @@ __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(Rotary r) {
   typedef typename RotaryVector<VEC>::type Vec;
   __shared__ f32x2 turns[kRotaryPairs];
   const int tid = threadIdx.x;
-  const int64_t row0 = (int64_t)blockIdx.x * r.tokens;
-  const int rows =
-      r.rows - row0 < r.tokens ? (int)(r.rows - row0) : r.tokens;
-  for (int i = tid; i < rows * r.half; i += kRotaryThreads) {
-    const int row = i / r.half, pair = i - row * r.half;
-    const int axis = (pair >= r.ends[0]) + (pair >= r.ends[1]) +
-                     (pair >= r.ends[2]);
-    const int position = r.positions[axis * r.position_stride + row0 + row];
-    const double turn =
-        (double)position * (double)r.frequencies[pair] * 0.15915494309189535;
-    float s, c;
-    sincospif((float)(2.0 * (turn - rint(turn))), &s, &c);
-    turns[i] = f32x2{c, s};
-  }
-  __syncthreads();
   const int heads = r.heads[0] + r.heads[1], items = heads * r.pieces;
-  for (int i = tid; i < rows * items; i += kRotaryThreads) {
-    const int row = i / items, at = i - row * items;
-    int head = at / r.pieces;
-    const int piece = at - head * r.pieces;
-    const int which = head >= r.heads[0];
-    head -= which ? r.heads[0] : 0;
-    const f16 *in = r.in[which] + (row0 + row) * r.in_strides[which][0] +
-                    head * r.in_strides[which][1];
-    f16 *out = r.out[which] + (row0 + row) * r.out_strides[which][0] +
-               head * r.out_strides[which][1];
-    const f32x2 *turn = turns + row * r.half;
-    if (piece >= r.rotated) {  // dims past the rotated ones
-      const int d = 2 * r.half + (piece - r.rotated) * VEC;
-      *(Vec *)(out + d) = *(const Vec *)(in + d);
-    } else if (INTERLEAVED && WIDE) {
-      const int d = piece * 8;
-      const f16x8 x = *(const f16x8 *)(in + d);
-      f16x8 y;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        f16 ya, yb;
-        turn_pair(x[2 * e], x[2 * e + 1], turn[d / 2 + e], &ya, &yb);
-        y[2 * e] = ya;
-        y[2 * e + 1] = yb;
-      }
-      *(f16x8 *)(out + d) = y;
-    } else if (WIDE) {
-      const int d = piece * 8;
-      const f16x8 a = *(const f16x8 *)(in + d);
-      const f16x8 b = *(const f16x8 *)(in + r.half + d);
-      f16x8 ya, yb;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        f16 y1, y2;
-        turn_pair(a[e], b[e], turn[d + e], &y1, &y2);
-        ya[e] = y1;
-        yb[e] = y2;
-      }
-      *(f16x8 *)(out + d) = ya;
-      *(f16x8 *)(out + r.half + d) = yb;
-    } else {
-      const int d1 = INTERLEAVED ? 2 * piece : piece;
-      const int d2 = INTERLEAVED ? 2 * piece + 1 : r.half + piece;
-      f16 y1, y2;
-      turn_pair(in[d1], in[d2], turn[piece], &y1, &y2);
-      out[d1] = y1;
-      out[d2] = y2;
+  for (int64_t row0 = (int64_t)blockIdx.x * r.tokens; row0 < r.rows;
+       row0 += (int64_t)gridDim.x * r.tokens) {
+    const int rows =
+        r.rows - row0 < r.tokens ? (int)(r.rows - row0) : r.tokens;
+    for (int i = tid; i < rows * r.half; i += kRotaryThreads) {
+      const int row = i / r.half, pair = i - row * r.half;
+      const int axis = (pair >= r.ends[0]) + (pair >= r.ends[1]) +
+                       (pair >= r.ends[2]);
+      const int position = r.positions[axis * r.position_stride + row0 + row];
+      const double turn =
+          (double)position * (double)r.frequencies[pair] * 0.15915494309189535;
+      float s, c;
+      sincospif((float)(2.0 * (turn - rint(turn))), &s, &c);
+      turns[i] = f32x2{c, s};
     }
+    __syncthreads();
+    for (int i = tid; i < rows * items; i += kRotaryThreads) {
+      const int row = i / items, at = i - row * items;
+      int head = at / r.pieces;
+      const int piece = at - head * r.pieces;
+      const int which = head >= r.heads[0];
+      head -= which ? r.heads[0] : 0;
+      const f16 *in = r.in[which] + (row0 + row) * r.in_strides[which][0] +
+                      head * r.in_strides[which][1];
+      f16 *out = r.out[which] + (row0 + row) * r.out_strides[which][0] +
+                 head * r.out_strides[which][1];
+      const f32x2 *turn = turns + row * r.half;
+      if (piece >= r.rotated) {  // dims past the rotated ones
+        const int d = 2 * r.half + (piece - r.rotated) * VEC;
+        *(Vec *)(out + d) = *(const Vec *)(in + d);
+      } else if (INTERLEAVED && WIDE) {
+        const int d = piece * 8;
+        const f16x8 x = *(const f16x8 *)(in + d);
+        f16x8 y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          f16 ya, yb;
+          turn_pair(x[2 * e], x[2 * e + 1], turn[d / 2 + e], &ya, &yb);
+          y[2 * e] = ya;
+          y[2 * e + 1] = yb;
+        }
+        *(f16x8 *)(out + d) = y;
+      } else if (WIDE) {
+        const int d = piece * 8;
+        const f16x8 a = *(const f16x8 *)(in + d);
+        const f16x8 b = *(const f16x8 *)(in + r.half + d);
+        f16x8 ya, yb;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          f16 y1, y2;
+          turn_pair(a[e], b[e], turn[d + e], &y1, &y2);
+          ya[e] = y1;
+          yb[e] = y2;
+        }
+        *(f16x8 *)(out + d) = ya;
+        *(f16x8 *)(out + r.half + d) = yb;
+      } else {
+        const int d1 = INTERLEAVED ? 2 * piece : piece;
+        const int d2 = INTERLEAVED ? 2 * piece + 1 : r.half + piece;
+        f16 y1, y2;
+        turn_pair(in[d1], in[d2], turn[piece], &y1, &y2);
+        out[d1] = y1;
+        out[d2] = y2;
+      }
+    }
+    __syncthreads();  // before the next tokens' turns
   }
 }
 
@@ -138,10 +141,12 @@ hipError_t launch_rotary(const Rotary &rotary, void *stream) {
       {(const void *)&rotary_kernel<true, false>,
        (const void *)&rotary_kernel<true, true>}};
   void *args[] = {&r};
-  return hipLaunchKernel(
-      kernels[r.wide][r.interleaved],
-      dim3((unsigned)(((int64_t)r.rows + r.tokens - 1) / r.tokens)),
-      dim3(kRotaryThreads), args, 0, (hipStream_t)stream);
+  // A launch has fewer than 2^32 threads.
+  const int64_t wgs = ((int64_t)r.rows + r.tokens - 1) / r.tokens;
+  const int64_t most_wgs = (int64_t)1 << 22;
+  return hipLaunchKernel(kernels[r.wide][r.interleaved],
+                         dim3((unsigned)(wgs < most_wgs ? wgs : most_wgs)),
+                         dim3(kRotaryThreads), args, 0, (hipStream_t)stream);
 }
 
 const KernelEntry *rotary_kernels(int *count) {

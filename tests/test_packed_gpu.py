@@ -728,6 +728,37 @@ def test_a_captured_step(pkg, dev):
             assert torch.equal(a.nan_to_num(7.0), b.nan_to_num(7.0))
 
 
+def test_captured_parts(pkg, dev):
+    """Calls of two launches in graphs of one stream, replayed beside eager calls
+    with the stream's own buffer."""
+    p = Packed([1500], 2, 2, 64, 64)
+    t = Tree([1500, 40], [60, 9], 8, 2, 64, 64, 16, 0, words=2, spare=90)
+    ps, ts = ints(p.starts), [ints(x) for x in (t.starts, t.lengths, t.table)]
+    masks = t.masks.cuda()
+    want_p, want_t = p.call(pkg), t.call(pkg)
+    p.check(want_p)
+    t.check(want_t)
+    outs = []
+    for _ in range(2):
+        po = torch.zeros_like(want_p)
+        to = torch.zeros_like(want_t)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            pkg.packed_attention(p.q, p.k, p.v, ps, o=po)
+            pkg.tree_attention(t.q, t.kc, t.vc, *ts, masks, o=to)
+        outs.append((graph, po, to))
+    for _ in range(3):
+        for graph, po, to in outs:
+            po.zero_()
+            to.zero_()
+            graph.replay()
+            p.call(pkg)
+            t.call(pkg)
+        torch.cuda.synchronize()
+        for _, po, to in outs:
+            assert torch.equal(po, want_p) and torch.equal(to, want_t)
+
+
 def test_another_stream(pkg, dev):
     """Calls that name another stream run in its order."""
     p = Packed([300, 41], 8, 2, 64, 64, pad=2)
