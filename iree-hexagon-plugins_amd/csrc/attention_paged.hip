@@ -1455,6 +1455,12 @@ attention_paged_kernel(PagedAttention) {
   }
 }
 
+// Whole tiles: up to so many requests their tiles are counted, four a lane; of
+// more, which would make every workgroup count long (4096 of 20 to 200 tokens, 12
+// heads of 64: 3692 us, searched 930; 1024 337 and 245, 256 the same, 128 32.5 and
+// 34.7), row_starts alone tell where they can begin.
+constexpr int kScannedRequests = 256;
+
 // Packed rows whose tiles are all whole: a workgroup takes one, found by the
 // requests' numbers of tiles alone (as a line of them 1.5 us longer: 48
 // sequences of 1 to 500 tokens, 12 heads of 64, 37.7 -> 34.2 us; prompts of 7195
@@ -1485,7 +1491,7 @@ void attention_packed_kernel(PagedAttention) {
   const int lane = threadIdx.x & 63;
   const int each = (p.batch + 63) >> 6;
   int begin = 0, end = 0, key0 = 0, key1 = 0;
-  if (lane * each < p.batch) {
+  if (p.batch <= kScannedRequests && lane * each < p.batch) {
     begin = row_start(p, lane * each);
     end = row_start(p, lane * each + 1);
     key0 = key_start(p, lane * each);
@@ -1519,66 +1525,93 @@ void attention_packed_kernel(PagedAttention) {
     const int shift = !WIDE || rows <= kNarrowRows ? 4 : 7;
     return (uint32_t)(rows + (1 << shift) - 1) >> shift;
   };
-  const int tiles_rows = rows_of(p, begin, end);
-  uint32_t tiles = tiles_of(begin, end);
-  for (int i = 1; i < each && lane * each + i < p.batch; ++i)
-    tiles += tiles_of(row_start(p, lane * each + i),
-                      row_start(p, lane * each + i + 1));
-  const uint32_t upto = lane_sums(tiles);
-  const uint32_t total = (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
-  if ((uint32_t)way >= total)
-    return;
   auto lane_at = [&](uint32_t first, uint32_t x) {  // the last first <= x
     return uniform(63 - __builtin_clzll(__ballot(first <= x) | 1));
   };
   auto of_lane = [&](uint32_t x, int l) {
     return (uint32_t)__builtin_amdgcn_readlane((int)x, l);
   };
-  int lane_of;
   uint32_t i;
-  if (p.levels) {
-    // Tile `way` of all by their keys, most first: among those of kLevelKeys *
-    // level keys and more but not of the next level.
-    const uint32_t keys = key1 > key0 ? (uint32_t)(key1 - key0) : 0;
-    const int shift = !WIDE || tiles_rows <= kNarrowRows ? 4 : 7;
-    auto with = [&](uint32_t level) {  // the request's tiles of so many keys
-      const uint32_t least = level * kLevelKeys;
-      const uint32_t n =
-          p.causal ? (uint32_t)((uint64_t)(keys - least) * p.group >> shift) + 1
-                   : tiles;
-      return keys < least ? 0 : n < tiles ? n : tiles;
-    };
-    uint32_t level = 0;
-    for (uint32_t step = (uint32_t)p.levels; step > 0; step >>= 1)
-      if (of_lane(lane_sums(with(level + step)), 63) > (uint32_t)way)
-        level += step;
-    const uint32_t more = with(level + 1);
-    const uint32_t mine = (level == 0 ? tiles : with(level)) - more;
-    const uint32_t rank =
-        (uint32_t)way - of_lane(lane_sums(more), 63);
-    const uint32_t before = lane_sums(mine) - mine;
-    lane_of = lane_at(before, rank);
-    i = of_lane(tiles - 1 - more, lane_of) - (rank - of_lane(before, lane_of));
-    if (i >= of_lane(tiles, lane_of))
-      return;  // (the sums may have wrapped)
-  } else {
-    const uint32_t at = total - 1 - (uint32_t)way;
-    lane_of = lane_at(upto - tiles, at);
-    i = at - of_lane(upto - tiles, lane_of);
-  }
-  begin = __builtin_amdgcn_readlane(begin, lane_of);
-  end = __builtin_amdgcn_readlane(end, lane_of);
-  key0 = __builtin_amdgcn_readlane(key0, lane_of);
-  key1 = __builtin_amdgcn_readlane(key1, lane_of);
-  for (int b = lane_of * each; i >= tiles_of(begin, end);) {
-    // (the sums may have wrapped: no further than the last request)
-    if (++b >= p.batch)
+  if (p.batch <= kScannedRequests) {
+    const int tiles_rows = rows_of(p, begin, end);
+    uint32_t tiles = tiles_of(begin, end);
+    for (int i = 1; i < each && lane * each + i < p.batch; ++i)
+      tiles += tiles_of(row_start(p, lane * each + i),
+                        row_start(p, lane * each + i + 1));
+    const uint32_t upto = lane_sums(tiles);
+    const uint32_t total = (uint32_t)__builtin_amdgcn_readlane((int)upto, 63);
+    if ((uint32_t)way >= total)
       return;
-    i -= tiles_of(begin, end);
+    int lane_of;
+    if (p.levels) {
+      // Tile `way` of all by their keys, most first: among those of kLevelKeys *
+      // level keys and more but not of the next level.
+      const uint32_t keys = key1 > key0 ? (uint32_t)(key1 - key0) : 0;
+      const int shift = !WIDE || tiles_rows <= kNarrowRows ? 4 : 7;
+      auto with = [&](uint32_t level) {  // the request's tiles of so many keys
+        const uint32_t least = level * kLevelKeys;
+        const uint32_t n =
+            p.causal
+                ? (uint32_t)((uint64_t)(keys - least) * p.group >> shift) + 1
+                : tiles;
+        return keys < least ? 0 : n < tiles ? n : tiles;
+      };
+      uint32_t level = 0;
+      for (uint32_t step = (uint32_t)p.levels; step > 0; step >>= 1)
+        if (of_lane(lane_sums(with(level + step)), 63) > (uint32_t)way)
+          level += step;
+      const uint32_t more = with(level + 1);
+      const uint32_t mine = (level == 0 ? tiles : with(level)) - more;
+      const uint32_t rank =
+          (uint32_t)way - of_lane(lane_sums(more), 63);
+      const uint32_t before = lane_sums(mine) - mine;
+      lane_of = lane_at(before, rank);
+      i = of_lane(tiles - 1 - more, lane_of) - (rank - of_lane(before, lane_of));
+      if (i >= of_lane(tiles, lane_of))
+        return;  // (the sums may have wrapped)
+    } else {
+      const uint32_t at = total - 1 - (uint32_t)way;
+      lane_of = lane_at(upto - tiles, at);
+      i = at - of_lane(upto - tiles, lane_of);
+    }
+    begin = __builtin_amdgcn_readlane(begin, lane_of);
+    end = __builtin_amdgcn_readlane(end, lane_of);
+    key0 = __builtin_amdgcn_readlane(key0, lane_of);
+    key1 = __builtin_amdgcn_readlane(key1, lane_of);
+    for (int b = lane_of * each; i >= tiles_of(begin, end);) {
+      // (the sums may have wrapped: no further than the last request)
+      if (++b >= p.batch)
+        return;
+      i -= tiles_of(begin, end);
+      begin = uniform(row_start(p, b));
+      end = uniform(row_start(p, b + 1));
+      key0 = uniform(key_start(p, b));
+      key1 = uniform(key_start(p, b + 1));
+    }
+  } else {
+    // Request b's tiles are numbered from (whole tiles of rows before it) + b on:
+    // always enough, and the numbers past its own are empty. The last request
+    // that begins at or before the way's number, by 64ths.
+    auto first_tile = [&](int b) {
+      return (row_start(p, b) * p.group >> (WIDE ? 7 : 4)) + b;
+    };
+    const int at = uniform(first_tile(p.batch)) - 1 - way;
+    int b = 0;
+    for (int span = p.batch; span > 1;) {
+      const int step = (span + 63) >> 6, mine = b + lane * step;
+      const bool holds = lane * step < span && first_tile(mine) <= at;
+      const int from =
+          uniform(63 - __builtin_clzll(__ballot(holds) | 1)) * step;
+      b += from;
+      span = step < span - from ? step : span - from;
+    }
     begin = uniform(row_start(p, b));
     end = uniform(row_start(p, b + 1));
     key0 = uniform(key_start(p, b));
     key1 = uniform(key_start(p, b + 1));
+    i = (uint32_t)(at - uniform(first_tile(b)));
+    if (at < 0 || i >= tiles_of(begin, end))
+      return;
   }
   const int rows = rows_of(p, begin, end);
   const int shift = !WIDE || rows <= kNarrowRows ? 4 : 7;

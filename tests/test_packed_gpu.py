@@ -566,6 +566,45 @@ def test_packed_ordered_tiles(pkg, dev):
         p.check(p.call(pkg))
 
 
+@pytest.mark.parametrize("batch,lo,hi,heads,hk,d,more", [
+    (257, 0, 140, 2, 1, 64, None),    # one more than are counted
+    (300, 0, 9, 2, 1, 256, 70),       # narrow tiles alone
+    (320, 10, 60, 1, 1, 256, None),
+    (700, 0, 40, 3, 1, 96, 90), (400, 1, 1, 8, 1, 128, 300),
+    (4200, 0, 12, 1, 1, 64, None)])   # three rounds of 64
+def test_packed_many_sequences(pkg, dev, batch, lo, hi, heads, hk, d, more):
+    """More sequences than a workgroup counts, empty ones among them."""
+    print(f"many {batch} {lo} {hi} {heads} {hk} {d} {more}", flush=True)
+    g = torch.Generator().manual_seed(batch)
+
+    def lengths(lo, hi):
+        n = torch.randint(lo, hi + 1, (batch,), generator=g)
+        # runs of sequences without rows, the first and the last among them
+        n[:3], n[70:90], n[-2:] = lo, lo, lo
+        return n.tolist()
+
+    added = lengths(lo, hi)
+    keys = lengths(0, more) if more else None
+    p = Packed(added, heads, hk, d, d, keys, causal=batch % 200 != 0, pad=5,
+               seed=d)
+    p.check(p.call(pkg))
+
+
+def test_packed_many_bad_starts(pkg, dev):
+    """Starts of many sequences that do not ascend: nothing outside is
+    written."""
+    p = Packed([200, 100], 4, 2, 64, 64)
+    top = 2 ** 31 - 1
+    for rows in ([0, 300] * 200, [300, 0] * 200, [-5, top] * 150,
+                 [300] * 301, [top] * 301, [0] * 301,
+                 list(range(300, -1, -1))):
+        print(f"starts {rows[:3]} {len(rows)}", flush=True)
+        buf = torch.full((302, 4, 64), 9.0, dtype=H, device="cuda")
+        pkg.packed_attention(p.q, p.k, p.v, ints(rows), None, buf[1:301])
+        torch.cuda.synchronize()
+        assert bool((buf[0] == 9).all() and (buf[301] == 9).all())
+
+
 def test_packed_infinities(pkg, dev):
     """A NaN in a sequence's query or key stays in its rows; infinite scores of
     either sign are the formula's; other sequences' rows are not read."""
