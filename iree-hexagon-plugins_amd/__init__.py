@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import operator
 import os
 import struct
 import threading
@@ -1727,7 +1728,7 @@ def packed_attention(q, k, v, row_starts, key_starts=None, o=None, *,
 
 @functools.lru_cache(maxsize=1024)
 def _sections(sections, axes, half, d) -> tuple:
-    """The four sections of iree_mi355x_rotary_t."""
+    """The four sections of iree_mi355x_rotary_t, of a tuple of ints."""
     if not 1 <= axes <= 4 or len(sections) != axes:
         raise ValueError(f"{len(sections)} sections for {axes} axes (1 to 4)")
     if sum(sections) != half or 2 * half > d or min(sections) < 0:
@@ -1771,8 +1772,15 @@ def rotary(q, k, positions, frequencies, sections=None, *, interleaved=False,
     half = frequencies.numel()
     if frequencies.stride() != (1,) and (frequencies.ndim != 1 or half > 1):
         raise ValueError("frequencies must be 1-D with unit column stride")
-    pairs = _sections((half,) if sections is None else tuple(sections), axes,
-                      half, d)
+    if sections is None:
+        sections = (half,)
+    else:  # (as keys of the cache below 64.0 and 64 are the same)
+        try:
+            sections = tuple(map(operator.index, sections))
+        except TypeError:
+            raise TypeError(f"sections must be integers, got {sections}") \
+                from None
+    pairs = _sections(sections, axes, half, d)
     qo, ko = (h * d, d), (hk * d, d)
     if q_out is not None:
         of_q, (*qo, _) = _rows_of(q_out, "q_out", 3)

@@ -55,6 +55,27 @@ def test_rotary_checks(pkg):
     bad("device", TypeError, k=None)
 
 
+def test_rotary_sections_are_integers(pkg):
+    """Refused in either order, and a refused call leaves nothing behind that a
+    good one of equal sections would be given."""
+    def call(sections, n, axes=None):
+        positions = i(5) if axes is None else i(axes, 5)
+        pkg.rotary(z(5, 4, 2 * n), None, positions, z(n, dtype=F), sections)
+
+    for n in (13, 29):
+        with pytest.raises(TypeError, match="sections must be integers"):
+            call((float(n),), n)
+        for good in ((n,), [n], None, torch.tensor([n])):
+            with pytest.raises(TypeError, match="device"):
+                call(good, n)
+        with pytest.raises(TypeError, match="sections must be integers"):
+            call((float(n),), n)
+    for bad in ((6.0, 1, 2), ("6", 1, 2), (None,) * 3, 9, torch.ones(3) * 3):
+        with pytest.raises(TypeError, match="sections must be integers"):
+            call(bad, 9, 3)
+    assert all(type(n) is int for n in pkg._sections((13,), 1, 13, 26))
+
+
 def test_tree_masks_checks(pkg):
     bad = refuses(pkg.tree_masks, dict(parents=i(9), row_starts=i(3),
                                        words=2))
