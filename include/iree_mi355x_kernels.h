@@ -339,10 +339,12 @@ int iree_mi355x_append_kv_f16(const iree_mi355x_kv_cache_t *cache,
                               const int64_t v_strides[2],
                               const int32_t *slots, void *stream);
 
-// Attention of packed rows over the cache, f16 in and out, f32 scores and
-// softmax. All requests share a prefix of prefix_length tokens in the pages
-// prefix_pages (0: none, paged attention); request b's own tokens are the
-// first lengths[b] of the pages block_table[b]. Row row_starts[b] + i sees
+// Attention of packed rows over the cache, f16 in and out; scores, softmax
+// statistics and sums in f32, the softmax's weights rounded to f16 (2^-11 of each,
+// an f16 result's own rounding) for their product with V.
+// All requests share a prefix of prefix_length tokens in the pages prefix_pages
+// (0: none, paged attention); request b's own tokens are the first lengths[b] of
+// the pages block_table[b]. Row row_starts[b] + i sees
 // the prefix and own tokens 0 .. lengths[b] - added[b] + i, added[b] =
 // row_starts[b + 1] - row_starts[b]: the new tokens are its last ones.
 //   o[row, h] = softmax(q[row, h] k^T * scale) v, KV head h / (heads /
@@ -421,9 +423,11 @@ int iree_mi355x_tree_attention_f16(const iree_mi355x_paged_attention_t *args,
 //
 // Whole sequences of different lengths as packed rows, without a cache.
 
-// Attention of packed sequences, f16 in, f16 or f32 (OUT_F32) out, f32 scores
-// and softmax. Sequence b's queries are rows row_starts[b] .. row_starts[b + 1]
-// - 1 of q and o, its keys rows key_starts[b] .. key_starts[b + 1] - 1 of k and
+// Attention of packed sequences, f16 in, f16 or f32 (OUT_F32) out; scores,
+// softmax statistics and sums in f32. For their product with V the softmax's
+// weights are rounded to f16, as in the calls above; with OUT_F32 to 22 bits (2^-22
+// of each), for up to about 1.4 times the time.
+// Sequence b's queries are rows row_starts[b] .. row_starts[b + 1] - 1 of q and o, its keys rows key_starts[b] .. key_starts[b + 1] - 1 of k and
 // v (the same array where they are the same rows). With n queries and m keys,
 // query i sees all keys, or with CAUSAL keys 0 .. m - n + i: the queries are
 // its last tokens.

@@ -323,14 +323,38 @@ __device__ __forceinline__ int64_t result_row(const PagedAttention &p,
          (int64_t)(kv_head * p.group + row - token * p.group) * p.o_head;
 }
 // Four columns of it.
-template <PagedKeys KIND>
+template <bool F32>
 __device__ __forceinline__ void store_result(const PagedAttention &p,
                                              int64_t at, f32x4 x) {
-  if (KIND == PagedKeys::kRows && p.out_f32)
+  if (F32)
     *(f32x4 *)((float *)p.o + at) = x;
   else
     *(f16x4 *)(p.o + at) = f16x4{(f16)x[0], (f16)x[1], (f16)x[2], (f16)x[3]};
 }
+// Two weights 2^(s - m) as the matrix instruction takes them, in f16: rounded by
+// at most 2^-11 of each or, the largest being 1, 2^-25; their sum is of the
+// rounded ones. That is of the size of an f16 result's own rounding. F32: a
+// result of 32 bits gets 22 bits of them, what the rounding leaves as a second
+// operand and half as many products again (one prompt of 8191 tokens, 32 / 8 heads
+// of 128: 783 us instead of 556, so f16 results do without). Both are 2^11 times
+// the weight, which the sums cancel: what neither holds is then 2^-22 of it or
+// 2^-36.
+struct Weights {
+  f16x2 f16s, rest;
+};
+template <bool F32>
+__device__ __forceinline__ Weights weights_of(float x, float y) {
+  Weights w = {};
+  if constexpr (F32) {
+    x *= 2048.0f;
+    y *= 2048.0f;
+  }
+  w.f16s = __builtin_convertvector(f32x2{x, y}, f16x2);
+  if constexpr (F32)
+    w.rest = f16x2{(f16)(x - (float)w.f16s[0]), (f16)(y - (float)w.f16s[1])};
+  return w;
+}
+
 __device__ __forceinline__ int64_t part_row(const PagedAttention &p,
                                             const PagedTile &t, int row) {
   return (int64_t)t.kv_head * p.part_rows + t.part + row;
@@ -340,7 +364,7 @@ __device__ __forceinline__ int64_t part_row(const PagedAttention &p,
 
 // A tile of up to 16 rows. DP: the row of a staged V (64, 128 or 256); DX: a
 // multiple of 32 up to it, at least V's head dim; DK: alike of Q's and K's.
-template <int DP, int DX, int DK, PagedKeys KIND>
+template <int DP, int DX, int DK, PagedKeys KIND, bool F32>
 __device__ __forceinline__ void narrow_tile(const PagedTile &t,
                                             const Requests &all, char *smem,
                                             float (*wave_m)[kNarrowRows],
@@ -506,18 +530,19 @@ __device__ __forceinline__ void narrow_tile(const PagedTile &t,
       for (int d = 0; d < DB; ++d)
         o[d] *= keep;
     }
-    // The weights are rounded to f16 for the matrix instruction, by at most
-    // 2^-11 of each or, the largest being 1, 2^-25; the sum is of the rounded
-    // ones.
     const float ref = m_ref == kNegInf ? 0.0f : m_ref;
-    i32x4 pf;
+    i32x4 pf, pf_rest;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const float x0 = s[e >> 1][2 * (e & 1)], x1 = s[e >> 1][2 * (e & 1) + 1];
-      const f16x2 p2 = {(f16)__builtin_amdgcn_exp2f(x0 - ref),
-                        (f16)__builtin_amdgcn_exp2f(x1 - ref)};
-      l_sum = __builtin_amdgcn_fdot2(p2, ones, l_sum, false);
-      pf[e] = __builtin_bit_cast(int, p2);
+      const Weights w = weights_of<F32>(__builtin_amdgcn_exp2f(x0 - ref),
+                                        __builtin_amdgcn_exp2f(x1 - ref));
+      l_sum = __builtin_amdgcn_fdot2(w.f16s, ones, l_sum, false);
+      pf[e] = __builtin_bit_cast(int, w.f16s);
+      if constexpr (F32) {
+        l_sum = __builtin_amdgcn_fdot2(w.rest, ones, l_sum, false);
+        pf_rest[e] = __builtin_bit_cast(int, w.rest);
+      }
     }
 
     // V through this wave's LDS tile; keys that are not there are zeros.
@@ -546,7 +571,10 @@ __device__ __forceinline__ void narrow_tile(const PagedTile &t,
       const i32x2 hi = __builtin_bit_cast(
           i32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                      (IHP_LDS s16x4 *)(at + 16 * (DP * 2))));
-      o[d] = Mfma16<f16>::mma(i32x4{lo[0], lo[1], hi[0], hi[1]}, pf, o[d]);
+      const i32x4 values = {lo[0], lo[1], hi[0], hi[1]};
+      o[d] = Mfma16<f16>::mma(values, pf, o[d]);
+      if constexpr (F32)
+        o[d] = Mfma16<f16>::mma(values, pf_rest, o[d]);
     }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
@@ -602,7 +630,7 @@ __device__ __forceinline__ void narrow_tile(const PagedTile &t,
 #pragma unroll
     for (int e = 0; e < CPT / 4; ++e)
       if (dq + 4 * e < p.dv)  // dv is a multiple of 8
-        store_result<KIND>(p, dst + 4 * e, acc[e] * inv);
+        store_result<F32>(p, dst + 4 * e, acc[e] * inv);
   } else {
     const int64_t at = part_row(p, t, row);
 #pragma unroll
@@ -628,7 +656,7 @@ __device__ __forceinline__ int wide_v_swizzle(int key) {
   return DP >= 128 ? 4 * (key & 3) : 4 * ((key >> 1) & 1);
 }
 
-template <int DP, int DX, int DK, PagedKeys KIND>
+template <int DP, int DX, int DK, PagedKeys KIND, bool F32>
 __device__ __forceinline__ void wide_tile(const PagedTile &t,
                                           const Requests &all, char *smem) {
   const PagedAttention &p = arguments();
@@ -645,9 +673,9 @@ __device__ __forceinline__ void wide_tile(const PagedTile &t,
   // Passes of K after which its swizzle, of 16 rows, is the same again.
   constexpr int TURN = kPagedWaves * KROWS < 16 ? 16 / (kPagedWaves * KROWS) : 1;
   // LDS reads whose waits are counted here, not by the compiler. A read that is
-  // still on its way must stay in its registers, so not where there are too few
-  // of them.
-  constexpr bool OWN_WAITS = DP < 256;
+  // still on its way must stay in its registers, so not where there are, or with
+  // F32's second operands might be, too few of them.
+  constexpr bool OWN_WAITS = DP < 256 && !F32;
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -960,8 +988,7 @@ __device__ __forceinline__ void wide_tile(const PagedTile &t,
         o[dt] *= keep;
     }
     const float m_use = m_run == kNegInf ? 0.0f : m_run;
-    // Weights rounded to f16 as in a narrow tile.
-    i32x4 pw[4];
+    i32x4 pw[4], pw_rest[4];
 #pragma unroll
     for (int f = 0; f < 4; ++f)
 #pragma unroll
@@ -970,8 +997,10 @@ __device__ __forceinline__ void wide_tile(const PagedTile &t,
             __builtin_fmaf(st[f >> 1][8 * (f & 1) + 2 * w], sc, -m_use));
         const float p1 = __builtin_amdgcn_exp2f(
             __builtin_fmaf(st[f >> 1][8 * (f & 1) + 2 * w + 1], sc, -m_use));
-        const f16x2 h = __builtin_convertvector(f32x2{p0, p1}, f16x2);
-        pw[f][w] = __builtin_bit_cast(int, h);
+        const Weights x = weights_of<F32>(p0, p1);
+        pw[f][w] = __builtin_bit_cast(int, x.f16s);
+        if constexpr (F32)
+          pw_rest[f][w] = __builtin_bit_cast(int, x.rest);
       }
 
     // O^T += V^T P^T, 16 keys an MFMA; the V^T fragments of the next key step
@@ -1016,13 +1045,19 @@ __device__ __forceinline__ void wide_tile(const PagedTile &t,
           const i32x4 vf = i32x4{vr[ST % 2][dt][0][0], vr[ST % 2][dt][0][1],
                                  vr[ST % 2][dt][1][0], vr[ST % 2][dt][1][1]};
           o[dt] = Mfma32<f16>::mma(vf, pw[ST], o[dt]);
+          if constexpr (F32)
+            o[dt] = Mfma32<f16>::mma(vf, pw_rest[ST], o[dt]);
         }
         psum[ST] = 0.0f;
+        auto add = [&](int two) {
+          psum[ST] = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, two),
+                                            f16x2{1, 1}, psum[ST], false);
+        };
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-          const int word = pw[ST][w];
-          psum[ST] = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, word),
-                                            f16x2{1, 1}, psum[ST], false);
+          add(pw[ST][w]);
+          if constexpr (F32)
+            add(pw_rest[ST][w]);
         }
       });
       l_run += (psum[0] + psum[1]) + (psum[2] + psum[3]);
@@ -1034,7 +1069,7 @@ __device__ __forceinline__ void wide_tile(const PagedTile &t,
   // the lane's row.
   const float sum = pair_sum(l_run);
   const int row = r_wave + l32;
-  if (KIND != PagedKeys::kPages && t.part < 0 && p.o_wide) {
+  if (KIND != PagedKeys::kPages && !F32 && t.part < 0 && p.o_wide) {
     // The row's lanes exchange halves of two quarters, so that each stores 16
     // bytes of one.
     const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
@@ -1071,7 +1106,7 @@ __device__ __forceinline__ void wide_tile(const PagedTile &t,
 #pragma unroll
       for (int q = 0; q < 4; ++q)
         if (32 * dt + 8 * q < p.dv)  // dv is a multiple of 8
-          store_result<KIND>(
+          store_result<F32>(
               p, dst + 32 * dt + 8 * q,
               f32x4{o[dt][4 * q] * inv, o[dt][4 * q + 1] * inv,
                     o[dt][4 * q + 2] * inv, o[dt][4 * q + 3] * inv});
@@ -1190,8 +1225,8 @@ constexpr int tile_bytes(int dp, int dk, bool wide) {
   return ring > v && ring > merge ? ring : v > merge ? v : merge;
 }
 
-// WIDE: requests of more than 16 rows have wide tiles.
-template <int DP, int DX, int DK, bool WIDE, PagedKeys KIND>
+// WIDE: requests of more than 16 rows have wide tiles. F32: o is (kRows).
+template <int DP, int DX, int DK, bool WIDE, PagedKeys KIND, bool F32 = false>
 __global__ __launch_bounds__(
     kPagedThreads, DP >= 256 || (WIDE && DK > 128) ? 1 : 2) void
 attention_paged_kernel(PagedAttention) {
@@ -1427,9 +1462,9 @@ attention_paged_kernel(PagedAttention) {
     line_at[wave] = {x,  x_end, start, per,        inv_per, t.kv_head,
                      way, b,    i,     small_rows, shared,  q};
     if (shift == 4)
-      narrow_tile<DP, DX, DK, KIND>(t, all, smem, wave_m, wave_l);
+      narrow_tile<DP, DX, DK, KIND, F32>(t, all, smem, wave_m, wave_l);
     else if constexpr (WIDE)
-      wide_tile<DP, DX, DK, KIND>(t, all, smem);
+      wide_tile<DP, DX, DK, KIND, F32>(t, all, smem);
     asm volatile("" ::: "memory");
     const Line &l = line_at[wave];
     x = (uint32_t)uniform((int)l.x);
@@ -1471,7 +1506,7 @@ constexpr int kScannedRequests = 256;
 // one's last tokens. Three workgroups a CU of 64 dims, whose registers just allow it: a
 // short sequence's tile is mostly waiting, for its place, its first keys and its
 // stores (the 48 sequences 44.7 -> 39.1 us).
-template <int DP, int DX, int DK, bool WIDE>
+template <int DP, int DX, int DK, bool WIDE, bool F32>
 __global__ __launch_bounds__(kPagedThreads, DP >= 256 || (WIDE && DK > 128) ? 1
                                             : DP == 64                      ? 3
                                                                             : 2)
@@ -1630,16 +1665,16 @@ void attention_packed_kernel(PagedAttention) {
   t.s_end = (t.seen + kStepKeys - 1) / kStepKeys;
   t.part = -1;
   if (shift == 4)
-    narrow_tile<DP, DX, DK, KIND>(t, all, smem, wave_m, wave_l);
+    narrow_tile<DP, DX, DK, KIND, F32>(t, all, smem, wave_m, wave_l);
   else if constexpr (WIDE)
-    wide_tile<DP, DX, DK, KIND>(t, all, smem);
+    wide_tile<DP, DX, DK, KIND, F32>(t, all, smem);
 }
 
 // Joins the parts of every row that has some: DP / 4 threads, 4 columns each,
 // for every GROUPS-th four of a row's parts, then the GROUPS sums through LDS.
 // A row's parts of one kind (the prefix's of a small request, its own or both
 // at once) are kWideRows rows apart; part_of tells the first and how many.
-template <int DP, int GROUPS, PagedKeys KIND>
+template <int DP, int GROUPS, bool F32>
 __global__ __launch_bounds__(kPagedThreads) void attention_paged_join_kernel(
     PagedAttention p) {
   constexpr int TPR = DP / 4, ROWS = kPagedThreads / TPR / GROUPS;
@@ -1733,7 +1768,7 @@ __global__ __launch_bounds__(kPagedThreads) void attention_paged_join_kernel(
   if (!real || parts == 0 || dq >= p.dv)
     return;
   const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
-  store_result<KIND>(p, result_row(p, kv_head, row) + dq, acc * inv);
+  store_result<F32>(p, result_row(p, kv_head, row) + dq, acc * inv);
 }
 
 // ----------------------------------------------------------------------------
@@ -1746,43 +1781,46 @@ struct PagedKernel {
   const char *name;
   PagedKeys keys;
   int dp, dx, dk, groups;  // groups: of a joined row's parts
-  bool wide;
+  bool wide, f32;
   const void *fn;
   const void *whole = nullptr;  // where no tile is split
 };
-// A join of kPages is also kTree's.
 const PagedKernel kPagedKernels[] = {
-#define IHP_PAGED(NAME, KIND, DP, DX, DK, WIDE)                                \
-  {"attention_" NAME, PagedKeys::KIND, DP, DX, DK, 0, WIDE,                    \
+#define IHP_PAGED(NAME, KIND, DP, DX, DK, WIDE, F32)                           \
+  {"attention_" NAME, PagedKeys::KIND, DP, DX, DK, 0, WIDE, F32,               \
    (const void *)&attention_paged_kernel<DP, DX, DK, WIDE, PagedKeys::KIND>}
-#define IHP_PAGED_ALL(NAME, KIND)                                              \
-  IHP_PAGED(NAME "_d64", KIND, 64, 64, 64, true),                              \
-      IHP_PAGED(NAME "_d96", KIND, 128, 96, 96, true),                         \
-      IHP_PAGED(NAME "_d128", KIND, 128, 128, 128, true),                      \
-      IHP_PAGED(NAME "_d192_128", KIND, 128, 128, 192, false),                 \
-      IHP_PAGED(NAME "_d192_128_rows", KIND, 128, 128, 192, true),             \
-      IHP_PAGED(NAME "_d256", KIND, 256, 256, 256, false)
-    IHP_PAGED_ALL("paged", kPages),
-    IHP_PAGED_ALL("tree", kTree),
+#define IHP_PAGED_ALL(NAME, KIND, F32)                                         \
+  IHP_PAGED(NAME "_d64", KIND, 64, 64, 64, true, F32),                         \
+      IHP_PAGED(NAME "_d96", KIND, 128, 96, 96, true, F32),                    \
+      IHP_PAGED(NAME "_d128", KIND, 128, 128, 128, true, F32),                 \
+      IHP_PAGED(NAME "_d192_128", KIND, 128, 128, 192, false, F32),            \
+      IHP_PAGED(NAME "_d192_128_rows", KIND, 128, 128, 192, true, F32),        \
+      IHP_PAGED(NAME "_d256", KIND, 256, 256, 256, false, F32)
+    IHP_PAGED_ALL("paged", kPages, false),
+    IHP_PAGED_ALL("tree", kTree, false),
 #undef IHP_PAGED
-#define IHP_PAGED(NAME, KIND, DP, DX, DK, WIDE)                                \
-  {"attention_" NAME, PagedKeys::KIND, DP, DX, DK, 0, WIDE,                    \
-   (const void *)&attention_paged_kernel<DP, DX, DK, WIDE, PagedKeys::KIND>,   \
-   (const void *)&attention_packed_kernel<DP, DX, DK, WIDE>}
-    IHP_PAGED_ALL("packed", kRows),
-    IHP_PAGED("packed_d256_rows", kRows, 256, 256, 256, true),
+#define IHP_PAGED(NAME, KIND, DP, DX, DK, WIDE, F32)                           \
+  {"attention_" NAME, PagedKeys::KIND, DP, DX, DK, 0, WIDE, F32,               \
+   (const void *)&attention_paged_kernel<DP, DX, DK, WIDE, PagedKeys::KIND,    \
+                                         F32>,                                 \
+   (const void *)&attention_packed_kernel<DP, DX, DK, WIDE, F32>}
+    IHP_PAGED_ALL("packed", kRows, false),
+    IHP_PAGED("packed_d256_rows", kRows, 256, 256, 256, true, false),
+    IHP_PAGED_ALL("packed_f32", kRows, true),
+    IHP_PAGED("packed_f32_d256_rows", kRows, 256, 256, 256, true, true),
 #undef IHP_PAGED_ALL
 #undef IHP_PAGED
-#define IHP_JOIN(NAME, KIND, DP, GROUPS)                                       \
-  {"attention_" NAME "_join_d" #DP "_g" #GROUPS, PagedKeys::KIND, DP, DP, DP,  \
-   GROUPS, false,                                                              \
-   (const void *)&attention_paged_join_kernel<DP, GROUPS, PagedKeys::KIND>}
-#define IHP_JOIN_ALL(NAME, KIND)                                               \
-  IHP_JOIN(NAME, KIND, 64, 1), IHP_JOIN(NAME, KIND, 64, 8),                    \
-      IHP_JOIN(NAME, KIND, 128, 1), IHP_JOIN(NAME, KIND, 128, 8),              \
-      IHP_JOIN(NAME, KIND, 256, 1), IHP_JOIN(NAME, KIND, 256, 4)
-    IHP_JOIN_ALL("paged", kPages),
-    IHP_JOIN_ALL("packed", kRows),
+// The joins are those of all kinds of keys.
+#define IHP_JOIN(NAME, DP, GROUPS, F32)                                        \
+  {"attention_" NAME "_join_d" #DP "_g" #GROUPS, PagedKeys::kPages, DP, DP,    \
+   DP, GROUPS, false, F32,                                                     \
+   (const void *)&attention_paged_join_kernel<DP, GROUPS, F32>}
+#define IHP_JOIN_ALL(NAME, F32)                                                \
+  IHP_JOIN(NAME, 64, 1, F32), IHP_JOIN(NAME, 64, 8, F32),                      \
+      IHP_JOIN(NAME, 128, 1, F32), IHP_JOIN(NAME, 128, 8, F32),                \
+      IHP_JOIN(NAME, 256, 1, F32), IHP_JOIN(NAME, 256, 4, F32)
+    IHP_JOIN_ALL("paged", false),
+    IHP_JOIN_ALL("packed_f32", true),
 #undef IHP_JOIN_ALL
 #undef IHP_JOIN
 };
@@ -1901,12 +1939,11 @@ hipError_t launch_attention_paged(PagedKeys keys,
       all <= (keys == PagedKeys::kPages ? kPagedFewRows : kTreeFewRows);
   const PagedKernel *kernel = nullptr, *join = nullptr;
   for (const PagedKernel &k : kPagedKernels)
-    if (k.dp == plan.dp) {
+    if (k.dp == plan.dp && k.f32 == (a.out_f32 != 0)) {
       if (k.groups == 0 && k.keys == keys && k.dx == plan.dx &&
           k.dk == plan.dk && k.wide == plan.wide)
         kernel = &k;
-      else if (k.groups > 0 && (k.groups > 1) == few &&
-               (k.keys == PagedKeys::kRows) == (keys == PagedKeys::kRows))
+      else if (k.groups > 0 && (k.groups > 1) == few)
         join = &k;
     }
   if (!kernel || !join)

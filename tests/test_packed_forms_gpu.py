@@ -1,0 +1,138 @@
+"""The forms of packed attention on the GPU: results of 32 bits, and tiles that
+are split along their keys, of every head-dim bucket.
+
+The definition in 64 bits is `Packed`'s, and so is the bound of an f16 result.
+"""
+import pytest
+import torch
+
+from test_packed_gpu import Packed
+
+pytestmark = pytest.mark.gpu
+H, F, D, I32 = torch.float16, torch.float32, torch.float64, torch.int32
+NAN, INF = float("nan"), float("inf")
+
+
+def parts(pkg, p):
+    """The workspace that the call asks for: 0 where tiles are whole."""
+    return pkg._packed_workspace_need(
+        p.rows, p.k.shape[0], len(p.added), p.heads, p.hk, p.d, p.dv)
+
+
+class Packed32(Packed):
+    """Packed with the bound of an f32 result.
+
+    A weight 2^(s - m) <= 2^4 is held as two f16 operands of 2^11 times it: the
+    first is off by 2^-11 of it, the second by 2^-11 of that, or, where either is
+    subnormal, 2^-25, which is 2^-36 of the weights' scale: with p the softmax,
+    A = sum p |v| + |o| and a largest weight of 1 at least
+      2^-22 A + n 2^-36 (max |v| + |o|).
+    exp2's last bits are 2^-22 A at most. The 32-bit sums have two products a
+    key, and a part, a rescaling and the last quotient a rounding each: (2 n +
+    16) 2^-24 A. The scores are off by (d + 8) 2^-24 S, S = max_j scale sum |q
+    k_j|, as an f16 result's. All to first order: 2 % more.
+    """
+
+    def check(self, got, scale=None):
+        scale = self.d ** -0.5 if scale is None else scale
+        assert got.dtype is F
+        group, worst = self.heads // self.hk, 0.0
+        got = got.double()
+        for b, (a, m) in enumerate(zip(self.added, self.keys)):
+            r0, k0 = self.starts[b], self.key_starts[b]
+            mine = got[r0:r0 + a]
+            sees = torch.ones(a, m, dtype=torch.bool, device="cuda")
+            if self.causal:
+                sees = sees.tril(m - a)
+            for h in range(self.heads if a and m else 0):
+                q = self.q[r0:r0 + a, h].double()
+                k = self.k[k0:k0 + m, h // group].double()
+                v = self.v[k0:k0 + m, h // group].double()
+                s = (q @ k.t() * scale).masked_fill(~sees, -INF)
+                p = torch.softmax(s, 1).nan_to_num(0.0)
+                r, n = p @ v, sees.sum(1, keepdim=True)
+                big = ((q.abs() @ k.abs().t()).masked_fill(~sees, 0.0)
+                       .amax(1, keepdim=True) * abs(scale))
+                spread = p @ v.abs() + r.abs()
+                far = (2 ** -21 * spread
+                       + n * 2 ** -36 * (v.abs().amax(0) + r.abs())
+                       + (2 * n + 16 + (self.d + 8) * big) * 2 ** -24 * spread)
+                off = (mine[:, h] - r).abs()
+                assert bool((off <= 1.02 * far).all()), (
+                    b, h, float((off / far.clamp(min=1e-30)).max()))
+                worst = max(worst, float((off / far.clamp(min=1e-30)).max()))
+            if not m:
+                assert bool((mine == 0).all())
+        assert bool((got[self.starts[-1]:] == 9).all()), "past the last"
+        return worst
+
+
+FORMS = [
+    # added, heads, kv heads, d, dv, keys, split
+    ([37, 0, 5], 3, 1, 64, 64, None, False),
+    ([300, 17], 2, 2, 64, 64, None, False),
+    ([70, 130], 6, 1, 96, 96, None, False),
+    ([129, 300], 4, 2, 128, 128, None, False),
+    ([90, 200], 4, 1, 192, 128, None, False),
+    ([1, 2, 3, 1], 4, 1, 192, 128, None, False),
+    ([70, 9, 300], 2, 2, 256, 256, None, False),
+    ([1, 1, 2], 2, 1, 256, 256, [400, 0, 30], False),
+    ([1, 20], 4, 2, 40, 24, [0, 70], False),
+    ([20] * 300, 1, 1, 64, 64, None, False),
+    # tiles in parts: many rows, joined one at a time, and few, by groups
+    ([1500], 2, 2, 64, 64, None, True),
+    ([800], 1, 1, 64, 64, None, True),
+    ([1500], 2, 2, 96, 96, None, True),
+    ([800], 1, 1, 80, 96, None, True),
+    ([1500], 2, 2, 128, 128, None, True),
+    ([3, 0, 500], 4, 1, 128, 128, [2000, 90, 700], True),
+    ([1500], 2, 2, 192, 128, None, True),
+    ([800], 1, 1, 192, 128, None, True),
+    ([1500], 2, 2, 256, 256, None, True),
+    ([0, 1, 200], 2, 2, 200, 232, [900, 1000, 1100], True),
+    # narrow tiles alone
+    ([1, 2], 4, 1, 192, 128, [3000, 4000], True),
+    ([4] * 40, 16, 4, 192, 128, [1500] * 40, True),
+    ([1, 2], 4, 1, 256, 256, [3000, 4000], True),
+    ([4] * 40, 16, 4, 256, 256, [1500] * 40, True)]
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("shape", FORMS)
+def test_packed_f32_has_its_bits(pkg, dev, shape, causal):
+    """A result of 32 bits is as near to the definition as its sums allow, not
+    as f16 weights would be."""
+    added, heads, hk, d, dv, keys, split = shape
+    print(f"f32 {added[:4]} {heads} {hk} {d} {dv} {causal}", flush=True)
+    p = Packed32(added, heads, hk, d, dv, keys, causal, pad=3, seed=d)
+    assert (parts(pkg, p) > 0) == split
+    worst = p.check(p.call(pkg, dtype=F))
+    print(f"of the bound: {worst:.3f}", flush=True)
+
+
+@pytest.mark.parametrize("rows", [1, 130])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_packed_small_weights(pkg, dev, rows, d):
+    """One key far ahead of 4000 that share the rest: weights of 3e-5, which
+    f16 holds with 9 bits; f32 results keep theirs, f16 ones their bound."""
+    print(f"small {rows} {d}", flush=True)
+    p = Packed32([rows], 2, 1, d, d, [4000], False, seed=d)
+    p.q.zero_()
+    p.k.zero_()
+    p.q[:, :, 0], p.k[1234, :, 0] = 8.0, 10.4 / 8 * d ** 0.5
+    p.k[:, :, 1] = torch.linspace(-1, 1, 4000).half().cuda()[:, None]
+    p.q[:, 1, 1] = 1.0
+    p.v.abs_()
+    p.check(p.call(pkg, dtype=F))
+    Packed.check(p, p.call(pkg))
+
+
+def test_packed_f32_views(pkg, dev):
+    """Outputs of 32 bits in the columns of a wider buffer, whole and split."""
+    for added, d in (([200, 3], 64), ([1500], 96), ([800], 256)):
+        p = Packed32(added, 2, 1, d, d)
+        for pad, at in ((8, 4), (4, 0)):
+            buf = torch.full((p.rows, 2, d + pad), 9.0, device="cuda")
+            p.check(p.call(pkg, buf[..., at:at + d]))
+            assert bool((buf[..., :at] == 9).all()
+                        and (buf[..., at + d:] == 9).all())
