@@ -136,3 +136,146 @@ def test_packed_f32_views(pkg, dev):
             p.check(p.call(pkg, buf[..., at:at + d]))
             assert bool((buf[..., :at] == 9).all()
                         and (buf[..., at + d:] == 9).all())
+
+
+# ------------------------------------------------------- tiles in parts, f16 --
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("shape", [s for s in FORMS if s[6]] + [
+    # more sequences than lanes
+    ([3, 0, 1, 9] * 25, 2, 1, 64, 64, [900, 5, 0, 2700] * 25, True),
+    ([1] * 200, 1, 1, 128, 128, [3, 1200] * 100, True),
+    ([2, 1, 0, 6] * 20, 1, 1, 256, 256, [1500, 0, 9, 1700] * 20, True)])
+def test_packed_parts(pkg, dev, shape, causal):
+    added, heads, hk, d, dv, keys, _ = shape
+    print(f"parts {added[:4]} {heads} {hk} {d} {dv} {causal}", flush=True)
+    p = Packed(added, heads, hk, d, dv, keys, causal, pad=3, seed=d + 1)
+    assert parts(pkg, p) > 0
+    p.check(p.call(pkg))
+
+
+SPLIT = [
+    # added, heads, kv heads, d, dv, keys
+    ([1500], 2, 2, 64, 64, None),
+    ([1400, 100], 2, 2, 96, 96, None),
+    ([1500], 2, 2, 192, 128, None),
+    ([1300], 2, 1, 256, 256, None),
+    ([300, 200], 4, 1, 128, 128, [1500, 900]),
+    ([1, 2], 4, 1, 192, 128, [3000, 1000]),
+    ([1, 2], 4, 1, 256, 256, [3000, 1000]),
+    ([40, 2], 1, 1, 64, 64, [60000, 200])]  # of many sequences too
+
+
+@pytest.mark.parametrize("shape", SPLIT)
+def test_packed_parts_nan(pkg, dev, shape):
+    """A NaN in a query stays in its row and head, one in a key in the rows that
+    see it, whatever part it is in."""
+    added, heads, hk, d, dv, keys = shape
+    print(f"nan {shape}", flush=True)
+    group = heads // hk
+    for dtype in (H, F):
+        p = Packed(added, heads, hk, d, dv, keys, seed=d)
+        assert parts(pkg, p) > 0
+        p.q.mul_(0.5)
+        clean = p.call(pkg, dtype=dtype)
+        want = torch.zeros(p.rows, heads, dtype=torch.bool, device="cuda")
+        p.q[0, heads - 1] = NAN
+        want[0, heads - 1] = True
+        # a key in the middle of the last sequence
+        a, n = p.added[-1], p.keys[-1]
+        j = n // 2
+        p.k[p.key_starts[-2] + j, 0] = NAN
+        want[p.starts[-2] + max(0, j - (n - a)):, :group] = True
+        got = p.call(pkg, dtype=dtype)
+        assert torch.equal(got.isnan().all(2), want)
+        assert torch.equal(got.isnan().any(2), want)
+        assert torch.equal(got[~want], clean[~want])
+
+
+@pytest.mark.parametrize("d,dv", [(64, 64), (96, 96), (128, 128), (192, 128),
+                                  (256, 256)])
+def test_packed_parts_infinite_scores(pkg, dev, d, dv):
+    """Keys of scores -inf have the weight 0, whole parts of them too: the rows
+    behind them are those of a sequence that begins there."""
+    lead, n = 400, 1500
+    p = Packed([n], 2, 2, d, dv, seed=d)
+    assert parts(pkg, p) > 0
+    p.q.abs_().clamp_(min=0.01)
+    p.k[:lead] = -INF
+    got = p.call(pkg)
+    rest = Packed32([n - lead], 2, 2, d, dv)
+    rest.q, rest.k, rest.v = p.q[lead:], p.k[lead:], p.v[lead:]
+    Packed.check(rest, got[lead:])
+    rest.check(p.call(pkg, dtype=F)[lead:])
+
+
+def raw(pkg, p, o, workspace, bytes_, starts, key_starts):
+    """The C entry on a workspace of the caller's."""
+    import ctypes
+    a = pkg.PackedAttentionArgs(
+        q=p.q.data_ptr(), k=p.k.data_ptr(), v=p.v.data_ptr(), o=o.data_ptr(),
+        row_starts=starts.data_ptr(), key_starts=key_starts.data_ptr(),
+        rows=p.rows, key_rows=p.k.shape[0], batch=starts.numel() - 1,
+        heads=p.heads, kv_heads=p.hk, head_dim=p.d, head_dim_v=p.dv,
+        scale=p.d ** -0.5, flags=(pkg.CAUSAL if p.causal else 0)
+        | (pkg.ATTENTION_OUT_F32 if o.dtype is F else 0))
+    for name, x in zip("qkvo", (p.q, p.k, p.v, o)):
+        getattr(a, name + "_strides")[:] = x.stride()[:2]
+    return pkg.library().iree_mi355x_packed_attention_f16(
+        ctypes.byref(a), workspace, bytes_,
+        torch.cuda.current_stream().cuda_stream)
+
+
+TOP = 2 ** 31 - 1
+BAD = [
+    # row and key starts, as shares of the rows and of the keys, or as they are
+    ([0, 1.0, 0.3, 1.0], [0, 0.7, 0.3, 1.0]),
+    ([-7, 0.5, TOP], [-TOP - 1, 0.4, TOP]),
+    ([1.0, 0, 1.0], [1.0, 0, 0.6]),
+    ([0, 1.0, 0, 1.0, 0, 1.0], [0, 1.0, 0, 1.0, 0, 1.0]),
+    ([0.5, 0.6, 0.9], [0.9, 0.1, 1.0]),
+    ([0, 0, 0, 1.0], [TOP, TOP, -1, TOP])]
+
+
+@pytest.mark.parametrize("shape", SPLIT)
+def test_packed_parts_bad_starts(pkg, dev, shape):
+    """Starts that do not ascend or lie outside the rows, in the split form: rows
+    hold anything, but nothing beside the output or the workspace is written,
+    whatever the workspace held, and the next call is right."""
+    added, heads, hk, d, dv, keys = shape
+    print(f"bad starts {shape}", flush=True)
+
+    def ints(x):
+        return torch.tensor(x, dtype=I32, device="cuda")
+
+    for causal, dtype in ((True, H), (False, F)):
+        p = Packed(added, heads, hk, d, dv, keys, causal, seed=d)
+        n, guard = p.k.shape[0], 4096
+        for rows, key_rows in BAD + [([0, 1.0] * 33, [0, 1.0] * 33),
+                                     ([1.0, 0] * 40, [0, 1.0] * 40)]:
+            starts, key_starts = (
+                ints([int(x * t) if isinstance(x, float) else x for x in s])
+                for s, t in ((rows, p.rows), (key_rows, n)))
+            need = pkg._packed_workspace_need(
+                p.rows, n, len(rows) - 1, heads, hk, d, dv)
+            if len(rows) <= 4 or n > 60000:
+                assert need > 0
+            for fill in (0, -1, 0x7f):
+                buf = torch.full((p.rows + 2, heads, dv), 9.0, dtype=dtype,
+                                 device="cuda")
+                ws = torch.full((need + 2 * guard,), fill, dtype=torch.int8,
+                                device="cuda")
+                ws[:guard] = ws[guard + need:] = 0x5a
+                assert raw(pkg, p, buf[1:-1], ws.data_ptr() + guard, need,
+                           starts, key_starts) == pkg.OK
+                torch.cuda.synchronize()
+                assert bool((buf[0] == 9).all() and (buf[-1] == 9).all())
+                assert bool((ws[:guard] == 0x5a).all()
+                            and (ws[guard + need:] == 0x5a).all())
+        # the same workspace, right starts
+        buf = torch.full((p.rows, heads, dv), 9.0, dtype=dtype, device="cuda")
+        need = parts(pkg, p)
+        ws = torch.full((need,), 0x7f, dtype=torch.int8, device="cuda")
+        assert raw(pkg, p, buf, ws.data_ptr(), need, ints(p.starts),
+                   ints(p.key_starts)) == pkg.OK
+        p.check(buf)
