@@ -381,18 +381,19 @@ struct TreeMasks {
 };
 hipError_t launch_tree_masks(const TreeMasks &masks, void *stream);
 
-// Rotated rows of q, then of k (rotary.hip): element strides (row, head).
-// A thread takes `pairs` pairs at a time: 8 of halves or 4 of neighbours, where
-// 16-byte loads can (checked on the host), or 1; then the dims past the rotated
-// ones, 8 or 1 at a time. A head's pieces are `pieces`, the first `rotated` of
-// them rotated ones.
+// Rotated rows of q, then of k (rotary.hip): element strides (row, head). Of the
+// `half` pairs, those from ends[0] on turn by the second axis' positions, and so
+// on. `wide` where 16-byte accesses fit all operands (checked on the host): a
+// thread then takes 8 pairs of halves, or 4 of neighbours (`interleaved`), at a
+// time, else 1. A head has `pieces` of those, the first `rotated` of them turned,
+// the others 8 dims, or 1, that are copied. A workgroup takes `tokens` rows.
 struct Rotary {
   const _Float16 *in[2];
   _Float16 *out[2];
   const int32_t *positions;
   const float *frequencies;
   int64_t in_strides[2][2], out_strides[2][2], position_stride;
-  int rows, heads[2], half, dim, ends[3], axes;
+  int rows, heads[2], half, ends[3];
   int tokens, pieces, rotated, interleaved, wide;
 };
 hipError_t launch_rotary(const Rotary &rotary, void *stream);

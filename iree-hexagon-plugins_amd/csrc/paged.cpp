@@ -498,13 +498,11 @@ int iree_mi355x_rotary_f16(const iree_mi355x_rotary_t *a, void *stream) {
   r.position_stride = a->position_stride;
   r.rows = (int)a->rows;
   r.half = (int)half;
-  r.dim = (int)a->head_dim;
   int64_t end = 0;
   for (int i = 0; i < 3; ++i) {  // axes that there are not begin past the pairs
     end = i + 1 < a->axes ? end + a->sections[i] : half;
     r.ends[i] = (int)end;
   }
-  r.axes = (int)a->axes;
   const int vec = wide ? 8 : 1;
   r.rotated = (int)(interleaved && wide ? half / 4 : half / vec);
   r.pieces = r.rotated + (int)((a->head_dim - 2 * half) / vec);
