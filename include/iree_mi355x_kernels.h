@@ -427,18 +427,21 @@ int iree_mi355x_tree_attention_f16(const iree_mi355x_paged_attention_t *args,
 // softmax statistics and sums in f32. For their product with V the softmax's
 // weights are rounded to f16, as in the calls above; with OUT_F32 to 22 bits (2^-22
 // of each), for up to about 1.4 times the time.
-// Sequence b's queries are rows row_starts[b] .. row_starts[b + 1] - 1 of q and o, its keys rows key_starts[b] .. key_starts[b + 1] - 1 of k and
-// v (the same array where they are the same rows). With n queries and m keys,
-// query i sees all keys, or with CAUSAL keys 0 .. m - n + i: the queries are
-// its last tokens.
+// Sequence b's queries are rows row_starts[b] .. row_starts[b + 1] - 1 of q and
+// o, its keys rows key_starts[b] .. key_starts[b + 1] - 1 of k and v (the same
+// array where they are the same rows). With n queries and m keys, query i sees all
+// keys, or with CAUSAL keys 0 .. m - n + i: the queries are its last tokens.
 //   o[row, h] = softmax(q[row, h] k^T * scale) v, KV head h / (heads /
 //   kv_heads); 0 for a row that sees no key, NaN for one with a NaN score
 // Rows from row_starts[batch] on are left as they were. A NaN or infinity in the V
 // of a key that a row does not see may reach it where another row of its tile
 // sees the key (0 times it). Head dims are multiples of 8 up to 256. The starts
 // must ascend from 0: where they do not, rows hold anything, but nothing
-// outside the tensors is read or written. The workspace is as
-// iree_mi355x_shared_prefix_attention_f16's.
+// outside the tensors is read or written. A launch has fewer than 2^32 threads, so
+// a call whose (batch + rows * heads / kv_heads / 128) * kv_heads reaches 2^24 is
+// UNSUPPORTED (/ 16 with head dims above 128 and at most 16 rows a sequence and KV
+// head on average): a million sequences of one token and 16 KV heads are. The
+// workspace is as iree_mi355x_shared_prefix_attention_f16's.
 typedef struct iree_mi355x_packed_attention_t {
   const void *q;              // [rows, heads, head_dim]
   const void *k;              // [key_rows, kv_heads, head_dim]

@@ -274,6 +274,19 @@ def test_packed_attention_argument_errors(pkg):
         assert packed(pkg, **kw) == pkg.OK, kw
 
 
+def test_packed_attention_of_too_many_tiles(pkg):
+    """2^24 (tile, KV head) pairs are more than a launch has."""
+    for batch, rows, heads, kv_heads, d in (
+            (1 << 20, 1 << 20, 16, 16, 64), (1 << 24, 1, 1, 1, 128),
+            (1, 1 << 27, 16, 16, 64), (1, 1 << 27, 64, 16, 128),
+            (1 << 20, 1 << 20, 16, 16, 256)):
+        assert packed(pkg, batch=batch, rows=rows, key_rows=rows, heads=heads,
+                      kv_heads=kv_heads, head_dim=d, head_dim_v=d,
+                      o_strides=(heads * d, d)) == \
+            pkg.UNSUPPORTED, (batch, rows)
+        assert "too large" in pkg.last_error()
+
+
 def test_packed_workspace(pkg):
     """Only prompts whose tiles are too few to keep the CUs busy, and whose keys
     are many, are split."""
