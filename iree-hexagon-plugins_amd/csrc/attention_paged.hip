@@ -40,8 +40,11 @@
 // Trees (kTree): of its request's new tokens a row sees those before it whose bit
 // its mask has. Only blocks that hold new tokens look: 64 bits of the mask, cut
 // from words at any bit, go into the test that hides keys past a row's own
-// (narrow tiles read them with the block's rows, ahead). The masks of chains cost
-// nothing measurable over kPages.
+// (narrow tiles read them with the block's rows, ahead; wide ones where they use
+// them, so that such a step also waits for the next block's copies). All blocks of
+// a prompt without cached tokens are such ones: a chain of 1000, 32 / 8 heads of
+// 128, takes 40.6 us, without masks 35.1; of 4096 217 and 184; of 1000 behind 4000
+// cached tokens 110 and 102.
 //
 // Packed rows (kRows): keys are rows too, so a block's place is a base and its
 // rows follow one another; there are no tables and no prefix. Where there are
@@ -1909,7 +1912,9 @@ hipError_t launch_attention_paged(PagedKeys keys,
   a.least = (int)plan.least;
   a.unit = (int)plan.unit;
   a.tile_units = (int)plan.tile_units;
-  // Requests of a lane each that may differ, and more tiles than run at once.
+  // Requests of a lane each that may differ, and more tiles than
+  // kPagedTargetWgs, which is what runs at once where a CU holds two workgroups
+  // (of 64 dims it holds three, above 128 dims one; the rule is the same).
   a.levels = a.batch > 1 && a.batch <= 64 && a.items > kPagedTargetWgs &&
                      a.key_rows / a.batch >= 2 * (int)kLevelKeys
                  ? 1

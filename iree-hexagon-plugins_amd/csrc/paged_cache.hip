@@ -31,7 +31,8 @@
 // LDS, as far as it holds a request's (4096 words), else in the output. Bound by
 // the chain of 64s in the longest request: 32 trees of 9 to 63 nodes 2.9 us, 48 of
 // up to 250 beside a chain of 500, 8 words, 9 to 10 (with the masks read back from
-// memory 14 to 16).
+// memory 14 to 16). A chain of 2048 takes 29 us, of 8192 112 (2 words, a call among
+// others).
 #include "device_common.h"
 #include "kernels_internal.h"
 
