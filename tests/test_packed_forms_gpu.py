@@ -279,3 +279,40 @@ def test_packed_parts_bad_starts(pkg, dev, shape):
         assert raw(pkg, p, buf, ws.data_ptr(), need, ints(p.starts),
                    ints(p.key_starts)) == pkg.OK
         p.check(buf)
+
+
+def test_packed_f32_captured(pkg, dev):
+    """Whole and split calls of 32 bits in a graph, replayed with other lengths
+    beside f16 calls on the stream's own workspace."""
+    calls = [Packed32([1500], 2, 2, 96, 96, pad=4, seed=1),
+             Packed32([200, 90], 2, 1, 64, 64, seed=2)]
+    assert [parts(pkg, p) > 0 for p in calls] == [True, False]
+    starts = [torch.tensor(p.starts, dtype=I32, device="cuda") for p in calls]
+    outs = [torch.full((p.rows, p.heads, p.dv), 9.0, device="cuda")
+            for p in calls]
+    for p in calls:
+        p.k[p.starts[-1]:] = p.v[p.starts[-1]:] = 1.0
+
+    def step():
+        for p, s, o in zip(calls, starts, outs):
+            pkg.packed_attention(p.q, p.k, p.v, s, o=o)
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for first, second in (([1500], [200, 90]), ([1504], [290, 0]),
+                          ([700], [1, 280])):
+        for p, s, o, added in zip(calls, starts, outs, (first, second)):
+            p.added = p.keys = added
+            p.starts = p.key_starts = [sum(added[:b])
+                                       for b in range(len(added) + 1)]
+            s.copy_(torch.tensor(p.starts, dtype=I32))
+            o.fill_(9.0)
+        graph.replay()
+        half = [p.call(pkg) for p in calls]
+        torch.cuda.synchronize()
+        for p, o, h in zip(calls, outs, half):
+            p.check(o)
+            Packed.check(p, h)
